@@ -9,6 +9,8 @@ const SOURCES: &[&str] = &[
         "rv_prologue.hip",
         "rv_decode.hip",
         "rv_prefill.hip",
+        "rv_q8.hip",
+        "rv_rows.hip",
         "rv_quant.hip",
         "rv_batched.hip",
         "rv_gemv_abi.cpp",

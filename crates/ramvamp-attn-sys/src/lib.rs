@@ -46,6 +46,7 @@ pub const RV_TUNE_DECODE_DEPTH: i32 = 9;
 pub const RV_TUNE_DECODE_MERGE: i32 = 11;
 pub const RV_ELEM_F16: i32 = 1;
 pub const RV_ELEM_F32: i32 = 2;
+pub const RV_ELEM_Q8_0: i32 = 4;
 pub const RV_QF_Q4_K: u32 = 1;
 pub const RV_QF_Q5_K: u32 = 2;
 pub const RV_QF_Q6_K: u32 = 3;
@@ -134,6 +135,9 @@ extern "C" {
     pub fn rv_kv_append_rows(kv: *mut rv_kv, layer: usize, k: *const f32, v: *const f32, rows: usize, row_len: usize, flags: u32, err: *mut rv_error) -> i32;
     pub fn rv_kv_clear(kv: *mut rv_kv);
     pub fn rv_kv_truncate(kv: *mut rv_kv, new_len: usize, err: *mut rv_error) -> i32;
+    pub fn rv_kv_truncate_layer(kv: *mut rv_kv, layer: usize, new_len: usize, err: *mut rv_error) -> i32;
+    pub fn rv_kv_append_each(kv: *mut rv_kv, layer0: usize, n: usize, k: *const f32, v: *const f32, row_len: usize, flags: u32, err: *mut rv_error) -> i32;
+    pub fn rv_kv_read_rows(kv: *const rv_kv, layer: usize, pos: usize, rows: usize, k: *mut f32, v: *mut f32, flags: u32, err: *mut rv_error) -> i32;
     pub fn rv_kv_k_layer(kv: *const rv_kv, layer: usize, dev: *mut *const c_void, n_elems: *mut usize, err: *mut rv_error) -> i32;
     pub fn rv_kv_v_layer(kv: *const rv_kv, layer: usize, dev: *mut *const c_void, n_elems: *mut usize, err: *mut rv_error) -> i32;
     pub fn rv_kv_read_row(kv: *const rv_kv, plane_v: c_int, layer: usize, pos: usize, dst: *mut c_void, err: *mut rv_error) -> i32;
@@ -145,6 +149,8 @@ extern "C" {
     pub fn rv_attention_at_in(kv: *const rv_kv, q: *const f32, q_len: usize, layer: usize, positions: usize, scale: f32, scratch_len: usize, out: *mut f32, out_len: usize, flags: u32, err: *mut rv_error) -> i32;
     pub fn rv_attention_at_kv_range_in(kv: *const rv_kv, q: *const f32, q_len: usize, layer: usize, positions: usize, scale: f32, kv_lo: usize, kv_hi: usize, scratch_len: usize, out: *mut f32, out_len: usize, flags: u32, err: *mut rv_error) -> i32;
     pub fn rv_attention_at_rows(kv: *const rv_kv, q_rows: *const f32, rows: usize, q_dim: usize, layer: usize, start: usize, scale: f32, out: *mut f32, flags: u32, err: *mut rv_error) -> i32;
+    pub fn rv_decode_attention_shared(prefix: *const rv_kv, prefix_layer: usize, prefix_positions: usize, tails: *const rv_kv, tail_layer: usize, q_rows: *const f32, n_seqs: usize, q_dim: usize, scale: f32, out: *mut f32, flags: u32, err: *mut rv_error) -> i32;
+    pub fn rv_decode_step_shared(prefix: *const rv_kv, prefix_layer: usize, prefix_positions: usize, tails: *mut rv_kv, tail_layer: usize, n_seqs: usize, q_rows: *const f32, k_rows: *const f32, v_rows: *const f32, q_dim: usize, q_norm_w: *const f32, q_norm_len: usize, k_norm_w: *const f32, k_norm_len: usize, eps: f32, theta: f32, scale: f32, out: *mut f32, flags: u32, err: *mut rv_error) -> i32;
     pub fn rv_decode_step(kv: *mut rv_kv, layer: usize, q: *const f32, q_len: usize, k: *const f32, k_len: usize, v: *const f32, v_len: usize, q_norm_w: *const f32, q_norm_len: usize, k_norm_w: *const f32, k_norm_len: usize, eps: f32, theta: f32, position: usize, scale: f32, out: *mut f32, out_len: usize, flags: u32, err: *mut rv_error) -> i32;
     pub fn rv_decode_step_dev(kv: *mut rv_kv, layer: usize, q: *const f32, q_len: usize, k: *const f32, k_len: usize, v: *const f32, v_len: usize, q_norm_w: *const f32, q_norm_len: usize, k_norm_w: *const f32, k_norm_len: usize, eps: f32, theta: f32, d_position: *const u32, max_position: usize, scale: f32, out: *mut f32, out_len: usize, flags: u32, err: *mut rv_error) -> i32;
     pub fn rv_kv_commit(kv: *mut rv_kv, layer: usize, rows: usize, err: *mut rv_error) -> i32;

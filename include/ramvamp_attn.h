@@ -73,8 +73,15 @@ typedef struct rv_error {
 /* Element type of the cache planes. RV_ELEM_F16 is the reference's own
  * format (f16 bits, round-to-nearest-even on append, kv/mod.rs:336-368);
  * RV_ELEM_F32 keeps the identical [layer][capacity][kv_dim] indexing with
- * 4-byte elements. */
-typedef enum rv_elem { RV_ELEM_F16 = 1, RV_ELEM_F32 = 2 } rv_elem;
+ * 4-byte elements. RV_ELEM_Q8_0 (no reference counterpart) keeps each head's
+ * row in blocks of 32 values, the codes and f16 scales of
+ * rv_quantize_row_q8_0 (8.5 bits a value); head_dim must be a multiple of 32,
+ * at most 512 (else RV_KV_INVALID_DIMS). What a reader sees of a value is
+ * f16(scale * code). A block whose scale times 127 would pass f16's range
+ * (magnitudes above 65468) saturates at scale 515.5; a block with an
+ * infinity or a NaN reads as 32 NaNs. Every call below takes such a cache but
+ * rv_kv_k_layer / rv_kv_v_layer. */
+typedef enum rv_elem { RV_ELEM_F16 = 1, RV_ELEM_F32 = 2, RV_ELEM_Q8_0 = 4 } rv_elem;
 
 /* flags */
 #define RV_HOST_PTRS 0x1u   /* tensor pointers are host memory */
@@ -83,7 +90,9 @@ typedef enum rv_elem { RV_ELEM_F16 = 1, RV_ELEM_F32 = 2 } rv_elem;
  * always fp32 arithmetic). Default (0) = RV_PREFILL_EXACT. EXACT and F16 take
  * their operands (q, K, V, and P <= 2^8) through f16: values must stay below
  * 65504 in magnitude, and EXACT keeps its ~2^-21 relative products only for
- * values above f16's normal minimum (2^-14); BF16 has fp32's range. */
+ * values above f16's normal minimum (2^-14); BF16 has fp32's range. On a
+ * Q8_0 cache K and V are f16 operands as stored; EXACT splits q and P into hi
+ * + lo halves, F16 and BF16 both round them to f16, q scaled into its range. */
 #define RV_PREFILL_EXACT 0x00u /* split-f16 MFMA, fp32-equivalent products */
 #define RV_PREFILL_F16 0x10u   /* single-pass f16 MFMA inputs, fp32 accumulate */
 #define RV_PREFILL_BF16 0x20u  /* single-pass bf16 MFMA inputs, fp32 accumulate */
@@ -107,13 +116,16 @@ size_t rv_scratch_len(size_t n_q_heads, size_t n_kv_heads, size_t head_dim,
 
 /* ---- KV cache (crates/core/src/kv/mod.rs) ---------------------------- */
 
-/* kv/mod.rs:237-259 `KvCache::projected_bytes`, for either element type
- * (2 planes * n_layers * capacity * n_kv_heads * head_dim * elem size). */
+/* kv/mod.rs:237-259 `KvCache::projected_bytes`, for each element type
+ * (2 planes * n_layers * capacity * n_kv_heads * head_dim * elem size; Q8_0: 34
+ * bytes per 32 elements). */
 int32_t rv_kv_projected_bytes(size_t n_layers, size_t n_kv_heads, size_t head_dim,
                               size_t capacity, rv_elem elem, uint64_t* bytes,
                               rv_error* err);
 
-/* kv/mod.rs:163-181 `KvCache::new`: zeroed planes on `device`, every cursor 0. */
+/* kv/mod.rs:163-181 `KvCache::new`: zeroed planes on `device`, every cursor 0.
+ * A Q8_0 cache pads its capacity to whole tiles of 128 rows in memory, and
+ * takes at most 2^31 - 256 rows (RV_ERR_UNSUPPORTED). */
 int32_t rv_kv_new(size_t n_layers, size_t n_kv_heads, size_t head_dim, size_t capacity,
                   rv_elem elem, int device, rv_kv** out, rv_error* err);
 void rv_kv_free(rv_kv* kv);
@@ -145,14 +157,33 @@ int32_t rv_kv_append_rows(rv_kv* kv, size_t layer, const float* k, const float* 
 /* kv/mod.rs:383-385 `clear` and :410-420 `truncate`. */
 void rv_kv_clear(rv_kv* kv);
 int32_t rv_kv_truncate(rv_kv* kv, size_t new_len, rv_error* err);
+/* No reference counterpart: `truncate` of one layer alone, whatever the
+ * others hold (a batch's layers are its sequences' rows, see
+ * rv_decode_attention_shared): new_len above the layer's length is
+ * RV_KV_TRUNCATE_BEYOND_LENGTH. */
+int32_t rv_kv_truncate_layer(rv_kv* kv, size_t layer, size_t new_len, rv_error* err);
+/* No reference counterpart: one row appended to each of the layers layer0 ..
+ * layer0 + n - 1, each at its own cursor, in one launch (per 256). k and v hold
+ * n * kv_dim f32. All or nothing: the first layer without room is
+ * RV_KV_CAPACITY_EXCEEDED. n == 0 is a no-op. */
+int32_t rv_kv_append_each(rv_kv* kv, size_t layer0, size_t n, const float* k, const float* v, size_t row_len,
+                          uint32_t flags, rv_error* err);
+/* No reference counterpart: rows pos .. pos + rows - 1 of a layer as f32, the
+ * values attention reads, whatever the element type: rows * kv_dim f32 into
+ * each of k and v (either may be null). Past the layer's length is
+ * RV_KV_POSITION_OUT_OF_RANGE (b = the last row asked for). */
+int32_t rv_kv_read_rows(const rv_kv* kv, size_t layer, size_t pos, size_t rows, float* k, float* v, uint32_t flags,
+                        rv_error* err);
 /* kv/mod.rs:449-460 `k_layer` / `v_layer`: the device address of a layer's
- * plane and the element count the view covers (`len(layer) * kv_dim`). */
+ * plane and the element count the view covers (`len(layer) * kv_dim`). A Q8_0
+ * plane holds no such elements: RV_ERR_UNSUPPORTED. */
 int32_t rv_kv_k_layer(const rv_kv* kv, size_t layer, const void** dev, size_t* n_elems,
                       rv_error* err);
 int32_t rv_kv_v_layer(const rv_kv* kv, size_t layer, const void** dev, size_t* n_elems,
                       rv_error* err);
 /* kv/mod.rs:428-441 `k_row` / `v_row`, copied to host memory: `dst` gets
- * kv_dim elements of the plane's type (u16 f16 bits or f32). */
+ * kv_dim elements of the plane's type (u16 f16 bits or f32); of a Q8_0 cache
+ * the row's kv_dim / 32 blocks of 34 bytes, f16 scale then 32 int8 codes. */
 int32_t rv_kv_read_row(const rv_kv* kv, int plane_v, size_t layer, size_t pos, void* dst,
                        rv_error* err);
 
@@ -220,6 +251,40 @@ int32_t rv_attention_at_rows(const rv_kv* kv, const float* q_rows, size_t rows, 
                              size_t layer, size_t start, float scale, float* out,
                              uint32_t flags, rv_error* err);
 
+/* ---- decode for a batch that shares a prefix (no reference counterpart) ----
+ * One token of each of n_seqs sequences that continue the same prompt (the
+ * server's reused prefix, server/src/engine.rs:388-417, for several requests
+ * at once): row i of q_rows (q_dim post-RoPE f32) attends rows 0 ..
+ * prefix_positions of `prefix`'s layer prefix_layer, then every row of its own,
+ * which are layer tail_layer + i of `tails` (a cache whose layers are the
+ * batch's slots: for a model of L layers make it with L * n_seqs layers and
+ * use tail_layer = layer * n_seqs; the lengths may be ragged). The prefix's
+ * rows are read once for the whole batch. prefix_positions may be 0; a
+ * sequence without any row at all is RV_ATTN_EMPTY_LAYER. out is n_seqs *
+ * q_dim. Equal to rv_decode_attention over a cache holding the prefix's rows
+ * and then the sequence's, within fp32 reassociation.
+ * Checks, in order: the two caches' geometry, element type, device and stream
+ * (RV_ERR_UNSUPPORTED where they differ), q_dim, the prefix's layer and
+ * positions, the tails' layers, empty sequences. Work is queued on that
+ * stream; `tails`' workspace is used. F32 planes pass through f16 hi + lo
+ * operands as RV_PREFILL_EXACT's do: magnitudes below 65504, and the full
+ * precision above 2^-14. */
+int32_t rv_decode_attention_shared(const rv_kv* prefix, size_t prefix_layer, size_t prefix_positions,
+                                   const rv_kv* tails, size_t tail_layer, const float* q_rows, size_t n_seqs,
+                                   size_t q_dim, float scale, float* out, uint32_t flags, rv_error* err);
+/* The batch's whole step for one layer, as rv_decode_step for each sequence:
+ * q and k rows RMSNormed and rotated at position prefix_positions + the
+ * sequence's own length, k and v rows appended to the sequence's layer of
+ * `tails`, then rv_decode_attention_shared. q_rows, k_rows and v_rows are
+ * pre-norm, n_seqs rows each. head_dim and the norm weights are checked first,
+ * then as above with RV_KV_CAPACITY_EXCEEDED for the first full layer in place
+ * of the empty one. */
+int32_t rv_decode_step_shared(const rv_kv* prefix, size_t prefix_layer, size_t prefix_positions, rv_kv* tails,
+                              size_t tail_layer, size_t n_seqs, const float* q_rows, const float* k_rows,
+                              const float* v_rows, size_t q_dim, const float* q_norm_w, size_t q_norm_len,
+                              const float* k_norm_w, size_t k_norm_len, float eps, float theta, float scale,
+                              float* out, uint32_t flags, rv_error* err);
+
 /* ---- fused layer steps ------------------------------------------------ */
 
 /* model/forward.rs:2622-2633, one decode token of one layer: per-head
@@ -256,7 +321,7 @@ int32_t rv_decode_step(rv_kv* kv, size_t layer, const float* q, size_t q_len, co
  * The first call for a (theta, max_position) builds the (cos, sin) table and
  * workspace and must not be captured; later calls may be. Device pointers
  * only (RV_HOST_PTRS is RV_ERR_UNSUPPORTED); head_dim 128 and a group of at
- * most 16 (else RV_ERR_UNSUPPORTED). Results equal rv_decode_step's within
+ * most 16 unless the cache is Q8_0 (else RV_ERR_UNSUPPORTED). Results equal rv_decode_step's within
  * fp32 reassociation (the splits follow max_position, not the length). */
 int32_t rv_decode_step_dev(rv_kv* kv, size_t layer, const float* q, size_t q_len, const float* k,
                            size_t k_len, const float* v, size_t v_len, const float* q_norm_w,

@@ -24,8 +24,10 @@ from .attention import (  # noqa: F401
     decode_attention_in,
     decode_attention_kv_range_in,
     decode_attention_noalloc,
+    decode_attention_shared,
     decode_step,
     decode_step_dev,
+    decode_step_shared,
     position_advance,
     prefill_chunk,
     scratch_len,

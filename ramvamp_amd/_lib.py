@@ -20,6 +20,7 @@ RV_PREFILL_F16 = 0x10
 RV_PREFILL_BF16 = 0x20
 RV_ELEM_F16 = 1
 RV_ELEM_F32 = 2
+RV_ELEM_Q8_0 = 4
 RV_TUNE_DECODE_SPLIT_LEN = 1
 RV_TUNE_PREFILL_KV_SPLIT = 2
 RV_TUNE_DECODE_WAVES = 3
@@ -82,6 +83,9 @@ SIGNATURES = {
     "rv_kv_append_rows": (c_int32, [_P, c_size_t, _P, _P, c_size_t, c_size_t, c_uint32, _E]),
     "rv_kv_clear": (None, [_P]),
     "rv_kv_truncate": (c_int32, [_P, c_size_t, _E]),
+    "rv_kv_truncate_layer": (c_int32, [_P, c_size_t, c_size_t, _E]),
+    "rv_kv_append_each": (c_int32, [_P, c_size_t, c_size_t, _P, _P, c_size_t, c_uint32, _E]),
+    "rv_kv_read_rows": (c_int32, [_P, c_size_t, c_size_t, c_size_t, _P, _P, c_uint32, _E]),
     "rv_kv_k_layer": (c_int32, [_P, c_size_t, POINTER(c_void_p), POINTER(c_size_t), _E]),
     "rv_kv_v_layer": (c_int32, [_P, c_size_t, POINTER(c_void_p), POINTER(c_size_t), _E]),
     "rv_kv_read_row": (c_int32, [_P, c_int, c_size_t, c_size_t, _P, _E]),
@@ -95,6 +99,10 @@ SIGNATURES = {
     "rv_attention_at_kv_range_in": (c_int32, [_P, _P, c_size_t, c_size_t, c_size_t, c_float, c_size_t, c_size_t,
                                               c_size_t, _P, c_size_t, c_uint32, _E]),
     "rv_attention_at_rows": (c_int32, [_P, _P, c_size_t, c_size_t, c_size_t, c_size_t, c_float, _P, c_uint32, _E]),
+    "rv_decode_attention_shared": (c_int32, [_P, c_size_t, c_size_t, _P, c_size_t, _P, c_size_t, c_size_t, c_float,
+                                             _P, c_uint32, _E]),
+    "rv_decode_step_shared": (c_int32, [_P, c_size_t, c_size_t, _P, c_size_t, c_size_t, _P, _P, _P, c_size_t, _P,
+                                        c_size_t, _P, c_size_t, c_float, c_float, c_float, _P, c_uint32, _E]),
     "rv_decode_step": (c_int32, [_P, c_size_t, _P, c_size_t, _P, c_size_t, _P, c_size_t, _P, c_size_t, _P, c_size_t,
                                  c_float, c_float, c_size_t, c_float, _P, c_size_t, c_uint32, _E]),
     "rv_decode_step_dev": (c_int32, [_P, c_size_t, _P, c_size_t, _P, c_size_t, _P, c_size_t, _P, c_size_t, _P,

@@ -7,7 +7,8 @@ reference read the same here. Differences, all forced by the device:
 
 - ``KvCache`` lives on a GPU (planes in HBM, cursors on the host) and takes
   an element type: ``"f16"`` is the reference's format, ``"f32"`` keeps the
-  same layout with 4-byte elements.
+  same layout with 4-byte elements, ``"q8_0"`` (no reference counterpart)
+  keeps rows in blocks of 32 8-bit codes with an f16 scale.
 - Tensors are either torch tensors on the cache's GPU (device pointers; the
   call is queued on torch's current stream) or numpy arrays (host pointers;
   the call copies in, computes, copies out and returns when done). One call
@@ -176,7 +177,9 @@ def _elem_code(elem) -> int:
         return L.RV_ELEM_F16
     if elem in ("f32", L.RV_ELEM_F32):
         return L.RV_ELEM_F32
-    raise ValueError(f"elem must be 'f16' or 'f32', got {elem!r}")
+    if elem in ("q8_0", L.RV_ELEM_Q8_0):
+        return L.RV_ELEM_Q8_0
+    raise ValueError(f"elem must be 'f16', 'f32' or 'q8_0', got {elem!r}")
 
 
 class KvCache:
@@ -188,7 +191,7 @@ class KvCache:
         _check(_lib().rv_kv_new(n_layers, n_kv_heads, head_dim, capacity, _elem_code(elem), device, byref(self._h),
                                 byref(err)), err)
         self.device = device
-        self.elem = "f16" if _elem_code(elem) == L.RV_ELEM_F16 else "f32"
+        self.elem = {L.RV_ELEM_F16: "f16", L.RV_ELEM_F32: "f32", L.RV_ELEM_Q8_0: "q8_0"}[_elem_code(elem)]
         self._stream = None
 
     new = classmethod(lambda cls, *a, **k: cls(*a, **k))
@@ -274,6 +277,42 @@ class KvCache:
         err = L.RvError()
         _check(_lib().rv_kv_truncate(self._h, new_len, byref(err)), err)
 
+    def truncate_layer(self, layer: int, new_len: int):
+        """rv_kv_truncate_layer (no reference counterpart): one layer's length
+        alone, for a cache whose layers are a batch's sequences."""
+        err = L.RvError()
+        _check(_lib().rv_kv_truncate_layer(self._h, layer, new_len, byref(err)), err)
+
+    def append_each(self, layer0: int, k_rows, v_rows):
+        """rv_kv_append_each (no reference counterpart): row i of k_rows and
+        v_rows to layer layer0 + i, each at its own cursor (all rows or none)."""
+        ka, va = _Arg(k_rows), _Arg(v_rows)
+        kv_dim = self.kv_dim()
+        if ka.n != va.n or ka.n % kv_dim:
+            raise ValueError("k_rows and v_rows must both be rows x kv_dim")
+        err = L.RvError()
+        _check(_lib().rv_kv_append_each(self._h, layer0, ka.n // kv_dim, ka.ptr, va.ptr, kv_dim,
+                                        _flags(self, (ka, va)), byref(err)), err)
+
+    def read_rows(self, layer: int, start: int, rows: int, k=None, v=None):
+        """rv_kv_read_rows (no reference counterpart): the values of rows
+        start .. start + rows as attention reads them, (k, v) float32 [rows]
+        [kv_dim], into the tensors (or numpy arrays) given, else into new
+        device tensors."""
+        if k is None and v is None:
+            import torch
+
+            k = torch.empty(rows, self.kv_dim(), dtype=torch.float32, device=f"cuda:{self.device}")
+            v = torch.empty_like(k)
+        ka, va = _Arg(k, writable=True), _Arg(v, writable=True)
+        for a in (ka, va):
+            if a.host is not None and a.n != rows * self.kv_dim():
+                raise ValueError("k and v must be rows x kv_dim")
+        err = L.RvError()
+        _check(_lib().rv_kv_read_rows(self._h, layer, start, rows, ka.ptr, va.ptr, _flags(self, (ka, va)),
+                                      byref(err)), err)
+        return k, v
+
     def commit(self, layer: int, rows: int):
         """rv_kv_commit (no reference counterpart): adds the rows that
         device-position steps wrote to the layer's length; a step refused on
@@ -318,7 +357,10 @@ class KvCache:
 
     def _row(self, plane_v: int, layer: int, pos: int) -> np.ndarray:
         self._bind_stream()  # the copy is ordered after work queued on torch's current stream
-        out = np.empty(self.kv_dim(), dtype=np.uint16 if self.elem == "f16" else np.float32)
+        if self.elem == "q8_0":  # blocks of 34 bytes: f16 scale, 32 int8 codes
+            out = np.empty((self.kv_dim() // 32, 34), dtype=np.uint8)
+        else:
+            out = np.empty(self.kv_dim(), dtype=np.uint16 if self.elem == "f16" else np.float32)
         err = L.RvError()
         _check(_lib().rv_kv_read_row(self._h, plane_v, layer, pos, out.ctypes.data_as(c_void_p), byref(err)), err)
         return out
@@ -446,6 +488,54 @@ def attention_at_rows(q_rows, cache: KvCache, layer: int, start: int, scale: flo
     flags = _flags(cache, (qa, oa)) | _MODES[mode]
     _check(_lib().rv_attention_at_rows(cache.handle, qa.ptr, rows, q_dim, layer, start, scale, oa.ptr, flags,
                                        byref(err)), err)
+    return out
+
+
+def _same_stream(prefix: KvCache, tails: KvCache):
+    """Both caches of a batch on torch's current stream (host arrays too: the two
+    have to agree)."""
+    prefix._bind_stream()
+    tails._bind_stream()
+
+
+def decode_attention_shared(q_rows, prefix: KvCache, prefix_layer: int, prefix_positions: int, tails: KvCache,
+                            tail_layer: int, scale: float, out):
+    """rv_decode_attention_shared (no reference counterpart): row i of q_rows
+    attends rows 0 .. prefix_positions of the prefix, then all rows of layer
+    tail_layer + i of ``tails``, a cache whose layers are the batch's slots."""
+    qa, oa = _Arg(q_rows), _Arg(out, writable=True)
+    q_dim = _row_width(q_rows, tails)
+    if oa.n != qa.n:
+        raise ValueError("out must have the shape of q_rows")
+    err = L.RvError()
+    _same_stream(prefix, tails)
+    flags = _flags(tails, (qa, oa))
+    _check(_lib().rv_decode_attention_shared(prefix.handle, prefix_layer, prefix_positions, tails.handle, tail_layer,
+                                             qa.ptr, qa.n // q_dim if q_dim else 0, q_dim, scale, oa.ptr, flags,
+                                             byref(err)), err)
+    return out
+
+
+def decode_step_shared(prefix: KvCache, prefix_layer: int, prefix_positions: int, tails: KvCache, tail_layer: int,
+                       q_rows, k_rows, v_rows, q_norm_w, k_norm_w, eps: float, theta: float, scale: float, out):
+    """rv_decode_step_shared (no reference counterpart): decode_step for each
+    sequence of a batch that shares a prefix, one row each: q/k RMSNorm + RoPE at
+    prefix_positions + the sequence's length, append to its layer of ``tails``,
+    then decode_attention_shared."""
+    qa, ka, va, oa = _Arg(q_rows), _Arg(k_rows), _Arg(v_rows), _Arg(out, writable=True)
+    wq, wk = _Arg(q_norm_w), _Arg(k_norm_w)
+    q_dim, kv_dim = _row_width(q_rows, tails), tails.kv_dim()
+    n = qa.n // q_dim if q_dim else 0
+    if ka.n != n * kv_dim or va.n != n * kv_dim:
+        raise ValueError("k_rows and v_rows must be rows x kv_dim with q_rows' rows")
+    if oa.n != qa.n:
+        raise ValueError("out must have the shape of q_rows")
+    err = L.RvError()
+    _same_stream(prefix, tails)
+    flags = _flags(tails, (qa, ka, va, wq, wk, oa))
+    _check(_lib().rv_decode_step_shared(prefix.handle, prefix_layer, prefix_positions, tails.handle, tail_layer, n,
+                                        qa.ptr, ka.ptr, va.ptr, q_dim, wq.ptr, wq.n, wk.ptr, wk.n, eps, theta, scale,
+                                        oa.ptr, flags, byref(err)), err)
     return out
 
 

@@ -2,7 +2,7 @@
 //
 // Host-side validation in the reference's precedence, the per-layer cursors
 // of the device KV cache, staging for host pointers, and dispatch to the
-// gfx950 kernels (rv_prologue.hip, rv_decode.hip, rv_prefill.hip). Nothing is
+// gfx950 kernels (rv_prologue.hip, rv_decode.hip, rv_prefill.hip, rv_q8.hip, rv_rows.hip). Nothing is
 // queued on the device before a call's validation has passed, so `out` is
 // untouched on every error, as in the reference (attention.rs:413-425).
 #include <hip/hip_runtime.h>
@@ -51,8 +51,6 @@ struct DeviceGuard {
     if (prev >= 0 && hipGetDevice(&cur) == hipSuccess && cur != prev) (void)hipSetDevice(prev);
   }
 };
-
-size_t elem_size(int elem) { return elem == RV_ELEM_F32 ? 4 : 2; }
 
 size_t sat_mul(size_t a, size_t b) {
   size_t r;
@@ -218,6 +216,87 @@ int32_t check_rope_dim(const rv_kv* kv, rv_error* err) {
   if (kv->head_dim / 2 > (size_t)rv::kMaxHalf)
     return fail(err, RV_ERR_UNSUPPORTED, kv->head_dim, 0, 0, 0, "head_dim above 512");
   return RV_OK;
+}
+
+// Layers [layer0, layer0 + n) exist.
+int32_t check_layers(const rv_kv* kv, size_t layer0, size_t n, rv_error* err) {
+  if (layer0 >= kv->n_layers) return fail(err, RV_KV_LAYER_OUT_OF_RANGE, layer0, kv->n_layers);
+  if (n > kv->n_layers - layer0) return fail(err, RV_KV_LAYER_OUT_OF_RANGE, kv->n_layers, kv->n_layers);
+  return RV_OK;
+}
+
+// Each of the layers has room for one more row.
+int32_t check_room(const rv_kv* kv, size_t layer0, size_t n, rv_error* err) {
+  for (size_t i = 0; i < n; ++i)
+    if (kv->lens[layer0 + i] == kv->capacity) return fail(err, RV_KV_CAPACITY_EXCEEDED, layer0 + i, kv->capacity);
+  return RV_OK;
+}
+
+// The destinations of rows [r0, r0 + n) of a call that writes one row to each
+// of the layers from layer0 on.
+rv::RowDst each_dst(const rv_kv* kv, size_t layer0, size_t r0, size_t n, size_t pos0) {
+  rv::RowDst d;
+  d.layer = layer0 + r0;
+  d.pos0 = (long)pos0;
+  d.each_n = (int)n;
+  for (size_t i = 0; i < n; ++i) d.len[i] = (uint32_t)kv->lens[layer0 + r0 + i];
+  return d;
+}
+
+constexpr size_t kMaxRows = 0x7FFFFF00u;  // the kernels' 32-bit positions
+
+// The checks that attention over a shared prefix and its batch's rows make, in
+// order; `one_more`: each sequence is about to gain a row.
+int32_t shared_check(const rv_kv* prefix, size_t prefix_layer, size_t prefix_positions, const rv_kv* tails,
+                     size_t tail_layer, size_t n_seqs, size_t q_dim, bool one_more, rv_error* err) {
+  const size_t hd = tails->head_dim, n_kv = tails->n_kv_heads;
+  if (prefix->head_dim != hd || prefix->n_kv_heads != n_kv)
+    return fail(err, RV_ERR_UNSUPPORTED, prefix->n_kv_heads, prefix->head_dim, n_kv, hd,
+                "prefix and tails of different geometry");
+  if (prefix->elem != tails->elem)
+    return fail(err, RV_ERR_UNSUPPORTED, (uint64_t)prefix->elem, (uint64_t)tails->elem, 0, 0,
+                "prefix and tails of different element types");
+  if (prefix->device != tails->device || prefix->stream != tails->stream)
+    return fail(err, RV_ERR_UNSUPPORTED, (uint64_t)prefix->device, (uint64_t)tails->device, 0, 0,
+                "prefix and tails on different devices or streams");
+  if (q_dim == 0 || q_dim % hd) return fail(err, RV_ATTN_Q_LEN_INDIVISIBLE, q_dim, hd);
+  if ((q_dim / hd) % n_kv) return fail(err, RV_ATTN_GQA_GROUP_MISMATCH, q_dim / hd, n_kv);
+  int32_t rc = check_layer(prefix, prefix_layer, err);
+  if (rc) return rc;
+  if (prefix_positions > prefix->lens[prefix_layer])
+    return fail(err, RV_KV_POSITION_OUT_OF_RANGE, prefix_layer, prefix_positions - 1, prefix->lens[prefix_layer]);
+  if ((rc = check_layers(tails, tail_layer, n_seqs, err))) return rc;
+  if (one_more) {
+    if ((rc = check_room(tails, tail_layer, n_seqs, err))) return rc;
+  } else {
+    for (size_t i = 0; i < n_seqs; ++i)
+      if (prefix_positions == 0 && tails->lens[tail_layer + i] == 0)
+        return fail(err, RV_ATTN_EMPTY_LAYER, tail_layer + i);
+  }
+  if (hd > 512) return fail(err, RV_ERR_UNSUPPORTED, hd, 0, 0, 0, "head_dim above 512");
+  size_t most = prefix_positions;
+  for (size_t i = 0; i < n_seqs; ++i) most = std::max(most, tails->lens[tail_layer + i] + 1);
+  if (most > kMaxRows) return fail(err, RV_ERR_UNSUPPORTED, most, 0, 0, 0, "position past 2^31");
+  if (sat_mul(n_seqs, q_dim / hd) > 0x7FFFFFFFu)
+    return fail(err, RV_ERR_UNSUPPORTED, n_seqs, 0, 0, 0, "query heads of the batch past 2^31");
+  return RV_OK;
+}
+
+rv::RowsCall shared_call(const rv_kv* prefix, size_t prefix_layer, size_t prefix_positions, const rv_kv* tails,
+                         size_t tail_layer, const float* q, size_t n_seqs, size_t q_dim, float scale, float* out) {
+  rv::RowsCall c;
+  c.main = prefix;
+  c.layer = prefix_layer;
+  c.positions = prefix_positions;
+  c.tails = tails;
+  c.tail_layer = tail_layer;
+  c.q = q;
+  c.rows = n_seqs;
+  c.n_q_heads = q_dim / tails->head_dim;
+  c.kv_hi = tails->n_kv_heads;
+  c.scale = scale;
+  c.out = out;
+  return c;
 }
 
 }  // namespace
@@ -393,7 +472,7 @@ int32_t decode_step_dev_check(const rv_kv* kv, size_t layer, size_t q_len, size_
   if ((rc = check_norm_weights(hd, q_norm_len, k_norm_len, err))) return rc;
   if ((rc = check_layer(kv, layer, err))) return rc;
   if (max_position >= kv->capacity) return fail(err, RV_KV_CAPACITY_EXCEEDED, layer, kv->capacity);
-  if (!decode_pro_supported(kv, q_len / hd))
+  if (kv->elem != RV_ELEM_Q8_0 && !decode_pro_supported(kv, q_len / hd))
     return fail(err, RV_ERR_UNSUPPORTED, hd, q_len / hd / kv->n_kv_heads, 0, 0,
                 "device-position step: head_dim 128 and a group of at most 16");
   return RV_OK;
@@ -445,12 +524,19 @@ size_t rv_scratch_len(size_t n_q_heads, size_t n_kv_heads, size_t head_dim, size
 
 int32_t rv_kv_projected_bytes(size_t n_layers, size_t n_kv_heads, size_t head_dim, size_t capacity, rv_elem elem,
                               uint64_t* bytes, rv_error* err) {
-  if (elem != RV_ELEM_F16 && elem != RV_ELEM_F32) return fail(err, RV_ERR_BAD_ELEM, (uint64_t)elem);
+  if (elem != RV_ELEM_F16 && elem != RV_ELEM_F32 && elem != RV_ELEM_Q8_0)
+    return fail(err, RV_ERR_BAD_ELEM, (uint64_t)elem);
   if (!bytes) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, "bytes");
   size_t kv_dim, plane, total, b2, b;
   int32_t rc = geometry(n_layers, n_kv_heads, head_dim, capacity, &kv_dim, &plane, &total, err);
   if (rc) return rc;
-  if (__builtin_mul_overflow(total, (size_t)2, &b2) || __builtin_mul_overflow(b2, elem_size(elem), &b))
+  const bool q8 = elem == RV_ELEM_Q8_0;
+  if (q8 && (head_dim % 32 || head_dim > 512))
+    return fail(err, RV_KV_INVALID_DIMS, n_layers, n_kv_heads, head_dim, capacity,
+                "Q8_0 rows need a head_dim that is a multiple of 32, at most 512");
+  // Q8_0: 34 bytes for every 32 elements.
+  if (__builtin_mul_overflow(q8 ? total / 32 : total, (size_t)2, &b2) ||
+      __builtin_mul_overflow(b2, q8 ? (size_t)34 : elem == RV_ELEM_F32 ? (size_t)4 : (size_t)2, &b))
     return fail(err, RV_KV_INVALID_DIMS, n_layers, n_kv_heads, head_dim, capacity,
                 "total size in bytes overflows usize");
   *bytes = (uint64_t)b;
@@ -463,6 +549,14 @@ int32_t rv_kv_new(size_t n_layers, size_t n_kv_heads, size_t head_dim, size_t ca
   uint64_t bytes;
   int32_t rc = rv_kv_projected_bytes(n_layers, n_kv_heads, head_dim, capacity, elem, &bytes, err);
   if (rc) return rc;
+  if (elem == RV_ELEM_Q8_0) {
+    // Its kernels count positions in 32 bits, and whole tiles past the last one.
+    if (capacity > 0x7FFFFF00u) return fail(err, RV_ERR_UNSUPPORTED, capacity, 0, 0, 0, "Q8_0 capacity past 2^31");
+    size_t padded;  // as many rows as it pads the capacity to, both planes
+    if (__builtin_mul_overflow(n_layers * n_kv_heads * head_dim, (capacity + 127) / 128 * 128 * 4, &padded))
+      return fail(err, RV_KV_INVALID_DIMS, n_layers, n_kv_heads, head_dim, capacity,
+                  "total size in bytes overflows usize");
+  }
   rv_kv* kv = new (std::nothrow) rv_kv();
   if (!kv) return fail(err, RV_ERR_HIP, (uint64_t)hipErrorOutOfMemory, 0, 0, 0, "host allocation");
   size_t total;
@@ -479,7 +573,7 @@ int32_t rv_kv_new(size_t n_layers, size_t n_kv_heads, size_t head_dim, size_t ca
   kv->staged_pos.assign(n_layers, 0);
   kv->staged_mode.assign(n_layers, 0);
   DeviceGuard dg(device);
-  const size_t plane_bytes = total * elem_size(elem);
+  const size_t plane_bytes = kv->plane_bytes();
   hipError_t e = hipMalloc(&kv->k, plane_bytes);
   if (e == hipSuccess) e = hipMalloc(&kv->v, plane_bytes);
   if (e == hipSuccess) e = hipMemset(kv->k, 0, plane_bytes);
@@ -612,7 +706,15 @@ int32_t rv_kv_append_rows(rv_kv* kv, size_t layer, const float* k, const float* 
     dv = st.in(v, n);
     if (st.e != hipSuccess) return hip_fail(err, st.e, "hipMemcpyAsync H2D");
   }
-  rv::HipStatus hs = rv::launch_append(kv, layer, len, dk, dv, rows, kv->stream);
+  rv::HipStatus hs;
+  if (kv->elem == RV_ELEM_Q8_0) {
+    rv::RowDst dst;
+    dst.layer = layer;
+    dst.row0 = (long)len;
+    hs = rv::launch_append_dst(kv, dst, dk, dv, rows, kv->stream);
+  } else {
+    hs = rv::launch_append(kv, layer, len, dk, dv, rows, kv->stream);
+  }
   if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
   kv->lens[layer] = len + rows;
   if (flags & (RV_HOST_PTRS | RV_SYNC)) {
@@ -652,10 +754,169 @@ int32_t rv_kv_truncate(rv_kv* kv, size_t new_len, rv_error* err) {
   return ok(err);
 }
 
+// No reference counterpart: one layer's cursor alone (a batch slot's sequence).
+int32_t rv_kv_truncate_layer(rv_kv* kv, size_t layer, size_t new_len, rv_error* err) {
+  if (!kv) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, "kv");
+  int32_t rc = check_layer(kv, layer, err);
+  if (rc) return rc;
+  if (new_len > kv->lens[layer]) return fail(err, RV_KV_TRUNCATE_BEYOND_LENGTH, new_len, kv->lens[layer]);
+  kv->lens[layer] = new_len;
+  kv->staged_pos[layer] = std::min(kv->staged_pos[layer], new_len);
+  return ok(err);
+}
+
+// No reference counterpart: a range of rows as f32, whatever the element type.
+int32_t rv_kv_read_rows(const rv_kv* ckv, size_t layer, size_t pos, size_t rows, float* k, float* v, uint32_t flags,
+                        rv_error* err) {
+  if (!ckv) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, "kv");
+  rv_kv* kv = const_cast<rv_kv*>(ckv);
+  int32_t rc = check_layer(kv, layer, err);
+  if (rc) return rc;
+  const size_t len = kv->lens[layer];
+  if (pos > len || rows > len - pos)
+    return fail(err, RV_KV_POSITION_OUT_OF_RANGE, layer, sat_add(pos, rows ? rows - 1 : 0), len);
+  if (rows == 0) return ok(err);
+  if (!k && !v) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, "k and v");
+  DeviceGuard dg(kv->device);
+  const size_t n = rows * kv->kv_dim;
+  float *dk = k, *dv = v;
+  if (flags & RV_HOST_PTRS) {
+    Stager st(kv);
+    if (!st.reserve(2 * Stager::align(n * 4))) return hip_fail(err, st.e, "hipMalloc stage");
+    dk = k ? st.carve(n) : nullptr;
+    dv = v ? st.carve(n) : nullptr;
+  }
+  rv::HipStatus hs = rv::launch_read_rows(kv, layer, pos, rows, dk, dv, kv->stream);
+  if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
+  if ((flags & RV_HOST_PTRS) && k && v) {
+    const hipError_t e = hipMemcpyAsync(k, dk, n * 4, hipMemcpyDeviceToHost, kv->stream);
+    if (e != hipSuccess) return hip_fail(err, e, "hipMemcpyAsync D2H");
+  }
+  return v ? finish(kv, flags, dv, v, n, err) : finish(kv, flags, dk, k, n, err);
+}
+
+// No reference counterpart: one row to each of n layers.
+int32_t rv_kv_append_each(rv_kv* kv, size_t layer0, size_t n, const float* k, const float* v, size_t row_len,
+                          uint32_t flags, rv_error* err) {
+  if (!kv) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, "kv");
+  if (n == 0) return ok(err);
+  int32_t rc = check_layers(kv, layer0, n, err);
+  if (rc) return rc;
+  if (row_len != kv->kv_dim) return fail(err, RV_KV_ROW_LEN_MISMATCH, row_len, kv->kv_dim, 0, 0, "k");
+  if ((rc = check_room(kv, layer0, n, err))) return rc;
+  if (kv->capacity > kMaxRows) return fail(err, RV_ERR_UNSUPPORTED, kv->capacity, 0, 0, 0, "position past 2^31");
+  if (!k || !v) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, !k ? "k" : "v");
+  DeviceGuard dg(kv->device);
+  const float *dk = k, *dv = v;
+  if (flags & RV_HOST_PTRS) {
+    Stager st(kv);
+    const size_t m = n * kv->kv_dim;
+    if (!st.reserve(2 * Stager::align(m * 4))) return hip_fail(err, st.e, "hipMalloc stage");
+    dk = st.in(k, m);
+    dv = st.in(v, m);
+    if (st.e != hipSuccess) return hip_fail(err, st.e, "hipMemcpyAsync H2D");
+  }
+  for (size_t r0 = 0; r0 < n; r0 += rv::kMaxEach) {
+    const size_t m = std::min<size_t>(rv::kMaxEach, n - r0);
+    const rv::HipStatus hs = rv::launch_append_dst(kv, each_dst(kv, layer0, r0, m, 0), dk + r0 * kv->kv_dim,
+                                                   dv + r0 * kv->kv_dim, m, kv->stream);
+    if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
+  }
+  for (size_t i = 0; i < n; ++i) kv->lens[layer0 + i] += 1;
+  if (flags & (RV_HOST_PTRS | RV_SYNC)) {
+    const hipError_t e = hipStreamSynchronize(kv->stream);
+    if (e != hipSuccess) return hip_fail(err, e, "hipStreamSynchronize");
+  }
+  return ok(err);
+}
+
+int32_t rv_decode_attention_shared(const rv_kv* prefix, size_t prefix_layer, size_t prefix_positions,
+                                   const rv_kv* ctails, size_t tail_layer, const float* q_rows, size_t n_seqs,
+                                   size_t q_dim, float scale, float* out, uint32_t flags, rv_error* err) {
+  if (!prefix || !ctails) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, !prefix ? "prefix" : "tails");
+  if (n_seqs == 0) return ok(err);
+  rv_kv* tails = const_cast<rv_kv*>(ctails);
+  int32_t rc =
+      shared_check(prefix, prefix_layer, prefix_positions, tails, tail_layer, n_seqs, q_dim, false, err);
+  if (rc) return rc;
+  if (!q_rows || !out) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, !q_rows ? "q_rows" : "out");
+  DeviceGuard dg(tails->device);
+  const size_t n = n_seqs * q_dim;
+  const float* dq = q_rows;
+  float* dout = out;
+  if (flags & RV_HOST_PTRS) {
+    Stager st(tails);
+    if (!st.reserve(2 * Stager::align(n * 4))) return hip_fail(err, st.e, "hipMalloc stage");
+    dq = st.in(q_rows, n);
+    dout = st.carve(n);
+    if (st.e != hipSuccess) return hip_fail(err, st.e, "hipMemcpyAsync H2D");
+  }
+  const rv::HipStatus hs = rv::launch_rows(
+      tails, shared_call(prefix, prefix_layer, prefix_positions, tails, tail_layer, dq, n_seqs, q_dim, scale, dout),
+      tails->stream);
+  if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
+  return finish(tails, flags, dout, out, n, err);
+}
+
+int32_t rv_decode_step_shared(const rv_kv* prefix, size_t prefix_layer, size_t prefix_positions, rv_kv* tails,
+                              size_t tail_layer, size_t n_seqs, const float* q_rows, const float* k_rows,
+                              const float* v_rows, size_t q_dim, const float* q_norm_w, size_t q_norm_len,
+                              const float* k_norm_w, size_t k_norm_len, float eps, float theta, float scale,
+                              float* out, uint32_t flags, rv_error* err) {
+  if (!prefix || !tails) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, !prefix ? "prefix" : "tails");
+  if (n_seqs == 0) return ok(err);
+  int32_t rc = check_rope_dim(tails, err);
+  if (rc) return rc;
+  if ((rc = check_norm_weights(tails->head_dim, q_norm_len, k_norm_len, err))) return rc;
+  if ((rc = shared_check(prefix, prefix_layer, prefix_positions, tails, tail_layer, n_seqs, q_dim, true, err)))
+    return rc;
+  if (!q_rows || !k_rows || !v_rows || !q_norm_w || !k_norm_w || !out)
+    return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, "tensor");
+  DeviceGuard dg(tails->device);
+  const size_t hd = tails->head_dim, kvd = tails->kv_dim, nq = n_seqs * q_dim, nk = n_seqs * kvd;
+  const float *dq = q_rows, *dk = k_rows, *dv = v_rows, *dwq = q_norm_w, *dwk = k_norm_w;
+  float* dout = out;
+  if (flags & RV_HOST_PTRS) {
+    Stager st(tails);
+    if (!st.reserve(2 * Stager::align(nq * 4) + 2 * Stager::align(nk * 4) + 2 * Stager::align(hd * 4)))
+      return hip_fail(err, st.e, "hipMalloc stage");
+    dq = st.in(q_rows, nq);
+    dk = st.in(k_rows, nk);
+    dv = st.in(v_rows, nk);
+    dwq = st.in(q_norm_w, hd);
+    dwk = st.in(k_norm_w, hd);
+    dout = st.carve(nq);
+    if (st.e != hipSuccess) return hip_fail(err, st.e, "hipMemcpyAsync H2D");
+  }
+  rv::InvFreq inv;
+  rv::fill_inv_freq(inv, hd, theta);
+  rv::HipStatus hs = rv::ensure_qbuf(tails, nq * sizeof(float));
+  const size_t n_q = q_dim / hd;
+  for (size_t r0 = 0; r0 < n_seqs && hs.e == hipSuccess; r0 += rv::kMaxEach) {
+    const size_t m = std::min<size_t>(rv::kMaxEach, n_seqs - r0);
+    hs = rv::launch_prologue_dst(tails, each_dst(tails, tail_layer, r0, m, prefix_positions), dq + r0 * q_dim,
+                                 tails->qbuf + r0 * q_dim, n_q, dk + r0 * kvd, dv + r0 * kvd, m, dwq, dwk, eps, inv,
+                                 tails->stream);
+  }
+  if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
+  for (size_t i = 0; i < n_seqs; ++i) tails->lens[tail_layer + i] += 1;
+  hs = rv::launch_rows(tails,
+                       shared_call(prefix, prefix_layer, prefix_positions, tails, tail_layer, tails->qbuf, n_seqs,
+                                   q_dim, scale, dout),
+                       tails->stream);
+  if (hs.e != hipSuccess) {
+    for (size_t i = 0; i < n_seqs; ++i) tails->lens[tail_layer + i] -= 1;
+    return hip_fail(err, hs.e, hs.what);
+  }
+  return finish(tails, flags, dout, out, nq, err);
+}
+
 static int32_t layer_view(const rv_kv* kv, int plane_v, size_t layer, const void** dev, size_t* n, rv_error* err) {
   if (!kv || !dev || !n) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, "kv/dev/n_elems");
   int32_t rc = check_layer(kv, layer, err);
   if (rc) return rc;
+  if (kv->elem == RV_ELEM_Q8_0)
+    return fail(err, RV_ERR_UNSUPPORTED, (uint64_t)kv->elem, 0, 0, 0, "a Q8_0 plane has no elements to view (read its rows)");
   *dev = plane_v ? kv->v_layer(layer) : kv->k_layer(layer);
   *n = kv->lens[layer] * kv->kv_dim;
   return ok(err);
@@ -675,6 +936,18 @@ int32_t rv_kv_read_row(const rv_kv* kv, int plane_v, size_t layer, size_t pos, v
   const size_t len = kv->lens[layer];
   if (pos >= len) return fail(err, RV_KV_POSITION_OUT_OF_RANGE, layer, pos, len);
   DeviceGuard dg(kv->device);
+  if (kv->elem == RV_ELEM_Q8_0) {
+    rv_kv* m = const_cast<rv_kv*>(kv);
+    Stager st(m);
+    const size_t bytes = kv->kv_dim / 32 * 34;
+    if (!st.reserve(Stager::align(bytes))) return hip_fail(err, st.e, "hipMalloc stage");
+    const rv::HipStatus hs = rv::launch_read_blocks(kv, plane_v, layer, pos, (uint8_t*)m->stage, kv->stream);
+    if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
+    hipError_t e = hipMemcpyAsync(dst, m->stage, bytes, hipMemcpyDeviceToHost, kv->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(kv->stream);
+    if (e != hipSuccess) return hip_fail(err, e, "read_row");
+    return ok(err);
+  }
   const size_t es = kv->elem_size();
   const char* src = (plane_v ? kv->v_layer(layer) : kv->k_layer(layer)) + pos * kv->kv_dim * es;
   hipError_t e = hipMemcpyAsync(dst, src, kv->kv_dim * es, hipMemcpyDeviceToHost, kv->stream);
@@ -766,7 +1039,22 @@ static int32_t rows_plan(const rv_kv* kv, size_t rows, size_t q_dim, size_t laye
 static int32_t run_rows(rv_kv* kv, const float* dq, size_t rows, size_t q_dim, size_t layer, size_t start,
                         const Plan& p, float scale, float* dout, uint32_t flags, rv_error* err) {
   rv::HipStatus hs;
-  if (rv::prefill_supported(kv, p.group, start + rows)) {
+  if (kv->elem == RV_ELEM_Q8_0) {
+    rv::RowsCall c;
+    c.main = kv;
+    c.layer = layer;
+    c.positions = start + rows;
+    c.causal = true;
+    c.start = start;
+    c.q = dq;
+    c.rows = rows;
+    c.n_q_heads = p.n_q_heads;
+    c.kv_hi = kv->n_kv_heads;
+    c.scale = scale;
+    c.out = dout;
+    c.split = (flags & RV_PREFILL_MODE_MASK) == RV_PREFILL_EXACT;
+    hs = rv::launch_rows(kv, c, kv->stream);
+  } else if (rv::prefill_supported(kv, p.group, start + rows)) {
     hs = rv::launch_prefill(kv, dq, rows, p.n_q_heads, layer, start, scale, dout, flags, nullptr, kv->stream);
   } else {
     for (size_t r = 0; r < rows && hs.e == hipSuccess; ++r)
@@ -863,8 +1151,16 @@ int32_t rv_decode_step(rv_kv* kv, size_t layer, const float* q, size_t q_len, co
   if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
   // q and k rotate at `position` (forward.rs:2628-2629); the row lands at
   // the layer's cursor.
-  hs = rv::launch_row_prologue(kv, layer, len, dq, kv->qbuf, n_q, dk, dv, 1, dwq, dwk, eps, inv, position, nullptr,
-                               nullptr, kv->stream);
+  if (kv->elem == RV_ELEM_Q8_0) {
+    rv::RowDst dst;
+    dst.layer = layer;
+    dst.row0 = (long)len;
+    dst.pos0 = (long)position;
+    hs = rv::launch_prologue_dst(kv, dst, dq, kv->qbuf, n_q, dk, dv, 1, dwq, dwk, eps, inv, kv->stream);
+  } else {
+    hs = rv::launch_row_prologue(kv, layer, len, dq, kv->qbuf, n_q, dk, dv, 1, dwq, dwk, eps, inv, position, nullptr,
+                                 nullptr, kv->stream);
+  }
   if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
   kv->lens[layer] = len + 1;
   hs = rv::launch_decode(kv, kv->qbuf, n_q, layer, len + 1, scale, 0, kv->n_kv_heads, dout, kv->stream);
@@ -888,6 +1184,35 @@ int32_t rv_decode_step_dev(rv_kv* kv, size_t layer, const float* q, size_t q_len
     return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, "tensor");
   if (flags & RV_HOST_PTRS) return fail(err, RV_ERR_UNSUPPORTED, flags, 0, 0, 0, "RV_HOST_PTRS (device pointers only)");
   DeviceGuard dg(kv->device);
+  if (kv->elem == RV_ELEM_Q8_0) {
+    rv::InvFreq inv;
+    rv::fill_inv_freq(inv, kv->head_dim, theta);
+    rv::HipStatus hs = rv::ensure_qbuf(kv, q_len * sizeof(float));
+    rv::RowDst dst;
+    dst.layer = layer;
+    dst.d_pos = d_position;
+    dst.max_pos = (uint32_t)max_position;
+    dst.status = rv::dev_status(kv);
+    const size_t n_q = q_len / kv->head_dim;
+    if (hs.e == hipSuccess)
+      hs = rv::launch_prologue_dst(kv, dst, q, kv->qbuf, n_q, k, v, 1, q_norm_w, k_norm_w, eps, inv, kv->stream);
+    if (hs.e == hipSuccess) {
+      rv::RowsCall c;
+      c.main = kv;
+      c.layer = layer;
+      c.positions = max_position + 1;
+      c.q = kv->qbuf;
+      c.rows = 1;
+      c.n_q_heads = n_q;
+      c.kv_hi = kv->n_kv_heads;
+      c.scale = scale;
+      c.out = out;
+      c.d_pos = d_position;
+      hs = rv::launch_rows(kv, c, kv->stream);
+    }
+    if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
+    return finish(kv, flags, out, out, q_len, err);
+  }
   rv::HipStatus hs = rv::ensure_rope_tab(kv, theta, max_position + 1);
   if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
   rv::DecodePro pro{k, v, q_norm_w, k_norm_w, eps, {}, {}, d_position, kv->rope_tab, (int)max_position,
@@ -928,7 +1253,7 @@ int32_t rv_kv_device_status(rv_kv* kv, rv_error* err) {
 
 int32_t rv_kv_device_bytes(rv_kv* kv, uint64_t* now, uint64_t* bound, rv_error* err) {
   if (!kv) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, "kv");
-  const size_t planes = 2 * kv->n_layers * kv->plane * kv->elem_size();
+  const size_t planes = 2 * kv->plane_bytes();
   size_t staged = 0;
   for (size_t b : kv->staged_bytes) staged += b;
   const size_t base = planes + kv->ws_bytes + kv->qbuf_bytes + kv->stage_bytes + kv->retired_bytes +
@@ -962,10 +1287,12 @@ int32_t rv_kv_projected_device_bytes(size_t n_layers, size_t n_kv_heads, size_t 
   g.head_dim = head_dim;
   g.capacity = capacity;
   g.elem = elem;
+  g.plane = capacity * n_kv_heads * head_dim;
   g.kv_dim = n_kv_heads * head_dim;
   const size_t ws = std::max<size_t>(rv::decode_ws_bound(&g), (size_t)1 << 20);
   const size_t staged = n_layers * rv::prefill_stage_bound(&g);
   const size_t tab = capacity * head_dim * sizeof(float);
+  if (elem == RV_ELEM_Q8_0) planes = 2 * g.plane_bytes();  // its capacity in whole tiles
   *bytes = planes + ws + rv::ticket_words(&g) * sizeof(unsigned) + staged + tab;
   return ok(err);
 }
@@ -1058,9 +1385,16 @@ int32_t rv_prefill_chunk(rv_kv* kv, size_t layer, const float* q_rows, const flo
     if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
   } else {
     hs = rv::ensure_qbuf(kv, nq * sizeof(float));
-    if (hs.e == hipSuccess)
+    if (hs.e == hipSuccess && kv->elem == RV_ELEM_Q8_0) {
+      rv::RowDst dst;
+      dst.layer = layer;
+      dst.row0 = (long)len;
+      dst.pos0 = (long)start;
+      hs = rv::launch_prologue_dst(kv, dst, dq, kv->qbuf, q_dim / hd, dk, dv, rows, dwq, dwk, eps, inv, kv->stream);
+    } else if (hs.e == hipSuccess) {
       hs = rv::launch_row_prologue(kv, layer, len, dq, kv->qbuf, q_dim / hd, dk, dv, rows, dwq, dwk, eps, inv, start,
                                    nullptr, nullptr, kv->stream);
+    }
     if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
     kv->lens[layer] = len + rows;
     rc = run_rows(kv, kv->qbuf, rows, q_dim, layer, start, p, scale, dout, flags, err);

@@ -1424,12 +1424,13 @@ static HipStatus tile_merge_args(rv_kv* kv, const TilePlan& p, int n_heads, int 
 }
 
 size_t decode_ws_bound(const rv_kv* kv) {
+  if (kv->elem == RV_ELEM_Q8_0) return rows_ws_bound(kv);
   if (kv->head_dim != kD) return 0;
   return tile_ws_bound(kv, (int)kv->n_kv_heads, 16) * sizeof(float);
 }
 
 bool decode_pro_supported(const rv_kv* kv, size_t n_q_heads) {
-  return kv->head_dim == kD && n_q_heads % kv->n_kv_heads == 0 && n_q_heads / kv->n_kv_heads <= 16 &&
+  return kv->elem != RV_ELEM_Q8_0 && kv->head_dim == kD && n_q_heads % kv->n_kv_heads == 0 && n_q_heads / kv->n_kv_heads <= 16 &&
          kv->tune_decode_impl != 1;
 }
 
@@ -1473,8 +1474,27 @@ HipStatus launch_decode_pro(rv_kv* kv, const float* q_raw, size_t n_q_heads, siz
   return st;
 }
 
+// One row of a Q8_0 cache: its attention is rv_rows.hip's.
+static RowsCall q8_decode(const rv_kv* kv, const float* q, size_t n_q_heads, size_t layer, size_t positions,
+                          float scale, size_t kv_lo, size_t kv_hi, float* out) {
+  RowsCall c;
+  c.main = kv;
+  c.layer = layer;
+  c.positions = positions;
+  c.q = q;
+  c.rows = 1;
+  c.n_q_heads = n_q_heads;
+  c.kv_lo = kv_lo;
+  c.kv_hi = kv_hi;
+  c.scale = scale;
+  c.out = out;
+  return c;
+}
+
 size_t decode_ws_need(const rv_kv* kv, size_t n_q_heads, size_t positions, size_t n_heads) {
   if (n_heads == 0) return 0;
+  if (kv->elem == RV_ELEM_Q8_0)
+    return rows_ws_need(kv, q8_decode(kv, nullptr, n_q_heads, 0, positions, 0.f, 0, n_heads, nullptr));
   const int group = (int)(n_q_heads / kv->n_kv_heads);
   if (kv->head_dim == kD && group <= 16 && kv->tune_decode_impl != 1)
     return tile_ws_floats(plan_tile(kv, (long)positions), (int)n_heads, group) * sizeof(float);
@@ -1489,6 +1509,8 @@ size_t decode_ws_need(const rv_kv* kv, size_t n_q_heads, size_t positions, size_
 HipStatus launch_decode(rv_kv* kv, const float* q, size_t n_q_heads, size_t layer, size_t positions,
                         float scale, size_t kv_lo, size_t kv_hi, float* out, hipStream_t s, const Workspace* ws) {
   HipStatus st;
+  if (kv->elem == RV_ELEM_Q8_0)
+    return kv_lo == kv_hi ? st : launch_rows(kv, q8_decode(kv, q, n_q_heads, layer, positions, scale, kv_lo, kv_hi, out), s, ws);
   if (ws && decode_ws_need(kv, n_q_heads, positions, kv_hi - kv_lo) > ws->bytes) {
     st.e = hipErrorInvalidValue;
     st.what = "decode scratch too small";

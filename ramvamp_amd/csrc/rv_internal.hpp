@@ -7,6 +7,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <type_traits>
 #include <vector>
 
 #include "../../include/ramvamp_attn.h"
@@ -15,7 +16,7 @@ struct rv_kv {
   size_t n_layers = 0, n_kv_heads = 0, head_dim = 0, capacity = 0, kv_dim = 0, plane = 0;
   int elem = RV_ELEM_F16;
   int device = 0;
-  void* k = nullptr;  // [n_layers][capacity][kv_dim], elem-sized, device
+  void* k = nullptr;  // [n_layers][capacity][kv_dim], elem-sized, device (Q8_0: rv_rows.hpp)
   void* v = nullptr;
   std::vector<size_t> lens;  // per-layer cursors (kv/mod.rs:147), host-side
   hipStream_t stream = nullptr;
@@ -84,9 +85,23 @@ struct rv_kv {
   double timed_ms = 0;
   uint64_t timed_n = 0;
 
-  size_t elem_size() const { return elem == RV_ELEM_F32 ? 4 : 2; }
-  char* k_layer(size_t layer) const { return (char*)k + layer * plane * elem_size(); }
-  char* v_layer(size_t layer) const { return (char*)v + layer * plane * elem_size(); }
+  // f32 and f16 planes only: a Q8_0 plane's codes are bytes, its scales follow
+  // the codes of all layers in the same allocation.
+  size_t elem_size() const { return elem == RV_ELEM_F32 ? 4 : elem == RV_ELEM_F16 ? 2 : 1; }
+  size_t row_cap() const { return elem == RV_ELEM_Q8_0 ? (capacity + 127) / 128 * 128 : capacity; }
+  size_t layer_bytes() const { return row_cap() * kv_dim * elem_size(); }
+  size_t layer_scales() const { return row_cap() * kv_dim / 32; }
+  size_t plane_bytes() const {
+    return n_layers * (layer_bytes() + (elem == RV_ELEM_Q8_0 ? layer_scales() * sizeof(uint16_t) : 0));
+  }
+  char* k_layer(size_t layer) const { return (char*)k + layer * layer_bytes(); }
+  char* v_layer(size_t layer) const { return (char*)v + layer * layer_bytes(); }
+  uint16_t* k_scales(size_t layer) const {
+    return (uint16_t*)((char*)k + n_layers * layer_bytes()) + layer * layer_scales();
+  }
+  uint16_t* v_scales(size_t layer) const {
+    return (uint16_t*)((char*)v + n_layers * layer_bytes()) + layer * layer_scales();
+  }
 };
 
 namespace rv {
@@ -314,5 +329,63 @@ int32_t decode_step_dev_check(const rv_kv* kv, size_t layer, size_t q_len, size_
                               size_t k_norm_len, rv_error* err);
 // The device-position step's (cos, sin) table covering positions [0, n).
 HipStatus ensure_rope_tab(rv_kv* kv, float theta, size_t n);
+
+// ---- the Q8_0 cache's rows (rv_q8.hip) ------------------------------------------
+// Where each of a call's rows lands and the position it rotates at. each_n
+// == 0: row r at row0 + r of `layer` and position pos0 + r. Otherwise row r
+// goes to layer `layer + r`, at row len[r] and position pos0 + len[r].
+// With d_pos (one row) both come from device memory: the position is *d_pos,
+// nothing is written past max_pos, and status (as DecodePro's) records it.
+constexpr int kMaxEach = 256;
+struct RowDst {
+  size_t layer = 0;
+  long row0 = 0;
+  long pos0 = 0;
+  int each_n = 0;
+  const uint32_t* d_pos = nullptr;
+  uint32_t max_pos = 0;
+  uint32_t* status = nullptr;
+  uint32_t len[kMaxEach] = {};
+};
+// Appends k and v rows as given, in the cache's element type.
+HipStatus launch_append_dst(const rv_kv* kv, const RowDst& dst, const float* k, const float* v, size_t rows,
+                            hipStream_t s);
+// q heads RMSNormed and rotated into q_out (n_q may be 0), k heads RMSNormed,
+// rotated and appended, v heads appended.
+HipStatus launch_prologue_dst(const rv_kv* kv, const RowDst& dst, const float* q, float* q_out, size_t n_q,
+                              const float* k, const float* v, size_t rows, const float* q_w, const float* k_w,
+                              float eps, const InvFreq& inv, hipStream_t s);
+// Rows [pos, pos + rows) of a layer as f32 (any element type); k or v may be null.
+HipStatus launch_read_rows(const rv_kv* kv, size_t layer, size_t pos, size_t rows, float* k, float* v, hipStream_t s);
+// One Q8_0 row's blocks in ggml's storage order (f16 scale, 32 codes).
+HipStatus launch_read_blocks(const rv_kv* kv, int plane_v, size_t layer, size_t pos, uint8_t* dst, hipStream_t s);
+
+// ---- attention of many query columns over one range of rows (rv_rows.hip) ---------
+// A column is one query head of one query row. Every column of a kv head
+// attends rows [0, limit) of `main` (null: none), limit = positions, or start
+// + row + 1 with causal; with `tails` the columns of row i also attend rows
+// [0, lens[i]) of layer tail_layer + i of that cache.
+struct RowsCall {
+  const rv_kv* main = nullptr;
+  size_t layer = 0;
+  size_t positions = 0;
+  bool causal = false;
+  size_t start = 0;
+  const rv_kv* tails = nullptr;
+  size_t tail_layer = 0;
+  const float* q = nullptr;
+  size_t rows = 0, n_q_heads = 0;
+  size_t kv_lo = 0, kv_hi = 0;
+  float scale = 0.f;
+  float* out = nullptr;
+  bool split = true;  // q and probabilities as f16 hi + lo (else rounded to f16)
+  // positions = *d_pos + 1, planned for `positions`; past it nothing is written.
+  const uint32_t* d_pos = nullptr;
+};
+// Workspace and stream are `owner`'s; `ws` as launch_decode's.
+HipStatus launch_rows(rv_kv* owner, const RowsCall& c, hipStream_t s, const Workspace* ws = nullptr);
+size_t rows_ws_need(const rv_kv* owner, const RowsCall& c);
+// The most a decode call of up to 16 query heads per kv head needs on this cache.
+size_t rows_ws_bound(const rv_kv* kv);
 
 }  // namespace rv

@@ -1671,17 +1671,17 @@ HipStatus ready_persistent(rv_kv* kv, size_t layer, uint32_t mode, hipStream_t s
 }  // namespace
 
 size_t prefill_stage_bound(const rv_kv* kv) {
-  if (kv->head_dim != kD) return 0;
+  if (kv->head_dim != kD || kv->elem == RV_ELEM_Q8_0) return 0;
   const size_t cap_tiles = (kv->capacity + kBT - 1) / kBT;
   return kv->n_kv_heads * cap_tiles * tile_bytes_of(RV_PREFILL_EXACT);
 }
 
 // head_dim 128 and a group that divides 64 (so a workgroup's 64 or 128
 // columns are whole rows of the group); any other geometry runs each row
-// through the decode kernels.
+// through the decode kernels, a Q8_0 cache's chunk through rv_rows.hip's.
 bool prefill_supported(const rv_kv* kv, size_t group, size_t positions) {
   (void)positions;
-  return kv->head_dim == kD && group >= 1 && 64 % group == 0;
+  return kv->elem != RV_ELEM_Q8_0 && kv->head_dim == kD && group >= 1 && 64 % group == 0;
 }
 
 HipStatus launch_prefill(rv_kv* kv, const float* q_rows, size_t rows, size_t n_q_heads, size_t layer,
