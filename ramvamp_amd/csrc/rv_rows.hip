@@ -83,16 +83,87 @@ __device__ __forceinline__ void split8(const float (&x)[8], f16x8& hi, f16x8& lo
   }
 }
 
-// Dims 8 j .. + 7 of kv head h's K row t as f16 (f32: hi and lo).
+// ---- few columns: a wave's tiles in registers --------------------------------------
+// 32 rows a tile on 16x16x32 products, 16 NB columns. K's lane (row li, quarter
+// lk) loads dims 32 lk .. + 31 of rows li and 16 + li (the dot product's order
+// of dims is free as long as q follows it: a Q8_0 block is one lane's, with one
+// scale); V's lane (li, lk) dims 8 li .. + 7 of the rows whose probabilities
+// the scores' C layout gives quarter lk: 4 lk .. + 3 and 16 + 4 lk .. + 3, so
+// that P needs no exchange. Output tile b holds dims 8 i + b.
 template <typename T>
-__device__ __forceinline__ void load_k8(const KvView& w, int h, long t, int j, f16x8& hi, f16x8& lo) {
+struct Raw;
+template <>
+struct Raw<Q8> {
+  u32x4 k[2][2];
+  uint32_t ks[2];
+  u32x2 v[8];
+  u32x2 vs[2];
+};
+template <>
+struct Raw<_Float16> {
+  f16x8 k[2][4];
+  f16x8 v[8];
+};
+template <>
+struct Raw<float> {
+  f32x4 k[2][8];
+  f32x4 v[8][2];
+};
+
+template <typename T>
+__device__ __forceinline__ void load_raw(Raw<T>& x, const KvView& w, int h, long p0, long last, int li, int lk) {
   if constexpr (std::is_same<T, Q8>::value) {
-    const size_t row = (size_t)h * w.rows + t;
-    const u32x2 c = *reinterpret_cast<const u32x2*>(w.k + row * kD + 8 * j);
-    const _Float16 s = __builtin_bit_cast(_Float16, w.ks[row * 4 + (j >> 2)]);
+    const char* kb = w.k + ((size_t)h * w.rows + p0) * kD;
+    const uint16_t* sb = w.ks + ((size_t)h * w.rows + p0) * 4;
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const int r = 16 * a + li;
+      x.k[a][0] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kb + r * kD + 32 * lk));
+      x.k[a][1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kb + r * kD + 32 * lk + 16));
+      x.ks[a] = sb[4 * r + lk];
+    }
+    const char* vb = w.v + ((size_t)h * w.rows + p0) * kD + 8 * li;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      x.v[i] = __builtin_nontemporal_load(
+          reinterpret_cast<const u32x2*>(vb + (16 * (i >> 2) + 4 * lk + (i & 3)) * kD));
+    const uint16_t* vs = w.vs + ((size_t)h * 4 + (li >> 2)) * w.rows + p0 + 4 * lk;
+    x.vs[0] = *reinterpret_cast<const u32x2*>(vs);
+    x.vs[1] = *reinterpret_cast<const u32x2*>(vs + 16);
+  } else {
+    const T* kb = reinterpret_cast<const T*>(w.k) + (size_t)h * kD + 32 * lk;
+    const T* vb = reinterpret_cast<const T*>(w.v) + (size_t)h * kD + 8 * li;
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const T* r = kb + (size_t)min(p0 + 16 * a + li, last) * w.kv_dim;
+      constexpr int n = std::is_same<T, float>::value ? 8 : 4;
+#pragma unroll
+      for (int c = 0; c < n; ++c)
+        x.k[a][c] = *reinterpret_cast<const std::remove_reference_t<decltype(x.k[0][0])>*>(r + 16 / sizeof(T) * c);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const T* r = vb + (size_t)min(p0 + 16 * (i >> 2) + 4 * lk + (i & 3), last) * w.kv_dim;
+      if constexpr (std::is_same<T, float>::value) {
+        x.v[i][0] = reinterpret_cast<const f32x4*>(r)[0];
+        x.v[i][1] = reinterpret_cast<const f32x4*>(r)[1];
+      } else {
+        x.v[i] = *reinterpret_cast<const f16x8*>(r);
+      }
+    }
+  }
+}
+
+// K operand of row tile a, dims 32 lk + 8 c .. + 7 (f32: hi and lo).
+template <typename T>
+__device__ __forceinline__ void raw_k(const Raw<T>& x, int a, int c, f16x8& hi, f16x8& lo) {
+  if constexpr (std::is_same<T, Q8>::value) {
+    const uint32_t w0 = x.k[a][c >> 1][2 * (c & 1)], w1 = x.k[a][c >> 1][2 * (c & 1) + 1];
     f16x2 p[4];
-    q8_widen(c[0], p[0], p[1]);
-    q8_widen(c[1], p[2], p[3]);
+    q8_widen(w0, p[0], p[1]);
+    q8_widen(w1, p[2], p[3]);
+    const uint16_t sb = (uint16_t)x.ks[a];
+    const _Float16 s = __builtin_bit_cast(_Float16, sb);
     const f16x2 ss = {s, s};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -100,211 +171,572 @@ __device__ __forceinline__ void load_k8(const KvView& w, int h, long t, int j, f
       hi[2 * i] = v[0];
       hi[2 * i + 1] = v[1];
     }
+  } else if constexpr (std::is_same<T, float>::value) {
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = x.k[a][2 * c + (e >> 2)][e & 3];
+    split8(f, hi, lo);
   } else {
-    const T* p = reinterpret_cast<const T*>(w.k) + (size_t)t * w.kv_dim + (size_t)h * kD + 8 * j;
-    if constexpr (std::is_same<T, float>::value) {
-      float x[8];
-      load8(p, x);
-      split8(x, hi, lo);
+    hi = x.k[a][c];
+  }
+}
+
+// Zeroes the rows past `last` (what a plane holds there may not be finite).
+template <typename T>
+__device__ __forceinline__ void mask_v(Raw<T>& x, long p0, long last, int lk) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (p0 + 16 * (i >> 2) + 4 * lk + (i & 3) <= last) continue;
+    if constexpr (std::is_same<T, Q8>::value) {
+      const uint32_t w = x.vs[i >> 2][(i & 3) >> 1];
+      x.vs[i >> 2][(i & 3) >> 1] = w & ((i & 1) ? 0x0000FFFFu : 0xFFFF0000u);
+    } else if constexpr (std::is_same<T, float>::value) {
+      x.v[i][0] = f32x4{};
+      x.v[i][1] = f32x4{};
     } else {
-      hi = *reinterpret_cast<const f16x8*>(p);
+      x.v[i] = f16x8{};
     }
   }
 }
 
-// Dims 8 j .. + 7 of eight V rows t0 + {0..3}, t0 + 8 + {0..3}, one f16x8 of
-// the rows per dim; rows past `last` are zeros (their probabilities are zero,
-// and what the plane holds there may not be finite).
+// V operands of output tiles 2 u and 2 u + 1.
 template <typename T>
-__device__ __forceinline__ void load_v8x8(const KvView& w, int h, long t0, long last, int j, f16x8 (&hi)[8],
-                                          f16x8 (&lo)[8]) {
+__device__ __forceinline__ void raw_v2(const Raw<T>& x, int u, f16x8 (&hi)[2], f16x8 (&lo)[2]) {
   if constexpr (std::is_same<T, Q8>::value) {
-    const uint16_t* sp = w.vs + ((size_t)h * 4 + (j >> 2)) * w.rows + t0;
-    const u32x2 sa = *reinterpret_cast<const u32x2*>(sp), sb = *reinterpret_cast<const u32x2*>(sp + 8);
-    const char* base = w.v + ((size_t)h * w.rows + t0) * kD + 8 * j;
-    u32x2 c[8];
+    const f16x2 off = {(_Float16)-1152.f, (_Float16)-1152.f};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = *reinterpret_cast<const u32x2*>(base + (size_t)((i & 3) + 8 * (i >> 2)) * kD);
-    // (Through scalars: a bit cast of a vector's element reads its element 0.)
-    const uint32_t sw[4] = {sa[0], sa[1], sb[0], sb[1]};
-    f16x2 s[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = __builtin_bit_cast(f16x2, sw[i]);
-    if (t0 + 11 > last) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (t0 + (i & 3) + 8 * (i >> 2) > last) s[i >> 1][i & 1] = (_Float16)0.f;
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t a = x.v[2 * i][u >> 1], b = x.v[2 * i + 1][u >> 1], sw = x.vs[i >> 1][i & 1];
+      const f16x2 s = __builtin_bit_cast(f16x2, sw);
+      // (a's byte, b's byte) of both dims, then each pair widened.
+      const uint32_t t = __builtin_amdgcn_perm(b, a, (u & 1) ? 0x07030602u : 0x05010400u);
+      const uint32_t t0 = __builtin_amdgcn_perm(0x64646464u, t, 0x04010400u);
+      const uint32_t t1 = __builtin_amdgcn_perm(0x64646464u, t, 0x04030402u);
+      const f16x2 v0 = (__builtin_bit_cast(f16x2, t0) + off) * s, v1 = (__builtin_bit_cast(f16x2, t1) + off) * s;
+      hi[0][2 * i] = v0[0];
+      hi[0][2 * i + 1] = v0[1];
+      hi[1][2 * i] = v1[0];
+      hi[1][2 * i + 1] = v1[1];
     }
-#define RV_DIM(W, D)                                                            \
-  {                                                                             \
-    _Pragma("unroll") for (int i = 0; i < 4; ++i) {                             \
-      const f16x2 v = q8_widen_pair<D>(c[2 * i][W], c[2 * i + 1][W]) * s[i];    \
-      hi[4 * W + D][2 * i] = v[0];                                              \
-      hi[4 * W + D][2 * i + 1] = v[1];                                          \
-    }                                                                           \
-  }
-    RV_DIM(0, 0) RV_DIM(0, 1) RV_DIM(0, 2) RV_DIM(0, 3) RV_DIM(1, 0) RV_DIM(1, 1) RV_DIM(1, 2) RV_DIM(1, 3)
-#undef RV_DIM
+  } else if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = x.v[i][u >> 1][2 * (u & 1) + k];
+      split8(f, hi[k], lo[k]);
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const long t = t0 + (i & 3) + 8 * (i >> 2);
-      const T* p = reinterpret_cast<const T*>(w.v) + (size_t)min(t, last) * w.kv_dim + (size_t)h * kD + 8 * j;
-      if constexpr (std::is_same<T, float>::value) {
-        float x[8];
-        load8(p, x);
-        if (t > last) {
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = 0.f;
-        }
-        f16x8 a, b;
-        split8(x, a, b);
+      for (int i = 0; i < 8; ++i) hi[k][i] = x.v[i][2 * u + k];
+  }
+}
+
+// The f16 hi and lo halves of a column's q', scaled by a power of two that
+// brings its largest value to [2^13, 2^14); N values a lane, the column's
+// lanes 16 and 32 apart (or 32 apart only). Returns the power back.
+template <int N, bool QUARTERS, bool HL>
+__device__ __forceinline__ float split_q(const float (&x)[N], f16x8 (&hi)[N / 8], f16x8 (&lo)[HL ? N / 8 : 1]) {
+  float amax = 0.f;
 #pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          hi[d][i] = a[d];
-          lo[d][i] = b[d];
+  for (int i = 0; i < N; ++i) amax = fmaxf(amax, fabsf(x[i]));
+  if constexpr (QUARTERS) amax = swap_max<16>(amax);
+  amax = swap_max<32>(amax);
+  int ex = 14;
+  if (amax > 0.f && amax < INFINITY) (void)frexpf(amax, &ex);
+  const int k = max(ex - 14, -100);
+  const float down = ldexpf(1.f, -k);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float v = x[i] * down;
+    const _Float16 h = (_Float16)v;
+    hi[i / 8][i % 8] = h;
+    if constexpr (HL) lo[i / 8][i % 8] = (_Float16)(v - (float)h);
+  }
+  return ldexpf(1.f, k);
+}
+
+__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Columns [col0, col0 + 16 NB) of kv head h over rows [t_begin, t_end) of `w`,
+// by the four waves `w0` .. + 3 of the workgroup (wave wv of them takes tiles
+// wv, wv + 4, ...). All waves of the workgroup call it together; `run` false:
+// nothing to do but the barriers. No causal limit.
+constexpr int narrow_lds(int nb) { return 3 * nb * 34 * 64 * 4; }
+
+template <typename T, int NB>
+__device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, int n_cols, int row0, long t_begin,
+                           long t_end, int slot, int wv, bool run, char* lds) {
+  constexpr bool LO = Lo<T>::value;
+  const int lane = threadIdx.x & 63, li = lane & 15, lk = lane >> 4;
+  const int hk = a.kv_lo + h;
+  const long last = t_end - 1;
+  float q_up[NB], m_run[NB], m_sub[NB], l_run[NB];
+  f32x4 o[NB][8];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    m_run[n] = -INFINITY;
+    m_sub[n] = 0.f;
+    l_run[n] = 0.f;
+#pragma unroll
+    for (int b = 0; b < 8; ++b) o[n][b] = f32x4{};
+  }
+  const int n_tiles = run ? (int)((t_end - t_begin + 31) >> 5) : 0;
+  if (wv < n_tiles) {
+    Raw<T> ra, rb;
+    load_raw<T>(ra, w, hk, t_begin + 32L * wv, last, li, lk);
+    f16x8 qh[NB][4], ql[NB][4];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const int col = col0 + 16 * n + li;
+      const bool live = col < n_cols;
+      const int cc = live ? col : n_cols - 1;
+      const float* qp =
+          a.q + ((size_t)(row0 + cc / a.group) * a.n_q_heads + (size_t)hk * a.group + cc % a.group) * kD + 32 * lk;
+      typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+      float x[32];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const f32x4 v = *reinterpret_cast<const f32x4u*>(qp + 4 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 * i + e] = live ? v[e] * a.qscale : 0.f;
+      }
+      q_up[n] = split_q<32, true, true>(x, qh[n], ql[n]);
+    }
+    auto compute = [&](Raw<T>& x, long p0) {
+      const bool edge = p0 + 32 > t_end;
+      f32x4 s[NB][2][2];
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[n][t][0] = s[n][t][1] = f32x4{};
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          f16x8 kh, kl;
+          raw_k<T>(x, t, c, kh, kl);
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            s[n][t][0] = mfma16(kh, qh[n][c], s[n][t][0]);
+            s[n][t][1] = mfma16(kh, ql[n][c], s[n][t][1]);
+            if constexpr (LO) s[n][t][1] = mfma16(kl, qh[n][c], s[n][t][1]);
+          }
         }
+      f16x8 ph[NB], pl[NB];
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        float y[8], mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          y[i] = (s[n][i >> 2][0][i & 3] + s[n][i >> 2][1][i & 3]) * q_up[n];
+          if (edge && p0 + 16 * (i >> 2) + 4 * lk + (i & 3) >= t_end) y[i] = -INFINITY;
+          mx = fmaxf(mx, y[i]);
+        }
+        mx = swap_max<16>(mx);
+        mx = swap_max<32>(mx);
+        if (__builtin_amdgcn_ballot_w64(mx > m_run[n] + kSlack) != 0) {
+          const float mn = fmaxf(m_run[n], mx), ms = mn == -INFINITY ? 0.f : mn;
+          const float alpha = __builtin_amdgcn_exp2f(m_run[n] - ms);
+          m_run[n] = mn;
+          m_sub[n] = ms;
+          l_run[n] *= alpha;
+#pragma unroll
+          for (int b = 0; b < 8; ++b) o[n][b] *= alpha;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float p = __builtin_amdgcn_exp2f(y[i] - m_sub[n]);
+          l_run[n] += p;
+          const float pp = p * kPScale;
+          const _Float16 hi = (_Float16)pp;
+          ph[n][i] = hi;
+          pl[n][i] = (_Float16)(pp - (float)hi);
+        }
+      }
+      if (edge) mask_v<T>(x, p0, last, lk);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        f16x8 vh[2], vl[2];
+        raw_v2<T>(x, u, vh, vl);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          o[n][2 * u] = mfma16(vh[0], ph[n], o[n][2 * u]);
+          o[n][2 * u + 1] = mfma16(vh[1], ph[n], o[n][2 * u + 1]);
+          o[n][2 * u] = mfma16(vh[0], pl[n], o[n][2 * u]);
+          o[n][2 * u + 1] = mfma16(vh[1], pl[n], o[n][2 * u + 1]);
+          if constexpr (LO) {
+            o[n][2 * u] = mfma16(vl[0], ph[n], o[n][2 * u]);
+            o[n][2 * u + 1] = mfma16(vl[1], ph[n], o[n][2 * u + 1]);
+          }
+        }
+      }
+    };
+    if constexpr (LO) {  // a tile fills the registers
+      for (int t = wv; t < n_tiles; t += 4) {
+        if (t != wv) load_raw<T>(ra, w, hk, t_begin + 32L * t, last, li, lk);
+        compute(ra, t_begin + 32L * t);
+      }
+      rb = ra;
+    } else {
+    // One tile computed while the wave's next one loads.
+    for (int t = wv; t < n_tiles; t += 8) {
+      const bool more = t + 4 < n_tiles;
+      if (more) load_raw<T>(rb, w, hk, t_begin + 32L * (t + 4), last, li, lk);
+      compute(ra, t_begin + 32L * t);
+      if (!more) break;
+      if (t + 8 < n_tiles) load_raw<T>(ra, w, hk, t_begin + 32L * (t + 8), last, li, lk);
+      compute(rb, t_begin + 32L * (t + 4));
+    }
+    }
+  }
+  // Each lane summed its own rows: the other quarters of the column's.
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    l_run[n] = swap_sum<16>(l_run[n]);
+    l_run[n] = swap_sum<32>(l_run[n]);
+  }
+  // The waves' partials meet in LDS, in wave order: [wave - 1][NB][34][64 lanes].
+  float* om = reinterpret_cast<float*>(lds);
+  constexpr int kBlock = 34 * 64;
+  if (wv > 0) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      float* d = om + ((wv - 1) * NB + n) * kBlock + lane;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) d[64 * i] = o[n][i >> 2][i & 3];
+      d[64 * 32] = m_run[n];
+      d[64 * 33] = l_run[n];
+    }
+  }
+  __syncthreads();
+  if (wv > 0 || !run) return;
+  constexpr float kDown = 1.f / kPScale;
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    for (int p = 1; p < min(4, n_tiles); ++p) {
+      const float* d = om + ((p - 1) * NB + n) * kBlock + lane;
+      const float m2 = d[64 * 32], l2 = d[64 * 33];
+      const float mn = fmaxf(m_run[n], m2), ms = mn == -INFINITY ? 0.f : mn;
+      const float f1 = __builtin_amdgcn_exp2f(m_run[n] - ms), f2 = __builtin_amdgcn_exp2f(m2 - ms);
+      m_run[n] = mn;
+      l_run[n] = l_run[n] * f1 + l2 * f2;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[n][i >> 2][i & 3] = o[n][i >> 2][i & 3] * f1 + d[64 * i] * f2;
+    }
+    const int col = col0 + 16 * n + li;
+    if (col >= n_cols) continue;
+    const int row = row0 + col / a.group, head = col % a.group;
+    // This lane's dims: 32 lk + 8 r + b.
+    if (a.single) {
+      const float inv = kDown / l_run[n];
+      float* dst = a.out + ((size_t)row * a.n_heads * a.group + (size_t)h * a.group + head) * kD + 32 * lk;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int b = 0; b < 8; ++b) dst[8 * r + b] = o[n][b][r] * inv;
+      continue;
+    }
+    const size_t column = (size_t)h * a.rows * a.group + (size_t)row0 * a.group + col;
+    const size_t at = (size_t)slot * a.n_heads * a.rows * a.group + column;
+    float* dst = a.part + at * kD + 32 * lk;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const f32x4 v = {o[n][4 * g][r] * kDown, o[n][4 * g + 1][r] * kDown, o[n][4 * g + 2][r] * kDown,
+                         o[n][4 * g + 3][r] * kDown};
+        *reinterpret_cast<f32x4*>(dst + 8 * r + 4 * g) = v;
+      }
+    if (lk == 0) {
+      a.ml[2 * at] = m_run[n];
+      a.ml[2 * at + 1] = l_run[n];
+    }
+  }
+}
+
+// ---- many columns: tiles staged through LDS -----------------------------------------
+// Eight waves; half of them stage K, half V. A thread's share of a step of S
+// rows in its raw type: K, units of 8 dims of one row; V, units of 4 dims of
+// the eight rows of one operand slot.
+template <typename T, int S>
+struct Share {
+  static constexpr int KU = S / 16, VU = S / 64;  // units a thread
+  static constexpr int kw = std::is_same<T, Q8>::value ? 2 : std::is_same<T, float>::value ? 8 : 4;
+  static constexpr int N = std::is_same<T, Q8>::value ? (KU * 3 > VU * 12 ? KU * 3 : VU * 12) : KU * kw;
+  uint32_t r[N];
+};
+
+template <typename T, int S>
+__device__ __forceinline__ void load_share(Share<T, S>& x, const KvView& w, int h, long t0, long last, bool is_v,
+                                           int tt) {
+  constexpr bool Q = std::is_same<T, Q8>::value;
+  if (!is_v) {
+    const int j = tt & 15;
+#pragma unroll
+    for (int i = 0; i < Share<T, S>::KU; ++i) {
+      const long t = t0 + (tt >> 4) + 16 * i;
+      if constexpr (Q) {
+        const size_t row = (size_t)h * w.rows + t;
+        const u32x2 c = *reinterpret_cast<const u32x2*>(w.k + row * kD + 8 * j);
+        x.r[3 * i] = c[0];
+        x.r[3 * i + 1] = c[1];
+        x.r[3 * i + 2] = w.ks[row * 4 + (j >> 2)];
       } else {
-        f16x8 x = *reinterpret_cast<const f16x8*>(p);
-        if (t > last) x = f16x8{};
+        const u32x4* p = reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(w.k) +
+                                                        (size_t)min(t, last) * w.kv_dim + (size_t)h * kD + 8 * j);
 #pragma unroll
-        for (int d = 0; d < 8; ++d) hi[d][i] = x[d];
+        for (int k = 0; k < Share<T, S>::kw / 4; ++k) {
+          const u32x4 c = p[k];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x.r[Share<T, S>::kw * i + 4 * k + e] = c[e];
+        }
+      }
+    }
+  } else {
+    const int j = tt & 31;
+#pragma unroll
+    for (int u = 0; u < Share<T, S>::VU; ++u) {
+      const int pg = (tt >> 5) + 8 * u;
+      const long b = t0 + 32 * (pg >> 2) + 16 * ((pg >> 1) & 1) + 4 * (pg & 1);
+      if constexpr (Q) {
+        const char* p = w.v + ((size_t)h * w.rows + b) * kD + 4 * j;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          x.r[12 * u + i] = *reinterpret_cast<const uint32_t*>(p + ((i & 3) + 8 * (i >> 2)) * kD);
+        const uint16_t* sp = w.vs + ((size_t)h * 4 + (j >> 3)) * w.rows + b;
+        const u32x2 s0 = *reinterpret_cast<const u32x2*>(sp), s1 = *reinterpret_cast<const u32x2*>(sp + 8);
+        x.r[12 * u + 8] = s0[0];
+        x.r[12 * u + 9] = s0[1];
+        x.r[12 * u + 10] = s1[0];
+        x.r[12 * u + 11] = s1[1];
+      } else {
+        constexpr int n = std::is_same<T, float>::value ? 4 : 2;  // words of 4 dims
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const long t = min(b + (i & 3) + 8 * (i >> 2), last);
+          const T* p = reinterpret_cast<const T*>(w.v) + (size_t)t * w.kv_dim + (size_t)h * kD + 4 * j;
+          typedef uint32_t uw __attribute__((ext_vector_type(n)));
+          const uw c = *reinterpret_cast<const uw*>(p);
+#pragma unroll
+          for (int e = 0; e < n; ++e) x.r[8 * n * u + n * i + e] = c[e];
+        }
       }
     }
   }
 }
 
-// ---- one work item ----------------------------------------------------------------
+// Converts a share and writes it to the tiles at `lds` (K of all subtiles, V,
+// then their lo halves). Rows past `last` go in as zeros (V). A Q8_0 row's NaN
+// scale makes its block NaN; it must not reach columns that do not see the row
+// (0 * NaN), so the block goes in as zeros and nan_rows[subtile][block] marks
+// the row.
+template <typename T, int S>
+__device__ __forceinline__ void store_share(const Share<T, S>& x, char* lds, long t0, long last, bool is_v, int tt,
+                                            uint32_t (*nan_rows)[4]) {
+  constexpr bool Q = std::is_same<T, Q8>::value, LO = Lo<T>::value;
+  constexpr int kPlane = S / 32 * kTileB;
+  if (!is_v) {
+    const int j = tt & 15;
+#pragma unroll
+    for (int i = 0; i < Share<T, S>::KU; ++i) {
+      const int p = (tt >> 4) + 16 * i;
+      f16x8 hi, lo;
+      if constexpr (Q) {
+        f16x2 c[4];
+        q8_widen(x.r[3 * i], c[0], c[1]);
+        q8_widen(x.r[3 * i + 1], c[2], c[3]);
+        const uint16_t sb = (uint16_t)x.r[3 * i + 2];
+        const _Float16 s = __builtin_bit_cast(_Float16, sb);
+        const f16x2 ss = {s, s};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const f16x2 v = c[k] * ss;
+          hi[2 * k] = v[0];
+          hi[2 * k + 1] = v[1];
+        }
+      } else if constexpr (LO) {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(x.r[8 * i + e]);
+        split8(f, hi, lo);
+      } else {
+        const u32x4 c = {x.r[4 * i], x.r[4 * i + 1], x.r[4 * i + 2], x.r[4 * i + 3]};
+        hi = __builtin_bit_cast(f16x8, c);
+      }
+      char* dst = lds + ((p >> 5) * 8 + (j >> 1)) * kFragB + k_slot(p & 31, j & 1) * 16;
+      *reinterpret_cast<f16x8*>(dst) = hi;
+      if constexpr (LO) *reinterpret_cast<f16x8*>(dst + 2 * kPlane) = lo;
+    }
+  } else {
+    const int j = tt & 31, dt = j >> 3;
+#pragma unroll
+    for (int u = 0; u < Share<T, S>::VU; ++u) {
+      const int pg = (tt >> 5) + 8 * u, st = pg >> 2, s = (pg >> 1) & 1, hh = pg & 1;
+      const long b = t0 + 32 * st + 16 * s + 4 * hh;
+      const bool edge = b + 11 > last;
+      f16x8 hi[4], lo[4];
+      if constexpr (Q) {
+        uint32_t sw[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sw[i] = x.r[12 * u + 8 + i];
+        // A scale's NaN: all exponent bits set (no scale is infinite).
+        uint32_t bad = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t half = (i & 1) ? 0xFFFF0000u : 0x0000FFFFu;
+          if (edge && b + (i & 3) + 8 * (i >> 2) > last)
+            sw[i >> 1] &= ~half;
+          else if ((sw[i >> 1] & half & 0x7C007C00u) == (half & 0x7C007C00u)) {
+            sw[i >> 1] &= ~half;
+            bad |= 1u << (16 * s + 4 * hh + (i & 3) + 8 * (i >> 2));
+          }
+        }
+        if (bad && (j & 7) == 0) atomicOr(&nan_rows[st][dt], bad);
+        const f16x2 off = {(_Float16)-1152.f, (_Float16)-1152.f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t a = x.r[12 * u + 2 * i], c = x.r[12 * u + 2 * i + 1];
+          const f16x2 sc = __builtin_bit_cast(f16x2, sw[i]);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t t = __builtin_amdgcn_perm(c, a, k ? 0x07030602u : 0x05010400u);
+            const uint32_t p0 = __builtin_amdgcn_perm(0x64646464u, t, 0x04010400u);
+            const uint32_t p1 = __builtin_amdgcn_perm(0x64646464u, t, 0x04030402u);
+            const f16x2 v0 = (__builtin_bit_cast(f16x2, p0) + off) * sc;
+            const f16x2 v1 = (__builtin_bit_cast(f16x2, p1) + off) * sc;
+            hi[2 * k][2 * i] = v0[0];
+            hi[2 * k][2 * i + 1] = v0[1];
+            hi[2 * k + 1][2 * i] = v1[0];
+            hi[2 * k + 1][2 * i + 1] = v1[1];
+          }
+        }
+      } else if constexpr (LO) {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          float f[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            f[i] = edge && b + (i & 3) + 8 * (i >> 2) > last ? 0.f : __uint_as_float(x.r[32 * u + 4 * i + d]);
+          split8(f, hi[d], lo[d]);
+        }
+      } else {
+        uint32_t c[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          c[i] = edge && b + ((i >> 1) & 3) + 8 * (i >> 3) > last ? 0u : x.r[16 * u + i];
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          u32x4 p;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            p[i] = __builtin_amdgcn_perm(c[4 * i + 2 + (d >> 1)], c[4 * i + (d >> 1)], (d & 1) ? 0x07060302u : 0x05040100u);
+          hi[d] = __builtin_bit_cast(f16x8, p);
+        }
+      }
+      char* base = lds + kPlane + (st * 8 + dt * 2 + s) * kFragB;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const int at = v_slot(dt, (j & 7) * 4 + d, hh) * 16;
+        *reinterpret_cast<f16x8*>(base + at) = hi[d];
+        if constexpr (LO) *reinterpret_cast<f16x8*>(base + at + 2 * kPlane) = lo[d];
+      }
+    }
+  }
+}
+
 // The columns [col0, col0 + 32 WC) of kv head h (column c: row c / group, head
-// c % group) over rows [t_begin, t_end) of `w`; wave (wc, wp) takes columns
-// 32 wc .. and the 32-position subtiles wp, wp + WP, ... of each step of the
-// workgroup. Every wave runs the same number of steps.
+// c % group) over rows [t_begin, t_end) of `w`, on 32x32x16 products; wave (wc,
+// wp) takes columns 32 wc .. and the 32-row subtiles wp, wp + WP, ... of each
+// step. The next step's rows are in flight while this one's are computed, and
+// its tiles the other half of the LDS.
+template <int WC>
+constexpr int wide_step() {
+  return WC == 2 ? 128 : 64;
+}
+template <typename T, int WC>
+constexpr int wide_lds() {
+  const int stages = 2 * stage_bytes<T>(wide_step<WC>());
+  const int merge = (8 / WC - 1) * WC * 66 * 64 * 4;
+  return stages > merge ? stages : merge;
+}
+
 template <typename T, int WC, bool HL>
-__device__ void run_item(const RowsArgs& a, const KvView& w, int h, int col0, int n_cols, int row0, long t_begin,
-                         long t_end, bool causal, int slot, char* lds) {
-  constexpr int WP = 4 / WC;
-  constexpr int S = WC == 1 ? 128 : 64;     // positions per step
-  constexpr int SUB = S / 32 / WP;          // subtiles of a wave per step
-  constexpr bool LO = Lo<T>::value;
-  constexpr int kPlane = S / 32 * kTileB;   // K hi, V hi, then K lo, V lo
+__device__ void run_wide(const RowsArgs& a, const KvView& w, int h, int col0, int n_cols, long t_begin, long t_end,
+                         bool causal, int slot, char* lds) {
+  constexpr int WP = 8 / WC, S = wide_step<WC>(), SUB = S / 32 / WP;
+  constexpr bool LO = Lo<T>::value, Q = std::is_same<T, Q8>::value;
+  constexpr int kPlane = S / 32 * kTileB, kStage = stage_bytes<T>(S);
+  __shared__ uint32_t nan_rows[3][S / 32][4];  // by step mod 3: cleared two steps ahead of its reads
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wc = wave % WC, wp = wave / WC;
+  const bool is_v = wave >= 4;
+  const int tt = tid & 255;
   const int lc = lane & 31, lh = lane >> 5;
   const int col = col0 + 32 * wc + lc;
   const bool live = col < n_cols;
   const int crow = (live ? col : n_cols - 1) / a.group, chead = (live ? col : n_cols - 1) % a.group;
-  const int q_row = row0 + crow;
-  const long limit = causal ? min((long)a.start + q_row + 1, t_end) : t_end;
+  const long limit = causal ? min((long)a.start + crow + 1, t_end) : t_end;
   // What the wave's first column sees, and its last.
   const int wcol0 = min(col0 + 32 * wc, n_cols - 1), wcol1 = min(col0 + 32 * wc + 31, n_cols - 1);
-  const long w_first = causal ? min((long)a.start + row0 + wcol0 / a.group + 1, t_end) : t_end;
-  const long w_last = causal ? min((long)a.start + row0 + wcol1 / a.group + 1, t_end) : t_end;
+  const long w_first = causal ? min((long)a.start + wcol0 / a.group + 1, t_end) : t_end;
+  const long w_last = causal ? min((long)a.start + wcol1 / a.group + 1, t_end) : t_end;
+  const int hk = a.kv_lo + h;
+  const long last = t_end - 1;
 
-  // q' of the column, dims 16 c + 8 lh .. + 7 of each chunk c, scaled by a
-  // power of two that brings its largest value to [2^13, 2^14).
+  Share<T, S> sh;
+  load_share<T, S>(sh, w, hk, t_begin, last, is_v, tt);
   f16x8 qh[8], ql[HL ? 8 : 1];
   float q_up;
-  {
-    const float* qp = a.q + ((size_t)q_row * a.n_q_heads + (size_t)(a.kv_lo + h) * a.group + chead) * kD;
-    float x[8][8];
-    float amax = 0.f;
+  {  // dims 16 c + 8 lh .. + 7 of each chunk c
+    const float* qp = a.q + ((size_t)crow * a.n_q_heads + (size_t)hk * a.group + chead) * kD;
+    float x[64];
 #pragma unroll
     for (int c = 0; c < 8; ++c)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[c][e] = live ? qp[16 * c + 8 * lh + e] * a.qscale : 0.f;
-        amax = fmaxf(amax, fabsf(x[c][e]));
-      }
-    amax = swap_max<32>(amax);
-    int ex = 14;
-    if (amax > 0.f && amax < INFINITY) (void)frexpf(amax, &ex);
-    const int k = max(ex - 14, -100);
-    const float down = ldexpf(1.f, -k);
-    q_up = ldexpf(1.f, k);
-#pragma unroll
-    for (int c = 0; c < 8; ++c)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = x[c][e] * down;
-        const _Float16 hi = (_Float16)v;
-        qh[c][e] = hi;
-        if constexpr (HL) ql[c][e] = (_Float16)(v - (float)hi);
-      }
+      for (int e = 0; e < 8; ++e) x[8 * c + e] = live ? qp[16 * c + 8 * lh + e] * a.qscale : 0.f;
+    q_up = split_q<64, false, HL>(x, qh, ql);
   }
+  if constexpr (Q) {
+    if (tid < 3 * (S / 32) * 4) (&nan_rows[0][0][0])[tid] = 0;
+    __syncthreads();
+  }
+  store_share<T, S>(sh, lds, t_begin, last, is_v, tt, Q ? nan_rows[0] : nullptr);
+  __syncthreads();
+
   f32x16 o[4];
 #pragma unroll
   for (int d = 0; d < 4; ++d) o[d] = f32x16{};
   float m_run = -INFINITY, m_sub = 0.f, l_run = 0.f;
   uint32_t taint = 0;  // Q8_0: this lane's dims met a NaN block in a row its column sees
-
-  __shared__ uint32_t nan_rows[4][4];  // [subtile of 32][block of 32 dims]: rows whose V scale is NaN
-
-  const int hk = a.kv_lo + h;
-  const long last = t_end - 1;
+  int buf = 0, n3 = 0;
   for (long t0 = t_begin; t0 < t_end; t0 += S) {
-    __syncthreads();  // the previous step's reads are done
-    if constexpr (std::is_same<T, Q8>::value) {
-      if (tid < 4 * (S / 32)) nan_rows[tid >> 2][tid & 3] = 0;
-      __syncthreads();
+    const bool more = t0 + S < t_end;
+    if (more && !LO) load_share<T, S>(sh, w, hk, t0 + S, last, is_v, tt);
+    if constexpr (Q) {
+      const int clear = n3 == 0 ? 2 : n3 - 1;  // (n3 + 2) mod 3
+      if (tid < (S / 32) * 4) (&nan_rows[clear][0][0])[tid] = 0;
     }
-    // K: thread -> (16-byte chunk j of a row, row); V: thread -> (8 dims, 8 rows).
-    for (int u = tid; u < S * 16; u += 256) {
-      const int j = u & 15, p = u >> 4;
-      f16x8 hi, lo;
-      load_k8<T>(w, hk, std::is_same<T, Q8>::value ? t0 + p : min(t0 + p, last), j, hi, lo);
-      char* dst = lds + ((p >> 5) * 8 + (j >> 1)) * kFragB + k_slot(p & 31, j & 1) * 16;
-      *reinterpret_cast<f16x8*>(dst) = hi;
-      if constexpr (LO) *reinterpret_cast<f16x8*>(dst + 2 * kPlane) = lo;
-    }
-    for (int u = tid; u < S * 2; u += 256) {
-      const int j = u & 15, pg = u >> 4, st = pg >> 2, s = (pg >> 1) & 1, hh = pg & 1;
-      f16x8 hi[8], lo[8];
-      load_v8x8<T>(w, hk, t0 + 32 * st + 16 * s + 4 * hh, last, j, hi, lo);
-      if constexpr (std::is_same<T, Q8>::value) {
-        // A NaN scale makes a row's whole block NaN; it must not reach columns
-        // that do not see the row (0 * NaN), so the block goes in as zeros and
-        // the columns that see it are marked.
-        uint32_t bad = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (hi[0][i] != hi[0][i]) bad |= 1u << (16 * s + 4 * hh + (i & 3) + 8 * (i >> 2));
-        if (bad) {
-          atomicOr(&nan_rows[st][j >> 2], bad);
-#pragma unroll
-          for (int d = 0; d < 8; ++d)
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (hi[d][i] != hi[d][i]) hi[d][i] = (_Float16)0.f;
-        }
-      }
-      const int dt = j >> 2;
-      char* base = lds + kPlane + (st * 8 + dt * 2 + s) * kFragB;
-#pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        const int at = v_slot(dt, (j & 3) * 8 + d, hh) * 16;
-        *reinterpret_cast<f16x8*>(base + at) = hi[d];
-        if constexpr (LO) *reinterpret_cast<f16x8*>(base + at + 2 * kPlane) = lo[d];
-      }
-    }
-    __syncthreads();
+    const char* tile = lds + buf * kStage;
 #pragma unroll
     for (int sub = 0; sub < SUB; ++sub) {
       const int st = wp + WP * sub;
       const long p0 = t0 + 32 * st;
       if (p0 >= w_last) continue;  // wave-uniform; barriers are outside
-      const char* kt = lds + st * kTileB;
-      const char* vt = lds + kPlane + st * kTileB;
+      const char* kt = tile + st * kTileB + k_slot(lc, lh) * 16;
+      const char* vt = tile + kPlane + st * kTileB;
       f32x16 s0 = {}, s1 = {};
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
-        const f16x8 kf = *reinterpret_cast<const f16x8*>(kt + c * kFragB + k_slot(lc, lh) * 16);
+        const f16x8 kf = *reinterpret_cast<const f16x8*>(kt + c * kFragB);
         s0 = mfma(kf, qh[c], s0);
         if constexpr (HL) s1 = mfma(kf, ql[c], s1);
-        if constexpr (LO) {
-          const f16x8 kl = *reinterpret_cast<const f16x8*>(kt + 2 * kPlane + c * kFragB + k_slot(lc, lh) * 16);
-          s1 = mfma(kl, qh[c], s1);
-        }
+        if constexpr (LO) s1 = mfma(*reinterpret_cast<const f16x8*>(kt + 2 * kPlane + c * kFragB), qh[c], s1);
       }
       float x[16], mx = -INFINITY;
       const bool edge = p0 + 32 > w_first;  // some column does not see all of it
@@ -316,8 +748,7 @@ __device__ void run_item(const RowsArgs& a, const KvView& w, int h, int col0, in
       }
       mx = swap_max<32>(mx);
       if (__builtin_amdgcn_ballot_w64(mx > m_run + kSlack) != 0) {
-        const float mn = fmaxf(m_run, mx);
-        const float ms = mn == -INFINITY ? 0.f : mn;
+        const float mn = fmaxf(m_run, mx), ms = mn == -INFINITY ? 0.f : mn;
         const float alpha = __builtin_amdgcn_exp2f(m_run - ms);
         m_run = mn;
         m_sub = ms;
@@ -335,43 +766,53 @@ __device__ void run_item(const RowsArgs& a, const KvView& w, int h, int col0, in
         ph[i >> 3][i & 7] = hi;
         if constexpr (HL) pl[i >> 3][i & 7] = (_Float16)(pp - (float)hi);
       }
-      if constexpr (std::is_same<T, Q8>::value) {
+      if constexpr (Q) {
         const long seen = limit - p0;  // rows of this subtile the column sees
         const uint32_t mask = seen >= 32 ? 0xFFFFFFFFu : seen <= 0 ? 0u : (1u << seen) - 1;
-        // Lane (column, lh) holds dims 32 dt + 8 a + 4 lh + r of every dt.
+        // Lane (column, lh) holds dims of every block d.
 #pragma unroll
         for (int d = 0; d < 4; ++d)
-          if (nan_rows[st][d] & mask) taint |= 1u << d;
+          if (nan_rows[n3][st][d] & mask) taint |= 1u << d;
       }
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+      for (int s = 0; s < 2; ++s) {
+        f16x8 vf[4];
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-          const f16x8 vf = *reinterpret_cast<const f16x8*>(vt + (d * 2 + s) * kFragB + v_slot(d, lc, lh) * 16);
-          o[d] = mfma(vf, ph[s], o[d]);
-          if constexpr (HL) o[d] = mfma(vf, pl[s], o[d]);
-          if constexpr (LO) {
-            const f16x8 vl =
-                *reinterpret_cast<const f16x8*>(vt + 2 * kPlane + (d * 2 + s) * kFragB + v_slot(d, lc, lh) * 16);
-            o[d] = mfma(vl, ph[s], o[d]);
-          }
+          vf[d] = *reinterpret_cast<const f16x8*>(vt + (d * 2 + s) * kFragB + v_slot(d, lc, lh) * 16);
+          o[d] = mfma(vf[d], ph[s], o[d]);
         }
+        if constexpr (HL) {
+#pragma unroll
+          for (int d = 0; d < 4; ++d) o[d] = mfma(vf[d], pl[s], o[d]);
+        }
+        if constexpr (LO) {
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+            o[d] = mfma(*reinterpret_cast<const f16x8*>(vt + 2 * kPlane + (d * 2 + s) * kFragB + v_slot(d, lc, lh) * 16),
+                        ph[s], o[d]);
+        }
+      }
     }
+    buf ^= 1;
+    n3 = n3 == 2 ? 0 : n3 + 1;
+    if (more && LO) load_share<T, S>(sh, w, hk, t0 + S, last, is_v, tt);  // (no registers to hold it meanwhile)
+    if (more) store_share<T, S>(sh, lds + buf * kStage, t0 + S, last, is_v, tt, Q ? nan_rows[n3] : nullptr);
+    __syncthreads();
   }
   // Each lane summed its own rows: the other half of the column's.
   l_run = swap_sum<32>(l_run);
-  if constexpr (std::is_same<T, Q8>::value) {
+  if constexpr (Q) {
     if (taint) {
 #pragma unroll
       for (int d = 0; d < 4; ++d)
         if (taint & (1u << d)) o[d] = o[d] * __builtin_nanf("");
     }
   }
-  // The position groups' partials meet in LDS, in wave order.
+  // The row groups' partials meet in LDS, in wave order.
   if constexpr (WP > 1) {
     float* om = reinterpret_cast<float*>(lds);  // [wp - 1][wc][64 registers][64 lanes], then (m, l)
     constexpr int kWave = 66 * 64;
-    __syncthreads();
     if (wp > 0) {
       float* d = om + ((wp - 1) * WC + wc) * kWave + lane;
 #pragma unroll
@@ -397,15 +838,15 @@ __device__ void run_item(const RowsArgs& a, const KvView& w, int h, int col0, in
   constexpr float kDown = 1.f / kPScale;
   if (a.single) {
     const float inv = kDown / l_run;
-    float* dst = a.out + ((size_t)q_row * a.n_heads * a.group + (size_t)h * a.group + chead) * kD;
+    float* dst = a.out + ((size_t)crow * a.n_heads * a.group + (size_t)h * a.group + chead) * kD;
 #pragma unroll
     for (int d = 0; d < 4; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) dst[32 * d + 8 * (i >> 2) + 4 * lh + (i & 3)] = o[d][i] * inv;
     return;
   }
-  const size_t column = (size_t)h * a.rows * a.group + (size_t)row0 * a.group + col;
-  const size_t at = (size_t)slot * a.n_heads * a.rows * a.group + column;
+  const size_t column = (size_t)h * n_cols + col;
+  const size_t at = (size_t)slot * a.n_heads * n_cols + column;
   float* dst = a.part + at * kD;
 #pragma unroll
   for (int d = 0; d < 4; ++d)
@@ -429,21 +870,65 @@ __device__ __forceinline__ bool device_positions(const uint32_t* d_pos, int plan
   return true;
 }
 
-template <typename T, int WC, bool HL, bool TAILS>
-__global__ __launch_bounds__(256) void rows_kernel(RowsArgs a, std::conditional_t<TAILS, TailLens, NoLens> lens) {
-  constexpr int kMain = stage_bytes<T>(WC == 1 ? 128 : 64), kTail = TAILS ? stage_bytes<T>(128) : 0;
-  constexpr int kMerge = (TAILS || WC == 1 ? 3 : WC == 2 ? 2 : 0) * 66 * 64 * 4;
-  constexpr int kBytes = kMain > kTail ? (kMain > kMerge ? kMain : kMerge) : (kTail > kMerge ? kTail : kMerge);
-  __shared__ __attribute__((aligned(1024))) char lds[kBytes];
-  int b = blockIdx.x;
+// A tail item by the four waves `wv` counts: sequence, column block of 16,
+// split (b past them: none, the waves only keep the barriers).
+template <typename T>
+__device__ void tail_item(const RowsArgs& a, const TailLens& lens, int b, int wv, char* lds) {
+  const int split = b % a.t_splits;
+  b /= a.t_splits;
+  const int cb = b % a.t_cb;
+  b /= a.t_cb;
+  const int h = b % a.n_heads, seq = b / a.n_heads;
+  const long len = seq < a.rows ? lens.len[seq] : 0, t_begin = (long)split * a.t_split_len;
+  KvView w = a.tail;
+  w.k += (size_t)seq * w.layer_bytes;
+  w.v += (size_t)seq * w.layer_bytes;
+  w.ks += (size_t)seq * w.layer_scales;
+  w.vs += (size_t)seq * w.layer_scales;
+  run_narrow<T, 1>(a, w, h, cb * 16, a.group, seq, t_begin, min(len, t_begin + a.t_split_len), a.n_splits + split, wv,
+                   t_begin < len, lds);
+}
+
+// Workgroup b of the main items: (kv head, split) units whose column blocks are
+// 8 apart, so that they run on one XCD and meet in its L2.
+__device__ __forceinline__ bool main_item(const RowsArgs& a, int b, int& h, int& split, int& cb) {
+  cb = (b % (8 * a.n_cb)) / 8;
+  const int u = (b / (8 * a.n_cb)) * 8 + b % 8;
+  if (u >= a.n_heads * a.n_splits) return false;
+  split = u % a.n_splits;
+  h = u / a.n_splits;
+  return true;
+}
+
+template <typename T, int NB, bool TAILS>
+__global__ __launch_bounds__(256) void rows_narrow_kernel(RowsArgs a, std::conditional_t<TAILS, TailLens, NoLens> lens) {
+  __shared__ __attribute__((aligned(16))) char lds[narrow_lds(NB)];
+  const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   int positions = a.positions;
   if (!device_positions(a.d_pos, a.positions, positions)) return;
+  const int b = blockIdx.x;
   if (!TAILS || b < a.main_items) {
-    const int split = b % a.n_splits;
-    b /= a.n_splits;
-    const int cb = b % a.n_cb, h = b / a.n_cb;
+    int h, split, cb;
+    if (!main_item(a, b, h, split, cb)) return;
+    const long t_begin = (long)split * a.split_len, t_end = min((long)positions, t_begin + a.split_len);
+    if (t_begin >= t_end) return;
+    run_narrow<T, NB>(a, a.main, h, cb * 16 * NB, a.rows * a.group, 0, t_begin, t_end, split, wv, true, lds);
+  } else if constexpr (TAILS) {
+    tail_item<T>(a, lens, b - a.main_items, wv, lds);
+  }
+}
+
+template <typename T, int WC, bool HL, bool TAILS>
+__global__ __launch_bounds__(512) void rows_wide_kernel(RowsArgs a, std::conditional_t<TAILS, TailLens, NoLens> lens) {
+  constexpr int kMain = wide_lds<T, WC>(), kTail = TAILS ? 2 * narrow_lds(1) : 0;
+  __shared__ __attribute__((aligned(1024))) char lds[kMain > kTail ? kMain : kTail];
+  const int b = blockIdx.x;
+  if (!TAILS || b < a.main_items) {
+    int h, split, cb;
+    if (!main_item(a, b, h, split, cb)) return;
+    if (a.causal) cb = a.n_cb - 1 - cb;  // the longest first
     const int n_cols = a.rows * a.group, col0 = cb * 32 * WC;
-    long t_end = positions;
+    long t_end = a.positions;
     if (a.causal) {  // the last column's limit
       const int r = (min(col0 + 32 * WC, n_cols) - 1) / a.group;
       t_end = min(t_end, (long)a.start + r + 1);
@@ -451,23 +936,11 @@ __global__ __launch_bounds__(256) void rows_kernel(RowsArgs a, std::conditional_
     const long t_begin = (long)split * a.split_len;
     t_end = min(t_end, t_begin + a.split_len);
     if (t_begin >= t_end) return;
-    run_item<T, WC, HL>(a, a.main, h, col0, n_cols, 0, t_begin, t_end, a.causal != 0, split, lds);
-  } else if constexpr (TAILS) {
-    b -= a.main_items;
-    const int split = b % a.t_splits;
-    b /= a.t_splits;
-    const int cb = b % a.t_cb;
-    b /= a.t_cb;
-    const int h = b % a.n_heads, seq = b / a.n_heads;
-    const long len = lens.len[seq], t_begin = (long)split * a.t_split_len;
-    if (t_begin >= len) return;
-    KvView w = a.tail;
-    w.k += (size_t)seq * w.layer_bytes;
-    w.v += (size_t)seq * w.layer_bytes;
-    w.ks += (size_t)seq * w.layer_scales;
-    w.vs += (size_t)seq * w.layer_scales;
-    run_item<T, 1, HL>(a, w, h, cb * 32, a.group, seq, t_begin, min(len, t_begin + a.t_split_len), false,
-                       a.n_splits + split, lds);
+    run_wide<T, WC, HL>(a, a.main, h, col0, n_cols, t_begin, t_end, a.causal != 0, split, lds);
+  } else if constexpr (TAILS) {  // two items, four waves each
+    const int half = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8);
+    tail_item<T>(a, lens, 2 * (b - a.main_items) + half, __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6) & 3),
+                 lds + half * narrow_lds(1));
   }
 }
 
@@ -581,21 +1054,22 @@ __global__ __launch_bounds__(256) void rows_generic_kernel(RowsArgs a, int hd,
 // ---- plans ------------------------------------------------------------------------
 struct RowsPlan {
   bool generic = false;
-  int wc = 1, n_cb = 0, n_splits = 0, split_len = 128;
+  int nb = 0, wc = 0;  // narrow: blocks of 16 columns; wide: waves of 32
+  int n_cb = 0, n_splits = 0, split_len = 128;
   int t_cb = 0, t_splits = 0, t_split_len = 128;
   size_t rows = 0;  // of one launch (sequences go in batches of kMaxEach)
   size_t slots() const { return (size_t)n_splits + t_splits; }
+  int columns() const { return nb ? 16 * nb : 32 * wc; }  // of a main item
 };
 
-constexpr long kWantItems = 2 * kCUs;
 constexpr int kPosStep = 128;
 
 // Splits of `positions` for `units` independent items so that the launch has
-// about kWantItems of them: lengths in whole steps.
-void split_positions(long positions, long units, int* n_splits, int* split_len) {
+// about `want` of them: lengths in whole steps.
+void split_positions(long positions, long units, long want, int* n_splits, int* split_len) {
   const long steps = (positions + kPosStep - 1) / kPosStep;
-  const long want = std::max<long>(1, std::min<long>(steps, kWantItems / std::max<long>(units, 1)));
-  const long per = (steps + want - 1) / want;
+  const long n = std::max<long>(1, std::min<long>(steps, want / std::max<long>(units, 1)));
+  const long per = (steps + n - 1) / n;
   *split_len = (int)(per * kPosStep);
   *n_splits = (int)((steps + per - 1) / per);
 }
@@ -607,11 +1081,15 @@ RowsPlan plan_rows(const RowsCall& c, const rv_kv* owner) {
   p.rows = c.tails ? std::min<size_t>(c.rows, kMaxEach) : c.rows;
   if (p.generic) return p;
   const long group = (long)(c.n_q_heads / g->n_kv_heads), heads = (long)(c.kv_hi - c.kv_lo);
+  const long cols = (long)p.rows * group;
+  const bool causal = c.causal && c.rows > 1;
+  if (cols <= 32 && !causal && c.split)
+    p.nb = cols <= 16 ? 1 : 2;
+  else
+    p.wc = cols <= 64 && g->elem != RV_ELEM_F32 ? 2 : cols <= 128 ? 4 : 8;
   if (c.main && c.positions) {
-    const long cols = (long)p.rows * group;
-    p.wc = cols <= 32 ? 1 : cols <= 64 ? 2 : 4;
-    p.n_cb = (int)((cols + 32 * p.wc - 1) / (32 * p.wc));
-    split_positions((long)c.positions, heads * p.n_cb, &p.n_splits, &p.split_len);
+    p.n_cb = (int)((cols + p.columns() - 1) / p.columns());
+    split_positions((long)c.positions, heads * p.n_cb, p.nb ? 2 * kCUs : kCUs, &p.n_splits, &p.split_len);
     if (owner->tune_decode_split_len > 0) {
       p.split_len = (int)((std::min<int64_t>(owner->tune_decode_split_len, 1 << 30) + kPosStep - 1) / kPosStep * kPosStep);
       p.n_splits = (int)((c.positions + p.split_len - 1) / p.split_len);
@@ -620,8 +1098,8 @@ RowsPlan plan_rows(const RowsCall& c, const rv_kv* owner) {
   if (c.tails) {
     size_t longest = 0;
     for (size_t i = 0; i < c.rows; ++i) longest = std::max(longest, c.tails->lens[c.tail_layer + i]);
-    p.t_cb = (int)((group + 31) / 32);
-    if (longest) split_positions((long)longest, heads * p.t_cb * (long)p.rows, &p.t_splits, &p.t_split_len);
+    p.t_cb = (int)((group + 15) / 16);
+    if (longest) split_positions((long)longest, heads * p.t_cb * (long)p.rows, 2 * kCUs, &p.t_splits, &p.t_split_len);
   }
   return p;
 }
@@ -632,19 +1110,24 @@ size_t plan_floats(const RowsPlan& p, const RowsCall& c) {
   return p.generic || p.slots() <= 1 ? 0 : p.slots() * cols * (kD + 2);
 }
 
-template <typename T, int WC, bool HL, bool TAILS, typename L>
-void launch_rows_kernel(const TimedPair& tp, const RowsArgs& a, unsigned items, hipStream_t s, const L& lens) {
-  launch_timed(tp, rows_kernel<T, WC, HL, TAILS>, dim3(items), dim3(256), s, a, lens);
-}
-
 template <typename T, bool HL, bool TAILS, typename L>
-void launch_wc(int wc, const TimedPair& tp, const RowsArgs& a, unsigned items, hipStream_t s, const L& lens) {
-  if (wc == 1)
-    launch_rows_kernel<T, 1, HL, TAILS>(tp, a, items, s, lens);
-  else if (wc == 2)
-    launch_rows_kernel<T, 2, HL, TAILS>(tp, a, items, s, lens);
-  else
-    launch_rows_kernel<T, 4, HL, TAILS>(tp, a, items, s, lens);
+void launch_plan(const RowsPlan& p, const TimedPair& tp, const RowsArgs& a, unsigned tail_items, hipStream_t s,
+                 const L& lens) {
+  if (p.nb) {
+    const dim3 grid((unsigned)a.main_items + tail_items);
+    if (p.nb == 1)
+      launch_timed(tp, rows_narrow_kernel<T, 1, TAILS>, grid, dim3(256), s, a, lens);
+    else
+      launch_timed(tp, rows_narrow_kernel<T, 2, TAILS>, grid, dim3(256), s, a, lens);
+    return;
+  }
+  const dim3 grid((unsigned)a.main_items + (tail_items + 1) / 2);
+  if (p.wc == 8)
+    launch_timed(tp, rows_wide_kernel<T, 8, HL, TAILS>, grid, dim3(512), s, a, lens);
+  else if (p.wc == 4)
+    launch_timed(tp, rows_wide_kernel<T, 4, HL, TAILS>, grid, dim3(512), s, a, lens);
+  else if constexpr (!Lo<T>::value)
+    launch_timed(tp, rows_wide_kernel<T, 2, HL, TAILS>, grid, dim3(512), s, a, lens);
 }
 
 }  // namespace
@@ -653,8 +1136,8 @@ size_t rows_ws_need(const rv_kv* owner, const RowsCall& c) { return plan_floats(
 
 size_t rows_ws_bound(const rv_kv* kv) {
   if (kv->head_dim != (size_t)kD) return 0;
-  // At most kWantItems items of 32 columns (one wave's), and one per kv head.
-  return (size_t)std::max<long>(kWantItems, (long)kv->n_kv_heads) * 32 * (kD + 2) * sizeof(float);
+  // A narrow launch's items: 2 kCUs, or one per kv head (and then no partials).
+  return (size_t)2 * kCUs * 16 * (kD + 2) * sizeof(float);
 }
 
 HipStatus launch_rows(rv_kv* owner, const RowsCall& c, hipStream_t s, const Workspace* ws) {
@@ -717,27 +1200,27 @@ HipStatus launch_rows(rv_kv* owner, const RowsCall& c, hipStream_t s, const Work
       const size_t cols = n * group * a.n_heads;
       a.part = base;
       a.ml = base ? base + p.slots() * cols * kD : nullptr;
-      a.n_cb = (int)((n * group + 32 * p.wc - 1) / (32 * p.wc));
+      a.n_cb = (int)((n * group + p.columns() - 1) / p.columns());
       a.n_splits = p.n_splits;
       a.split_len = p.split_len;
       a.t_cb = p.t_cb;
       a.t_splits = p.t_splits;
       a.t_split_len = p.t_split_len;
-      a.main_items = a.n_heads * a.n_cb * a.n_splits;
+      a.main_items = (a.n_heads * a.n_splits + 7) / 8 * 8 * a.n_cb;
       a.single = p.slots() == 1;
-      const unsigned items = (unsigned)(a.main_items + n * a.n_heads * a.t_cb * a.t_splits);
+      const unsigned tail_items = (unsigned)(n * a.n_heads * a.t_cb * a.t_splits);
       const TimedPair tp = ws ? TimedPair{} : timing_pair(owner, s);
       if (c.tails) {
         if (g->elem == RV_ELEM_Q8_0)
-          launch_wc<Q8, true, true>(p.wc, tp, a, items, s, lens);
+          launch_plan<Q8, true, true>(p, tp, a, tail_items, s, lens);
         else if (g->elem == RV_ELEM_F32)
-          launch_wc<float, true, true>(p.wc, tp, a, items, s, lens);
+          launch_plan<float, true, true>(p, tp, a, tail_items, s, lens);
         else
-          launch_wc<_Float16, true, true>(p.wc, tp, a, items, s, lens);
+          launch_plan<_Float16, true, true>(p, tp, a, tail_items, s, lens);
       } else if (c.split) {
-        launch_wc<Q8, true, false>(p.wc, tp, a, items, s, NoLens{});
+        launch_plan<Q8, true, false>(p, tp, a, 0, s, NoLens{});
       } else {
-        launch_wc<Q8, false, false>(p.wc, tp, a, items, s, NoLens{});
+        launch_plan<Q8, false, false>(p, tp, a, 0, s, NoLens{});
       }
       if (!a.single) {
         const dim3 grid((unsigned)((cols + 7) / 8)), block(256);
