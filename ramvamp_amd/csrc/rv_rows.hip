@@ -21,8 +21,10 @@ namespace {
 
 constexpr int kD = 128;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kSlack = 8.f;    // p may reach 2^kSlack before the maximum moves
-constexpr float kPScale = 64.f;  // p * kPScale <= 2^14, inside f16
+// The running maximum moves when a score passes it by more than kSlack, and
+// probabilities carry a factor of 2^kUp (it cancels in o / l): they stay at or
+// below 2^14, inside f16, and small ones are kept off its subnormals.
+constexpr float kSlack = 8.f, kUp = 6.f;
 
 struct NoLens {};
 struct TailLens {
@@ -33,8 +35,14 @@ struct RowsArgs {
   KvView main, tail;      // at the call's layers
   const float* q;
   float* out;             // written when there is one slot in all
-  float* part;            // [slot][column][kD]
-  float* ml;              // [slot][column][2]: maximum, sum
+  // Partials, a 16-column block's (narrow and tail items) or a 32-column
+  // block's (wide items) rows in the order of its wave's registers, so that
+  // stores and the merge's loads are whole lines: [slot][block][16 bytes i][64
+  // lanes]. ml: maximum and sum by [slot][column].
+  float* part;
+  float* ml;
+  size_t slot_floats;     // of part, from one main slot to the next
+  size_t t_base, t_slot_floats;  // of part: the first tail slot, from one to the next
   const uint32_t* d_pos;  // positions from device memory
   int rows, n_q_heads, group, kv_lo, n_heads;
   int positions, start;   // limit of row r: causal ? start + r + 1 : positions
@@ -258,6 +266,33 @@ __device__ __forceinline__ float split_q(const float (&x)[N], f16x8 (&hi)[N / 8]
   return ldexpf(1.f, k);
 }
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// N probabilities as f16 hi (and lo) operand halves, and their sum added to l:
+// p = 2^(s * up + shift).
+template <int N, bool HL>
+__device__ __forceinline__ void probabilities(const float (&s)[N], float up, float shift, f16x8 (&hi)[N / 8],
+                                              f16x8 (&lo)[N / 8], float& l) {
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const f32x2 p = {__builtin_amdgcn_exp2f(__builtin_fmaf(s[i], up, shift)),
+                     __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + 1], up, shift))};
+    sum += p[0];
+    sum += p[1];
+    const f16x2 h = __builtin_convertvector(p, f16x2);
+    hi[i / 8][i % 8] = h[0];
+    hi[i / 8][i % 8 + 1] = h[1];
+    if constexpr (HL) {
+      const f32x2 r = {__builtin_fmaf((float)h[0], -1.f, p[0]), __builtin_fmaf((float)h[1], -1.f, p[1])};
+      const f16x2 t = __builtin_convertvector(r, f16x2);
+      lo[i / 8][i % 8] = t[0];
+      lo[i / 8][i % 8 + 1] = t[1];
+    }
+  }
+  l += sum;
+}
+
 __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
@@ -265,12 +300,15 @@ __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
 // Columns [col0, col0 + 16 NB) of kv head h over rows [t_begin, t_end) of `w`,
 // by the four waves `w0` .. + 3 of the workgroup (wave wv of them takes tiles
 // wv, wv + 4, ...). All waves of the workgroup call it together; `run` false:
-// nothing to do but the barriers. No causal limit.
+// nothing to do but the barriers. No causal limit. `part` and `ml` are those of
+// the item's slot, kv head and (a tail's) sequence. AHEAD: a wave's next tile
+// loads while it computes one, where the registers hold two (an f32 tile is 128
+// of them).
 constexpr int narrow_lds(int nb) { return 3 * nb * 34 * 64 * 4; }
 
-template <typename T, int NB>
+template <typename T, int NB, bool AHEAD>
 __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, int n_cols, int row0, long t_begin,
-                           long t_end, int slot, int wv, bool run, char* lds) {
+                           long t_end, float* part, float* ml, int wv, bool run, char* lds) {
   constexpr bool LO = Lo<T>::value;
   const int lane = threadIdx.x & 63, li = lane & 15, lk = lane >> 4;
   const int hk = a.kv_lo + h;
@@ -287,7 +325,7 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
   }
   const int n_tiles = run ? (int)((t_end - t_begin + 31) >> 5) : 0;
   if (wv < n_tiles) {
-    Raw<T> ra, rb;
+    Raw<T> ra;
     load_raw<T>(ra, w, hk, t_begin + 32L * wv, last, li, lk);
     f16x8 qh[NB][4], ql[NB][4];
 #pragma unroll
@@ -332,13 +370,17 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
       for (int n = 0; n < NB; ++n) {
         float y[8], mx = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          y[i] = (s[n][i >> 2][0][i & 3] + s[n][i >> 2][1][i & 3]) * q_up[n];
-          if (edge && p0 + 16 * (i >> 2) + 4 * lk + (i & 3) >= t_end) y[i] = -INFINITY;
-          mx = fmaxf(mx, y[i]);
+        for (int i = 0; i < 8; ++i) y[i] = s[n][i >> 2][0][i & 3] + s[n][i >> 2][1][i & 3];
+        if (edge) {
+          const int seen = (int)(t_end - p0) - 4 * lk;  // of this quarter's rows 16 t + r
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (16 * (i >> 2) + (i & 3) >= seen) y[i] = -INFINITY;
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mx = fmaxf(mx, y[i]);
         mx = swap_max<16>(mx);
-        mx = swap_max<32>(mx);
+        mx = swap_max<32>(mx) * q_up[n];
         if (__builtin_amdgcn_ballot_w64(mx > m_run[n] + kSlack) != 0) {
           const float mn = fmaxf(m_run[n], mx), ms = mn == -INFINITY ? 0.f : mn;
           const float alpha = __builtin_amdgcn_exp2f(m_run[n] - ms);
@@ -348,15 +390,10 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
 #pragma unroll
           for (int b = 0; b < 8; ++b) o[n][b] *= alpha;
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float p = __builtin_amdgcn_exp2f(y[i] - m_sub[n]);
-          l_run[n] += p;
-          const float pp = p * kPScale;
-          const _Float16 hi = (_Float16)pp;
-          ph[n][i] = hi;
-          pl[n][i] = (_Float16)(pp - (float)hi);
-        }
+        f16x8 h1[1], l1[1];
+        probabilities<8, true>(y, q_up[n], kUp - m_sub[n], h1, l1, l_run[n]);
+        ph[n] = h1[0];
+        pl[n] = l1[0];
       }
       if (edge) mask_v<T>(x, p0, last, lk);
 #pragma unroll
@@ -376,22 +413,21 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
         }
       }
     };
-    if constexpr (LO) {  // a tile fills the registers
+    if constexpr (!AHEAD) {
       for (int t = wv; t < n_tiles; t += 4) {
         if (t != wv) load_raw<T>(ra, w, hk, t_begin + 32L * t, last, li, lk);
         compute(ra, t_begin + 32L * t);
       }
-      rb = ra;
     } else {
-    // One tile computed while the wave's next one loads.
-    for (int t = wv; t < n_tiles; t += 8) {
-      const bool more = t + 4 < n_tiles;
-      if (more) load_raw<T>(rb, w, hk, t_begin + 32L * (t + 4), last, li, lk);
-      compute(ra, t_begin + 32L * t);
-      if (!more) break;
-      if (t + 8 < n_tiles) load_raw<T>(ra, w, hk, t_begin + 32L * (t + 8), last, li, lk);
-      compute(rb, t_begin + 32L * (t + 4));
-    }
+      Raw<T> rb;
+      for (int t = wv; t < n_tiles; t += 8) {
+        const bool more = t + 4 < n_tiles;
+        if (more) load_raw<T>(rb, w, hk, t_begin + 32L * (t + 4), last, li, lk);
+        compute(ra, t_begin + 32L * t);
+        if (!more) break;
+        if (t + 8 < n_tiles) load_raw<T>(ra, w, hk, t_begin + 32L * (t + 8), last, li, lk);
+        compute(rb, t_begin + 32L * (t + 4));
+      }
     }
   }
   // Each lane summed its own rows: the other quarters of the column's.
@@ -415,7 +451,6 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
   }
   __syncthreads();
   if (wv > 0 || !run) return;
-  constexpr float kDown = 1.f / kPScale;
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     for (int p = 1; p < min(4, n_tiles); ++p) {
@@ -430,10 +465,10 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
     }
     const int col = col0 + 16 * n + li;
     if (col >= n_cols) continue;
-    const int row = row0 + col / a.group, head = col % a.group;
-    // This lane's dims: 32 lk + 8 r + b.
     if (a.single) {
-      const float inv = kDown / l_run[n];
+      // This lane's dims: 32 lk + 8 r + b.
+      const int row = row0 + col / a.group, head = col % a.group;
+      const float inv = 1.f / l_run[n];
       float* dst = a.out + ((size_t)row * a.n_heads * a.group + (size_t)h * a.group + head) * kD + 32 * lk;
 #pragma unroll
       for (int r = 0; r < 4; ++r)
@@ -441,20 +476,16 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
         for (int b = 0; b < 8; ++b) dst[8 * r + b] = o[n][b][r] * inv;
       continue;
     }
-    const size_t column = (size_t)h * a.rows * a.group + (size_t)row0 * a.group + col;
-    const size_t at = (size_t)slot * a.n_heads * a.rows * a.group + column;
-    float* dst = a.part + at * kD + 32 * lk;
+    float* dst = part + (size_t)(col / 16) * (16 * kD) + 4 * lane;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const f32x4 v = {o[n][4 * g][r] * kDown, o[n][4 * g + 1][r] * kDown, o[n][4 * g + 2][r] * kDown,
-                         o[n][4 * g + 3][r] * kDown};
-        *reinterpret_cast<f32x4*>(dst + 8 * r + 4 * g) = v;
-      }
+    for (int i = 0; i < 8; ++i) {  // dims 32 lk + 4 i .. + 3
+      const f32x4 v = {o[n][4 * (i & 1)][i >> 1], o[n][4 * (i & 1) + 1][i >> 1], o[n][4 * (i & 1) + 2][i >> 1],
+                       o[n][4 * (i & 1) + 3][i >> 1]};
+      *reinterpret_cast<f32x4*>(dst + 256 * i) = v;
+    }
     if (lk == 0) {
-      a.ml[2 * at] = m_run[n];
-      a.ml[2 * at + 1] = l_run[n];
+      ml[2 * col] = m_run[n];
+      ml[2 * col + 1] = l_run[n];
     }
   }
 }
@@ -578,22 +609,31 @@ __device__ __forceinline__ void store_share(const Share<T, S>& x, char* lds, lon
     for (int u = 0; u < Share<T, S>::VU; ++u) {
       const int pg = (tt >> 5) + 8 * u, st = pg >> 2, s = (pg >> 1) & 1, hh = pg & 1;
       const long b = t0 + 32 * st + 16 * s + 4 * hh;
-      const bool edge = b + 11 > last;
+      const bool edge = t0 + S - 1 > last;  // (of the step)
       f16x8 hi[4], lo[4];
       if constexpr (Q) {
         uint32_t sw[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) sw[i] = x.r[12 * u + 8 + i];
-        // A scale's NaN: all exponent bits set (no scale is infinite).
-        uint32_t bad = 0;
+        if (edge) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t half = (i & 1) ? 0xFFFF0000u : 0x0000FFFFu;
-          if (edge && b + (i & 3) + 8 * (i >> 2) > last)
-            sw[i >> 1] &= ~half;
-          else if ((sw[i >> 1] & half & 0x7C007C00u) == (half & 0x7C007C00u)) {
-            sw[i >> 1] &= ~half;
-            bad |= 1u << (16 * s + 4 * hh + (i & 3) + 8 * (i >> 2));
+          for (int i = 0; i < 8; ++i)
+            if (b + (i & 3) + 8 * (i >> 2) > last) sw[i >> 1] &= (i & 1) ? 0x0000FFFFu : 0xFFFF0000u;
+        }
+        // A scale's NaN: all exponent bits set (no scale is infinite), so that
+        // adding one to the exponent reaches the (clear) sign.
+        uint32_t nan = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) nan |= ((sw[i] & 0x7C007C00u) + 0x04000400u);
+        uint32_t bad = 0;
+        if (nan & 0x80008000u) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t half = (i & 1) ? 0xFFFF0000u : 0x0000FFFFu;
+            if ((sw[i >> 1] & half & 0x7C007C00u) == (half & 0x7C007C00u)) {
+              sw[i >> 1] &= ~half;
+              bad |= 1u << (16 * s + 4 * hh + (i & 3) + 8 * (i >> 2));
+            }
           }
         }
         if (bad && (j & 7) == 0) atomicOr(&nan_rows[st][dt], bad);
@@ -667,11 +707,11 @@ constexpr int wide_lds() {
 
 template <typename T, int WC, bool HL>
 __device__ void run_wide(const RowsArgs& a, const KvView& w, int h, int col0, int n_cols, long t_begin, long t_end,
-                         bool causal, int slot, char* lds) {
+                         bool causal, int split, char* lds) {
   constexpr int WP = 8 / WC, S = wide_step<WC>(), SUB = S / 32 / WP;
   constexpr bool LO = Lo<T>::value, Q = std::is_same<T, Q8>::value;
   constexpr int kPlane = S / 32 * kTileB, kStage = stage_bytes<T>(S);
-  __shared__ uint32_t nan_rows[3][S / 32][4];  // by step mod 3: cleared two steps ahead of its reads
+  __shared__ __attribute__((aligned(16))) uint32_t nan_rows[3][S / 32][4];  // by step mod 3: cleared two steps ahead of its reads
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wc = wave % WC, wp = wave / WC;
@@ -730,23 +770,26 @@ __device__ void run_wide(const RowsArgs& a, const KvView& w, int h, int col0, in
       if (p0 >= w_last) continue;  // wave-uniform; barriers are outside
       const char* kt = tile + st * kTileB + k_slot(lc, lh) * 16;
       const char* vt = tile + kPlane + st * kTileB;
-      f32x16 s0 = {}, s1 = {};
+      f32x16 acc = {};
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         const f16x8 kf = *reinterpret_cast<const f16x8*>(kt + c * kFragB);
-        s0 = mfma(kf, qh[c], s0);
-        if constexpr (HL) s1 = mfma(kf, ql[c], s1);
-        if constexpr (LO) s1 = mfma(*reinterpret_cast<const f16x8*>(kt + 2 * kPlane + c * kFragB), qh[c], s1);
+        acc = mfma(kf, qh[c], acc);
+        if constexpr (HL) acc = mfma(kf, ql[c], acc);
+        if constexpr (LO) acc = mfma(*reinterpret_cast<const f16x8*>(kt + 2 * kPlane + c * kFragB), qh[c], acc);
       }
       float x[16], mx = -INFINITY;
-      const bool edge = p0 + 32 > w_first;  // some column does not see all of it
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        x[i] = (HL || LO ? s0[i] + s1[i] : s0[i]) * q_up;
-        if (edge && p0 + 8 * (i >> 2) + (i & 3) + 4 * lh >= limit) x[i] = -INFINITY;
-        mx = fmaxf(mx, x[i]);
+      for (int i = 0; i < 16; ++i) x[i] = acc[i];
+      if (p0 + 32 > w_first) {  // some column does not see all of it
+        const int seen = (int)max(limit - p0, 0L) - 4 * lh;  // of this half's rows 8 t + r
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (8 * (i >> 2) + (i & 3) >= seen) x[i] = -INFINITY;
       }
-      mx = swap_max<32>(mx);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[i]);
+      mx = swap_max<32>(mx) * q_up;
       if (__builtin_amdgcn_ballot_w64(mx > m_run + kSlack) != 0) {
         const float mn = fmaxf(m_run, mx), ms = mn == -INFINITY ? 0.f : mn;
         const float alpha = __builtin_amdgcn_exp2f(m_run - ms);
@@ -757,22 +800,17 @@ __device__ void run_wide(const RowsArgs& a, const KvView& w, int h, int col0, in
         for (int d = 0; d < 4; ++d) o[d] *= alpha;
       }
       f16x8 ph[2], pl[2];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float p = __builtin_amdgcn_exp2f(x[i] - m_sub);
-        l_run += p;
-        const float pp = p * kPScale;
-        const _Float16 hi = (_Float16)pp;
-        ph[i >> 3][i & 7] = hi;
-        if constexpr (HL) pl[i >> 3][i & 7] = (_Float16)(pp - (float)hi);
-      }
+      probabilities<16, HL>(x, q_up, kUp - m_sub, ph, pl, l_run);
       if constexpr (Q) {
-        const long seen = limit - p0;  // rows of this subtile the column sees
-        const uint32_t mask = seen >= 32 ? 0xFFFFFFFFu : seen <= 0 ? 0u : (1u << seen) - 1;
         // Lane (column, lh) holds dims of every block d.
+        const u32x4 bad = *reinterpret_cast<const u32x4*>(nan_rows[n3][st]);
+        if (__builtin_amdgcn_readfirstlane(bad[0] | bad[1] | bad[2] | bad[3])) {
+          const long seen = limit - p0;  // rows of this subtile the column sees
+          const uint32_t mask = seen >= 32 ? 0xFFFFFFFFu : seen <= 0 ? 0u : (1u << seen) - 1;
 #pragma unroll
-        for (int d = 0; d < 4; ++d)
-          if (nan_rows[n3][st][d] & mask) taint |= 1u << d;
+          for (int d = 0; d < 4; ++d)
+            if (bad[d] & mask) taint |= 1u << d;
+        }
       }
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
@@ -835,9 +873,8 @@ __device__ void run_wide(const RowsArgs& a, const KvView& w, int h, int col0, in
     }
   }
   if (wp != 0 || !live) return;
-  constexpr float kDown = 1.f / kPScale;
   if (a.single) {
-    const float inv = kDown / l_run;
+    const float inv = 1.f / l_run;
     float* dst = a.out + ((size_t)crow * a.n_heads * a.group + (size_t)h * a.group + chead) * kD;
 #pragma unroll
     for (int d = 0; d < 4; ++d)
@@ -845,19 +882,17 @@ __device__ void run_wide(const RowsArgs& a, const KvView& w, int h, int col0, in
       for (int i = 0; i < 16; ++i) dst[32 * d + 8 * (i >> 2) + 4 * lh + (i & 3)] = o[d][i] * inv;
     return;
   }
-  const size_t column = (size_t)h * n_cols + col;
-  const size_t at = (size_t)slot * a.n_heads * n_cols + column;
-  float* dst = a.part + at * kD;
+  float* dst = a.part + split * a.slot_floats + ((size_t)h * ((n_cols + 31) / 32) + col / 32) * (32 * kD) + 4 * lane;
 #pragma unroll
-  for (int d = 0; d < 4; ++d)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const f32x4 v = {o[d][4 * g] * kDown, o[d][4 * g + 1] * kDown, o[d][4 * g + 2] * kDown, o[d][4 * g + 3] * kDown};
-      *reinterpret_cast<f32x4*>(dst + 32 * d + 8 * g + 4 * lh) = v;
-    }
+  for (int i = 0; i < 16; ++i) {  // dims 8 i + 4 lh .. + 3
+    const f32x4 v = {o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1], o[i >> 2][4 * (i & 3) + 2],
+                     o[i >> 2][4 * (i & 3) + 3]};
+    *reinterpret_cast<f32x4*>(dst + 256 * i) = v;
+  }
   if (lh == 0) {
-    a.ml[2 * at] = m_run;
-    a.ml[2 * at + 1] = l_run;
+    float* ml = a.ml + 2 * (((size_t)split * a.n_heads + h) * n_cols + col);
+    ml[0] = m_run;
+    ml[1] = l_run;
   }
 }
 
@@ -872,7 +907,7 @@ __device__ __forceinline__ bool device_positions(const uint32_t* d_pos, int plan
 
 // A tail item by the four waves `wv` counts: sequence, column block of 16,
 // split (b past them: none, the waves only keep the barriers).
-template <typename T>
+template <typename T, bool AHEAD>
 __device__ void tail_item(const RowsArgs& a, const TailLens& lens, int b, int wv, char* lds) {
   const int split = b % a.t_splits;
   b /= a.t_splits;
@@ -885,7 +920,9 @@ __device__ void tail_item(const RowsArgs& a, const TailLens& lens, int b, int wv
   w.v += (size_t)seq * w.layer_bytes;
   w.ks += (size_t)seq * w.layer_scales;
   w.vs += (size_t)seq * w.layer_scales;
-  run_narrow<T, 1>(a, w, h, cb * 16, a.group, seq, t_begin, min(len, t_begin + a.t_split_len), a.n_splits + split, wv,
+  run_narrow<T, 1, AHEAD>(a, w, h, cb * 16, a.group, seq, t_begin, min(len, t_begin + a.t_split_len),
+                   a.part + a.t_base + split * a.t_slot_floats + ((size_t)seq * a.n_heads + h) * a.t_cb * (16 * kD),
+                   a.ml + 2 * (((size_t)(a.n_splits + split) * a.n_heads + h) * a.rows + seq) * a.group, wv,
                    t_begin < len, lds);
 }
 
@@ -912,9 +949,12 @@ __global__ __launch_bounds__(256) void rows_narrow_kernel(RowsArgs a, std::condi
     if (!main_item(a, b, h, split, cb)) return;
     const long t_begin = (long)split * a.split_len, t_end = min((long)positions, t_begin + a.split_len);
     if (t_begin >= t_end) return;
-    run_narrow<T, NB>(a, a.main, h, cb * 16 * NB, a.rows * a.group, 0, t_begin, t_end, split, wv, true, lds);
+    const int n_cols = a.rows * a.group;
+    run_narrow<T, NB, !Lo<T>::value>(a, a.main, h, cb * 16 * NB, n_cols, 0, t_begin, t_end,
+                      a.part + split * a.slot_floats + (size_t)h * ((n_cols + 15) / 16) * (16 * kD),
+                      a.ml + 2 * ((size_t)split * a.n_heads + h) * n_cols, wv, true, lds);
   } else if constexpr (TAILS) {
-    tail_item<T>(a, lens, b - a.main_items, wv, lds);
+    tail_item<T, !Lo<T>::value>(a, lens, b - a.main_items, wv, lds);
   }
 }
 
@@ -939,40 +979,98 @@ __global__ __launch_bounds__(512) void rows_wide_kernel(RowsArgs a, std::conditi
     run_wide<T, WC, HL>(a, a.main, h, col0, n_cols, t_begin, t_end, a.causal != 0, split, lds);
   } else if constexpr (TAILS) {  // two items, four waves each
     const int half = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8);
-    tail_item<T>(a, lens, 2 * (b - a.main_items) + half, __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6) & 3),
+    tail_item<T, std::is_same<T, Q8>::value>(a, lens, 2 * (b - a.main_items) + half, __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6) & 3),
                  lds + half * narrow_lds(1));
   }
 }
 
-// Folds a column's partials: 32 lanes a column, 4 dims each, slots in order.
-template <bool TAILS>
-__global__ __launch_bounds__(256) void rows_merge_kernel(RowsArgs a, std::conditional_t<TAILS, TailLens, NoLens> lens) {
+// Folds the columns' partials, slots in an order that depends on their number
+// alone. A wave has 16 bytes (i = 0..15) of a block of 32 columns, lane (column,
+// half) dims 8 i + 4 half .. + 3; G waves share the slots of one, four loads in
+// flight each, and meet in LDS.
+template <int G, bool TAILS>
+__global__ __launch_bounds__(64 * (G < 4 ? 4 : G)) void rows_merge_kernel(
+    RowsArgs a, int narrow, std::conditional_t<TAILS, TailLens, NoLens> lens) {
+  constexpr int W = G < 4 ? 4 : G;
+  __shared__ f32x4 sm_o[G > 1 ? W : 1][64];
+  __shared__ float sm_m[G > 1 ? W : 1][64], sm_l[G > 1 ? W : 1][64];
   int positions = a.positions;
   if (!device_positions(a.d_pos, a.positions, positions)) return;
-  const int n = a.n_heads * a.rows * a.group;
-  const int column = blockIdx.x * 8 + (threadIdx.x >> 5), l = threadIdx.x & 31;
-  if (column >= n) return;
-  const int h = column / (a.rows * a.group), c = column % (a.rows * a.group), row = c / a.group;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int lc = lane & 31, lh = lane >> 5;
+  const int n_cols = a.rows * a.group, blocks = (n_cols + 31) / 32;
+  const int item = (int)blockIdx.x * (W / G) + wave / G, sub = wave % G;
+  const int i = item % 16, block = item / 16 % blocks, h = item / 16 / blocks;
+  const int col = 32 * block + lc;
+  const bool live = h < a.n_heads && col < n_cols;
+  if (G == 1 && !live) return;
+  const int c = live ? col : 0, hh = live ? h : 0, row = c / a.group;
   long limit = positions;
   if (a.causal) limit = min(limit, (long)a.start + row + 1);
   const int n_main = (int)((limit + a.split_len - 1) / a.split_len);
   int n_all = n_main;
-  if constexpr (TAILS) n_all += (int)((lens.len[row] + a.t_split_len - 1) / a.t_split_len);
+  const float* part = a.part + (narrow ? ((size_t)hh * ((n_cols + 15) / 16) + c / 16) * (16 * kD) +
+                                             256 * (2 * (i & 3) + lh) + 4 * ((c & 15) + 16 * (i >> 2))
+                                       : ((size_t)hh * blocks + block) * (32 * kD) + 256 * i + 4 * lane);
+  const float* ml = a.ml + 2 * ((size_t)hh * n_cols + c);
+  const size_t ml_slot = 2 * (size_t)a.n_heads * n_cols;
+  const float* tail = nullptr;
+  if constexpr (TAILS) {
+    n_all += (int)((lens.len[row] + a.t_split_len - 1) / a.t_split_len);
+    const int g = c % a.group;  // its block of 16, and dims 8 i + 4 lh = 32 lk + 4 j
+    tail = a.part + a.t_base + (((size_t)row * a.n_heads + hh) * a.t_cb + g / 16) * (16 * kD) +
+           256 * (2 * (i & 3) + lh) + 4 * ((g & 15) + 16 * (i >> 2));
+  }
   float M = -INFINITY, L = 0.f;
   f32x4 O = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < n_all; ++i) {
-    const int slot = i < n_main ? i : a.n_splits + i - n_main;
-    const size_t at = (size_t)slot * n + column;
-    const float m = a.ml[2 * at], s = a.ml[2 * at + 1];
-    const f32x4 v = *reinterpret_cast<const f32x4*>(a.part + at * kD + 4 * l);
-    const float mn = fmaxf(M, m), ms = mn == -INFINITY ? 0.f : mn;
-    const float f1 = __builtin_amdgcn_exp2f(M - ms), f2 = __builtin_amdgcn_exp2f(m - ms);
+  for (int k0 = sub; k0 < n_all; k0 += 4 * G) {
+    float m[4], s[4];
+    f32x4 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int j = min(k0 + k * G, n_all - 1);
+      const bool is_tail = TAILS && j >= n_main;
+      const float* p = is_tail ? tail + (j - n_main) * a.t_slot_floats : part + j * a.slot_floats;
+      const float* q = ml + (size_t)(is_tail ? a.n_splits + j - n_main : j) * ml_slot;
+      m[k] = q[0];
+      s[k] = q[1];
+      v[k] = *reinterpret_cast<const f32x4*>(p);
+    }
+    float mn = M;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k0 + k * G < n_all) mn = fmaxf(mn, m[k]);
+    const float ms = mn == -INFINITY ? 0.f : mn;
+    const float f = __builtin_amdgcn_exp2f(M - ms);
     M = mn;
-    L = L * f1 + s * f2;
-    O = O * f1 + v * f2;
+    L *= f;
+    O *= f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (k0 + k * G < n_all) {
+        const float e = __builtin_amdgcn_exp2f(m[k] - ms);
+        L += s[k] * e;
+        O += v[k] * e;
+      }
   }
+  if constexpr (G > 1) {
+    sm_o[wave][lane] = O;
+    sm_m[wave][lane] = M;
+    sm_l[wave][lane] = L;
+    __syncthreads();
+    if (sub != 0) return;
+#pragma unroll
+    for (int k = 1; k < G; ++k) {
+      const float m2 = sm_m[wave + k][lane], mn = fmaxf(M, m2), ms = mn == -INFINITY ? 0.f : mn;
+      const float f1 = __builtin_amdgcn_exp2f(M - ms), f2 = __builtin_amdgcn_exp2f(m2 - ms);
+      M = mn;
+      L = L * f1 + sm_l[wave + k][lane] * f2;
+      O = O * f1 + sm_o[wave + k][lane] * f2;
+    }
+  }
+  if (!live) return;
   const f32x4 r = O / L;
-  float* dst = a.out + ((size_t)row * a.n_heads * a.group + (size_t)h * a.group + c % a.group) * kD + 4 * l;
+  float* dst = a.out + ((size_t)row * a.n_heads * a.group + (size_t)h * a.group + c % a.group) * kD + 8 * i + 4 * lh;
 #pragma unroll
   for (int e = 0; e < 4; ++e) dst[e] = r[e];  // out may be only 4-byte aligned
 }
@@ -1104,10 +1202,30 @@ RowsPlan plan_rows(const RowsCall& c, const rv_kv* owner) {
   return p;
 }
 
+// Floats of one main slot's and one tail slot's partials (whole blocks of
+// columns), for `n` rows.
+size_t main_floats(const RowsPlan& p, size_t n, size_t group, size_t heads) {
+  const size_t b = p.nb ? 16 : 32;
+  return heads * ((n * group + b - 1) / b) * b * kD;
+}
+size_t tail_floats(const RowsPlan& p, size_t n, size_t heads) { return n * heads * p.t_cb * 16 * kD; }
+
 size_t plan_floats(const RowsPlan& p, const RowsCall& c) {
+  if (p.generic || p.slots() <= 1) return 0;
   const rv_kv* g = c.main ? c.main : c.tails;
-  const size_t cols = p.rows * (c.n_q_heads / g->n_kv_heads) * (c.kv_hi - c.kv_lo);
-  return p.generic || p.slots() <= 1 ? 0 : p.slots() * cols * (kD + 2);
+  const size_t group = c.n_q_heads / g->n_kv_heads, heads = c.kv_hi - c.kv_lo;
+  return p.n_splits * main_floats(p, p.rows, group, heads) + p.t_splits * tail_floats(p, p.rows, heads) +
+         2 * p.slots() * p.rows * group * heads;
+}
+
+template <int G>
+void launch_merge_g(const RowsArgs& a, int items, bool narrow, const TailLens* lens, hipStream_t s) {
+  constexpr int W = G < 4 ? 4 : G;
+  const dim3 grid((unsigned)((items + W / G - 1) / (W / G))), block(64 * W);
+  if (lens)
+    hipLaunchKernelGGL((rows_merge_kernel<G, true>), grid, block, 0, s, a, (int)narrow, *lens);
+  else
+    hipLaunchKernelGGL((rows_merge_kernel<G, false>), grid, block, 0, s, a, (int)narrow, NoLens{});
 }
 
 template <typename T, bool HL, bool TAILS, typename L>
@@ -1197,9 +1315,11 @@ HipStatus launch_rows(rv_kv* owner, const RowsCall& c, hipStream_t s, const Work
       }
 #undef RV_GENERIC
     } else {
-      const size_t cols = n * group * a.n_heads;
       a.part = base;
-      a.ml = base ? base + p.slots() * cols * kD : nullptr;
+      a.slot_floats = main_floats(p, n, group, a.n_heads);
+      a.t_base = p.n_splits * a.slot_floats;
+      a.t_slot_floats = tail_floats(p, n, a.n_heads);
+      a.ml = base ? base + a.t_base + p.t_splits * a.t_slot_floats : nullptr;
       a.n_cb = (int)((n * group + p.columns() - 1) / p.columns());
       a.n_splits = p.n_splits;
       a.split_len = p.split_len;
@@ -1223,11 +1343,14 @@ HipStatus launch_rows(rv_kv* owner, const RowsCall& c, hipStream_t s, const Work
         launch_plan<Q8, false, false>(p, tp, a, 0, s, NoLens{});
       }
       if (!a.single) {
-        const dim3 grid((unsigned)((cols + 7) / 8)), block(256);
-        if (c.tails)
-          hipLaunchKernelGGL(rows_merge_kernel<true>, grid, block, 0, s, a, lens);
+        const int merges = 16 * a.n_heads * (int)((n * group + 31) / 32);
+        const TailLens* tl = c.tails ? &lens : nullptr;
+        if (p.slots() <= 4)
+          launch_merge_g<1>(a, merges, p.nb != 0, tl, s);
+        else if (p.slots() <= 32)
+          launch_merge_g<4>(a, merges, p.nb != 0, tl, s);
         else
-          hipLaunchKernelGGL(rows_merge_kernel<false>, grid, block, 0, s, a, NoLens{});
+          launch_merge_g<16>(a, merges, p.nb != 0, tl, s);
       }
     }
     st.e = hipGetLastError();
