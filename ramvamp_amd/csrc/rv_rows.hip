@@ -19,6 +19,8 @@
 namespace rv {
 namespace {
 
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // as a caller's rows may be
+
 constexpr int kD = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 // The running maximum moves when a score passes it by more than kSlack, and
@@ -335,7 +337,6 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
       const int cc = live ? col : n_cols - 1;
       const float* qp =
           a.q + ((size_t)(row0 + cc / a.group) * a.n_q_heads + (size_t)hk * a.group + cc % a.group) * kD + 32 * lk;
-      typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
       float x[32];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -736,10 +737,11 @@ __device__ void run_wide(const RowsArgs& a, const KvView& w, int h, int col0, in
   {  // dims 16 c + 8 lh .. + 7 of each chunk c
     const float* qp = a.q + ((size_t)crow * a.n_q_heads + (size_t)hk * a.group + chead) * kD;
     float x[64];
+    f32x4 v[16];
 #pragma unroll
-    for (int c = 0; c < 8; ++c)
+    for (int i = 0; i < 16; ++i) v[i] = *reinterpret_cast<const f32x4u*>(qp + 16 * (i >> 1) + 8 * lh + 4 * (i & 1));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[8 * c + e] = live ? qp[16 * c + 8 * lh + e] * a.qscale : 0.f;
+    for (int i = 0; i < 64; ++i) x[i] = live ? v[i >> 2][i & 3] * a.qscale : 0.f;
     q_up = split_q<64, false, HL>(x, qh, ql);
   }
   if constexpr (Q) {
