@@ -751,6 +751,7 @@ __device__ void run_wide(const RowsArgs& a, const KvView& w, int h, int col0, in
   store_share<T, S>(sh, lds, t_begin, last, is_v, tt, Q ? nan_rows[0] : nullptr);
   __syncthreads();
 
+  if (wave >= 4) __builtin_amdgcn_s_setprio(1);
   f32x16 o[4];
 #pragma unroll
   for (int d = 0; d < 4; ++d) o[d] = f32x16{};
