@@ -121,7 +121,7 @@ struct Raw<float> {
 };
 
 template <typename T>
-__device__ __forceinline__ void load_raw(Raw<T>& x, const KvView& w, int h, long p0, long last, int li, int lk) {
+__device__ __forceinline__ void load_raw_k(Raw<T>& x, const KvView& w, int h, long p0, long last, int li, int lk) {
   if constexpr (std::is_same<T, Q8>::value) {
     const char* kb = w.k + ((size_t)h * w.rows + p0) * kD;
     const uint16_t* sb = w.ks + ((size_t)h * w.rows + p0) * 4;
@@ -132,6 +132,22 @@ __device__ __forceinline__ void load_raw(Raw<T>& x, const KvView& w, int h, long
       x.k[a][1] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(kb + r * kD + 32 * lk + 16));
       x.ks[a] = sb[4 * r + lk];
     }
+  } else {
+    const T* kb = reinterpret_cast<const T*>(w.k) + (size_t)h * kD + 32 * lk;
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const T* r = kb + (size_t)min(p0 + 16 * a + li, last) * w.kv_dim;
+      constexpr int n = std::is_same<T, float>::value ? 8 : 4;
+#pragma unroll
+      for (int c = 0; c < n; ++c)
+        x.k[a][c] = *reinterpret_cast<const std::remove_reference_t<decltype(x.k[0][0])>*>(r + 16 / sizeof(T) * c);
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_raw_v(Raw<T>& x, const KvView& w, int h, long p0, long last, int li, int lk) {
+  if constexpr (std::is_same<T, Q8>::value) {
     const char* vb = w.v + ((size_t)h * w.rows + p0) * kD + 8 * li;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -141,16 +157,7 @@ __device__ __forceinline__ void load_raw(Raw<T>& x, const KvView& w, int h, long
     x.vs[0] = *reinterpret_cast<const u32x2*>(vs);
     x.vs[1] = *reinterpret_cast<const u32x2*>(vs + 16);
   } else {
-    const T* kb = reinterpret_cast<const T*>(w.k) + (size_t)h * kD + 32 * lk;
     const T* vb = reinterpret_cast<const T*>(w.v) + (size_t)h * kD + 8 * li;
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      const T* r = kb + (size_t)min(p0 + 16 * a + li, last) * w.kv_dim;
-      constexpr int n = std::is_same<T, float>::value ? 8 : 4;
-#pragma unroll
-      for (int c = 0; c < n; ++c)
-        x.k[a][c] = *reinterpret_cast<const std::remove_reference_t<decltype(x.k[0][0])>*>(r + 16 / sizeof(T) * c);
-    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const T* r = vb + (size_t)min(p0 + 16 * (i >> 2) + 4 * lk + (i & 3), last) * w.kv_dim;
@@ -303,12 +310,10 @@ __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
 // by the four waves `w0` .. + 3 of the workgroup (wave wv of them takes tiles
 // wv, wv + 4, ...). All waves of the workgroup call it together; `run` false:
 // nothing to do but the barriers. No causal limit. `part` and `ml` are those of
-// the item's slot, kv head and (a tail's) sequence. AHEAD: a wave's next tile
-// loads while it computes one, where the registers hold two (an f32 tile is 128
-// of them).
+// the item's slot, kv head and (a tail's) sequence.
 constexpr int narrow_lds(int nb) { return 3 * nb * 34 * 64 * 4; }
 
-template <typename T, int NB, bool AHEAD>
+template <typename T, int NB>
 __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, int n_cols, int row0, long t_begin,
                            long t_end, float* part, float* ml, int wv, bool run, char* lds) {
   constexpr bool LO = Lo<T>::value;
@@ -327,8 +332,12 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
   }
   const int n_tiles = run ? (int)((t_end - t_begin + 31) >> 5) : 0;
   if (wv < n_tiles) {
-    Raw<T> ra;
-    load_raw<T>(ra, w, hk, t_begin + 32L * wv, last, li, lk);
+    // A wave's loads run ahead of its products: K of the next tile is loaded into
+    // the registers that this one's scores have read, V into those that its
+    // output has.
+    Raw<T> x;
+    load_raw_k<T>(x, w, hk, t_begin + 32L * wv, last, li, lk);
+    load_raw_v<T>(x, w, hk, t_begin + 32L * wv, last, li, lk);
     f16x8 qh[NB][4], ql[NB][4];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
@@ -346,7 +355,8 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
       }
       q_up[n] = split_q<32, true, true>(x, qh[n], ql[n]);
     }
-    auto compute = [&](Raw<T>& x, long p0) {
+    for (int tile = wv; tile < n_tiles; tile += 4) {
+      const long p0 = t_begin + 32L * tile;
       const bool edge = p0 + 32 > t_end;
       f32x4 s[NB][2][2];
 #pragma unroll
@@ -366,6 +376,7 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
             if constexpr (LO) s[n][t][1] = mfma16(kl, qh[n][c], s[n][t][1]);
           }
         }
+      if (tile + 4 < n_tiles) load_raw_k<T>(x, w, hk, p0 + 128, last, li, lk);
       f16x8 ph[NB], pl[NB];
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
@@ -413,22 +424,7 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
           }
         }
       }
-    };
-    if constexpr (!AHEAD) {
-      for (int t = wv; t < n_tiles; t += 4) {
-        if (t != wv) load_raw<T>(ra, w, hk, t_begin + 32L * t, last, li, lk);
-        compute(ra, t_begin + 32L * t);
-      }
-    } else {
-      Raw<T> rb;
-      for (int t = wv; t < n_tiles; t += 8) {
-        const bool more = t + 4 < n_tiles;
-        if (more) load_raw<T>(rb, w, hk, t_begin + 32L * (t + 4), last, li, lk);
-        compute(ra, t_begin + 32L * t);
-        if (!more) break;
-        if (t + 8 < n_tiles) load_raw<T>(ra, w, hk, t_begin + 32L * (t + 8), last, li, lk);
-        compute(rb, t_begin + 32L * (t + 4));
-      }
+      if (tile + 4 < n_tiles) load_raw_v<T>(x, w, hk, p0 + 128, last, li, lk);
     }
   }
   // Each lane summed its own rows: the other quarters of the column's.
@@ -910,7 +906,7 @@ __device__ __forceinline__ bool device_positions(const uint32_t* d_pos, int plan
 
 // A tail item by the four waves `wv` counts: sequence, column block of 16,
 // split (b past them: none, the waves only keep the barriers).
-template <typename T, bool AHEAD>
+template <typename T>
 __device__ void tail_item(const RowsArgs& a, const TailLens& lens, int b, int wv, char* lds) {
   const int split = b % a.t_splits;
   b /= a.t_splits;
@@ -923,7 +919,7 @@ __device__ void tail_item(const RowsArgs& a, const TailLens& lens, int b, int wv
   w.v += (size_t)seq * w.layer_bytes;
   w.ks += (size_t)seq * w.layer_scales;
   w.vs += (size_t)seq * w.layer_scales;
-  run_narrow<T, 1, AHEAD>(a, w, h, cb * 16, a.group, seq, t_begin, min(len, t_begin + a.t_split_len),
+  run_narrow<T, 1>(a, w, h, cb * 16, a.group, seq, t_begin, min(len, t_begin + a.t_split_len),
                    a.part + a.t_base + split * a.t_slot_floats + ((size_t)seq * a.n_heads + h) * a.t_cb * (16 * kD),
                    a.ml + 2 * (((size_t)(a.n_splits + split) * a.n_heads + h) * a.rows + seq) * a.group, wv,
                    t_begin < len, lds);
@@ -953,11 +949,11 @@ __global__ __launch_bounds__(256) void rows_narrow_kernel(RowsArgs a, std::condi
     const long t_begin = (long)split * a.split_len, t_end = min((long)positions, t_begin + a.split_len);
     if (t_begin >= t_end) return;
     const int n_cols = a.rows * a.group;
-    run_narrow<T, NB, !Lo<T>::value>(a, a.main, h, cb * 16 * NB, n_cols, 0, t_begin, t_end,
+    run_narrow<T, NB>(a, a.main, h, cb * 16 * NB, n_cols, 0, t_begin, t_end,
                       a.part + split * a.slot_floats + (size_t)h * ((n_cols + 15) / 16) * (16 * kD),
                       a.ml + 2 * ((size_t)split * a.n_heads + h) * n_cols, wv, true, lds);
   } else if constexpr (TAILS) {
-    tail_item<T, !Lo<T>::value>(a, lens, b - a.main_items, wv, lds);
+    tail_item<T>(a, lens, b - a.main_items, wv, lds);
   }
 }
 
@@ -982,7 +978,7 @@ __global__ __launch_bounds__(512) void rows_wide_kernel(RowsArgs a, std::conditi
     run_wide<T, WC, HL>(a, a.main, h, col0, n_cols, t_begin, t_end, a.causal != 0, split, lds);
   } else if constexpr (TAILS) {  // two items, four waves each
     const int half = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8);
-    tail_item<T, std::is_same<T, Q8>::value>(a, lens, 2 * (b - a.main_items) + half, __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6) & 3),
+    tail_item<T>(a, lens, 2 * (b - a.main_items) + half, __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6) & 3),
                  lds + half * narrow_lds(1));
   }
 }
@@ -1175,6 +1171,62 @@ void split_positions(long positions, long units, long want, int* n_splits, int* 
   *n_splits = (int)((steps + per - 1) / per);
 }
 
+// A wide launch's shape: how many columns an item has, and into how many splits
+// it and the tails are cut, by the time each choice would take. The times (us)
+// are fitted on this card over chunks of 77..1000 rows and batches of 7..64
+// sequences at 900 .. 16000 positions; what counts is that they rank the choices
+// as those measure (77 rows at 901: 2, 4, 8 waves of columns 21.7, 22.7, 24.1; 512
+// at 3449: 4, 8 waves 85.8, 81; 64 x 16000 f16 in 16, 21, 25, 32 splits 64.7, 54.7,
+// 67, 70). An item takes 14 to start, load its queries and store, and `c` per 128
+// positions (one workgroup a CU); a tail's four waves 10 and 2 per 128; a
+// partial's floats are written and read once.
+void plan_wide(RowsPlan& p, long positions, long cols, long heads, int elem, long tails, long longest) {
+  const long steps = (positions + kPosStep - 1) / kPosStep;
+  double best = 1e300;
+  for (long t_want : {kCUs / 2, kCUs, 2 * kCUs}) {
+    int t_splits = 0, t_len = kPosStep;
+    long t_wgs = 0;
+    double t_tail = 1;  // (none)
+    if (tails && longest) {
+      split_positions(longest, tails, t_want, &t_splits, &t_len);
+      t_wgs = (tails * t_splits + 1) / 2;
+      t_tail = 10 + 2.0 * (t_len / kPosStep);
+    } else if (t_want != kCUs) {
+      continue;
+    }
+    for (int wc : {2, 4, 8}) {
+      if (wc == 2 && elem == RV_ELEM_F32) continue;  // (its LDS tiles are twice as large)
+      const double c = elem == RV_ELEM_F32 ? (wc == 4 ? 5.5 : 9.0)
+                       : elem == RV_ELEM_F16 ? (wc == 2 ? 2.4 : wc == 4 ? 3.05 : 5.0)
+                                             : (wc == 2 ? 2.7 : wc == 4 ? 3.5 : 5.9);
+      const long units = heads * ((cols + 32 * wc - 1) / (32 * wc));
+      long n = 1;
+      for (long prev = 0; n <= steps; n = n == steps ? n + 1 : std::min(steps, n < 4 ? n + 1 : n * 5 / 4 + 1)) {
+        const long per = (steps + n - 1) / n, splits = (steps + per - 1) / per;
+        if (splits == prev) continue;
+        prev = splits;
+        const long items = units * splits;
+        if (items > 4 * kCUs && n > 1) break;
+        const double t = 14 + c * per;
+        // CUs the tails take meanwhile, one after the other on each.
+        const long in_a_row = std::max(1L, (long)(t / t_tail)), t_cus = (t_wgs + in_a_row - 1) / in_a_row;
+        const long rounds = items + t_cus <= kCUs ? 1 : (long)((items * t + t_wgs * t_tail) / (kCUs * t)) + 1;
+        const long slots = splits + t_splits;
+        double total = std::max(t * rounds, t_tail);
+        if (slots > 1) total += 3 + slots * cols * heads * (kD + 2) * 8 / 6.0e6;
+        if (total < best) {
+          best = total;
+          p.wc = wc;
+          p.n_splits = (int)splits;
+          p.split_len = (int)(per * kPosStep);
+          p.t_splits = t_splits;
+          p.t_split_len = t_len;
+        }
+      }
+    }
+  }
+}
+
 RowsPlan plan_rows(const RowsCall& c, const rv_kv* owner) {
   RowsPlan p;
   const rv_kv* g = c.main ? c.main : c.tails;
@@ -1183,25 +1235,30 @@ RowsPlan plan_rows(const RowsCall& c, const rv_kv* owner) {
   if (p.generic) return p;
   const long group = (long)(c.n_q_heads / g->n_kv_heads), heads = (long)(c.kv_hi - c.kv_lo);
   const long cols = (long)p.rows * group;
-  const bool causal = c.causal && c.rows > 1;
-  if (cols <= 32 && !causal && c.split)
-    p.nb = cols <= 16 ? 1 : 2;
-  else
-    p.wc = cols <= 64 && g->elem != RV_ELEM_F32 ? 2 : cols <= 128 ? 4 : 8;
-  if (c.main && c.positions) {
-    p.n_cb = (int)((cols + p.columns() - 1) / p.columns());
-    split_positions((long)c.positions, heads * p.n_cb, p.nb ? 2 * kCUs : kCUs, &p.n_splits, &p.split_len);
-    if (owner->tune_decode_split_len > 0) {
-      p.split_len = (int)((std::min<int64_t>(owner->tune_decode_split_len, 1 << 30) + kPosStep - 1) / kPosStep * kPosStep);
-      p.n_splits = (int)((c.positions + p.split_len - 1) / p.split_len);
-    }
-  }
+  const long positions = c.main ? (long)c.positions : 0;
+  long longest = 0;
   if (c.tails) {
-    size_t longest = 0;
-    for (size_t i = 0; i < c.rows; ++i) longest = std::max(longest, c.tails->lens[c.tail_layer + i]);
     p.t_cb = (int)((group + 15) / 16);
-    if (longest) split_positions((long)longest, heads * p.t_cb * (long)p.rows, 2 * kCUs, &p.t_splits, &p.t_split_len);
+    for (size_t i = 0; i < c.rows; ++i) longest = std::max(longest, (long)c.tails->lens[c.tail_layer + i]);
   }
+  const long tails = heads * p.t_cb * (long)p.rows;
+  // Few columns: one or two 16-column blocks in registers, unless rows see
+  // different lengths or the operands are single (neither is a decode).
+  if (cols <= 32 && !(c.causal && c.rows > 1) && c.split) {
+    p.nb = cols <= 16 ? 1 : 2;
+    if (positions) split_positions(positions, heads, 2 * kCUs, &p.n_splits, &p.split_len);
+    if (longest) split_positions(longest, tails, 2 * kCUs, &p.t_splits, &p.t_split_len);
+  } else if (positions) {
+    plan_wide(p, positions, cols, heads, g->elem, tails, longest);
+  } else {  // tails alone
+    p.nb = 1;
+    if (longest) split_positions(longest, tails, 2 * kCUs, &p.t_splits, &p.t_split_len);
+  }
+  if (positions && owner->tune_decode_split_len > 0) {
+    p.split_len = (int)((std::min<int64_t>(owner->tune_decode_split_len, 1 << 30) + kPosStep - 1) / kPosStep * kPosStep);
+    p.n_splits = (int)((positions + p.split_len - 1) / p.split_len);
+  }
+  if (p.columns()) p.n_cb = (int)((cols + p.columns() - 1) / p.columns());
   return p;
 }
 
