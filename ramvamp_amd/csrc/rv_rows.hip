@@ -27,6 +27,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // probabilities carry a factor of 2^kUp (it cancels in o / l): they stay at or
 // below 2^14, inside f16, and small ones are kept off its subnormals.
 constexpr float kSlack = 8.f, kUp = 6.f;
+constexpr int kFold = 16;  // splits of a kv head that the launch folds itself
 
 struct NoLens {};
 struct TailLens {
@@ -43,6 +44,7 @@ struct RowsArgs {
   // lanes]. ml: maximum and sum by [slot][column].
   float* part;
   float* ml;
+  unsigned* tickets;      // narrow main items fold in the launch: one per kv head, 128 bytes apart
   size_t slot_floats;     // of part, from one main slot to the next
   size_t t_base, t_slot_floats;  // of part: the first tail slot, from one to the next
   const uint32_t* d_pos;  // positions from device memory
@@ -306,58 +308,83 @@ __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Columns [col0, col0 + 16 NB) of kv head h over rows [t_begin, t_end) of `w`,
-// by the four waves `w0` .. + 3 of the workgroup (wave wv of them takes tiles
-// wv, wv + 4, ...). All waves of the workgroup call it together; `run` false:
-// nothing to do but the barriers. No causal limit. `part` and `ml` are those of
-// the item's slot, kv head and (a tail's) sequence.
-constexpr int narrow_lds(int nb) { return 3 * nb * 34 * 64 * 4; }
+// Where an item's partials go, and how they are folded.
+struct PartDst {
+  float* part;  // of the item's slot, kv head and (a tail's) sequence
+  float* ml;
+  // Folded by the last of the unit's `n` items to finish (ticket != null):
+  // `part` and `ml` are then the first slot's, this item's `slot`.
+  unsigned* ticket = nullptr;
+  int n = 0, slot = 0;
+  size_t slot_floats = 0, ml_slot = 0;
+};
 
-template <typename T, int NB>
+// A store and a load that another XCD's L2 sees: the store goes through this
+// one's, the load past it.
+constexpr int kDeviceScope = 16;  // the sc1 bit of a buffer instruction's cache policy
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t device_rsrc(const float* base) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), (short)0, 0x7FFFFFFF, 0x00020000);
+}
+
+constexpr int kRegB = 34 * 64 * 4;  // a wave's block: 32 output values, maximum and sum by lane
+constexpr int NW = 4;
+constexpr int narrow_lds(int nb) { return NW * nb * kRegB; }
+
+// Columns [col0, col0 + 16 NB) of kv head h over rows [t_begin, t_end) of `w`,
+// by four waves of the workgroup (wave wv of them takes tiles wv, wv + 4, ...).
+// All waves of the workgroup call it together; `run` false: nothing to do but
+// the barriers. causal: column c sees start + row + 1 rows.
+template <typename T, int NB, bool CAUSAL>
 __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, int n_cols, int row0, long t_begin,
-                           long t_end, float* part, float* ml, int wv, bool run, char* lds) {
-  constexpr bool LO = Lo<T>::value;
+                           long t_end, const PartDst& to, int wv, bool run, char* lds) {
+  constexpr bool LO = Lo<T>::value, Q = std::is_same<T, Q8>::value;
   const int lane = threadIdx.x & 63, li = lane & 15, lk = lane >> 4;
   const int hk = a.kv_lo + h;
   const long last = t_end - 1;
-  float q_up[NB], m_run[NB], m_sub[NB], l_run[NB];
+  float m_run[NB], l_run[NB];
+  uint32_t taint = 0;  // bit n: column block n saw a NaN row of this lane's dims (Q8_0, causal)
   f32x4 o[NB][8];
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     m_run[n] = -INFINITY;
-    m_sub[n] = 0.f;
     l_run[n] = 0.f;
 #pragma unroll
     for (int b = 0; b < 8; ++b) o[n][b] = f32x4{};
   }
   const int n_tiles = run ? (int)((t_end - t_begin + 31) >> 5) : 0;
   if (wv < n_tiles) {
+    float q_up[NB], m_sub[NB];
+    long limit[NB];
+    f32x4 qv[NB][8];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      m_sub[n] = 0.f;
+      const int cc = min(col0 + 16 * n + li, n_cols - 1);
+      const int r = a.rows == 1 ? 0 : row0 + cc / a.group;
+      limit[n] = CAUSAL ? min((long)a.start + r + 1, t_end) : t_end;
+      const float* qp = a.q + ((size_t)r * a.n_q_heads + (size_t)hk * a.group + (cc - (r - row0) * a.group)) * kD + 32 * lk;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) qv[n][i] = *reinterpret_cast<const f32x4u*>(qp + 4 * i);
+    }
     // A wave's loads run ahead of its products: K of the next tile is loaded into
     // the registers that this one's scores have read, V into those that its
     // output has.
     Raw<T> x;
     load_raw_k<T>(x, w, hk, t_begin + 32L * wv, last, li, lk);
     load_raw_v<T>(x, w, hk, t_begin + 32L * wv, last, li, lk);
+    // What every column sees at least.
+    const long w_first = CAUSAL ? min((long)a.start + row0 + min(col0, n_cols - 1) / a.group + 1, t_end) : t_end;
     f16x8 qh[NB][4], ql[NB][4];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-      const int col = col0 + 16 * n + li;
-      const bool live = col < n_cols;
-      const int cc = live ? col : n_cols - 1;
-      const float* qp =
-          a.q + ((size_t)(row0 + cc / a.group) * a.n_q_heads + (size_t)hk * a.group + cc % a.group) * kD + 32 * lk;
-      float x[32];
+      const bool live = col0 + 16 * n + li < n_cols;
+      float y[32];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const f32x4 v = *reinterpret_cast<const f32x4u*>(qp + 4 * i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[4 * i + e] = live ? v[e] * a.qscale : 0.f;
-      }
-      q_up[n] = split_q<32, true, true>(x, qh[n], ql[n]);
+      for (int i = 0; i < 32; ++i) y[i] = live ? qv[n][i >> 2][i & 3] * a.qscale : 0.f;
+      q_up[n] = split_q<32, true, true>(y, qh[n], ql[n]);
     }
-    for (int tile = wv; tile < n_tiles; tile += 4) {
+    for (int tile = wv; tile < n_tiles; tile += NW) {
       const long p0 = t_begin + 32L * tile;
-      const bool edge = p0 + 32 > t_end;
       f32x4 s[NB][2][2];
 #pragma unroll
       for (int n = 0; n < NB; ++n)
@@ -376,15 +403,15 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
             if constexpr (LO) s[n][t][1] = mfma16(kl, qh[n][c], s[n][t][1]);
           }
         }
-      if (tile + 4 < n_tiles) load_raw_k<T>(x, w, hk, p0 + 128, last, li, lk);
+      if (tile + NW < n_tiles) load_raw_k<T>(x, w, hk, p0 + 32 * NW, last, li, lk);
       f16x8 ph[NB], pl[NB];
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
         float y[8], mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = s[n][i >> 2][0][i & 3] + s[n][i >> 2][1][i & 3];
-        if (edge) {
-          const int seen = (int)(t_end - p0) - 4 * lk;  // of this quarter's rows 16 t + r
+        if (p0 + 32 > w_first) {
+          const int seen = (int)max(limit[n] - p0, 0L) - 4 * lk;  // of this quarter's rows 16 t + r
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             if (16 * (i >> 2) + (i & 3) >= seen) y[i] = -INFINITY;
@@ -407,7 +434,35 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
         ph[n] = h1[0];
         pl[n] = l1[0];
       }
-      if (edge) mask_v<T>(x, p0, last, lk);
+      if (p0 + 32 > t_end) mask_v<T>(x, p0, last, lk);
+      if constexpr (Q && CAUSAL) {
+        // A row's NaN scale makes its block NaN; it must not reach columns that do
+        // not see the row (0 * NaN): it goes in as zero and the columns that see it
+        // are marked. (NaN: all exponent bits set, no scale is infinite, so adding
+        // one to the exponent reaches the sign, which is clear.)
+        uint32_t bad = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bad |= (x.vs[i >> 1][i & 1] & 0x7C007C00u) + 0x04000400u;
+        if (__builtin_amdgcn_ballot_w64((bad & 0x80008000u) != 0) != 0) {
+          uint32_t rows = 0;  // of the tile, NaN in this lane's output dims (block lk)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t half = (i & 1) ? 0xFFFF0000u : 0x0000FFFFu, sw = x.vs[i >> 2][(i & 3) >> 1];
+            const bool nan = (sw & half & 0x7C007C00u) == (half & 0x7C007C00u);
+            x.vs[i >> 2][(i & 3) >> 1] = nan ? sw & ~half : sw;
+            const uint64_t who = __builtin_amdgcn_ballot_w64(nan);  // lane (4 block, quarter): its row
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (who >> (4 * lk + 16 * k) & 1) rows |= 1u << (16 * (i >> 2) + 4 * k + (i & 3));
+          }
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            const long seen = limit[n] - p0;
+            const uint32_t mask = seen >= 32 ? 0xFFFFFFFFu : seen <= 0 ? 0u : (1u << seen) - 1;
+            if (rows & mask) taint |= 1u << n;
+          }
+        }
+      }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         f16x8 vh[2], vl[2];
@@ -424,66 +479,150 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
           }
         }
       }
-      if (tile + 4 < n_tiles) load_raw_v<T>(x, w, hk, p0 + 128, last, li, lk);
+      if (tile + NW < n_tiles) load_raw_v<T>(x, w, hk, p0 + 32 * NW, last, li, lk);
     }
   }
-  // Each lane summed its own rows: the other quarters of the column's.
+  // The waves' partials meet in LDS, and each wave folds its share of the values,
+  // in wave order. A lane's 16 bytes i are dims 32 lk + 4 i .. + 3 of column li.
+  const int used = min(NW, n_tiles);
+  f32x4* om = reinterpret_cast<f32x4*>(lds);
+  float* sums = reinterpret_cast<float*>(lds + NW * NB * 32 * 64 * 4);  // [wave][NB][2][64]
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
+    // Each lane summed its own rows: the other quarters of the column's.
     l_run[n] = swap_sum<16>(l_run[n]);
     l_run[n] = swap_sum<32>(l_run[n]);
-  }
-  // The waves' partials meet in LDS, in wave order: [wave - 1][NB][34][64 lanes].
-  float* om = reinterpret_cast<float*>(lds);
-  constexpr int kBlock = 34 * 64;
-  if (wv > 0) {
+    if (Q && CAUSAL && (taint & (1u << n))) {
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      float* d = om + ((wv - 1) * NB + n) * kBlock + lane;
+      for (int b = 0; b < 8; ++b) o[n][b] *= __builtin_nanf("");
+    }
+    if (wv < used) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) d[64 * i] = o[n][i >> 2][i & 3];
-      d[64 * 32] = m_run[n];
-      d[64 * 33] = l_run[n];
+      for (int i = 0; i < 8; ++i)
+        om[((wv * NB + n) * 8 + i) * 64 + lane] = f32x4{o[n][4 * (i & 1)][i >> 1], o[n][4 * (i & 1) + 1][i >> 1],
+                                                        o[n][4 * (i & 1) + 2][i >> 1], o[n][4 * (i & 1) + 3][i >> 1]};
+      sums[((wv * NB + n) * 2) * 64 + lane] = m_run[n];
+      sums[((wv * NB + n) * 2 + 1) * 64 + lane] = l_run[n];
     }
   }
   __syncthreads();
-  if (wv > 0 || !run) return;
+  constexpr int IW = 8 / NW;  // 16-byte pieces a wave folds
+  if (run) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      float f[NW], M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int k = 0; k < NW; ++k) {
+        f[k] = k < used ? sums[((k * NB + n) * 2) * 64 + lane] : -INFINITY;
+        M = fmaxf(M, f[k]);
+      }
+      const float ms = M == -INFINITY ? 0.f : M;
+#pragma unroll
+      for (int k = 0; k < NW; ++k) {
+        f[k] = __builtin_amdgcn_exp2f(f[k] - ms);
+        if (k < used) L += f[k] * sums[((k * NB + n) * 2 + 1) * 64 + lane];
+      }
+      const int col = col0 + 16 * n + li;
+      if (col >= n_cols) continue;
+#pragma unroll
+      for (int j = 0; j < IW; ++j) {
+        const int i = wv * IW + j;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < NW; ++k)
+          if (k < used) v += om[((k * NB + n) * 8 + i) * 64 + lane] * f[k];
+        if (a.single) {
+          const int row = a.rows == 1 ? 0 : row0 + col / a.group;
+          float* dst = a.out + ((size_t)row * a.n_heads * a.group + (size_t)h * a.group + (col - (row - row0) * a.group)) * kD +
+                       32 * lk + 4 * i;
+          const f32x4 r = v / L;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dst[e] = r[e];
+        } else if (to.ticket) {
+          __builtin_amdgcn_raw_buffer_store_b128(
+              v, device_rsrc(to.part + to.slot * to.slot_floats),
+              (int)(((size_t)(col / 16) * (16 * kD) + 4 * lane + 256 * i) * sizeof(float)), 0, kDeviceScope);
+        } else {
+          *reinterpret_cast<f32x4*>(to.part + (size_t)(col / 16) * (16 * kD) + 4 * lane + 256 * i) = v;
+        }
+      }
+      if (!a.single && wv == 0 && lk == 0) {
+        if (to.ticket) {
+          const __amdgpu_buffer_rsrc_t rs = device_rsrc(to.ml + to.slot * to.ml_slot);
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(M), rs, 8 * col, 0, kDeviceScope);
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_int(L), rs, 8 * col + 4, 0, kDeviceScope);
+        } else {
+          to.ml[2 * col] = M;
+          to.ml[2 * col + 1] = L;
+        }
+      }
+    }
+  }
+  if (!to.ticket) return;  // (workgroup-uniform)
+  // The last item of the unit folds all of them, slots in order, so that the
+  // result does not depend on which one it is; it resets the ticket.
+  __shared__ unsigned drawn;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's stores are where other XCDs see them
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    drawn = __hip_atomic_fetch_add(to.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (drawn == (unsigned)to.n - 1) __hip_atomic_store(to.ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (drawn != (unsigned)to.n - 1) return;
+  const __amdgpu_buffer_rsrc_t rp = device_rsrc(to.part), rm = device_rsrc(to.ml);
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    for (int p = 1; p < min(4, n_tiles); ++p) {
-      const float* d = om + ((p - 1) * NB + n) * kBlock + lane;
-      const float m2 = d[64 * 32], l2 = d[64 * 33];
-      const float mn = fmaxf(m_run[n], m2), ms = mn == -INFINITY ? 0.f : mn;
-      const float f1 = __builtin_amdgcn_exp2f(m_run[n] - ms), f2 = __builtin_amdgcn_exp2f(m2 - ms);
-      m_run[n] = mn;
-      l_run[n] = l_run[n] * f1 + l2 * f2;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) o[n][i >> 2][i & 3] = o[n][i >> 2][i & 3] * f1 + d[64 * i] * f2;
-    }
     const int col = col0 + 16 * n + li;
     if (col >= n_cols) continue;
-    if (a.single) {
-      // This lane's dims: 32 lk + 8 r + b.
-      const int row = row0 + col / a.group, head = col % a.group;
-      const float inv = 1.f / l_run[n];
-      float* dst = a.out + ((size_t)row * a.n_heads * a.group + (size_t)h * a.group + head) * kD + 32 * lk;
+    float M = -INFINITY, L = 0.f;
+    f32x4 r[IW];
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+    for (int j = 0; j < IW; ++j) r[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    constexpr int C = 8;  // slots in flight
+    for (int k0 = 0; k0 < to.n; k0 += C) {
+      float f[C], s[C];
+      f32x4 v[IW][C];
 #pragma unroll
-        for (int b = 0; b < 8; ++b) dst[8 * r + b] = o[n][b][r] * inv;
-      continue;
-    }
-    float* dst = part + (size_t)(col / 16) * (16 * kD) + 4 * lane;
+      for (int k = 0; k < C; ++k) {
+        const int slot = min(k0 + k, to.n - 1);
+        const int mo = (int)((slot * to.ml_slot + 2 * col) * sizeof(float));
+        f[k] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(rm, mo, 0, kDeviceScope));
+        s[k] = __int_as_float(__builtin_amdgcn_raw_buffer_load_b32(rm, mo + 4, 0, kDeviceScope));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {  // dims 32 lk + 4 i .. + 3
-      const f32x4 v = {o[n][4 * (i & 1)][i >> 1], o[n][4 * (i & 1) + 1][i >> 1], o[n][4 * (i & 1) + 2][i >> 1],
-                       o[n][4 * (i & 1) + 3][i >> 1]};
-      *reinterpret_cast<f32x4*>(dst + 256 * i) = v;
+        for (int j = 0; j < IW; ++j) {
+          const auto raw = __builtin_amdgcn_raw_buffer_load_b128(
+              rp,
+              (int)((slot * to.slot_floats + (size_t)(col / 16) * (16 * kD) + 4 * lane + 256 * (wv * IW + j)) *
+                    sizeof(float)),
+              0, kDeviceScope);
+          v[j][k] = __builtin_bit_cast(f32x4, raw);
+        }
+      }
+      float mn = M;
+#pragma unroll
+      for (int k = 0; k < C; ++k)
+        if (k0 + k < to.n) mn = fmaxf(mn, f[k]);
+      const float ms = mn == -INFINITY ? 0.f : mn, g = __builtin_amdgcn_exp2f(M - ms);
+      M = mn;
+      L *= g;
+#pragma unroll
+      for (int j = 0; j < IW; ++j) r[j] *= g;
+#pragma unroll
+      for (int k = 0; k < C; ++k)
+        if (k0 + k < to.n) {
+          const float e = __builtin_amdgcn_exp2f(f[k] - ms);
+          L += s[k] * e;
+#pragma unroll
+          for (int j = 0; j < IW; ++j) r[j] += v[j][k] * e;
+        }
     }
-    if (lk == 0) {
-      ml[2 * col] = m_run[n];
-      ml[2 * col + 1] = l_run[n];
-    }
+    const int row = a.rows == 1 ? 0 : row0 + col / a.group;
+    float* dst = a.out + ((size_t)row * a.n_heads * a.group + (size_t)h * a.group + (col - (row - row0) * a.group)) * kD + 32 * lk;
+#pragma unroll
+    for (int j = 0; j < IW; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dst[4 * (wv * IW + j) + e] = r[j][e] / L;
   }
 }
 
@@ -919,10 +1058,11 @@ __device__ void tail_item(const RowsArgs& a, const TailLens& lens, int b, int wv
   w.v += (size_t)seq * w.layer_bytes;
   w.ks += (size_t)seq * w.layer_scales;
   w.vs += (size_t)seq * w.layer_scales;
-  run_narrow<T, 1>(a, w, h, cb * 16, a.group, seq, t_begin, min(len, t_begin + a.t_split_len),
-                   a.part + a.t_base + split * a.t_slot_floats + ((size_t)seq * a.n_heads + h) * a.t_cb * (16 * kD),
-                   a.ml + 2 * (((size_t)(a.n_splits + split) * a.n_heads + h) * a.rows + seq) * a.group, wv,
-                   t_begin < len, lds);
+  PartDst to;
+  to.part = a.part + a.t_base + split * a.t_slot_floats + ((size_t)seq * a.n_heads + h) * a.t_cb * (16 * kD);
+  to.ml = a.ml + 2 * (((size_t)(a.n_splits + split) * a.n_heads + h) * a.rows + seq) * a.group;
+  run_narrow<T, 1, false>(a, w, h, cb * 16, a.group, seq, t_begin, min(len, t_begin + a.t_split_len), to, wv,
+                             t_begin < len, lds);
 }
 
 // Workgroup b of the main items: (kv head, split) units whose column blocks are
@@ -936,25 +1076,47 @@ __device__ __forceinline__ bool main_item(const RowsArgs& a, int b, int& h, int&
   return true;
 }
 
-template <typename T, int NB, bool TAILS>
-__global__ __launch_bounds__(256) void rows_narrow_kernel(RowsArgs a, std::conditional_t<TAILS, TailLens, NoLens> lens) {
+template <typename T, int NB, bool TAILS, bool CAUSAL>
+__global__ __launch_bounds__(256) void rows_narrow_kernel(RowsArgs a,
+                                                              std::conditional_t<TAILS, TailLens, NoLens> lens) {
   __shared__ __attribute__((aligned(16))) char lds[narrow_lds(NB)];
   const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   int positions = a.positions;
   if (!device_positions(a.d_pos, a.positions, positions)) return;
-  const int b = blockIdx.x;
-  if (!TAILS || b < a.main_items) {
-    int h, split, cb;
-    if (!main_item(a, b, h, split, cb)) return;
-    const long t_begin = (long)split * a.split_len, t_end = min((long)positions, t_begin + a.split_len);
-    if (t_begin >= t_end) return;
-    const int n_cols = a.rows * a.group;
-    run_narrow<T, NB>(a, a.main, h, cb * 16 * NB, n_cols, 0, t_begin, t_end,
-                      a.part + split * a.slot_floats + (size_t)h * ((n_cols + 15) / 16) * (16 * kD),
-                      a.ml + 2 * ((size_t)split * a.n_heads + h) * n_cols, wv, true, lds);
-  } else if constexpr (TAILS) {
-    tail_item<T>(a, lens, b - a.main_items, wv, lds);
+  int split, h, cb = 0;
+  if constexpr (TAILS) {
+    if ((int)blockIdx.x >= a.main_items) {
+      tail_item<T>(a, lens, (int)blockIdx.x - a.main_items, wv, lds);
+      return;
+    }
+    if (!main_item(a, blockIdx.x, h, split, cb)) return;
+  } else {  // grid (splits, kv heads, column blocks)
+    split = blockIdx.x;
+    h = blockIdx.y;
+    cb = blockIdx.z;
   }
+  const int n_cols = a.rows * a.group, col0 = cb * 16 * NB;
+  long t_end = positions;
+  if constexpr (CAUSAL) t_end = min(t_end, (long)a.start + (min(col0 + 16 * NB, n_cols) - 1) / a.group + 1);
+  const long t_begin = (long)split * a.split_len;
+  const long t_all = t_end;
+  t_end = min(t_end, t_begin + a.split_len);
+  if (t_begin >= t_end) return;
+  PartDst to;
+  const size_t part = (size_t)h * ((n_cols + 15) / 16) * (16 * kD), ml_slot = 2 * (size_t)a.n_heads * n_cols;
+  to.part = a.part + part;
+  to.ml = a.ml + 2 * (size_t)h * n_cols;
+  if (!TAILS && !CAUSAL && a.tickets) {
+    to.ticket = a.tickets + 32 * h;
+    to.n = (int)((t_all + a.split_len - 1) / a.split_len);
+    to.slot = split;
+    to.slot_floats = a.slot_floats;
+    to.ml_slot = ml_slot;
+  } else {
+    to.part += split * a.slot_floats;
+    to.ml += split * ml_slot;
+  }
+  run_narrow<T, NB, CAUSAL>(a, a.main, h, col0, n_cols, 0, t_begin, t_end, to, wv, true, lds);
 }
 
 template <typename T, int WC, bool HL, bool TAILS>
@@ -1152,6 +1314,7 @@ __global__ __launch_bounds__(256) void rows_generic_kernel(RowsArgs a, int hd,
 struct RowsPlan {
   bool generic = false;
   int nb = 0, wc = 0;  // narrow: blocks of 16 columns; wide: waves of 32
+  bool fold = false;           // narrow: in the launch
   int n_cb = 0, n_splits = 0, split_len = 128;
   int t_cb = 0, t_splits = 0, t_split_len = 128;
   size_t rows = 0;  // of one launch (sequences go in batches of kMaxEach)
@@ -1171,35 +1334,37 @@ void split_positions(long positions, long units, long want, int* n_splits, int* 
   *n_splits = (int)((steps + per - 1) / per);
 }
 
-// A wide launch's shape: how many columns an item has, and into how many splits
-// it and the tails are cut, by the time each choice would take. The times (us)
-// are fitted on this card over chunks of 77..1000 rows and batches of 7..64
-// sequences at 900 .. 16000 positions; what counts is that they rank the choices
-// as those measure (77 rows at 901: 2, 4, 8 waves of columns 21.7, 22.7, 24.1; 512
-// at 3449: 4, 8 waves 85.8, 81; 64 x 16000 f16 in 16, 21, 25, 32 splits 64.7, 54.7,
-// 67, 70). An item takes 14 to start, load its queries and store, and `c` per 128
-// positions (one workgroup a CU); a tail's four waves 10 and 2 per 128; a
-// partial's floats are written and read once.
-void plan_wide(RowsPlan& p, long positions, long cols, long heads, int elem, long tails, long longest) {
+// A launch's shape by the time each choice would take: whether its main items
+// are narrow (32 columns, 4 waves) or wide and of how many columns, and into how
+// many splits they and the tails are cut. The times (us) are fitted on this card
+// over chunks of 2..1000 rows and batches of 7..64 sequences at 0 .. 16000
+// positions; what counts is that they rank the choices as those measure (77 rows
+// at 901: narrow in 1, 3 splits 19.0, 16.3, wide with 2, 4, 8 waves of columns
+// 21.7, 22.7, 24.1; 200 at 1000: narrow 22.4, wide 31.3; 200 at 4000: 58.7, 53.0;
+// 512 at 3449: 100, wide with 4, 8 waves 85.8, 81; 64 x 16000 f16 in 16, 21, 25, 32
+// splits 64.7, 54.7, 67, 70). A wide item takes 14 to start, load its queries
+// and store, and `c` per 128 positions (one workgroup a CU); a narrow one 6.4 and
+// 1.6 (f32 3.2), two a CU in 1.8 times that; a tail's four waves beside wide items
+// 10 and 2; a partial's floats are written and read once.
+void plan_shape(RowsPlan& p, long positions, long cols, long heads, int elem, long tails, long longest) {
   const long steps = (positions + kPosStep - 1) / kPosStep;
   double best = 1e300;
   for (long t_want : {kCUs / 2, kCUs, 2 * kCUs}) {
     int t_splits = 0, t_len = kPosStep;
-    long t_wgs = 0;
-    double t_tail = 1;  // (none)
-    if (tails && longest) {
+    if (tails && longest)
       split_positions(longest, tails, t_want, &t_splits, &t_len);
-      t_wgs = (tails * t_splits + 1) / 2;
-      t_tail = 10 + 2.0 * (t_len / kPosStep);
-    } else if (t_want != kCUs) {
+    else if (t_want != kCUs)
       continue;
-    }
-    for (int wc : {2, 4, 8}) {
+    const double t_steps = t_len / kPosStep;
+    for (int wc : {0, 2, 4, 8}) {
       if (wc == 2 && elem == RV_ELEM_F32) continue;  // (its LDS tiles are twice as large)
-      const double c = elem == RV_ELEM_F32 ? (wc == 4 ? 5.5 : 9.0)
+      const double c = wc == 0                 ? (elem == RV_ELEM_F32 ? 3.2 : 1.6)
+                       : elem == RV_ELEM_F32 ? (wc == 4 ? 5.5 : 9.0)
                        : elem == RV_ELEM_F16 ? (wc == 2 ? 2.4 : wc == 4 ? 3.05 : 5.0)
                                              : (wc == 2 ? 2.7 : wc == 4 ? 3.5 : 5.9);
-      const long units = heads * ((cols + 32 * wc - 1) / (32 * wc));
+      const double fixed = wc ? 14 : 6.4, t_tail = !t_splits ? 1 : wc ? 10 + 2.0 * t_steps : 6.4 + 1.2 * t_steps;
+      const long t_wgs = wc ? (tails * t_splits + 1) / 2 : tails * t_splits;
+      const long units = heads * ((cols + (wc ? 32 * wc : 32) - 1) / (wc ? 32 * wc : 32));
       long n = 1;
       for (long prev = 0; n <= steps; n = n == steps ? n + 1 : std::min(steps, n < 4 ? n + 1 : n * 5 / 4 + 1)) {
         const long per = (steps + n - 1) / n, splits = (steps + per - 1) / per;
@@ -1207,15 +1372,21 @@ void plan_wide(RowsPlan& p, long positions, long cols, long heads, int elem, lon
         prev = splits;
         const long items = units * splits;
         if (items > 4 * kCUs && n > 1) break;
-        const double t = 14 + c * per;
-        // CUs the tails take meanwhile, one after the other on each.
-        const long in_a_row = std::max(1L, (long)(t / t_tail)), t_cus = (t_wgs + in_a_row - 1) / in_a_row;
-        const long rounds = items + t_cus <= kCUs ? 1 : (long)((items * t + t_wgs * t_tail) / (kCUs * t)) + 1;
+        const double t = fixed + c * per;
+        double total;
+        if (wc) {
+          // CUs the tails take meanwhile, one after the other on each.
+          const long in_a_row = std::max(1L, (long)(t / t_tail)), t_cus = (t_wgs + in_a_row - 1) / in_a_row;
+          const long rounds = items + t_cus <= kCUs ? 1 : (long)((items * t + t_wgs * t_tail) / (kCUs * t)) + 1;
+          total = std::max(t * rounds, t_tail);
+        } else {
+          total = std::max(std::max(t, t_tail), 0.9 * (items * t + t_wgs * t_tail) / kCUs);
+        }
         const long slots = splits + t_splits;
-        double total = std::max(t * rounds, t_tail);
         if (slots > 1) total += 3 + slots * cols * heads * (kD + 2) * 8 / 6.0e6;
         if (total < best) {
           best = total;
+          p.nb = wc ? 0 : 2;
           p.wc = wc;
           p.n_splits = (int)splits;
           p.split_len = (int)(per * kPosStep);
@@ -1236,28 +1407,36 @@ RowsPlan plan_rows(const RowsCall& c, const rv_kv* owner) {
   const long group = (long)(c.n_q_heads / g->n_kv_heads), heads = (long)(c.kv_hi - c.kv_lo);
   const long cols = (long)p.rows * group;
   const long positions = c.main ? (long)c.positions : 0;
+  const bool causal = c.causal && c.rows > 1;  // (one row: its limit is `positions`)
   long longest = 0;
   if (c.tails) {
     p.t_cb = (int)((group + 15) / 16);
     for (size_t i = 0; i < c.rows; ++i) longest = std::max(longest, (long)c.tails->lens[c.tail_layer + i]);
   }
   const long tails = heads * p.t_cb * (long)p.rows;
-  // Few columns: one or two 16-column blocks in registers, unless rows see
-  // different lengths or the operands are single (neither is a decode).
-  if (cols <= 32 && !(c.causal && c.rows > 1) && c.split) {
+  if (positions && (cols > 32 || causal)) {
+    plan_shape(p, positions, cols, heads, g->elem, tails, longest);
+  } else {
+    // One narrow block of columns a kv head. A decode's splits, 32 query heads over
+    // 4 kv heads, us: 200 positions whole 6.3, in two 7.5; 400 in four 7.8, whole
+    // 8.0; 1000 in eight 7.8, in four 8.6; 2000 in 16 8.7, in 8 9.6; 4096 in 16 9.7,
+    // in 32 10.0; 16384 in 64 12.0, in 128 14.3; 131000 in 64 32.5, in 128 32.2.
     p.nb = cols <= 16 ? 1 : 2;
-    if (positions) split_positions(positions, heads, 2 * kCUs, &p.n_splits, &p.split_len);
-    if (longest) split_positions(longest, tails, 2 * kCUs, &p.t_splits, &p.t_split_len);
-  } else if (positions) {
-    plan_wide(p, positions, cols, heads, g->elem, tails, longest);
-  } else {  // tails alone
-    p.nb = 1;
+    if (positions && positions <= 2 * kPosStep) {
+      p.n_splits = 1;
+      p.split_len = 2 * kPosStep;
+    } else if (positions) {
+      split_positions(positions, heads, positions <= 2 * kFold * kPosStep ? kFold * heads : kCUs, &p.n_splits, &p.split_len);
+    }
     if (longest) split_positions(longest, tails, 2 * kCUs, &p.t_splits, &p.t_split_len);
   }
   if (positions && owner->tune_decode_split_len > 0) {
     p.split_len = (int)((std::min<int64_t>(owner->tune_decode_split_len, 1 << 30) + kPosStep - 1) / kPosStep * kPosStep);
     p.n_splits = (int)((positions + p.split_len - 1) / p.split_len);
   }
+  // Splits folded by the launch: 1.3 us of its own against 4.3 for a second one,
+  // while they are few.
+  p.fold = cols <= 32 && !c.tails && !causal && p.n_splits > 1 && p.n_splits <= kFold;
   if (p.columns()) p.n_cb = (int)((cols + p.columns() - 1) / p.columns());
   return p;
 }
@@ -1292,11 +1471,21 @@ template <typename T, bool HL, bool TAILS, typename L>
 void launch_plan(const RowsPlan& p, const TimedPair& tp, const RowsArgs& a, unsigned tail_items, hipStream_t s,
                  const L& lens) {
   if (p.nb) {
-    const dim3 grid((unsigned)a.main_items + tail_items);
-    if (p.nb == 1)
-      launch_timed(tp, rows_narrow_kernel<T, 1, TAILS>, grid, dim3(256), s, a, lens);
-    else
-      launch_timed(tp, rows_narrow_kernel<T, 2, TAILS>, grid, dim3(256), s, a, lens);
+    if constexpr (TAILS) {
+      const dim3 grid((unsigned)a.main_items + tail_items);
+      if (p.nb == 1)
+        launch_timed(tp, rows_narrow_kernel<T, 1, true, false>, grid, dim3(256), s, a, lens);
+      else
+        launch_timed(tp, rows_narrow_kernel<T, 2, true, false>, grid, dim3(256), s, a, lens);
+    } else {
+      const dim3 grid((unsigned)a.n_splits, (unsigned)a.n_heads, (unsigned)a.n_cb);
+      if (a.causal)
+        launch_timed(tp, rows_narrow_kernel<T, 2, false, true>, grid, dim3(256), s, a, lens);
+      else if (p.nb == 2)
+        launch_timed(tp, rows_narrow_kernel<T, 2, false, false>, grid, dim3(256), s, a, lens);
+      else
+        launch_timed(tp, rows_narrow_kernel<T, 1, false, false>, grid, dim3(256), s, a, lens);
+    }
     return;
   }
   const dim3 grid((unsigned)a.main_items + (tail_items + 1) / 2);
@@ -1314,8 +1503,8 @@ size_t rows_ws_need(const rv_kv* owner, const RowsCall& c) { return plan_floats(
 
 size_t rows_ws_bound(const rv_kv* kv) {
   if (kv->head_dim != (size_t)kD) return 0;
-  // A narrow launch's items: 2 kCUs, or one per kv head (and then no partials).
-  return (size_t)2 * kCUs * 16 * (kD + 2) * sizeof(float);
+  // A decode's items: kFold or fewer per kv head, or kCUs in all.
+  return std::max<size_t>(kCUs, kFold * kv->n_kv_heads) * 16 * (kD + 2) * sizeof(float);
 }
 
 HipStatus launch_rows(rv_kv* owner, const RowsCall& c, hipStream_t s, const Workspace* ws) {
@@ -1356,7 +1545,7 @@ HipStatus launch_rows(rv_kv* owner, const RowsCall& c, hipStream_t s, const Work
     a.n_heads = (int)(c.kv_hi - c.kv_lo);
     a.positions = (int)c.positions;
     a.start = (int)c.start;
-    a.causal = c.causal;
+    a.causal = c.causal && c.rows > 1;  // (one row: its limit is `positions`)
     a.d_pos = c.d_pos;
     a.qscale = c.scale * kLog2e;
     if (p.generic) {
@@ -1388,6 +1577,7 @@ HipStatus launch_rows(rv_kv* owner, const RowsCall& c, hipStream_t s, const Work
       a.t_split_len = p.t_split_len;
       a.main_items = (a.n_heads * a.n_splits + 7) / 8 * 8 * a.n_cb;
       a.single = p.slots() == 1;
+      a.tickets = p.fold ? xcd_tickets(owner) : nullptr;
       const unsigned tail_items = (unsigned)(n * a.n_heads * a.t_cb * a.t_splits);
       const TimedPair tp = ws ? TimedPair{} : timing_pair(owner, s);
       if (c.tails) {
@@ -1402,7 +1592,7 @@ HipStatus launch_rows(rv_kv* owner, const RowsCall& c, hipStream_t s, const Work
       } else {
         launch_plan<Q8, false, false>(p, tp, a, 0, s, NoLens{});
       }
-      if (!a.single) {
+      if (!a.single && !p.fold) {
         const int merges = 16 * a.n_heads * (int)((n * group + 31) / 32);
         const TailLens* tl = c.tails ? &lens : nullptr;
         if (p.slots() <= 4)
