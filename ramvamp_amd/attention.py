@@ -163,10 +163,13 @@ class _Arg:
 
 
 def _flags(cache: "KvCache", args) -> int:
-    kinds = {a.host for a in args if a.host is not None}
-    if len(kinds) > 1:
-        raise TypeError("one call takes either device tensors or host arrays, not both")
-    if kinds == {True}:
+    host = None
+    for a in args:
+        if a.host is not None and a.host is not host:
+            if host is not None:
+                raise TypeError("one call takes either device tensors or host arrays, not both")
+            host = a.host
+    if host:
         return L.RV_HOST_PTRS
     cache._bind_stream()
     return 0
@@ -193,6 +196,8 @@ class KvCache:
         self.device = device
         self.elem = {L.RV_ELEM_F16: "f16", L.RV_ELEM_F32: "f32", L.RV_ELEM_Q8_0: "q8_0"}[_elem_code(elem)]
         self._stream = None
+        self._kv_dim = n_kv_heads * head_dim
+        self._torch_device = None
 
     new = classmethod(lambda cls, *a, **k: cls(*a, **k))
 
@@ -263,7 +268,7 @@ class KvCache:
     def append_rows(self, layer: int, k_rows, v_rows):
         """The loop of model/prefill.rs:2081-2087 in one call (all rows or none)."""
         ka, va = _Arg(k_rows), _Arg(v_rows)
-        kv_dim = self.kv_dim()
+        kv_dim = self._kv_dim
         if ka.n != va.n or ka.n % kv_dim:
             raise ValueError("k_rows and v_rows must both be rows x kv_dim")
         err = L.RvError()
@@ -287,7 +292,7 @@ class KvCache:
         """rv_kv_append_each (no reference counterpart): row i of k_rows and
         v_rows to layer layer0 + i, each at its own cursor (all rows or none)."""
         ka, va = _Arg(k_rows), _Arg(v_rows)
-        kv_dim = self.kv_dim()
+        kv_dim = self._kv_dim
         if ka.n != va.n or ka.n % kv_dim:
             raise ValueError("k_rows and v_rows must both be rows x kv_dim")
         err = L.RvError()
@@ -302,11 +307,13 @@ class KvCache:
         if k is None and v is None:
             import torch
 
-            k = torch.empty(rows, self.kv_dim(), dtype=torch.float32, device=f"cuda:{self.device}")
+            if self._torch_device is None:
+                self._torch_device = torch.device("cuda", self.device)
+            k = torch.empty((rows, self._kv_dim), dtype=torch.float32, device=self._torch_device)
             v = torch.empty_like(k)
         ka, va = _Arg(k, writable=True), _Arg(v, writable=True)
         for a in (ka, va):
-            if a.host is not None and a.n != rows * self.kv_dim():
+            if a.host is not None and a.n != rows * self._kv_dim:
                 raise ValueError("k and v must be rows x kv_dim")
         err = L.RvError()
         _check(_lib().rv_kv_read_rows(self._h, layer, start, rows, ka.ptr, va.ptr, _flags(self, (ka, va)),

@@ -12,10 +12,14 @@
 // NaN gets a NaN scale, so that its 32 values all read as NaN (a code cannot
 // carry one).
 //
-// Bound by bytes: 4 in and 34/32 out per value. One thread takes four values
-// (a 16-byte load, a 4-byte store), eight lanes a block (the maximum over them
-// is three DPP steps).
+// Bound by bytes, 4 in and 34/32 out per value, as long as a thread's share of a
+// block is large enough to spread the block's own work (two divisions, the
+// scale's rounding) over it: eight values a thread, four lanes a block (the
+// maximum over them is two DPP steps); with four values a thread and roundf
+// 4096 rows of 512 took 8.8 us, bound by vector operations.
 #include "rv_rows.hpp"
+
+#include <algorithm>
 
 namespace rv {
 namespace {
@@ -37,78 +41,73 @@ struct DstArgs {
 
 constexpr float kMaxScale = 515.5f;  // 127 * 515.5 rounds to 65472; the next f16, 516, to infinity
 
-// Four values of a block held by 8 lanes: their codes (+ 128) and the scale.
-__device__ __forceinline__ uint32_t q8_quad(const f32x4 x, uint16_t& scale) {
+// Eight values of a block held by 4 lanes: their codes (+ 128) and the scale.
+struct Oct {
+  f32x4 a, b;
+  __device__ __forceinline__ float operator[](int e) const { return e < 4 ? a[e] : b[e - 4]; }
+};
+
+__device__ __forceinline__ u32x2 q8_oct(const Oct& x, uint16_t& scale) {
 #pragma clang fp contract(off)
-  // Finite blocks only: the largest magnitude's bits order as integers, and a
-  // NaN or an infinity has larger bits than any finite value.
+  // The largest magnitude's bits order as integers, and a NaN or an infinity has
+  // larger bits than any finite value.
   uint32_t m = 0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) m = max(m, __float_as_uint(fabsf(x[e])));
+  for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(x[e]) & 0x7FFFFFFFu);
   m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, DPP_QUAD_XOR1, 0xF, 0xF, false));
   m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, DPP_QUAD_XOR2, 0xF, 0xF, false));
-  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, DPP_ROW_HALF_MIRROR, 0xF, 0xF, false));
   const bool finite = m < 0x7F800000u;
   float d = finite ? __uint_as_float(m) / 127.f : 0.f;
-  if (f32_to_f16_bits(d) > f32_to_f16_bits(kMaxScale)) d = kMaxScale;
+  if (d >= 515.75f) d = kMaxScale;  // (halfway to 516, the even one of the two)
   // Below the smallest normal float the reciprocal may overflow; the f16 scale
   // is zero there and the codes stand for nothing.
   const float id = d >= 1.17549435e-38f ? 1.f / d : 0.f;
-  scale = finite ? f32_to_f16_bits(d) : (uint16_t)0x7E00;
-  uint32_t w = 0;
+  scale = finite ? __builtin_bit_cast(uint16_t, (_Float16)d) : (uint16_t)0x7E00;
+  uint32_t w[2] = {0, 0};
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float y = finite ? fminf(fmaxf(roundf(x[e] * id), -127.f), 127.f) : 0.f;
-    w |= (uint32_t)((int)y + 128) << (8 * e);
+  for (int e = 0; e < 8; ++e) {
+    // Half away from zero: the conversion truncates, and adding the float below
+    // one half rounds up to the next whole number from exactly one half on.
+    const float y = __builtin_amdgcn_fmed3f(x[e] * id, -127.f, 127.f);
+    const int c = finite ? (int)(y + __builtin_copysignf(0x1.fffffep-2f, y)) : 0;
+    w[e >> 2] |= (uint32_t)(c + 128) << (8 * (e & 3));
   }
-  return w;
-}
-
-// Stores four values [d, d + 4) of kv head h at row t of the layer `w` (+ its
-// offsets) as the cache's type. For Q8 every lane of the 8 that hold a block
-// calls it together.
-template <typename T, bool V>
-__device__ __forceinline__ void store_quad(const KvView& w, size_t lb, size_t ls, int hd, int h, long t, int d,
-                                           const f32x4 x) {
-  char* base = const_cast<char*>(V ? w.v : w.k) + lb;
-  if constexpr (std::is_same<T, Q8>::value) {
-    uint16_t s;
-    const uint32_t c = q8_quad(x, s);
-    const size_t row = (size_t)h * w.rows + t;
-    *reinterpret_cast<uint32_t*>(base + row * hd + d) = c;
-    if (d % 32 == 0) {
-      const int nb = hd / 32, b = d / 32;
-      if (V)
-        const_cast<uint16_t*>(w.vs)[ls + ((size_t)h * nb + b) * w.rows + t] = s;
-      else
-        const_cast<uint16_t*>(w.ks)[ls + row * nb + b] = s;
-    }
-  } else {
-    T* p = reinterpret_cast<T*>(base) + (size_t)t * w.kv_dim + (size_t)h * hd + d;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if constexpr (std::is_same<T, float>::value)
-        p[e] = x[e];
-      else
-        p[e] = f32_to_f16_bits(x[e]);
-    }
-  }
+  return u32x2{w[0], w[1]};
 }
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
-// One thread per four consecutive values of one plane (blockIdx.y: K, V).
-template <typename T, bool EACH>
-__global__ __launch_bounds__(256) void append_dst_kernel(KvView w, DstArgs a, const float* __restrict__ k,
-                                                         const float* __restrict__ v, int rows, int hd,
-                                                         std::conditional_t<EACH, EachLens, NoLens> lens) {
-  const int quads = (int)w.kv_dim / 4;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  const int r = (int)(i / quads), j = (int)(i % quads);
-  if (r >= rows) return;
+// Quantizes eight values [d, d + 8) of kv head h and stores them at row t of the
+// layer `w` (+ its offsets). The 4 lanes that hold a block call it together.
+template <bool V>
+__device__ __forceinline__ void store_oct(const KvView& w, size_t lb, size_t ls, int hd, int h, long t, int d,
+                                          const Oct& x) {
+  uint16_t s;
+  const u32x2 c = q8_oct(x, s);
+  const size_t row = (size_t)h * w.rows + t;
+  *reinterpret_cast<u32x2*>(const_cast<char*>(V ? w.v : w.k) + lb + row * hd + d) = c;
+  if (d % 32 == 0) {
+    const int nb = hd / 32, b = d / 32;
+    if (V)
+      const_cast<uint16_t*>(w.vs)[ls + ((size_t)h * nb + b) * w.rows + t] = s;
+    else
+      const_cast<uint16_t*>(w.ks)[ls + row * nb + b] = s;
+  }
+}
+
+// Eight consecutive values a thread, of one plane (blockIdx.y: K, V), into a Q8_0
+// cache.
+template <bool EACH>
+__global__ __launch_bounds__(256) void append_q8_kernel(KvView w, DstArgs a, const float* __restrict__ k,
+                                                        const float* __restrict__ v, uint32_t n_octs, int hd,
+                                                        std::conditional_t<EACH, EachLens, NoLens> lens) {
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= n_octs) return;  // (the four lanes of a block together)
   const bool is_v = blockIdx.y != 0;
-  const f32x4 x = *reinterpret_cast<const f32x4u*>((is_v ? v : k) + (size_t)r * w.kv_dim + 4 * j);
-  const int h = 4 * j / hd, d = 4 * j % hd;
+  const f32x4u* src = reinterpret_cast<const f32x4u*>((is_v ? v : k) + 8 * (size_t)i);  // (rows are contiguous)
+  const Oct x{__builtin_nontemporal_load(src), __builtin_nontemporal_load(src + 1)};
+  const uint32_t per_row = (uint32_t)w.kv_dim / 8;
+  const uint32_t r = i / per_row, j = 8 * (i - r * per_row), h = j / (uint32_t)hd, d = j - h * hd;
   long t;
   if constexpr (EACH)
     t = lens.len[r];
@@ -116,26 +115,21 @@ __global__ __launch_bounds__(256) void append_dst_kernel(KvView w, DstArgs a, co
     t = a.row0 + r;
   const size_t lb = (size_t)r * a.layer_bytes, ls = (size_t)r * a.layer_scales;
   if (is_v)
-    store_quad<T, true>(w, lb, ls, hd, h, t, d, x);
+    store_oct<true>(w, lb, ls, hd, h, t, d, x);
   else
-    store_quad<T, false>(w, lb, ls, hd, h, t, d, x);
+    store_oct<false>(w, lb, ls, hd, h, t, d, x);
 }
 
-// As append_dst_kernel for any head size: one thread per value.
-template <typename T, bool EACH>
+// One row to each layer of an f16 or f32 cache: one thread per value.
+template <typename T>
 __global__ __launch_bounds__(256) void append_each_kernel(KvView w, DstArgs a, const float* __restrict__ k,
-                                                          const float* __restrict__ v, int rows,
-                                                          std::conditional_t<EACH, EachLens, NoLens> lens) {
+                                                          const float* __restrict__ v, int rows, EachLens lens) {
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   const int r = (int)(i / w.kv_dim), j = (int)(i % w.kv_dim);
   if (r >= rows) return;
   const bool is_v = blockIdx.y != 0;
   const float x = (is_v ? v : k)[(size_t)r * w.kv_dim + j];
-  long t;
-  if constexpr (EACH)
-    t = lens.len[r];
-  else
-    t = a.row0 + r;
+  const long t = lens.len[r];
   T* p = reinterpret_cast<T*>(const_cast<char*>(is_v ? w.v : w.k) + (size_t)r * a.layer_bytes) + (size_t)t * w.kv_dim + j;
   if constexpr (std::is_same<T, float>::value)
     *p = x;
@@ -148,8 +142,8 @@ constexpr int kMaxHd = 512;
 // grid (rows, q heads + k heads + v heads), one wave each. Lane l owns the
 // rotation's pairs (i, i + half), i = l + 64 p; the f32 operations are
 // norm.rs:18-26 and rope.rs:31-45's, one rounding each, the mean of squares
-// and the angles in f64 (as rv_prologue.hip's). k and v heads pass through LDS
-// to the store's order, four consecutive values a lane.
+// and the angles in f64 (as rv_prologue.hip's). k and v heads of a Q8_0 cache pass
+// through LDS to the store's order, eight consecutive values a lane.
 template <typename T, bool EACH>
 __global__ __launch_bounds__(64) void prologue_dst_kernel(KvView w, DstArgs a, const float* __restrict__ q,
                                                           float* __restrict__ q_out, int n_q,
@@ -158,7 +152,7 @@ __global__ __launch_bounds__(64) void prologue_dst_kernel(KvView w, DstArgs a, c
                                                           const float* __restrict__ k_w, float eps, InvFreq inv,
                                                           std::conditional_t<EACH, EachLens, NoLens> lens) {
 #pragma clang fp contract(off)
-  __shared__ float row[kMaxHd];
+  __shared__ __attribute__((aligned(16))) float row[kMaxHd];
   constexpr int NP = kMaxHd / 2 / 64;
   const int r = blockIdx.x, lane = threadIdx.x, half = hd / 2;
   int s = blockIdx.y;
@@ -236,13 +230,15 @@ __global__ __launch_bounds__(64) void prologue_dst_kernel(KvView w, DstArgs a, c
       row[i + half] = y1[p];
     }
     __syncthreads();
-    // Whole groups of 8 lanes are past the row's end together (hd % 32 == 0).
-    for (int d = 4 * lane; d < hd; d += 256) {
-      const f32x4 y = {row[d], row[d + 1], row[d + 2], row[d + 3]};
+    // Whole groups of 4 lanes are past the row's end together (hd % 32 == 0).
+    const int d = 8 * lane;
+    if (d < hd) {
+      const f32x4* y = reinterpret_cast<const f32x4*>(row + d);
+      const Oct x{y[0], y[1]};
       if (is_v)
-        store_quad<T, true>(w, lb, ls, hd, h, t, d, y);
+        store_oct<true>(w, lb, ls, hd, h, t, d, x);
       else
-        store_quad<T, false>(w, lb, ls, hd, h, t, d, y);
+        store_oct<false>(w, lb, ls, hd, h, t, d, x);
     }
   } else {
     T* dst = reinterpret_cast<T*>(const_cast<char*>(is_v ? w.v : w.k) + lb) + (size_t)t * w.kv_dim + (size_t)h * hd;
@@ -261,39 +257,43 @@ __global__ __launch_bounds__(64) void prologue_dst_kernel(KvView w, DstArgs a, c
   }
 }
 
-// Rows [pos, pos + rows) of one plane (blockIdx.y: K, V) as f32, four values a
-// thread where W == 4.
+// Rows [pos, pos + ..) of one plane (blockIdx.y: K, V) as f32, W values a thread.
 template <typename T, int W>
-__global__ __launch_bounds__(256) void read_rows_kernel(KvView w, int hd, long pos, int rows, float* __restrict__ k,
-                                                        float* __restrict__ v) {
-  const long n = w.kv_dim / W;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  const long r = i / n;
-  const int j = (int)(i % n) * W;
-  if (r >= rows) return;
+__global__ __launch_bounds__(256) void read_rows_kernel(KvView w, int hd, long pos, uint32_t n_pieces,
+                                                        float* __restrict__ k, float* __restrict__ v) {
+  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
   const bool is_v = blockIdx.y != 0;
   float* dst = is_v ? v : k;
-  if (!dst) return;
-  const int h = j / hd, d = j % hd;
+  if (i >= n_pieces || !dst) return;
+  const uint32_t per_row = (uint32_t)w.kv_dim / W;
+  const uint32_t r = i / per_row, j = (i - r * per_row) * W, h = j / (uint32_t)hd, d = j - h * hd;
   const long t = pos + r;
   float x[W];
-  if constexpr (std::is_same<T, Q8>::value && W == 4) {
+  if constexpr (std::is_same<T, Q8>::value) {
+    static_assert(W == 8, "pieces inside a block");
     const int nb = hd / 32;
     const size_t row = (size_t)h * w.rows + t;
-    const uint32_t c = *reinterpret_cast<const uint32_t*>((is_v ? w.v : w.k) + row * hd + d);
-    const uint16_t s = is_v ? w.vs[((size_t)h * nb + d / 32) * w.rows + t] : w.ks[row * nb + d / 32];
+    const u32x2 c = *reinterpret_cast<const u32x2*>((is_v ? w.v : w.k) + row * hd + d);
+    const uint16_t sb = is_v ? w.vs[((size_t)h * nb + d / 32) * w.rows + t] : w.ks[row * nb + d / 32];
+    const _Float16 s = __builtin_bit_cast(_Float16, sb);
+    f16x2 p[4];
+    q8_widen(c[0], p[0], p[1]);
+    q8_widen(c[1], p[2], p[3]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = q8_value((uint8_t)(c >> (8 * e)), s);
+    for (int e = 0; e < 8; ++e) x[e] = (float)(_Float16)(p[e >> 1][e & 1] * s);
   } else {
 #pragma unroll
     for (int e = 0; e < W; ++e)
       x[e] = is_v ? kv_value<T, true>(w, hd, h, t, d + e) : kv_value<T, false>(w, hd, h, t, d + e);
   }
-  float* o = dst + (size_t)r * w.kv_dim + j;
-  if constexpr (W == 4)
-    *reinterpret_cast<f32x4u*>(o) = f32x4{x[0], x[1], x[2], x[3]};
-  else
+  float* o = dst + (size_t)i * W;
+  if constexpr (W >= 4) {
+#pragma unroll
+    for (int e = 0; e < W; e += 4)
+      *reinterpret_cast<f32x4u*>(o + e) = f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+  } else {
     *o = x[0];
+  }
 }
 
 // One Q8_0 row in ggml's block_q8_0 order, 34 bytes a block.
@@ -343,23 +343,37 @@ HipStatus launched(const char* what) {
 
 unsigned blocks_of(size_t threads) { return (unsigned)((threads + 255) / 256); }
 
+// Rows a launch takes: the kernels count its pieces in 32 bits.
+size_t rows_at_once(size_t kv_dim) { return std::max<size_t>(1, ((size_t)1 << 30) / kv_dim); }
+
 }  // namespace
 
 HipStatus launch_append_dst(const rv_kv* kv, const RowDst& dst, const float* k, const float* v, size_t rows,
                             hipStream_t s) {
   if (rows == 0) return HipStatus{};
   const KvView w = kv_view(kv, dst.layer);
-  const DstArgs a = dst_args(dst, w);
-  const int hd = (int)kv->head_dim, n = (int)rows;
-  const dim3 quads(blocks_of(rows * kv->kv_dim / 4), 2), vals(blocks_of(rows * kv->kv_dim), 2), block(256);
-  if (kv->elem == RV_ELEM_Q8_0 && dst.each_n)
-    hipLaunchKernelGGL((append_dst_kernel<Q8, true>), quads, block, 0, s, w, a, k, v, n, hd, each_lens(dst));
-  else if (kv->elem == RV_ELEM_Q8_0)
-    hipLaunchKernelGGL((append_dst_kernel<Q8, false>), quads, block, 0, s, w, a, k, v, n, hd, NoLens{});
+  DstArgs a = dst_args(dst, w);
+  const int hd = (int)kv->head_dim;
+  const dim3 block(256);
+  if (kv->elem == RV_ELEM_Q8_0 && !dst.each_n) {
+    for (size_t r0 = 0, n; r0 < rows; r0 += n) {
+      n = std::min(rows - r0, rows_at_once(kv->kv_dim));
+      const size_t octs = n * kv->kv_dim / 8;
+      hipLaunchKernelGGL(append_q8_kernel<false>, dim3(blocks_of(octs), 2), block, 0, s, w, a, k + r0 * kv->kv_dim,
+                         v + r0 * kv->kv_dim, (uint32_t)octs, hd, NoLens{});
+      a.row0 += (long)n;
+    }
+    return launched("append launch");
+  }
+  const size_t octs = rows * kv->kv_dim / 8;  // (at most kMaxEach rows)
+  const dim3 vals(blocks_of(rows * kv->kv_dim), 2);
+  if (kv->elem == RV_ELEM_Q8_0)
+    hipLaunchKernelGGL(append_q8_kernel<true>, dim3(blocks_of(octs), 2), block, 0, s, w, a, k, v, (uint32_t)octs, hd,
+                       each_lens(dst));
   else if (kv->elem == RV_ELEM_F32)
-    hipLaunchKernelGGL((append_each_kernel<float, true>), vals, block, 0, s, w, a, k, v, n, each_lens(dst));
+    hipLaunchKernelGGL(append_each_kernel<float>, vals, block, 0, s, w, a, k, v, (int)rows, each_lens(dst));
   else
-    hipLaunchKernelGGL((append_each_kernel<uint16_t, true>), vals, block, 0, s, w, a, k, v, n, each_lens(dst));
+    hipLaunchKernelGGL(append_each_kernel<uint16_t>, vals, block, 0, s, w, a, k, v, (int)rows, each_lens(dst));
   return launched("append launch");
 }
 
@@ -392,20 +406,25 @@ HipStatus launch_read_rows(const rv_kv* kv, size_t layer, size_t pos, size_t row
   const KvView w = kv_view(kv, layer);
   const int hd = (int)kv->head_dim;
   const bool four = hd % 4 == 0;
-  const dim3 grid(blocks_of(rows * kv->kv_dim / (four ? 4 : 1)), 2), block(256);
-#define RV_READ(T)                                                                                                  \
-  if (four)                                                                                                         \
-    hipLaunchKernelGGL((read_rows_kernel<T, 4>), grid, block, 0, s, w, hd, (long)pos, (int)rows, k, v);             \
-  else                                                                                                              \
-    hipLaunchKernelGGL((read_rows_kernel<T, 1>), grid, block, 0, s, w, hd, (long)pos, (int)rows, k, v)
-  if (kv->elem == RV_ELEM_Q8_0) {
-    hipLaunchKernelGGL((read_rows_kernel<Q8, 4>), grid, block, 0, s, w, hd, (long)pos, (int)rows, k, v);
-  } else if (kv->elem == RV_ELEM_F32) {
-    RV_READ(float);
-  } else {
-    RV_READ(_Float16);
-  }
+  for (size_t r0 = 0, n; r0 < rows; r0 += n) {
+    n = std::min(rows - r0, rows_at_once(kv->kv_dim));
+    const size_t pieces = n * kv->kv_dim / (kv->elem == RV_ELEM_Q8_0 ? 8 : four ? 4 : 1);
+    const dim3 grid(blocks_of(pieces), 2), block(256);
+    float *dk = k ? k + r0 * kv->kv_dim : nullptr, *dv = v ? v + r0 * kv->kv_dim : nullptr;
+#define RV_READ(T, W)                                                                                            \
+  hipLaunchKernelGGL((read_rows_kernel<T, W>), grid, block, 0, s, w, hd, (long)(pos + r0), (uint32_t)pieces, dk, dv)
+    if (kv->elem == RV_ELEM_Q8_0)
+      RV_READ(Q8, 8);
+    else if (kv->elem == RV_ELEM_F32 && four)
+      RV_READ(float, 4);
+    else if (kv->elem == RV_ELEM_F32)
+      RV_READ(float, 1);
+    else if (four)
+      RV_READ(_Float16, 4);
+    else
+      RV_READ(_Float16, 1);
 #undef RV_READ
+  }
   return launched("read rows launch");
 }
 
