@@ -1381,6 +1381,7 @@ void plan_shape(RowsPlan& p, long positions, long cols, long heads, int elem, lo
           total = std::max(t * rounds, t_tail);
         } else {
           total = std::max(std::max(t, t_tail), 0.9 * (items * t + t_wgs * t_tail) / kCUs);
+          if (items > kCUs) total = std::max(total, 1.8 * t);  // some CU has two
         }
         const long slots = splits + t_splits;
         if (slots > 1) total += 3 + slots * cols * heads * (kD + 2) * 8 / 6.0e6;
