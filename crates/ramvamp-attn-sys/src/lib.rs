@@ -44,6 +44,7 @@ pub const RV_TUNE_DECODE_IMPL: i32 = 6;
 pub const RV_TUNE_KERNEL_TIMING: i32 = 7;
 pub const RV_TUNE_DECODE_DEPTH: i32 = 9;
 pub const RV_TUNE_DECODE_MERGE: i32 = 11;
+pub const RV_TUNE_ROWS_COLUMNS: i32 = 12;
 pub const RV_ELEM_F16: i32 = 1;
 pub const RV_ELEM_F32: i32 = 2;
 pub const RV_ELEM_Q8_0: i32 = 4;

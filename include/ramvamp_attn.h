@@ -370,6 +370,8 @@ int32_t rv_prefill_chunk(rv_kv* kv, size_t layer, const float* q_rows, const flo
 #define RV_TUNE_DECODE_DEPTH 9     /* 16-position tiles in flight per decode wave: 1 (default), 2 or 4 (f16 planes) */
 #define RV_TUNE_DECODE_MERGE 11    /* decode split merge: 0 auto, 1 inside the tile launch (a first level inside each
                                       XCD's L2, then across XCDs), 2 a second kernel */
+#define RV_TUNE_ROWS_COLUMNS 12    /* query columns (heads x rows) per workgroup of the row attention (Q8_0 chunks,
+                                      shared prefixes): 32, 64, 128 or 256 (0: by size); 64 not for f32 planes */
 int32_t rv_kv_set_tuning(rv_kv* kv, int32_t knob, int64_t value, rv_error* err);
 
 /* No reference counterpart: benchmark instrumentation. With

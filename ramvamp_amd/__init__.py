@@ -42,5 +42,6 @@ from ._lib import (  # noqa: F401  (knobs of KvCache.set_tuning)
     RV_TUNE_KERNEL_TIMING,
     RV_TUNE_PREFILL_KV_SPLIT,
     RV_TUNE_PREFILL_ROWS,
+    RV_TUNE_ROWS_COLUMNS,
 )
 from . import block, projections, router  # noqa: F401,E402

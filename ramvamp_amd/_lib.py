@@ -30,6 +30,7 @@ RV_TUNE_DECODE_IMPL = 6
 RV_TUNE_KERNEL_TIMING = 7
 RV_TUNE_DECODE_DEPTH = 9
 RV_TUNE_DECODE_MERGE = 11
+RV_TUNE_ROWS_COLUMNS = 12
 RV_NOALLOC_SCRATCH_BYTES = 8 << 20
 # include/ramvamp_gemv.h
 RV_QF_Q4_K = 1

@@ -1415,6 +1415,7 @@ int32_t rv_kv_set_tuning(rv_kv* kv, int32_t knob, int64_t value, rv_error* err) 
     case RV_TUNE_KERNEL_TIMING: kv->timing = value != 0; break;
     case RV_TUNE_DECODE_DEPTH: kv->tune_decode_depth = value; break;
     case RV_TUNE_DECODE_MERGE: kv->tune_decode_merge = value; break;
+    case RV_TUNE_ROWS_COLUMNS: kv->tune_rows_columns = value; break;
     default: return fail(err, RV_ERR_UNSUPPORTED, (uint64_t)knob, 0, 0, 0, "tuning knob");
   }
   return ok(err);

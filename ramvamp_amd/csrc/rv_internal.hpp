@@ -72,6 +72,7 @@ struct rv_kv {
   int64_t tune_decode_hg = 0;
   int64_t tune_decode_impl = 0;  // 0 auto (MFMA tiles: head_dim 128, group <= 16), 1 VALU subgroups, 3 LDS-staged tiles
   int64_t tune_decode_depth = 0;  // tiles in flight per wave (1, 2, 4); 0 auto
+  int64_t tune_rows_columns = 0;  // query columns per item of rv_rows.hip: 32, 64, 128, 256; 0 by size
   int64_t tune_decode_merge = 0;  // 0 auto, 1 in-launch XCD merge, 2 separate merge kernel
   // The dispatcher deals a launch's workgroups to the XCDs round robin on this
   // device (checked at rv_kv_new): the XCD merge may rely on it.

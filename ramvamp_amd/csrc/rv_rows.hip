@@ -1346,7 +1346,7 @@ void split_positions(long positions, long units, long want, int* n_splits, int* 
 // and store, and `c` per 128 positions (one workgroup a CU); a narrow one 6.4 and
 // 1.6 (f32 3.2), two a CU in 1.8 times that; a tail's four waves beside wide items
 // 10 and 2; a partial's floats are written and read once.
-void plan_shape(RowsPlan& p, long positions, long cols, long heads, int elem, long tails, long longest) {
+void plan_shape(RowsPlan& p, long positions, long cols, long heads, int elem, long tails, long longest, long columns) {
   const long steps = (positions + kPosStep - 1) / kPosStep;
   double best = 1e300;
   for (long t_want : {kCUs / 2, kCUs, 2 * kCUs}) {
@@ -1358,6 +1358,7 @@ void plan_shape(RowsPlan& p, long positions, long cols, long heads, int elem, lo
     const double t_steps = t_len / kPosStep;
     for (int wc : {0, 2, 4, 8}) {
       if (wc == 2 && elem == RV_ELEM_F32) continue;  // (its LDS tiles are twice as large)
+      if (columns && columns != (wc ? 32 * wc : 32)) continue;
       const double c = wc == 0                 ? (elem == RV_ELEM_F32 ? 3.2 : 1.6)
                        : elem == RV_ELEM_F32 ? (wc == 4 ? 5.5 : 9.0)
                        : elem == RV_ELEM_F16 ? (wc == 2 ? 2.4 : wc == 4 ? 3.05 : 5.0)
@@ -1416,7 +1417,9 @@ RowsPlan plan_rows(const RowsCall& c, const rv_kv* owner) {
   }
   const long tails = heads * p.t_cb * (long)p.rows;
   if (positions && (cols > 32 || causal)) {
-    plan_shape(p, positions, cols, heads, g->elem, tails, longest);
+    const long k = (long)owner->tune_rows_columns;
+    const bool known = k == 32 || (k == 64 && g->elem != RV_ELEM_F32) || k == 128 || k == 256;
+    plan_shape(p, positions, cols, heads, g->elem, tails, longest, known ? k : 0);
   } else {
     // One narrow block of columns a kv head. A decode's splits, 32 query heads over
     // 4 kv heads, us: 200 positions whole 6.3, in two 7.5; 400 in four 7.8, whole
@@ -1433,6 +1436,11 @@ RowsPlan plan_rows(const RowsCall& c, const rv_kv* owner) {
   }
   if (positions && owner->tune_decode_split_len > 0) {
     p.split_len = (int)((std::min<int64_t>(owner->tune_decode_split_len, 1 << 30) + kPosStep - 1) / kPosStep * kPosStep);
+    p.n_splits = (int)((positions + p.split_len - 1) / p.split_len);
+  }
+  if (positions && causal && owner->tune_prefill_kv_split > 0) {
+    const long n = std::min<long>(owner->tune_prefill_kv_split, (positions + kPosStep - 1) / kPosStep);
+    p.split_len = (int)(((positions + n - 1) / n + kPosStep - 1) / kPosStep * kPosStep);
     p.n_splits = (int)((positions + p.split_len - 1) / p.split_len);
   }
   // Splits folded by the launch: 1.3 us of its own against 4.3 for a second one,

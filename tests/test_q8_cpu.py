@@ -67,3 +67,26 @@ def test_null_arguments(lib):
     assert err.what == b"prefix"
     assert lib.rv_decode_step_shared(None, 0, 0, None, 0, 1, None, None, None, 1, None, 1, None, 1, 1e-6, 1e6, 1.0,
                                      None, 0, e) == 32
+
+
+def test_the_row_kernels_keep_their_operands_in_registers(tmp_path):
+    """What the compiled kernels ask of the card, read from the built library."""
+    import os
+    import re
+    import subprocess
+
+    from test_device_code import READELF, code_objects
+
+    if not os.path.exists(READELF):
+        pytest.skip("no llvm-readelf")
+    path, found = tmp_path / "object", 0
+    for obj in code_objects():
+        path.write_bytes(obj)
+        notes = subprocess.run([READELF, "--notes", str(path)], capture_output=True, text=True, check=True).stdout
+        for entry in notes.split("\n  - ")[1:]:
+            name = re.findall(r"^\s*\.name:\s+(_Z\S+)", entry, re.M)
+            if name and re.search(r"rows_(narrow|wide|merge)_kernel", name[-1]):
+                v = {k: int(x) for k, x in re.findall(r"^\s*\.(\w+):\s+(\d+)$", entry, re.M)}
+                assert v["vgpr_spill_count"] == 0 and v["private_segment_fixed_size"] == 0, name[-1]
+                found += 1
+    assert found >= 20
