@@ -1124,12 +1124,14 @@ __global__ __launch_bounds__(512) void rows_wide_kernel(RowsArgs a, std::conditi
   constexpr int kMain = wide_lds<T, WC>(), kTail = TAILS ? 2 * narrow_lds(1) : 0;
   __shared__ __attribute__((aligned(1024))) char lds[kMain > kTail ? kMain : kTail];
   const int b = blockIdx.x;
+  int positions = a.positions;
+  if (!device_positions(a.d_pos, a.positions, positions)) return;
   if (!TAILS || b < a.main_items) {
     int h, split, cb;
     if (!main_item(a, b, h, split, cb)) return;
     if (a.causal) cb = a.n_cb - 1 - cb;  // the longest first
     const int n_cols = a.rows * a.group, col0 = cb * 32 * WC;
-    long t_end = a.positions;
+    long t_end = positions;
     if (a.causal) {  // the last column's limit
       const int r = (min(col0 + 32 * WC, n_cols) - 1) / a.group;
       t_end = min(t_end, (long)a.start + r + 1);
@@ -1418,7 +1420,8 @@ RowsPlan plan_rows(const RowsCall& c, const rv_kv* owner) {
   const long tails = heads * p.t_cb * (long)p.rows;
   if (positions && (cols > 32 || causal)) {
     const long k = (long)owner->tune_rows_columns;
-    const bool known = k == 32 || (k == 64 && g->elem != RV_ELEM_F32) || k == 128 || k == 256;
+    // (narrow column blocks are a grid's z, 65535 at most)
+    const bool known = (k == 32 && cols <= 32 * 65535L) || (k == 64 && g->elem != RV_ELEM_F32) || k == 128 || k == 256;
     plan_shape(p, positions, cols, heads, g->elem, tails, longest, known ? k : 0);
   } else {
     // One narrow block of columns a kv head. A decode's splits, 32 query heads over

@@ -363,6 +363,32 @@ def test_device_position_step_in_a_graph():
                 assert np.array_equal(host(a), host(b))
 
 
+@pytest.mark.parametrize("n_kv,group,hd", [(2, 1, 128), (2, 20, 128), (2, 40, 128), (1, 72, 128), (2, 5, 64)])
+@pytest.mark.parametrize("n,most", [(0, 0), (3, 700), (300, 300), (300, 2500), (1030, 2500)])
+def test_device_position_of_every_group(n_kv, group, hd, n, most):
+    """What lies between the token's position and the planned one is not read:
+    rows of NaN."""
+    torch = torch_cuda()
+    say(f"case q8 device position {n_kv}x{group}x{hd} at {n} of {most}")
+    rng = np.random.default_rng(n + group)
+    kvd, qd, cap = n_kv * hd, n_kv * group * hd, 2501
+    kvs = [cache(np.random.default_rng(5), 1, n_kv, hd, n, cap=cap)[0] for _ in range(2)]
+    if most > n:
+        past = torch.full((most - n, kvd), float("nan"), device="cuda")
+        kvs[0].append_rows(0, past, past)
+    kvs[0].truncate(n)
+    q, k, v = (dev(rng.standard_normal(d).astype(np.float32)) for d in (qd, kvd, kvd))
+    wq, wk = (dev(rng.uniform(0.9, 1.1, hd).astype(np.float32)) for _ in range(2))
+    pos = torch.tensor([n], dtype=torch.int32, device="cuda")
+    got, want = (torch.full((qd,), float("nan"), device="cuda") for _ in range(2))
+    rv.decode_step_dev(kvs[0], 0, q, k, v, wq, wk, EPS, THETA, pos, most, scale_of(hd), got)
+    rv.decode_step(kvs[1], 0, q, k, v, wq, wk, EPS, THETA, n, scale_of(hd), want)
+    w = host(want)
+    # The same rows and query bits; the splits follow the plan's length.
+    d = np.abs(host(got).astype(np.float64) - w)
+    assert np.all(np.isfinite(w)) and d.max() <= 2.0 ** -17 * np.abs(w).max(), d.max()
+
+
 def test_graph_of_decodes_without_a_first_call():
     """rv_kv_new reserves what a decode needs: captured at once, replayed between
     eager calls that use the same workspace."""
