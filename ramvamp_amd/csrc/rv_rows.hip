@@ -253,31 +253,47 @@ __device__ __forceinline__ void raw_v2(const Raw<T>& x, int u, f16x8 (&hi)[2], f
   }
 }
 
-// The f16 hi and lo halves of a column's q', scaled by a power of two that
-// brings its largest value to [2^13, 2^14); N values a lane, the column's
-// lanes 16 and 32 apart (or 32 apart only). Returns the power back.
-template <int N, bool QUARTERS, bool HL>
-__device__ __forceinline__ float split_q(const float (&x)[N], f16x8 (&hi)[N / 8], f16x8 (&lo)[HL ? N / 8 : 1]) {
-  float amax = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) amax = fmaxf(amax, fabsf(x[i]));
-  if constexpr (QUARTERS) amax = swap_max<16>(amax);
-  amax = swap_max<32>(amax);
-  int ex = 14;
-  if (amax > 0.f && amax < INFINITY) (void)frexpf(amax, &ex);
-  const int k = max(ex - 14, -100);
-  const float down = ldexpf(1.f, -k);
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float v = x[i] * down;
-    const _Float16 h = (_Float16)v;
-    hi[i / 8][i % 8] = h;
-    if constexpr (HL) lo[i / 8][i % 8] = (_Float16)(v - (float)h);
-  }
-  return ldexpf(1.f, k);
+// x - hi, one instruction that reads the f16 half where it is. (A plain
+// subtraction widens the half first; the constant is kept from the compiler,
+// which would turn the product by it back into one.)
+__device__ __forceinline__ float minus_f16(float x, _Float16 hi) {
+  float minus_one = -1.f;
+  asm("" : "+s"(minus_one));
+  return __builtin_fmaf((float)hi, minus_one, x);
 }
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// The f16 hi and lo halves of a column's q' = q * qscale, scaled by a power of
+// two that brings its largest value to [2^13, 2^14); N values a lane, the
+// column's lanes 16 and 32 apart (or 32 apart only). Returns the power back.
+template <int N, bool QUARTERS, bool HL>
+__device__ __forceinline__ float split_q(const f32x4 (&q)[N / 4], float qscale, f16x8 (&hi)[N / 8],
+                                         f16x8 (&lo)[HL ? N / 8 : 1]) {
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) amax = fmaxf(fmaxf(amax, fabsf(q[i / 4][i % 4])), fabsf(q[i / 4][i % 4 + 1]));
+  if constexpr (QUARTERS) amax = swap_max<16>(amax);
+  amax = swap_max<32>(amax) * fabsf(qscale);
+  int ex = 14;
+  if (amax > 0.f && amax < INFINITY) (void)frexpf(amax, &ex);
+  const int k = max(ex - 14, -100);
+  const float c = ldexpf(qscale, -k);
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const f32x2 v = {q[i / 4][i % 4] * c, q[i / 4][i % 4 + 1] * c};
+    const f16x2 h = __builtin_convertvector(v, f16x2);
+    hi[i / 8][i % 8] = h[0];
+    hi[i / 8][i % 8 + 1] = h[1];
+    if constexpr (HL) {
+      const f32x2 r = {minus_f16(v[0], h[0]), minus_f16(v[1], h[1])};
+      const f16x2 t = __builtin_convertvector(r, f16x2);
+      lo[i / 8][i % 8] = t[0];
+      lo[i / 8][i % 8 + 1] = t[1];
+    }
+  }
+  return ldexpf(1.f, k);
+}
 
 // N probabilities as f16 hi (and lo) operand halves, and their sum added to l:
 // p = 2^(s * up + shift).
@@ -295,7 +311,7 @@ __device__ __forceinline__ void probabilities(const float (&s)[N], float up, flo
     hi[i / 8][i % 8] = h[0];
     hi[i / 8][i % 8 + 1] = h[1];
     if constexpr (HL) {
-      const f32x2 r = {__builtin_fmaf((float)h[0], -1.f, p[0]), __builtin_fmaf((float)h[1], -1.f, p[1])};
+      const f32x2 r = {minus_f16(p[0], h[0]), minus_f16(p[1], h[1])};
       const f16x2 t = __builtin_convertvector(r, f16x2);
       lo[i / 8][i % 8] = t[0];
       lo[i / 8][i % 8 + 1] = t[1];
@@ -376,13 +392,7 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
     const long w_first = CAUSAL ? min((long)a.start + row0 + min(col0, n_cols - 1) / a.group + 1, t_end) : t_end;
     f16x8 qh[NB][4], ql[NB][4];
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      const bool live = col0 + 16 * n + li < n_cols;
-      float y[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) y[i] = live ? qv[n][i >> 2][i & 3] * a.qscale : 0.f;
-      q_up[n] = split_q<32, true, true>(y, qh[n], ql[n]);
-    }
+    for (int n = 0; n < NB; ++n) q_up[n] = split_q<32, true, true>(qv[n], a.qscale, qh[n], ql[n]);
     for (int tile = wv; tile < n_tiles; tile += NW) {
       const long p0 = t_begin + 32L * tile;
       f32x4 s[NB][2][2];
@@ -871,13 +881,10 @@ __device__ void run_wide(const RowsArgs& a, const KvView& w, int h, int col0, in
   float q_up;
   {  // dims 16 c + 8 lh .. + 7 of each chunk c
     const float* qp = a.q + ((size_t)crow * a.n_q_heads + (size_t)hk * a.group + chead) * kD;
-    float x[64];
     f32x4 v[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = *reinterpret_cast<const f32x4u*>(qp + 16 * (i >> 1) + 8 * lh + 4 * (i & 1));
-#pragma unroll
-    for (int i = 0; i < 64; ++i) x[i] = live ? v[i >> 2][i & 3] * a.qscale : 0.f;
-    q_up = split_q<64, false, HL>(x, qh, ql);
+    q_up = split_q<64, false, HL>(v, a.qscale, qh, ql);
   }
   if constexpr (Q) {
     if (tid < 3 * (S / 32) * 4) (&nan_rows[0][0][0])[tid] = 0;
