@@ -135,10 +135,11 @@ __device__ __forceinline__ void load_raw_k(Raw<T>& x, const KvView& w, int h, lo
       x.ks[a] = sb[4 * r + lk];
     }
   } else {
-    const T* kb = reinterpret_cast<const T*>(w.k) + (size_t)h * kD + 32 * lk;
+    const T* kb = reinterpret_cast<const T*>(w.k) + (size_t)p0 * w.kv_dim + (size_t)h * kD;
+    const int left = (int)min(last - p0, 31L);
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
-      const T* r = kb + (size_t)min(p0 + 16 * a + li, last) * w.kv_dim;
+      const T* r = kb + ((uint32_t)min(16 * a + li, left) * (uint32_t)w.kv_dim + 32 * lk);
       constexpr int n = std::is_same<T, float>::value ? 8 : 4;
 #pragma unroll
       for (int c = 0; c < n; ++c)
@@ -159,10 +160,11 @@ __device__ __forceinline__ void load_raw_v(Raw<T>& x, const KvView& w, int h, lo
     x.vs[0] = *reinterpret_cast<const u32x2*>(vs);
     x.vs[1] = *reinterpret_cast<const u32x2*>(vs + 16);
   } else {
-    const T* vb = reinterpret_cast<const T*>(w.v) + (size_t)h * kD + 8 * li;
+    const T* vb = reinterpret_cast<const T*>(w.v) + (size_t)p0 * w.kv_dim + (size_t)h * kD;
+    const int left = (int)min(last - p0, 31L);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const T* r = vb + (size_t)min(p0 + 16 * (i >> 2) + 4 * lk + (i & 3), last) * w.kv_dim;
+      const T* r = vb + ((uint32_t)min(16 * (i >> 2) + 4 * lk + (i & 3), left) * (uint32_t)w.kv_dim + 8 * li);
       if constexpr (std::is_same<T, float>::value) {
         x.v[i][0] = reinterpret_cast<const f32x4*>(r)[0];
         x.v[i][1] = reinterpret_cast<const f32x4*>(r)[1];
@@ -1083,8 +1085,13 @@ __device__ __forceinline__ bool main_item(const RowsArgs& a, int b, int& h, int&
   return true;
 }
 
+template <typename T>
+constexpr int narrow_waves(int nb) {
+  return nb == 2 && !std::is_same<T, Q8>::value ? 1 : 2;
+}
+
 template <typename T, int NB, bool TAILS, bool CAUSAL>
-__global__ __launch_bounds__(256) void rows_narrow_kernel(RowsArgs a,
+__global__ __launch_bounds__(256, narrow_waves<T>(NB)) void rows_narrow_kernel(RowsArgs a,
                                                               std::conditional_t<TAILS, TailLens, NoLens> lens) {
   __shared__ __attribute__((aligned(16))) char lds[narrow_lds(NB)];
   const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
