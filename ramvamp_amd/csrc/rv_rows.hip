@@ -397,31 +397,43 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
     for (int n = 0; n < NB; ++n) q_up[n] = split_q<32, true, true>(qv[n], a.qscale, qh[n], ql[n]);
     for (int tile = wv; tile < n_tiles; tile += NW) {
       const long p0 = t_begin + 32L * tile;
-      f32x4 s[NB][2][2];
+      // Products of one sum follow each other at a distance: with one block of
+      // columns hi and lo are summed apart, with two in turn.
+      constexpr int SA = NB == 1 ? 2 : 1;
+      f32x4 s[NB][2][SA];
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) s[n][t][0] = s[n][t][1] = f32x4{};
+        for (int t = 0; t < 2; ++t) s[n][t][0] = s[n][t][SA - 1] = f32x4{};
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int c = 0; c < 4; ++c) {
+        f16x8 kh[2], kl[2];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          f16x8 kh, kl;
-          raw_k<T>(x, t, c, kh, kl);
+        for (int t = 0; t < 2; ++t) raw_k<T>(x, t, c, kh[t], kl[t]);
 #pragma unroll
-          for (int n = 0; n < NB; ++n) {
-            s[n][t][0] = mfma16(kh, qh[n][c], s[n][t][0]);
-            s[n][t][1] = mfma16(kh, ql[n][c], s[n][t][1]);
-            if constexpr (LO) s[n][t][1] = mfma16(kl, qh[n][c], s[n][t][1]);
-          }
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) s[n][t][0] = mfma16(kh[t], qh[n][c], s[n][t][0]);
+#pragma unroll
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) s[n][t][SA - 1] = mfma16(kh[t], ql[n][c], s[n][t][SA - 1]);
+        if constexpr (LO) {
+#pragma unroll
+          for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) s[n][t][SA - 1] = mfma16(kl[t], qh[n][c], s[n][t][SA - 1]);
         }
-      if (tile + NW < n_tiles) load_raw_k<T>(x, w, hk, p0 + 32 * NW, last, li, lk);
+      }
+      // (f16 by 32 columns has the registers for it one product later)
+      constexpr bool K_LATE = std::is_same<T, _Float16>::value && NB == 2;
+      if (!K_LATE && tile + NW < n_tiles) load_raw_k<T>(x, w, hk, p0 + 32 * NW, last, li, lk);
       f16x8 ph[NB], pl[NB];
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
         float y[8], mx = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = s[n][i >> 2][0][i & 3] + s[n][i >> 2][1][i & 3];
+        for (int i = 0; i < 8; ++i) y[i] = SA == 1 ? s[n][i >> 2][0][i & 3] : s[n][i >> 2][0][i & 3] + s[n][i >> 2][SA - 1][i & 3];
         if (p0 + 32 > w_first) {
           const int seen = (int)max(limit[n] - p0, 0L) - 4 * lk;  // of this quarter's rows 16 t + r
 #pragma unroll
@@ -490,6 +502,7 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
             o[n][2 * u + 1] = mfma16(vl[1], ph[n], o[n][2 * u + 1]);
           }
         }
+        if (K_LATE && u == 0 && tile + NW < n_tiles) load_raw_k<T>(x, w, hk, p0 + 32 * NW, last, li, lk);
       }
       if (tile + NW < n_tiles) load_raw_v<T>(x, w, hk, p0 + 32 * NW, last, li, lk);
     }
@@ -1087,7 +1100,7 @@ __device__ __forceinline__ bool main_item(const RowsArgs& a, int b, int& h, int&
 
 template <typename T>
 constexpr int narrow_waves(int nb) {
-  return nb == 2 && !std::is_same<T, Q8>::value ? 1 : 2;
+  return nb == 2 && Lo<T>::value ? 1 : 2;
 }
 
 template <typename T, int NB, bool TAILS, bool CAUSAL>
