@@ -1366,17 +1366,28 @@ void split_positions(long positions, long units, long want, int* n_splits, int* 
 // A launch's shape by the time each choice would take: whether its main items
 // are narrow (32 columns, 4 waves) or wide and of how many columns, and into how
 // many splits they and the tails are cut. The times (us) are fitted on this card
-// over chunks of 2..1000 rows and batches of 7..64 sequences at 0 .. 16000
-// positions; what counts is that they rank the choices as those measure (77 rows
-// at 901: narrow in 1, 3 splits 19.0, 16.3, wide with 2, 4, 8 waves of columns
-// 21.7, 22.7, 24.1; 200 at 1000: narrow 22.4, wide 31.3; 200 at 4000: 58.7, 53.0;
-// 512 at 3449: 100, wide with 4, 8 waves 85.8, 81; 64 x 16000 f16 in 16, 21, 25, 32
-// splits 64.7, 54.7, 67, 70). A wide item takes 14 to start, load its queries
-// and store, and `c` per 128 positions (one workgroup a CU); a narrow one 6.4 and
-// 1.6 (f32 3.2), two a CU in 1.8 times that; a tail's four waves beside wide items
-// 10 and 2; a partial's floats are written and read once.
-void plan_shape(RowsPlan& p, long positions, long cols, long heads, int elem, long tails, long longest, long columns) {
+// to 55 shapes, chunks of 5..1000 rows and batches of 8..128 sequences at 0..20000
+// positions, each in every column count and up to 25 split lengths; what counts is
+// that they rank the choices as those measure (the choice is the best one or
+// within 4 % of it in 51 of them, 6 to 11 % off in four). Both sides, us:
+// 77 rows at 901, narrow in 2, 3, 4 splits 16.3, 16.0, 18.6, wide with 2, 4, 8 waves
+// of columns 21.2, 22.4, 23.8; 200 at 4000, narrow whole, in 2, 5 splits 53.1, 49.9,
+// 56.4, wide 57.3, 52.4, 52.1; 512 at 1000, narrow 35.6, wide 57.9, 46.2, 43.7; 1000
+// at 12000, narrow 485, wide 539, 449, 386; 64 x 4000 Q8_0, narrow 26.8, wide 32.9,
+// 31.9, 34.3; 64 x 16000 f16 55.5, and 62.8, 53.8, 52.4.
+// A wide item takes a CU for 7.7 (starting, loading its queries, storing) and `c`
+// per 128 positions. A narrow one takes 5.3 and `n1` alone on its CU, 7.8 and `n2`
+// beside another (f32's registers leave no room for one). What the card does not
+// hold at once goes in rounds, which a chunk's items, the later ones longer, fill
+// in part. A tail is four waves' work of 1 to 2 per 128 positions, beside the main
+// items. A partial's floats are written and read once.
+void plan_shape(RowsPlan& p, long positions, long cols, long heads, int elem, long tails, long longest, long columns,
+                long chunk) {
   const long steps = (positions + kPosStep - 1) / kPosStep;
+  const bool f32 = elem == RV_ELEM_F32, f16 = elem == RV_ELEM_F16;
+  const double n1 = f32 ? 2.83 : f16 ? 1.3 : 1.28, n2 = f32 ? n1 : f16 ? 1.99 : 2.18;
+  const double share = 1 - 0.5 * chunk / positions;  // of the positions, that a chunk's rows see on the average
+  const long room = (f32 ? 1 : 2) * kCUs;  // narrow items at once
   double best = 1e300;
   for (long t_want : {kCUs / 2, kCUs, 2 * kCUs}) {
     int t_splits = 0, t_len = kPosStep;
@@ -1386,13 +1397,12 @@ void plan_shape(RowsPlan& p, long positions, long cols, long heads, int elem, lo
       continue;
     const double t_steps = t_len / kPosStep;
     for (int wc : {0, 2, 4, 8}) {
-      if (wc == 2 && elem == RV_ELEM_F32) continue;  // (its LDS tiles are twice as large)
+      if (wc == 2 && f32) continue;  // (its LDS tiles are twice as large)
       if (columns && columns != (wc ? 32 * wc : 32)) continue;
-      const double c = wc == 0                 ? (elem == RV_ELEM_F32 ? 3.2 : 1.6)
-                       : elem == RV_ELEM_F32 ? (wc == 4 ? 5.5 : 9.0)
-                       : elem == RV_ELEM_F16 ? (wc == 2 ? 2.4 : wc == 4 ? 3.05 : 5.0)
-                                             : (wc == 2 ? 2.7 : wc == 4 ? 3.5 : 5.9);
-      const double fixed = wc ? 14 : 6.4, t_tail = !t_splits ? 1 : wc ? 10 + 2.0 * t_steps : 6.4 + 1.2 * t_steps;
+      const double c = f32   ? (wc == 4 ? 6.2 : 9.1)
+                       : f16 ? (wc == 2 ? 2.5 : wc == 4 ? 3.4 : 5.55)
+                             : (wc == 2 ? 2.7 : wc == 4 ? 4.15 : 6.7);
+      const double t_tail = !t_splits ? 1 : wc ? 8.5 + 2.0 * t_steps : 5.3 + 1.13 * t_steps;
       const long t_wgs = wc ? (tails * t_splits + 1) / 2 : tails * t_splits;
       const long units = heads * ((cols + (wc ? 32 * wc : 32) - 1) / (wc ? 32 * wc : 32));
       long n = 1;
@@ -1402,19 +1412,36 @@ void plan_shape(RowsPlan& p, long positions, long cols, long heads, int elem, lo
         prev = splits;
         const long items = units * splits;
         if (items > 4 * kCUs && n > 1) break;
-        const double t = fixed + c * per;
         double total;
         if (wc) {
+          const double t = 7.7 + c * per, mean = 7.7 + c * per * share;
           // CUs the tails take meanwhile, one after the other on each.
           const long in_a_row = std::max(1L, (long)(t / t_tail)), t_cus = (t_wgs + in_a_row - 1) / in_a_row;
-          const long rounds = items + t_cus <= kCUs ? 1 : (long)((items * t + t_wgs * t_tail) / (kCUs * t)) + 1;
-          total = std::max(t * rounds, t_tail);
+          if (items + t_cus <= kCUs) {
+            total = std::max(t, t_tail);
+          } else {
+            total = t * ((items + kCUs - 1) / kCUs);
+            if (chunk)
+              total = std::max(t, std::min(total, items * mean / kCUs + 0.76 * t));
+            else
+              total = std::max(total, (items * t + t_wgs * t_tail) / kCUs + 0.1 * t);
+          }
         } else {
-          total = std::max(std::max(t, t_tail), 0.9 * (items * t + t_wgs * t_tail) / kCUs);
-          if (items > kCUs) total = std::max(total, 1.8 * t);  // some CU has two
+          const double alone = 5.3 + n1 * per, beside = f32 ? alone : 7.8 + n2 * per;
+          if (items + t_wgs <= kCUs) {
+            total = std::max(alone, t_tail);
+          } else if (items + t_wgs <= room) {
+            total = std::max(items > kCUs ? beside : alone + 0.24 * (beside - alone), t_tail);
+          } else {
+            const long rounds = (items + room - 1) / room;
+            const long fit = (rounds * room - items) * (long)(beside / t_tail);
+            total = rounds * beside;
+            if (chunk) total = std::max(beside, std::min(total, items * (7.8 + n2 * per * share) / room + 0.32 * beside));
+            total += 1.83 * t_tail * std::max(0L, t_wgs - fit) / room;
+          }
         }
         const long slots = splits + t_splits;
-        if (slots > 1) total += 3 + slots * cols * heads * (kD + 2) * 8 / 6.0e6;
+        if (slots > 1) total += 5.2 + slots * cols * heads * (kD + 2) * 8 / 7.6e6;
         if (total < best) {
           best = total;
           p.nb = wc ? 0 : 2;
@@ -1449,7 +1476,7 @@ RowsPlan plan_rows(const RowsCall& c, const rv_kv* owner) {
     const long k = (long)owner->tune_rows_columns;
     // (narrow column blocks are a grid's z, 65535 at most)
     const bool known = (k == 32 && cols <= 32 * 65535L) || (k == 64 && g->elem != RV_ELEM_F32) || k == 128 || k == 256;
-    plan_shape(p, positions, cols, heads, g->elem, tails, longest, known ? k : 0);
+    plan_shape(p, positions, cols, heads, g->elem, tails, longest, known ? k : 0, causal ? (long)c.rows : 0);
   } else {
     // One narrow block of columns a kv head. A decode's splits, 32 query heads over
     // 4 kv heads, us: 200 positions whole 6.3, in two 7.5; 400 in four 7.8, whole
