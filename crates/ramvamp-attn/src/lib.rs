@@ -46,6 +46,9 @@ pub enum Elem {
     F16,
     /// 4-byte f32 elements, the same [layer][capacity][kv_dim] indexing.
     F32,
+    /// Blocks of 32 values, int8 codes and an f16 scale (no counterpart there):
+    /// 8.5 bits a value. Rows are read with `read_rows`.
+    Q8_0,
 }
 
 fn no_error() -> sys::rv_error {
@@ -206,6 +209,7 @@ impl KvCache {
         let code = match elem {
             Elem::F16 => sys::RV_ELEM_F16,
             Elem::F32 => sys::RV_ELEM_F32,
+            Elem::Q8_0 => sys::RV_ELEM_Q8_0,
         };
         let rc = unsafe { sys::rv_kv_new(n_layers, n_kv_heads, head_dim, capacity, code, device, &mut raw, &mut e) };
         kv_result(rc, &e, (n_layers, n_kv_heads, head_dim, capacity))?;
@@ -311,7 +315,7 @@ impl KvCache {
                 n_kv_heads: self.n_kv_heads(),
                 head_dim: self.head_dim(),
                 capacity: self.capacity(),
-                reason: "f16 rows of an f32 cache: use k_row_f32 / v_row_f32",
+                reason: "f16 rows of another cache: use k_row_f32 / v_row_f32 (f32) or read_rows",
             });
         }
         let mut out = vec![0u16; self.kv_dim()];
@@ -330,7 +334,7 @@ impl KvCache {
                 n_kv_heads: self.n_kv_heads(),
                 head_dim: self.head_dim(),
                 capacity: self.capacity(),
-                reason: "f32 rows of an f16 cache: use k_row / v_row",
+                reason: "f32 rows of another cache: use k_row / v_row (f16) or read_rows",
             });
         }
         let mut out = vec![0f32; self.kv_dim()];
@@ -360,6 +364,44 @@ impl KvCache {
     /// `v_row` of an f32 cache.
     pub fn v_row_f32(&self, layer: usize, pos: usize) -> Result<Vec<f32>, KvError> {
         self.row_f32(1, layer, pos)
+    }
+
+    /// Rows `pos .. pos + rows` of a layer as f32, (k, v), whatever the element
+    /// type (no counterpart there).
+    pub fn read_rows(&self, layer: usize, pos: usize, rows: usize) -> Result<(Vec<f32>, Vec<f32>), KvError> {
+        let n = rows.checked_mul(self.kv_dim()).filter(|_| rows <= self.capacity()).unwrap_or(0);
+        let (mut k, mut v) = (vec![0f32; n], vec![0f32; n]);
+        let mut e = no_error();
+        let rc = unsafe {
+            sys::rv_kv_read_rows(self.raw.as_ptr(), layer, pos, rows, k.as_mut_ptr(), v.as_mut_ptr(), sys::RV_HOST_PTRS,
+                                 &mut e)
+        };
+        kv_result(rc, &e, self.geometry())?;
+        Ok((k, v))
+    }
+
+    /// One row to each of the `k.len() / kv_dim` layers from `layer0` on, all or
+    /// none (no counterpart there: a batch's sequences as layers).
+    pub fn append_each(&mut self, layer0: usize, k: &[f32], v: &[f32]) -> Result<(), KvError> {
+        let d = self.kv_dim();
+        for (len, what) in [(k.len(), "k"), (v.len(), "v")] {
+            if len % d != 0 || len != k.len() {
+                return Err(KvError::RowLenMismatch { what, got: len, expected: k.len() / d * d });
+            }
+        }
+        let mut e = no_error();
+        let rc = unsafe {
+            sys::rv_kv_append_each(self.raw.as_ptr(), layer0, k.len() / d, k.as_ptr(), v.as_ptr(), d, sys::RV_HOST_PTRS,
+                                   &mut e)
+        };
+        kv_result(rc, &e, self.geometry())
+    }
+
+    /// `truncate` of one layer (no counterpart there).
+    pub fn truncate_layer(&mut self, layer: usize, new_len: usize) -> Result<(), KvError> {
+        let mut e = no_error();
+        let rc = unsafe { sys::rv_kv_truncate_layer(self.raw.as_ptr(), layer, new_len, &mut e) };
+        kv_result(rc, &e, self.geometry())
     }
 
     fn layer_view(&self, plane_v: bool, layer: usize) -> Result<DeviceSlice<'_>, KvError> {
@@ -586,4 +628,34 @@ pub fn attention_at_kv_range_in_dispatch(
 ) -> Result<(), AttentionError> {
     let _ = force_scalar;
     attention_at_kv_range_in(q, cache, layer, positions, scale, kv_heads, scratch, out)
+}
+
+/// One token of each of `q_rows.len() / q_dim` sequences that share the first
+/// `prefix_positions` rows of `prefix`'s layer `prefix_layer`; sequence i's own
+/// rows are layer `tail_layer + i` of `tails` (no counterpart there: the server's
+/// reused prefix for several requests at once).
+pub fn decode_attention_shared(
+    q_rows: &[f32],
+    q_dim: usize,
+    prefix: &KvCache,
+    prefix_layer: usize,
+    prefix_positions: usize,
+    tails: &KvCache,
+    tail_layer: usize,
+    scale: f32,
+    out: &mut [f32],
+) -> Result<(), AttentionError> {
+    if q_dim == 0 || q_rows.len() % q_dim != 0 {
+        return Err(AttentionError::QLenIndivisible { q_len: q_rows.len(), head_dim: tails.head_dim() });
+    }
+    if out.len() != q_rows.len() {
+        return Err(AttentionError::OutLenMismatch { out_len: out.len(), expected: q_rows.len() });
+    }
+    let mut e = no_error();
+    let rc = unsafe {
+        sys::rv_decode_attention_shared(prefix.raw(), prefix_layer, prefix_positions, tails.raw(), tail_layer,
+                                        q_rows.as_ptr(), q_rows.len() / q_dim, q_dim, scale, out.as_mut_ptr(),
+                                        sys::RV_HOST_PTRS, &mut e)
+    };
+    attn_result(rc, &e)
 }

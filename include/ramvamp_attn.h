@@ -92,7 +92,7 @@ typedef enum rv_elem { RV_ELEM_F16 = 1, RV_ELEM_F32 = 2, RV_ELEM_Q8_0 = 4 } rv_e
  * 65504 in magnitude, and EXACT keeps its ~2^-21 relative products only for
  * values above f16's normal minimum (2^-14); BF16 has fp32's range. On a
  * Q8_0 cache K and V are f16 operands as stored; EXACT splits q and P into hi
- * + lo halves, F16 and BF16 both round them to f16, q scaled into its range. */
+ * + lo halves, F16 and BF16 both may round them to f16, q scaled into its range. */
 #define RV_PREFILL_EXACT 0x00u /* split-f16 MFMA, fp32-equivalent products */
 #define RV_PREFILL_F16 0x10u   /* single-pass f16 MFMA inputs, fp32 accumulate */
 #define RV_PREFILL_BF16 0x20u  /* single-pass bf16 MFMA inputs, fp32 accumulate */
@@ -278,7 +278,7 @@ int32_t rv_decode_attention_shared(const rv_kv* prefix, size_t prefix_layer, siz
  * `tails`, then rv_decode_attention_shared. q_rows, k_rows and v_rows are
  * pre-norm, n_seqs rows each. head_dim and the norm weights are checked first,
  * then as above with RV_KV_CAPACITY_EXCEEDED for the first full layer in place
- * of the empty one. */
+ * of the empty one. A captured call replays with the lengths of its capture. */
 int32_t rv_decode_step_shared(const rv_kv* prefix, size_t prefix_layer, size_t prefix_positions, rv_kv* tails,
                               size_t tail_layer, size_t n_seqs, const float* q_rows, const float* k_rows,
                               const float* v_rows, size_t q_dim, const float* q_norm_w, size_t q_norm_len,

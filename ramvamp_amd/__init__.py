@@ -5,7 +5,9 @@ ABI in include/ramvamp_attn.h, ramvamp_gemv.h and ramvamp_block.h). This package
 builds it (``build``), loads it (``_lib``), mirrors the reference's Rust
 attention API (``attention``) and quantized projections (``projections``)
 over it, one layer's attention block as a single device call (``block``),
-and makes seeded synthetic inputs (``synth``).
+and makes seeded synthetic inputs (``synth``). Beyond the reference, a cache may
+hold its rows in Q8_0 blocks (``KvCache(..., "q8_0")``), and a batch of sequences
+may decode over a prefix held once (``decode_step_shared``).
 """
 from .attention import (  # noqa: F401
     AttentionError,

@@ -15,8 +15,10 @@
 // Bound by bytes, 4 in and 34/32 out per value, as long as a thread's share of a
 // block is large enough to spread the block's own work (two divisions, the
 // scale's rounding) over it: eight values a thread, four lanes a block (the
-// maximum over them is two DPP steps); with four values a thread and roundf
-// 4096 rows of 512 took 8.8 us, bound by vector operations.
+// maximum over them is two DPP steps). 4096 rows of 512, both planes: 16.8 MB in
+// and 4.5 out in 6.0 us (3.5 TB/s; vector instructions are 60 % of the cycles),
+// where four values a thread and roundf took 8.8; the rows read back, 4.5 in and
+// 16.8 out, in 6.9 (3.1 TB/s, mostly stores).
 #include "rv_rows.hpp"
 
 #include <algorithm>

@@ -11,7 +11,11 @@
 // with q' = q * scale * log2(e) and m the running maximum. K and V are f16
 // matrix operands as stored (Q8_0: f16(scale * code); f32 planes: hi + lo
 // halves); q' and p are split into f16 hi + lo halves whose products are
-// summed in f32, which keeps fp32-equivalent products.
+// summed in f32, which keeps fp32-equivalent products: a column over a position
+// of 128 dims is 1024 operations (f32 planes 1536), and K and V are read once for
+// all columns of an item. One token is bound by those bytes or, up to some
+// thousand positions, by the launch's own latencies; from about 100 columns a kv
+// head on by the matrix and vector instructions.
 #include "rv_rows.hpp"
 
 #include <algorithm>
@@ -102,6 +106,16 @@ __device__ __forceinline__ void split8(const float (&x)[8], f16x8& hi, f16x8& lo
 // scale); V's lane (li, lk) dims 8 li .. + 7 of the rows whose probabilities
 // the scores' C layout gives quarter lk: 4 lk .. + 3 and 16 + 4 lk .. + 3, so
 // that P needs no exchange. Output tile b holds dims 8 i + b.
+//
+// For one token's columns it is the bytes that count: 131000 Q8_0 positions, 143
+// MB, 29 us (4.9 TB/s, a large copy's rate); 4097 positions 6.1 and the merge 4.3; of
+// 100 positions' 5.4 us 1.6 are the tile, the rest the way to its loads and the
+// waves' fold. With the tiles through LDS the whole calls took 166, 26 and 13.6
+// where they now take 33, 10.3 and 6.1. With 32 columns, a tile is 64 products
+// (1024 cycles of a SIMD) and about 360 vector instructions (1440), 208 of them the
+// codes' conversion, and two workgroups a CU, which 256 registers a wave allow,
+// run one's products beside the other's vector work: 32 sequences over 8192
+// positions 31.4 us with one, 25.8 with two.
 template <typename T>
 struct Raw;
 template <>
@@ -855,6 +869,15 @@ __device__ __forceinline__ void store_share(const Share<T, S>& x, char* lds, lon
 // wp) takes columns 32 wc .. and the 32-row subtiles wp, wp + WP, ... of each
 // step. The next step's rows are in flight while this one's are computed, and
 // its tiles the other half of the LDS.
+//
+// Eight waves convert a tile once for up to 256 columns, where the narrow items
+// would convert it eight times: a step of 64 rows by 256 columns takes 3.5 us, half
+// of it matrix instructions, the softmax and the conversion the rest (1000 rows
+// at 12000 positions: 57 % and 34 % of the SIMDs' cycles; 410 GFLOP in 380 us, 1.08
+// PFLOP/s, as much as a large f16 product reaches on this card under its power
+// limit). Two such workgroups a CU with half the columns each, the
+// instruction priority moved with the phases, or K's staging between the
+// subtiles measured the same or slower (512 rows at 3449: 79, 80 and 79 us).
 template <int WC>
 constexpr int wide_step() {
   return WC == 2 ? 128 : 64;
@@ -1177,7 +1200,10 @@ __global__ __launch_bounds__(512) void rows_wide_kernel(RowsArgs a, std::conditi
 // Folds the columns' partials, slots in an order that depends on their number
 // alone. A wave has 16 bytes (i = 0..15) of a block of 32 columns, lane (column,
 // half) dims 8 i + 4 half .. + 3; G waves share the slots of one, four loads in
-// flight each, and meet in LDS.
+// flight each, and meet in LDS. Bound by the partials' bytes where there are many
+// (1000 rows in two splits: 33 MB in, 16 out, 11.8 us, 4.2 TB/s), by a launch and two
+// dependent loads, 4 us, where there are few. G by the slots: 33 slots by one
+// wave of 4 loads at a time would be 9 trips to memory, by 16 waves it is one.
 template <int G, bool TAILS>
 __global__ __launch_bounds__(64 * (G < 4 ? 4 : G)) void rows_merge_kernel(
     RowsArgs a, int narrow, std::conditional_t<TAILS, TailLens, NoLens> lens) {
