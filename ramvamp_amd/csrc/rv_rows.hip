@@ -89,13 +89,29 @@ constexpr int stage_bytes(int positions) {
   return positions / 32 * 2 * kTileB * (Lo<T>::value ? 2 : 1);
 }
 
+// x - hi, one instruction that reads the f16 half where it is. (A plain
+// subtraction widens the half first; the constant is kept from the compiler,
+// which would turn the product by it back into one.)
+__device__ __forceinline__ float minus_f16(float x, _Float16 hi) {
+  float minus_one = -1.f;
+  asm("" : "+s"(minus_one));
+  return __builtin_fmaf((float)hi, minus_one, x);
+}
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
 // Eight f32 values as f16 hi and lo halves.
 __device__ __forceinline__ void split8(const float (&x)[8], f16x8& hi, f16x8& lo) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const _Float16 h = (_Float16)x[e];
-    hi[e] = h;
-    lo[e] = (_Float16)(x[e] - (float)h);
+  for (int e = 0; e < 8; e += 2) {
+    const f32x2 v = {x[e], x[e + 1]};
+    const f16x2 h = __builtin_convertvector(v, f16x2);
+    const f32x2 r = {minus_f16(v[0], h[0]), minus_f16(v[1], h[1])};
+    const f16x2 l = __builtin_convertvector(r, f16x2);
+    hi[e] = h[0];
+    hi[e + 1] = h[1];
+    lo[e] = l[0];
+    lo[e + 1] = l[1];
   }
 }
 
@@ -268,17 +284,6 @@ __device__ __forceinline__ void raw_v2(const Raw<T>& x, int u, f16x8 (&hi)[2], f
       for (int i = 0; i < 8; ++i) hi[k][i] = x.v[i][2 * u + k];
   }
 }
-
-// x - hi, one instruction that reads the f16 half where it is. (A plain
-// subtraction widens the half first; the constant is kept from the compiler,
-// which would turn the product by it back into one.)
-__device__ __forceinline__ float minus_f16(float x, _Float16 hi) {
-  float minus_one = -1.f;
-  asm("" : "+s"(minus_one));
-  return __builtin_fmaf((float)hi, minus_one, x);
-}
-
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // The f16 hi and lo halves of a column's q' = q * qscale, scaled by a power of
 // two that brings its largest value to [2^13, 2^14); N values a lane, the
