@@ -266,9 +266,9 @@ int32_t rv_attention_at_rows(const rv_kv* kv, const float* q_rows, size_t rows, 
  * Checks, in order: the two caches' geometry, element type, device and stream
  * (RV_ERR_UNSUPPORTED where they differ), q_dim, the prefix's layer and
  * positions, the tails' layers, empty sequences. Work is queued on that
- * stream; `tails`' workspace is used. F32 planes pass through f16 hi + lo
- * operands as RV_PREFILL_EXACT's do: magnitudes below 65504, and the full
- * precision above 2^-14. */
+ * stream; `tails`' workspace is used. F32 planes take any finite values: they
+ * pass through f16 hi + lo operands, rows scaled by powers of two, to 2^-22 of
+ * themselves or 2^-34 of the largest row's. */
 int32_t rv_decode_attention_shared(const rv_kv* prefix, size_t prefix_layer, size_t prefix_positions,
                                    const rv_kv* tails, size_t tail_layer, const float* q_rows, size_t n_seqs,
                                    size_t q_dim, float scale, float* out, uint32_t flags, rv_error* err);

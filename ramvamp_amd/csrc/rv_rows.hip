@@ -89,6 +89,61 @@ constexpr int stage_bytes(int positions) {
   return positions / 32 * 2 * kTileB * (Lo<T>::value ? 2 : 1);
 }
 
+// ---- the range of f32 planes ----------------------------------------------------------
+// hi + lo f16 halves hold a value to 2^-22 of itself between 2^-3 and 2^15, and
+// to 2^-25 below. Rows computed together are scaled by a power of two that keeps
+// their largest magnitude in [2^9, 2^15), so that any finite values keep 2^-22 of
+// themselves or 2^-34 of the largest: K's per tile, undone on the scores; V's by a
+// running exponent that follows the largest value seen, the outputs so far scaled
+// along.
+__device__ __forceinline__ float wave_max(float x) { return swap_max<32>(swap_max<16>(group_max<16>(x))); }
+__device__ __forceinline__ uint32_t uniform_bits(float x) {
+  return (uint32_t)__builtin_amdgcn_readfirstlane(__float_as_int(x));
+}
+__device__ __forceinline__ float power(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+
+// The largest magnitude of N values (NaN does not count).
+template <int N, typename F>
+__device__ __forceinline__ float largest(const F& at) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) m = fmaxf(fmaxf(m, fabsf(at(i))), fabsf(at(i + 1)));
+  return m;
+}
+
+// The exponent for values whose largest magnitude has the bits `m` (wave-uniform),
+// `e` if that still holds them (or they hold an infinity).
+__device__ __forceinline__ int range_exponent(uint32_t m, int e) {
+  if (m == 0 || m >= 0x7F800000u) return e;
+  const int x = (int)(m >> 23) - 127;  // in [2^x, 2^(x + 1)); subnormal: -127
+  return x >= e + 15 || x < e + 9 ? min(max(x - 13, -110), 114) : e;
+}
+
+struct VRange {  // wave-uniform
+  int e = 0;
+  uint32_t seen = 0;
+  // Takes in values of largest magnitude m (its bits, which order as it does).
+  // True: the outputs so far are to be scaled by `by`.
+  __device__ __forceinline__ bool take(uint32_t m, float& by) {
+    const bool outputs = seen != 0;
+    if (m < 0x7F800000u) seen = max(seen, m);
+    const int before = e;
+    e = range_exponent(seen, e);
+    by = power(max(before - e, -126));
+    return outputs && e != before;
+  }
+  // The partial's outputs unscaled. Past 2^60 it takes another form of the same
+  // value, o, l and 2^m by 2^40, so that p v stays finite.
+  template <typename O>
+  __device__ __forceinline__ void undo(float& m, float& l, const O& scale_outputs) const {
+    if (e == 0) return;
+    const int sh = e > 60 ? 40 : 0;
+    m += (float)sh;
+    l *= power(-sh);
+    scale_outputs(power(e - sh));
+  }
+};
+
 // x - hi, one instruction that reads the f16 half where it is. (A plain
 // subtraction widens the half first; the constant is kept from the compiler,
 // which would turn the product by it back into one.)
@@ -381,6 +436,7 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
   float m_run[NB], l_run[NB];
   uint32_t taint = 0;  // bit n: column block n saw a NaN row of this lane's dims (Q8_0, causal)
   f32x4 o[NB][8];
+  VRange range;  // (f32)
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     m_run[n] = -INFINITY;
@@ -416,6 +472,15 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
     for (int n = 0; n < NB; ++n) q_up[n] = split_q<32, true, true>(qv[n], a.qscale, qh[n], ql[n]);
     for (int tile = wv; tile < n_tiles; tile += NW) {
       const long p0 = t_begin + 32L * tile;
+      float k_up = 1.f;
+      if constexpr (LO) {
+        const int e = range_exponent(uniform_bits(wave_max(largest<64>([&](int i) { return x.k[i >> 5][(i >> 2) & 7][i & 3]; }))), 0);
+        if (e != 0) {
+          k_up = power(e);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x.k[i >> 3][i & 7] *= power(-e);
+        }
+      }
       // Products of one sum follow each other at a distance: with one block of
       // columns hi and lo are summed apart, with two in turn.
       constexpr int SA = NB == 1 ? 2 : 1;
@@ -444,8 +509,8 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
             for (int t = 0; t < 2; ++t) s[n][t][SA - 1] = mfma16(kl[t], qh[n][c], s[n][t][SA - 1]);
         }
       }
-      // (f16 by 32 columns has the registers for it one product later)
-      constexpr bool K_LATE = std::is_same<T, _Float16>::value && NB == 2;
+      // (f16 and f32 by 32 columns have the registers for it one product later)
+      constexpr bool K_LATE = !Q && NB == 2;
       if (!K_LATE && tile + NW < n_tiles) load_raw_k<T>(x, w, hk, p0 + 32 * NW, last, li, lk);
       f16x8 ph[NB], pl[NB];
 #pragma unroll
@@ -461,8 +526,9 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) mx = fmaxf(mx, y[i]);
+        const float up = LO ? q_up[n] * k_up : q_up[n];
         mx = swap_max<16>(mx);
-        mx = swap_max<32>(mx) * q_up[n];
+        mx = swap_max<32>(mx) * up;
         if (__builtin_amdgcn_ballot_w64(mx > m_run[n] + kSlack) != 0) {
           const float mn = fmaxf(m_run[n], mx), ms = mn == -INFINITY ? 0.f : mn;
           const float alpha = __builtin_amdgcn_exp2f(m_run[n] - ms);
@@ -473,11 +539,22 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
           for (int b = 0; b < 8; ++b) o[n][b] *= alpha;
         }
         f16x8 h1[1], l1[1];
-        probabilities<8, true>(y, q_up[n], kUp - m_sub[n], h1, l1, l_run[n]);
+        probabilities<8, true>(y, up, kUp - m_sub[n], h1, l1, l_run[n]);
         ph[n] = h1[0];
         pl[n] = l1[0];
       }
       if (p0 + 32 > t_end) mask_v<T>(x, p0, last, lk);
+      if constexpr (LO) {
+        float f;
+        if (range.take(uniform_bits(wave_max(largest<64>([&](int i) { return x.v[i >> 3][(i >> 2) & 1][i & 3]; }))), f)) {
+#pragma unroll
+          for (int i = 0; i < 8 * NB; ++i) o[i >> 3][i & 7] *= f;
+        }
+        if (range.e != 0) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x.v[i >> 1][i & 1] *= power(-range.e);
+        }
+      }
       if constexpr (Q && CAUSAL) {
         // A row's NaN scale makes its block NaN; it must not reach columns that do
         // not see the row (0 * NaN): it goes in as zero and the columns that see it
@@ -536,6 +613,11 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
     // Each lane summed its own rows: the other quarters of the column's.
     l_run[n] = swap_sum<16>(l_run[n]);
     l_run[n] = swap_sum<32>(l_run[n]);
+    if constexpr (LO)
+      range.undo(m_run[n], l_run[n], [&](float f) {
+#pragma unroll
+        for (int b = 0; b < 8; ++b) o[n][b] *= f;
+      });
     if (Q && CAUSAL && (taint & (1u << n))) {
 #pragma unroll
       for (int b = 0; b < 8; ++b) o[n][b] *= __builtin_nanf("");
@@ -698,8 +780,9 @@ __device__ __forceinline__ void load_share(Share<T, S>& x, const KvView& w, int 
         x.r[3 * i + 1] = c[1];
         x.r[3 * i + 2] = w.ks[row * 4 + (j >> 2)];
       } else {
-        const u32x4* p = reinterpret_cast<const u32x4*>(reinterpret_cast<const T*>(w.k) +
-                                                        (size_t)min(t, last) * w.kv_dim + (size_t)h * kD + 8 * j);
+        const T* base = reinterpret_cast<const T*>(w.k) + (size_t)t0 * w.kv_dim + (size_t)h * kD;
+        const uint32_t at = (uint32_t)min((tt >> 4) + 16 * i, (int)min(last - t0, S - 1L)) * (uint32_t)w.kv_dim + 8 * j;
+        const u32x4* p = reinterpret_cast<const u32x4*>(base + at);
 #pragma unroll
         for (int k = 0; k < Share<T, S>::kw / 4; ++k) {
           const u32x4 c = p[k];
@@ -729,8 +812,9 @@ __device__ __forceinline__ void load_share(Share<T, S>& x, const KvView& w, int 
         constexpr int n = std::is_same<T, float>::value ? 4 : 2;  // words of 4 dims
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const long t = min(b + (i & 3) + 8 * (i >> 2), last);
-          const T* p = reinterpret_cast<const T*>(w.v) + (size_t)t * w.kv_dim + (size_t)h * kD + 4 * j;
+          const T* base = reinterpret_cast<const T*>(w.v) + (size_t)t0 * w.kv_dim + (size_t)h * kD;
+          const int row = (int)(b - t0) + (i & 3) + 8 * (i >> 2);
+          const T* p = base + ((uint32_t)min(row, (int)min(last - t0, S - 1L)) * (uint32_t)w.kv_dim + 4 * j);
           typedef uint32_t uw __attribute__((ext_vector_type(n)));
           const uw c = *reinterpret_cast<const uw*>(p);
 #pragma unroll
@@ -929,17 +1013,44 @@ __device__ void run_wide(const RowsArgs& a, const KvView& w, int h, int col0, in
     for (int i = 0; i < 16; ++i) v[i] = *reinterpret_cast<const f32x4u*>(qp + 16 * (i >> 1) + 8 * lh + 4 * (i & 1));
     q_up = split_q<64, false, HL>(v, a.qscale, qh, ql);
   }
-  if constexpr (Q) {
-    if (tid < 3 * (S / 32) * 4) (&nan_rows[0][0][0])[tid] = 0;
+  f32x16 o[4];
+#pragma unroll
+  for (int d = 0; d < 4; ++d) o[d] = f32x16{};
+  // f32: the largest magnitudes of a step's K and V rows, by all waves that stage
+  // them, before any converts its share.
+  __shared__ uint32_t range_bits[2][2];
+  VRange range;
+  float k_up = 1.f;
+  const auto scale_share = [&](int slot) {
+    const float m = is_v ? largest<Share<T, S>::VU * 32>([&](int i) { return __uint_as_float(sh.r[i]); })
+                         : largest<Share<T, S>::KU * 8>([&](int i) { return __uint_as_float(sh.r[i]); });
+    const float w = wave_max(m);
+    if (lane == 0) atomicMax(&range_bits[slot][is_v], __float_as_uint(w));
+    __syncthreads();
+    const int ke = range_exponent(__builtin_amdgcn_readfirstlane(range_bits[slot][0]), 0);
+    k_up = power(ke);
+    if (tid < 2) range_bits[slot ^ 1][tid] = 0;
+    float f;
+    if (range.take(__builtin_amdgcn_readfirstlane(range_bits[slot][1]), f)) {
+#pragma unroll
+      for (int d = 0; d < 4; ++d) o[d] *= f;
+    }
+    const int e = is_v ? range.e : ke;
+    if (e != 0) {
+#pragma unroll
+      for (int i = 0; i < Share<T, S>::N; ++i) sh.r[i] = __float_as_uint(__uint_as_float(sh.r[i]) * power(-e));
+    }
+  };
+  if constexpr (Q || LO) {
+    if (Q && tid < 3 * (S / 32) * 4) (&nan_rows[0][0][0])[tid] = 0;
+    if (LO && tid < 2) range_bits[0][tid] = 0;
     __syncthreads();
   }
+  if constexpr (LO) scale_share(0);
   store_share<T, S>(sh, lds, t_begin, last, is_v, tt, Q ? nan_rows[0] : nullptr);
   __syncthreads();
 
   if (wave >= 4) __builtin_amdgcn_s_setprio(1);
-  f32x16 o[4];
-#pragma unroll
-  for (int d = 0; d < 4; ++d) o[d] = f32x16{};
   float m_run = -INFINITY, m_sub = 0.f, l_run = 0.f;
   uint32_t taint = 0;  // Q8_0: this lane's dims met a NaN block in a row its column sees
   int buf = 0, n3 = 0;
@@ -977,7 +1088,8 @@ __device__ void run_wide(const RowsArgs& a, const KvView& w, int h, int col0, in
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[i]);
-      mx = swap_max<32>(mx) * q_up;
+      const float up = LO ? q_up * k_up : q_up;
+      mx = swap_max<32>(mx) * up;
       if (__builtin_amdgcn_ballot_w64(mx > m_run + kSlack) != 0) {
         const float mn = fmaxf(m_run, mx), ms = mn == -INFINITY ? 0.f : mn;
         const float alpha = __builtin_amdgcn_exp2f(m_run - ms);
@@ -988,7 +1100,7 @@ __device__ void run_wide(const RowsArgs& a, const KvView& w, int h, int col0, in
         for (int d = 0; d < 4; ++d) o[d] *= alpha;
       }
       f16x8 ph[2], pl[2];
-      probabilities<16, HL>(x, q_up, kUp - m_sub, ph, pl, l_run);
+      probabilities<16, HL>(x, up, kUp - m_sub, ph, pl, l_run);
       if constexpr (Q) {
         // Lane (column, lh) holds dims of every block d.
         const u32x4 bad = *reinterpret_cast<const u32x4*>(nan_rows[n3][st]);
@@ -1022,12 +1134,22 @@ __device__ void run_wide(const RowsArgs& a, const KvView& w, int h, int col0, in
     }
     buf ^= 1;
     n3 = n3 == 2 ? 0 : n3 + 1;
-    if (more && LO) load_share<T, S>(sh, w, hk, t0 + S, last, is_v, tt);  // (no registers to hold it meanwhile)
+    if constexpr (LO) {
+      if (more) {
+        load_share<T, S>(sh, w, hk, t0 + S, last, is_v, tt);  // (no registers to hold it meanwhile)
+        scale_share(buf);
+      }
+    }
     if (more) store_share<T, S>(sh, lds + buf * kStage, t0 + S, last, is_v, tt, Q ? nan_rows[n3] : nullptr);
     __syncthreads();
   }
   // Each lane summed its own rows: the other half of the column's.
   l_run = swap_sum<32>(l_run);
+  if constexpr (LO)
+    range.undo(m_run, l_run, [&](float f) {
+#pragma unroll
+      for (int d = 0; d < 4; ++d) o[d] *= f;
+    });
   if constexpr (Q) {
     if (taint) {
 #pragma unroll

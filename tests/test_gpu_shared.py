@@ -5,7 +5,7 @@ import pytest
 
 import ramvamp_amd as rv
 from gpu_util import dev, host, say, torch_cuda
-from rows_util import attend, check, stored
+from rows_util import EPS32, LOG2E, attend, check, stored
 
 pytestmark = pytest.mark.gpu
 
@@ -84,6 +84,75 @@ def test_shared_decode(elem, n_kv, group, hd, prefix, tails):
     ho = np.full(q.shape, np.nan, np.float32)
     rv.decode_attention_shared(q, p, 1, prefix, t, 2, scale_of(hd), ho)
     assert np.array_equal(ho.view(np.uint32), got.view(np.uint32))
+
+
+@pytest.mark.parametrize("columns", [0, 32, 128, 256])
+@pytest.mark.parametrize("case", ["v_1e6", "v_1e-30", "v_1e37", "v_rows_1e-30_to_1e6", "v_later_larger", "v_later_smaller",
+                                  "v_zero_then_1e-30", "v_dims_1e-5", "k_rows_1e-25_to_1", "k_1e20_q_1e-20",
+                                  "k_1e-20_q_1e20", "k_1e-30"])
+def test_f32_planes_of_any_range(case, columns):
+    """Finite f32 values far outside f16's range, K's, V's and q's. On top of
+    rows_util's bounds, each value is held to 2^-22 of itself or 2^-34 of the
+    largest of the rows computed with it, whichever is larger."""
+    torch_cuda()
+    say(f"case f32 range {case} {columns}")
+    rng = np.random.default_rng(len(case))
+    n_kv, group, hd, prefix, tails = 2, 8, 128, 700, [0, 3, 70, 130, 31, 64, 1, 5, 9]
+    n, kvd = prefix, n_kv * hd
+    total = prefix + sum(tails)
+    k, v = (rng.standard_normal((total, kvd)) for _ in range(2))
+    q = rng.standard_normal((len(tails), n_kv * group * hd))
+    decades = rng.uniform(0, 1, (total, 1))
+    order = np.arange(total)[:, None]
+    if case == "v_1e6":
+        v *= 1e6
+    elif case == "v_1e-30":
+        v *= 1e-30
+    elif case == "v_1e37":
+        v *= 1e37
+    elif case == "v_rows_1e-30_to_1e6":
+        v *= 10.0 ** (-30 + 36 * decades)
+    elif case == "v_later_larger":
+        v *= np.where(order % prefix < 300, 1e-12, 1e4)
+    elif case == "v_later_smaller":
+        v *= np.where(order % prefix < 300, 1e9, 1e-6)
+    elif case == "v_zero_then_1e-30":
+        v *= np.where(order % prefix < 400, 0.0, 1e-30)
+    elif case == "v_dims_1e-5":
+        v[:, ::3] *= 1e-5
+    elif case == "k_rows_1e-25_to_1":
+        k *= 10.0 ** (-25 + 25 * decades)
+    elif case == "k_1e20_q_1e-20":
+        k, q = k * 1e20, q * 1e-20
+    elif case == "k_1e-20_q_1e20":
+        k, q = k * 1e-20, q * 1e20
+    elif case == "k_1e-30":
+        k *= 1e-30
+    k, v, q = (x.astype(np.float32) for x in (k, v, q))
+    p = rv.KvCache(1, n_kv, hd, prefix, "f32")
+    p.append_rows(0, dev(k[:n]), dev(v[:n]))
+    t = rv.KvCache(len(tails), n_kv, hd, max(tails), "f32")
+    for c in (p, t):
+        c.set_tuning(rv.RV_TUNE_ROWS_COLUMNS, columns)
+    out = dev(np.full(q.shape, np.nan, np.float32))
+    seqs, at = [], n
+    for i, m in enumerate(tails):
+        if m:
+            t.append_rows(i, dev(k[at:at + m]), dev(v[at:at + m]))
+        seqs.append((np.concatenate([k[:n], k[at:at + m]]), np.concatenate([v[:n], v[at:at + m]])))
+        at += m
+    rv.decode_attention_shared(dev(q), p, 0, n, t, 0, scale_of(hd), out)
+    got = host(out)
+    assert np.all(np.isfinite(got))
+    for i, (ki, vi) in enumerate(seqs):
+        want, a = attend(q[i], ki, vi, n_kv, hd, scale_of(hd))
+        terms, _ = attend(q[i], ki, np.abs(vi), n_kv, hd, scale_of(hd))
+        q1 = np.abs(q[i].reshape(-1, hd).astype(np.float64)).sum(-1).max() * scale_of(hd) * LOG2E
+        score = 37 * EPS32 * a + 2.0 ** -34 * q1 * np.abs(ki).max()
+        prob = np.log(2.0) * score + 2.0 ** -22
+        bound = terms * (2 * prob + 2.0 ** -22 + 96 * EPS32) + 2.0 ** -34 * float(np.abs(vi).max())
+        err = np.abs(got[i].astype(np.float64) - want)
+        assert np.all(err <= bound), (i, float(np.max(err / np.maximum(bound, 1e-300))))
 
 
 def test_more_sequences_than_one_launch_takes():
