@@ -1654,8 +1654,8 @@ RowsPlan plan_rows(const RowsCall& c, const rv_kv* owner) {
     p.n_splits = (int)((positions + p.split_len - 1) / p.split_len);
   }
   // Splits folded by the launch: 1.3 us of its own against 4.3 for a second one,
-  // while they are few.
-  p.fold = cols <= 32 && !c.tails && !causal && p.n_splits > 1 && p.n_splits <= kFold;
+  // while they are few (and their offsets within 31 bits).
+  p.fold = cols <= 32 && !c.tails && !causal && p.n_splits > 1 && p.n_splits <= kFold && heads < 4096;
   if (p.columns()) p.n_cb = (int)((cols + p.columns() - 1) / p.columns());
   return p;
 }
@@ -1740,7 +1740,9 @@ HipStatus launch_rows(rv_kv* owner, const RowsCall& c, hipStream_t s, const Work
     }
     base = (float*)ws->base;
   } else if (need) {
-    st = ensure_workspace(owner, need);
+    // Doubled (up to a GiB more), so that what a growing context or batch has
+    // outgrown, kept for the graphs captured over it, does not add up.
+    st = ensure_workspace(owner, need, std::min(2 * owner->ws_bytes, need + ((size_t)1 << 30)));
     if (st.e != hipSuccess) return st;
     base = (float*)owner->ws;
   }

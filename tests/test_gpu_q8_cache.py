@@ -389,6 +389,25 @@ def test_device_position_of_every_group(n_kv, group, hd, n, most):
     assert np.all(np.isfinite(w)) and d.max() <= 2.0 ** -17 * np.abs(w).max(), d.max()
 
 
+def test_the_workspace_of_a_growing_context_is_not_kept_at_every_size():
+    torch = torch_cuda()
+    say("case q8 workspace")
+    n_kv, group, hd, steps = 4, 8, 128, 200
+    kv = rv.KvCache(1, n_kv, hd, 128 * steps, "q8_0")
+    kv.set_tuning(rv.RV_TUNE_DECODE_SPLIT_LEN, 128)
+    x = torch.randn(128, n_kv * hd, device="cuda")
+    q = torch.randn(n_kv * group * hd, device="cuda")
+    out = torch.empty_like(q)
+    before = kv.device_bytes()[0]
+    for _ in range(steps):
+        kv.append_rows(0, x, x)
+        rv.decode_attention(q, kv, 0, scale_of(hd), None, out)
+    # The last call's splits, their 16 columns' values, maximum and sum each.
+    need = n_kv * steps * 16 * (hd + 2) * 4
+    # A buffer is at most twice what its call needed, those before it sum to no more.
+    assert kv.device_bytes()[0] - before <= 4 * need
+
+
 def test_graph_of_decodes_without_a_first_call():
     """rv_kv_new reserves what a decode needs: captured at once, replayed between
     eager calls that use the same workspace."""
