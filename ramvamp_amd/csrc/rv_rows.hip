@@ -19,6 +19,7 @@
 #include "rv_rows.hpp"
 
 #include <algorithm>
+#include <cfloat>
 
 namespace rv {
 namespace {
@@ -526,7 +527,7 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) mx = fmaxf(mx, y[i]);
-        const float up = LO ? q_up[n] * k_up : q_up[n];
+        const float up = LO ? fmaxf(q_up[n] * k_up, FLT_MIN) : q_up[n];  // (above zero: a masked score is -inf)
         mx = swap_max<16>(mx);
         mx = swap_max<32>(mx) * up;
         if (__builtin_amdgcn_ballot_w64(mx > m_run[n] + kSlack) != 0) {
@@ -1088,7 +1089,7 @@ __device__ void run_wide(const RowsArgs& a, const KvView& w, int h, int col0, in
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[i]);
-      const float up = LO ? q_up * k_up : q_up;
+      const float up = LO ? fmaxf(q_up * k_up, FLT_MIN) : q_up;  // (above zero: a masked score is -inf)
       mx = swap_max<32>(mx) * up;
       if (__builtin_amdgcn_ballot_w64(mx > m_run + kSlack) != 0) {
         const float mn = fmaxf(m_run, mx), ms = mn == -INFINITY ? 0.f : mn;

@@ -89,7 +89,7 @@ def test_shared_decode(elem, n_kv, group, hd, prefix, tails):
 @pytest.mark.parametrize("columns", [0, 32, 128, 256])
 @pytest.mark.parametrize("case", ["v_1e6", "v_1e-30", "v_1e37", "v_rows_1e-30_to_1e6", "v_later_larger", "v_later_smaller",
                                   "v_zero_then_1e-30", "v_dims_1e-5", "k_rows_1e-25_to_1", "k_1e20_q_1e-20",
-                                  "k_1e-20_q_1e20", "k_1e-30"])
+                                  "k_1e-20_q_1e20", "k_1e-30", "k_1e-33_q_1e-30"])
 def test_f32_planes_of_any_range(case, columns):
     """Finite f32 values far outside f16's range, K's, V's and q's. On top of
     rows_util's bounds, each value is held to 2^-22 of itself or 2^-34 of the
@@ -128,6 +128,8 @@ def test_f32_planes_of_any_range(case, columns):
         k, q = k * 1e-20, q * 1e20
     elif case == "k_1e-30":
         k *= 1e-30
+    elif case == "k_1e-33_q_1e-30":  # the scores' scale itself underflows
+        k, q = k * 1e-33, q * 1e-30
     k, v, q = (x.astype(np.float32) for x in (k, v, q))
     p = rv.KvCache(1, n_kv, hd, prefix, "f32")
     p.append_rows(0, dev(k[:n]), dev(v[:n]))
