@@ -197,6 +197,7 @@ class KvCache:
         self.elem = {L.RV_ELEM_F16: "f16", L.RV_ELEM_F32: "f32", L.RV_ELEM_Q8_0: "q8_0"}[_elem_code(elem)]
         self._stream = None
         self._kv_dim = n_kv_heads * head_dim
+        self._capacity = capacity
         self._torch_device = None
 
     new = classmethod(lambda cls, *a, **k: cls(*a, **k))
@@ -309,11 +310,12 @@ class KvCache:
 
             if self._torch_device is None:
                 self._torch_device = torch.device("cuda", self.device)
-            k = torch.empty((rows, self._kv_dim), dtype=torch.float32, device=self._torch_device)
+            n = rows if 0 <= rows <= self._capacity else 0  # (past it the call below refuses)
+            k = torch.empty((n, self._kv_dim), dtype=torch.float32, device=self._torch_device)
             v = torch.empty_like(k)
         ka, va = _Arg(k, writable=True), _Arg(v, writable=True)
         for a in (ka, va):
-            if a.host is not None and a.n != rows * self._kv_dim:
+            if a.host is not None and a.n != rows * self._kv_dim and 0 <= rows <= self._capacity:
                 raise ValueError("k and v must be rows x kv_dim")
         err = L.RvError()
         _check(_lib().rv_kv_read_rows(self._h, layer, start, rows, ka.ptr, va.ptr, _flags(self, (ka, va)),

@@ -128,6 +128,15 @@ def test_read_rows(elem, hd):
         kv.read_rows(2, 0, 3, k=k)
 
 
+@pytest.mark.parametrize("count", [134, 1 << 40, -1])
+def test_read_rows_past_the_capacity_allocates_nothing(count):
+    torch_cuda()
+    kv = rv.KvCache(1, 2, 128, 133, "q8_0")
+    with pytest.raises(rv.KvError) as e:
+        kv.read_rows(0, 0, count)
+    assert e.value.variant == "PositionOutOfRange"
+
+
 @pytest.mark.parametrize("n_kv,group,hd,n", GEOMETRIES)
 def test_decode(n_kv, group, hd, n):
     torch = torch_cuda()
