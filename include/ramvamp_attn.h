@@ -87,7 +87,8 @@ typedef enum rv_elem { RV_ELEM_F16 = 1, RV_ELEM_F32 = 2, RV_ELEM_Q8_0 = 4 } rv_e
 #define RV_HOST_PTRS 0x1u   /* tensor pointers are host memory */
 #define RV_SYNC 0x2u        /* synchronise the cache's stream before returning */
 /* Prefill arithmetic (rv_attention_at_rows / rv_prefill_chunk only; decode is
- * always fp32 arithmetic). Default (0) = RV_PREFILL_EXACT. EXACT and F16 take
+ * always fp32 arithmetic, on a Q8_0 cache and over a shared prefix split-f16
+ * products of its precision). Default (0) = RV_PREFILL_EXACT. EXACT and F16 take
  * their operands (q, K, V, and P <= 2^8) through f16: values must stay below
  * 65504 in magnitude, and EXACT keeps its ~2^-21 relative products only for
  * values above f16's normal minimum (2^-14); BF16 has fp32's range. On a
