@@ -203,3 +203,52 @@ def test_a_large_chunk_and_a_large_batch():
              for i in look]
     check(got[look], np.stack([w for w, _ in wants]), max(a for _, a in wants), np.abs(v16).max(), "batch")
     assert np.all(np.isfinite(got))
+
+
+@pytest.mark.parametrize("elem,row_bytes", [("q8_0", 128), ("f16", 256), ("f32", 512)])
+def test_planes_past_4_gib(elem, row_bytes):
+    """A layer whose rows pass 2^32 bytes: rows of zeros (score 0, value 0), but
+    some thousand around that offset, which carry all but 2^-15 of the weight."""
+    torch = torch_cuda()
+    say(f"case past 4 GiB {elem}")
+    rng = np.random.default_rng(row_bytes)
+    mark, group, d = (1 << 32) // row_bytes, 2, 128
+    lo, n = mark - 2500, mark + 1777
+    kv = rv.KvCache(2, 1, d, n, elem)
+    zeros = torch.zeros(1 << 20, d, device="cuda")
+    for at in range(0, lo, 1 << 20):
+        z = zeros[:min(1 << 20, lo - at)]
+        kv.append_rows(1, z, z)
+    k, v = rows(rng, n - lo, d), rows(rng, n - lo, d)
+    kv.append_rows(1, dev(k), dev(v))
+    got_k, got_v = kv.read_rows(1, n - 9, 9)
+    ks, vs = stored(k, elem), stored(v, elem)
+    assert np.array_equal(host(got_k), ks[-9:]) and np.array_equal(host(got_v), vs[-9:])
+    q = (8 * rng.standard_normal((3 if elem == "q8_0" else 20, group * d))).astype(np.float32)
+
+    def want(i, count):  # over the zero rows too, each a term of e^0 below
+        x = q[i].reshape(group, d).astype(np.float64) @ ks[:count].astype(np.float64).T * SCALE
+        p = np.exp(x - x.max(-1, keepdims=True))
+        below = p.sum(-1, keepdims=True) + lo * np.exp(-x.max(-1, keepdims=True))
+        a = np.abs(q[i].reshape(group, d)).astype(np.float64) @ np.abs(ks[:count]).T.astype(np.float64)
+        assert (lo * np.exp(-x.max(-1)) / below[:, 0]).max() < 2.0 ** -15
+        return (p / below @ vs[:count].astype(np.float64)).reshape(-1), a.max() * SCALE * 1.4426950408889634
+
+    vmax = np.abs(vs).max()
+    out = torch.full(q.shape, float("nan"), device="cuda")
+    if elem == "q8_0":
+        rv.decode_attention(dev(q[0]), kv, 1, SCALE, None, out[0])
+        w, a = want(0, n - lo)
+        check(host(out[0]), w, a, vmax, "decode")
+        rv.attention_at_rows(dev(q), kv, 1, n - 3, SCALE, out)
+        for i in range(3):
+            w, a = want(i, n - lo - 2 + i)
+            check(host(out[i]), w, a, vmax, f"chunk row {i}")
+    else:
+        tails = rv.KvCache(20, 1, d, 1, elem)
+        for columns in (32, 128):
+            tails.set_tuning(rv.RV_TUNE_ROWS_COLUMNS, columns)
+            rv.decode_attention_shared(dev(q), kv, 1, n, tails, 0, SCALE, out)
+            for i in (0, 11, 19):
+                w, a = want(i, n - lo)
+                check(host(out[i]), w, a, vmax, f"sequence {i}")
