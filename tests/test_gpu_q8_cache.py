@@ -486,6 +486,72 @@ def test_split_lengths_agree():
         check(host(out), want, a, np.abs(held[0][1]).max(), f"split {length}")
 
 
+def block_weights(rng, hidden, n_kv, group, hd):
+    torch = torch_cuda()
+    qd, kvd = n_kv * group * hd, n_kv * hd
+
+    def q80(rows_, cols):
+        b = np.zeros((rows_ * cols // 32, 34), np.uint8)
+        b[:, :2] = np.float16(0.003).tobytes()[0], np.float16(0.003).tobytes()[1]
+        b[:, 2:] = rng.integers(0, 256, (b.shape[0], 32))
+        return torch.from_numpy(b.reshape(-1)).cuda()
+
+    def q6k(rows_, cols):
+        b = rng.integers(0, 256, (rows_ * cols // 256, 210)).astype(np.uint8)
+        b[:, 192:208] = rng.integers(0, 20, (b.shape[0], 16))
+        b[:, 208:210] = np.frombuffer(np.float16(0.0004).tobytes(), np.uint8)
+        return torch.from_numpy(b.reshape(-1)).cuda()
+
+    return B.AttnBlockWeights(torch.ones(hidden, device="cuda"), P.Q6_K, q6k(qd, hidden), q80(kvd, hidden), P.Q6_K,
+                              q6k(kvd, hidden), torch.ones(hd, device="cuda"), torch.ones(hd, device="cuda"), P.Q6_K,
+                              q6k(hidden, qd))
+
+
+def test_the_block_s_token_graph():
+    """rv_attn_block_decode_dev captured once and replayed for every token over a
+    Q8_0 cache is rv_attn_block_decode (one split of the positions either way: the
+    same bits); a token past the plan leaves its residual as it was."""
+    torch = torch_cuda()
+    say("case q8 block graph")
+    rng = np.random.default_rng(18)
+    hidden, n_kv, group, hd, n, cap = 512, 4, 8, 128, 70, 75
+    qd = n_kv * group * hd
+    w = block_weights(rng, hidden, n_kv, group, hd)
+    graph_kv, eager_kv = (cache(np.random.default_rng(2), 1, n_kv, hd, n, cap=cap)[0] for _ in range(2))
+    pos = torch.tensor([n], dtype=torch.int32, device="cuda")
+    res = torch.zeros(hidden, device="cuda")
+    scratch = torch.empty(max(256, B.scratch_bytes(hidden, qd, n_kv * hd)), dtype=torch.uint8, device="cuda")
+
+    def token():
+        B.attn_block_decode_dev(graph_kv, 0, res, qd, w, EPS, THETA, pos, cap - 2, scale_of(hd), scratch)
+        rv.position_advance(graph_kv, pos)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        token()  # sizes the buffers
+        pos.fill_(n)
+        s.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            token()
+        for t in range(cap - 1 - n):
+            x = dev(rng.standard_normal(hidden).astype(np.float32))
+            res.copy_(x)
+            g.replay()
+            s.synchronize()
+            B.attn_block_decode(eager_kv, 0, x, qd, w, EPS, THETA, n + t, scale_of(hd))
+            assert np.array_equal(host(res), host(x)), t
+        x = dev(rng.standard_normal(hidden).astype(np.float32))
+        res.copy_(x)
+        g.replay()
+        s.synchronize()
+        assert np.array_equal(host(res), host(x))
+        with pytest.raises(rv.KvError) as e:
+            graph_kv.commit(0, cap - 1 - n)
+        assert e.value.variant == "CapacityExceeded"
+
+
 def test_the_layer_s_attention_block():
     """rv_attn_block_decode and _prefill over a Q8_0 cache are their parts."""
     torch = torch_cuda()
