@@ -1240,12 +1240,15 @@ __device__ void tail_item(const RowsArgs& a, const TailLens& lens, int b, int wv
                              t_begin < len, lds);
 }
 
-// Workgroup b of the main items: (kv head, split) units whose column blocks are
-// 8 apart, so that they run on one XCD and meet in its L2.
+// Workgroup b of the main items. Those of one XCD (b mod 8) are consecutive in
+// the order (kv head, split, column block), so that the column blocks of a split
+// meet in its L2, and every XCD has as many (600 rows at 3400, 19 blocks of 12
+// splits: 169 us with whole splits to an XCD, 90 so).
 __device__ __forceinline__ bool main_item(const RowsArgs& a, int b, int& h, int& split, int& cb) {
-  cb = (b % (8 * a.n_cb)) / 8;
-  const int u = (b / (8 * a.n_cb)) * 8 + b % 8;
-  if (u >= a.n_heads * a.n_splits) return false;
+  const int n = a.n_heads * a.n_splits * a.n_cb, i = (b & 7) * (a.main_items >> 3) + (b >> 3);
+  if (i >= n) return false;
+  cb = i % a.n_cb;
+  const int u = i / a.n_cb;
   split = u % a.n_splits;
   h = u / a.n_splits;
   return true;
@@ -1802,7 +1805,7 @@ HipStatus launch_rows(rv_kv* owner, const RowsCall& c, hipStream_t s, const Work
       a.t_cb = p.t_cb;
       a.t_splits = p.t_splits;
       a.t_split_len = p.t_split_len;
-      a.main_items = (a.n_heads * a.n_splits + 7) / 8 * 8 * a.n_cb;
+      a.main_items = (a.n_heads * a.n_splits * a.n_cb + 7) / 8 * 8;
       a.single = p.slots() == 1;
       a.tickets = p.fold ? xcd_tickets(owner) : nullptr;
       const unsigned tail_items = (unsigned)(n * a.n_heads * a.t_cb * a.t_splits);
