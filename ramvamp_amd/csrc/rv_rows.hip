@@ -1528,17 +1528,18 @@ void split_positions(long positions, long units, long want, int* n_splits, int* 
 // A launch's shape by the time each choice would take: whether its main items
 // are narrow (32 columns, 4 waves) or wide and of how many columns, and into how
 // many splits they and the tails are cut. The times (us) are fitted on this card
-// to 50 shapes, chunks of 5..1000 rows and batches of 8..128 sequences at 0..20000
-// positions, each in every column count and up to 25 split lengths; what counts is
-// that they rank the choices as those measure (the choice is the best one or
-// within 3 % of it in 47 of them, 7 to 10 % off in three). Both sides, us:
+// to 45 shapes, chunks of 5..1000 rows and batches of 8..100 sequences at 0..16000
+// positions, each in every column count and its better split lengths, four caches
+// in turn, as a model's layers are; what counts is that they rank the choices as
+// those measure (the choice is 0.8 % off the best one on the average). Both sides,
+// us, of one cache unless said:
 // 77 rows at 901, narrow in 2, 3, 4 splits 16.3, 16.0, 18.6, wide with 2, 4, 8 waves
-// of columns 21.2, 22.4, 23.8; 200 at 4000, narrow whole, in 2, 5 splits 53.1, 49.9,
-// 56.4, wide 57.3, 52.4, 52.1; 512 at 1000, narrow 35.6, wide 57.9, 46.2, 43.7; 1000
+// of columns 21.2, 22.4, 23.8; 200 at 4000, four caches, narrow 60.9, wide with 4, 8
+// waves 49.8, 47.1; 512 at 1000, narrow 35.6, wide 57.9, 46.2, 43.7; 1000
 // at 12000, narrow 485, wide 539, 449, 386; 64 x 4000 Q8_0, narrow 26.8, wide 32.9,
 // 31.9, 34.3; 64 x 16000 f16 55.5, and 62.8, 53.8, 52.4.
-// A wide item takes a CU for 7.3 (starting, loading its queries, storing) and `c`
-// per 128 positions. A narrow one takes 4.6 and `n1` alone on its CU, 7.2 and `n2`
+// A wide item takes a CU for 7.4 (starting, loading its queries, storing) and `c`
+// per 128 positions. A narrow one takes 5.4 and `n1` alone on its CU, 7.0 and `n2`
 // beside another (f32's registers leave no room for one). What the card does not
 // hold at once goes in rounds, which a chunk's items, the later ones longer, fill
 // in part. A tail is four waves' work of 1 to 2 per 128 positions, beside the main
@@ -1547,7 +1548,7 @@ void plan_shape(RowsPlan& p, long positions, long cols, long heads, int elem, lo
                 long chunk) {
   const long steps = (positions + kPosStep - 1) / kPosStep;
   const bool f32 = elem == RV_ELEM_F32, f16 = elem == RV_ELEM_F16;
-  const double n1 = f32 ? 3.2 : 1.24, n2 = f32 ? n1 : f16 ? 2.23 : 2.16;
+  const double n1 = f32 ? 2.87 : f16 ? 1.3 : 1.42, n2 = f32 ? n1 : f16 ? 2.39 : 2.27;
   const double share = 1 - 0.5 * chunk / positions;  // of the positions, that a chunk's rows see on the average
   const long room = (f32 ? 1 : 2) * kCUs;  // narrow items at once
   double best = 1e300;
@@ -1561,10 +1562,10 @@ void plan_shape(RowsPlan& p, long positions, long cols, long heads, int elem, lo
     for (int wc : {0, 2, 4, 8}) {
       if (wc == 2 && f32) continue;  // (its LDS tiles are twice as large)
       if (columns && columns != (wc ? 32 * wc : 32)) continue;
-      const double c = f32   ? (wc == 4 ? 7.45 : 10.4)
-                       : f16 ? (wc == 2 ? 2.57 : wc == 4 ? 3.35 : 5.96)
-                             : (wc == 2 ? 2.55 : wc == 4 ? 4.0 : 6.45);
-      const double t_tail = !t_splits ? 1 : wc ? 9.5 + 2.0 * t_steps : 4.6 + 1.07 * t_steps;
+      const double c = f32   ? (wc == 4 ? 7.86 : 10.1)
+                       : f16 ? (wc == 2 ? 2.72 : wc == 4 ? 3.62 : 5.96)
+                             : (wc == 2 ? 2.5 : wc == 4 ? 4.07 : 6.23);
+      const double t_tail = !t_splits ? 1 : wc ? 10.9 + 2.0 * t_steps : 5.4 + 1.05 * t_steps;
       const long t_wgs = wc ? (tails * t_splits + 1) / 2 : tails * t_splits;
       const long units = heads * ((cols + (wc ? 32 * wc : 32) - 1) / (wc ? 32 * wc : 32));
       long n = 1;
@@ -1576,7 +1577,7 @@ void plan_shape(RowsPlan& p, long positions, long cols, long heads, int elem, lo
         if (items > 4 * kCUs && n > 1) break;
         double total;
         if (wc) {
-          const double t = 7.3 + c * per, mean = 7.3 + c * per * share;
+          const double t = 7.4 + c * per, mean = 7.4 + c * per * share;
           // CUs the tails take meanwhile, one after the other on each.
           const long in_a_row = std::max(1L, (long)(t / t_tail)), t_cus = (t_wgs + in_a_row - 1) / in_a_row;
           if (items + t_cus <= kCUs) {
@@ -1584,26 +1585,26 @@ void plan_shape(RowsPlan& p, long positions, long cols, long heads, int elem, lo
           } else {
             total = t * ((items + kCUs - 1) / kCUs);
             if (chunk)
-              total = std::max(t, std::min(total, items * mean / kCUs + 0.84 * t));
+              total = std::max(t, std::min(total, items * mean / kCUs + 0.97 * t));
             else
-              total = std::max(total, (items * t + t_wgs * t_tail) / kCUs + 0.13 * t);
+              total = std::max(total, (items * t + t_wgs * t_tail) / kCUs + 0.12 * t);
           }
         } else {
-          const double alone = 4.6 + n1 * per, beside = f32 ? alone : 7.2 + n2 * per;
+          const double alone = 5.4 + n1 * per, beside = f32 ? alone : 7.0 + n2 * per;
           if (items + t_wgs <= kCUs) {
             total = std::max(alone, t_tail);
           } else if (items + t_wgs <= room) {
-            total = std::max(items > kCUs ? beside : alone + 0.52 * (beside - alone) * std::min(1.0, t_tail / alone), t_tail);
+            total = std::max(items > kCUs ? beside : alone + 0.3 * (beside - alone) * std::min(1.0, t_tail / alone), t_tail);
           } else {
             const long rounds = (items + room - 1) / room;
             const long fit = (rounds * room - items) * (long)(beside / t_tail);
             total = rounds * beside;
-            if (chunk) total = std::max(beside, std::min(total, items * (7.2 + n2 * per * share) / room + 0.34 * beside));
-            total += 2.0 * t_tail * std::max(0L, t_wgs - fit) / room;
+            if (chunk) total = std::max(beside, std::min(total, items * (7.0 + n2 * per * share) / room + 0.32 * beside));
+            total += 2.15 * t_tail * std::max(0L, t_wgs - fit) / room;
           }
         }
         const long slots = splits + t_splits;
-        if (slots > 1) total += 5.2 + slots * cols * heads * (kD + 2) * 8 / 7.8e6;
+        if (slots > 1) total += 4.6 + slots * cols * heads * (kD + 2) * 8 / 7.5e6;
         if (total < best) {
           best = total;
           p.nb = wc ? 0 : 2;
