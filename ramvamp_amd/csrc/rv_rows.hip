@@ -8,7 +8,7 @@
 //
 //   o[c] = sum_t p[c][t] v[t] / sum_t p[c][t],  p[c][t] = 2^(q'[c] . k[t] - m[c])
 //
-// with q' = q * scale * log2(e) and m the running maximum. K and V are f16
+// with q' = q * scale * log2(e) and m a base that follows the running maximum. K and V are f16
 // matrix operands as stored (Q8_0: f16(scale * code); f32 planes: hi + lo
 // halves); q' and p are split into f16 hi + lo halves whose products are
 // summed in f32, which keeps fp32-equivalent products: a column over a position
@@ -28,9 +28,9 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // as a c
 
 constexpr int kD = 128;
 constexpr float kLog2e = 1.4426950408889634f;
-// The running maximum moves when a score passes it by more than kSlack, and
-// probabilities carry a factor of 2^kUp (it cancels in o / l): they stay at or
-// below 2^14, inside f16, and small ones are kept off its subnormals.
+// Probabilities are taken relative to a base kUp below the running maximum (it
+// cancels in o / l), which moves when a score passes it by more than kUp + kSlack:
+// they stay at or below 2^14, inside f16.
 constexpr float kSlack = 8.f, kUp = 6.f;
 constexpr int kFold = 16;  // splits of a kv head that the launch folds itself
 
@@ -134,11 +134,12 @@ struct VRange {  // wave-uniform
     return outputs && e != before;
   }
   // The partial's outputs unscaled. Past 2^60 it takes another form of the same
-  // value, o, l and 2^m by 2^40, so that p v stays finite.
+  // value, o, l and 2^m by 2^64, so that p v stays finite (m's sum is exact up to
+  // scores of 2^30).
   template <typename O>
   __device__ __forceinline__ void undo(float& m, float& l, const O& scale_outputs) const {
     if (e == 0) return;
-    const int sh = e > 60 ? 40 : 0;
+    const int sh = e > 60 ? 64 : 0;
     m += (float)sh;
     l *= power(-sh);
     scale_outputs(power(e - sh));
@@ -152,6 +153,14 @@ __device__ __forceinline__ float minus_f16(float x, _Float16 hi) {
   float minus_one = -1.f;
   asm("" : "+s"(minus_one));
   return __builtin_fmaf((float)hi, minus_one, x);
+}
+
+// The base for scores of maximum mx. A score minus its base is exact, whatever the
+// scores' size; where their last bit weighs as much as kUp (from 2^25 on) mx - kUp
+// may round further down than that, and the base is the maximum itself.
+__device__ __forceinline__ float base_of(float mx) {
+  const float b = mx - kUp;
+  return mx - b > kUp ? mx : b;
 }
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -373,15 +382,15 @@ __device__ __forceinline__ float split_q(const f32x4 (&q)[N / 4], float qscale, 
 }
 
 // N probabilities as f16 hi (and lo) operand halves, and their sum added to l:
-// p = 2^(s * up + shift).
+// p = 2^(s * up - base), up a power of two.
 template <int N, bool HL>
-__device__ __forceinline__ void probabilities(const float (&s)[N], float up, float shift, f16x8 (&hi)[N / 8],
+__device__ __forceinline__ void probabilities(const float (&s)[N], float up, float base, f16x8 (&hi)[N / 8],
                                               f16x8 (&lo)[N / 8], float& l) {
   float sum = 0.f;
 #pragma unroll
   for (int i = 0; i < N; i += 2) {
-    const f32x2 p = {__builtin_amdgcn_exp2f(__builtin_fmaf(s[i], up, shift)),
-                     __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + 1], up, shift))};
+    const f32x2 p = {__builtin_amdgcn_exp2f(__builtin_fmaf(s[i], up, -base)),
+                     __builtin_amdgcn_exp2f(__builtin_fmaf(s[i + 1], up, -base))};
     sum += p[0];
     sum += p[1];
     const f16x2 h = __builtin_convertvector(p, f16x2);
@@ -531,8 +540,8 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
         const float up = LO ? fmaxf(q_up[n] * k_up, FLT_MIN) : q_up[n];  // (above zero: a masked score is -inf)
         mx = swap_max<16>(mx);
         mx = swap_max<32>(mx) * up;
-        if (__builtin_amdgcn_ballot_w64(mx > m_run[n] + kSlack) != 0) {
-          const float mn = fmaxf(m_run[n], mx), ms = mn == -INFINITY ? 0.f : mn;
+        if (__builtin_amdgcn_ballot_w64(mx - m_run[n] > kUp + kSlack) != 0) {
+          const float mn = fmaxf(m_run[n], base_of(mx)), ms = mn == -INFINITY ? 0.f : mn;
           const float alpha = __builtin_amdgcn_exp2f(m_run[n] - ms);
           m_run[n] = mn;
           m_sub[n] = ms;
@@ -541,7 +550,7 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
           for (int b = 0; b < 8; ++b) o[n][b] *= alpha;
         }
         f16x8 h1[1], l1[1];
-        probabilities<8, true>(y, up, kUp - m_sub[n], h1, l1, l_run[n]);
+        probabilities<8, true>(y, up, m_sub[n], h1, l1, l_run[n]);
         ph[n] = h1[0];
         pl[n] = l1[0];
       }
@@ -1093,8 +1102,8 @@ __device__ void run_wide(const RowsArgs& a, const KvView& w, int h, int col0, in
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[i]);
       const float up = LO ? fmaxf(q_up * k_up, FLT_MIN) : q_up;  // (above zero: a masked score is -inf)
       mx = swap_max<32>(mx) * up;
-      if (__builtin_amdgcn_ballot_w64(mx > m_run + kSlack) != 0) {
-        const float mn = fmaxf(m_run, mx), ms = mn == -INFINITY ? 0.f : mn;
+      if (__builtin_amdgcn_ballot_w64(mx - m_run > kUp + kSlack) != 0) {
+        const float mn = fmaxf(m_run, base_of(mx)), ms = mn == -INFINITY ? 0.f : mn;
         const float alpha = __builtin_amdgcn_exp2f(m_run - ms);
         m_run = mn;
         m_sub = ms;
@@ -1103,7 +1112,7 @@ __device__ void run_wide(const RowsArgs& a, const KvView& w, int h, int col0, in
         for (int d = 0; d < 4; ++d) o[d] *= alpha;
       }
       f16x8 ph[2], pl[2];
-      probabilities<16, HL>(x, up, kUp - m_sub, ph, pl, l_run);
+      probabilities<16, HL>(x, up, m_sub, ph, pl, l_run);
       if constexpr (Q) {
         // Lane (column, lh) holds dims of every block d.
         const u32x4 bad = *reinterpret_cast<const u32x4*>(nan_rows[n3][st]);
