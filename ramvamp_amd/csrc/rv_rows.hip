@@ -30,8 +30,17 @@ constexpr int kD = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 // Probabilities are taken relative to a base kUp below the running maximum (it
 // cancels in o / l), which moves when a score passes it by more than kUp + kSlack:
-// they stay at or below 2^14, inside f16.
-constexpr float kSlack = 8.f, kUp = 6.f;
+// they stay at or below 2^15, inside f16, and the lo half of a small one, which
+// shares f16's last bit of 2^-24, still holds 2^-36 of the largest.
+constexpr float kSlack = 4.f, kUp = 11.f;
+// An f32 sum drops the terms below 2^-24 of it, all of them where one row's weight
+// towers over the others' (as the first token's often does): 2^-28 a row, 16 rows
+// a term. So after this many rows a wave's sums of o and l join those that it has
+// put aside and are begun again: what is dropped stays below 2^-15 (wide) and 2^-18
+// (narrow) of the weight, however long the split. A wide item's sums go
+// through memory (128 KiB out and in; 4096 rows at 131000 14.9 -> 15.1 ms), a narrow
+// one's through the LDS that its waves meet in.
+constexpr int kWalkWide = 8192, kWalkNarrow = 32 * 32;
 constexpr int kFold = 16;  // splits of a kv head that the launch folds itself
 
 struct NoLens {};
@@ -49,6 +58,7 @@ struct RowsArgs {
   // lanes]. ml: maximum and sum by [slot][column].
   float* part;
   float* ml;
+  f32x4* aside;           // wide main items longer than kWalkWide: [item][wave][17 x 16 bytes][64 lanes]
   unsigned* tickets;      // narrow main items fold in the launch: one per kv head, 128 bytes apart
   size_t slot_floats;     // of part, from one main slot to the next
   size_t t_base, t_slot_floats;  // of part: the first tail slot, from one to the next
@@ -133,18 +143,23 @@ struct VRange {  // wave-uniform
     by = power(max(before - e, -126));
     return outputs && e != before;
   }
-  // The partial's outputs unscaled. Past 2^60 it takes another form of the same
-  // value, o, l and 2^m by 2^64, so that p v stays finite (m's sum is exact up to
-  // scores of 2^30).
-  template <typename O>
-  __device__ __forceinline__ void undo(float& m, float& l, const O& scale_outputs) const {
-    if (e == 0) return;
+  // The factor that unscales a partial's outputs. Past 2^60 it takes another form
+  // of the same value, o, l and 2^m by 2^64, so that p v stays finite (m's sum is
+  // exact up to scores of 2^30).
+  __device__ __forceinline__ float undo(float& m, float& l) const {
     const int sh = e > 60 ? 64 : 0;
     m += (float)sh;
     l *= power(-sh);
-    scale_outputs(power(e - sh));
+    return power(e - sh);
   }
 };
+
+// x as computed here: addresses made from it are not kept from before a loop in
+// registers that the loop has better use for.
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 
 // x - hi, one instruction that reads the f16 half where it is. (A plain
 // subtraction widens the half first; the constant is kept from the compiler,
@@ -436,12 +451,12 @@ constexpr int narrow_lds(int nb) { return NW * nb * kRegB; }
 // Columns [col0, col0 + 16 NB) of kv head h over rows [t_begin, t_end) of `w`,
 // by four waves of the workgroup (wave wv of them takes tiles wv, wv + 4, ...).
 // All waves of the workgroup call it together; `run` false: nothing to do but
-// the barriers. causal: column c sees start + row + 1 rows.
-template <typename T, int NB, bool CAUSAL>
+// the barriers. causal: column c sees start + row + 1 rows. WALK: longer than
+// kWalkNarrow rows a wave.
+template <typename T, int NB, bool CAUSAL, bool WALK>
 __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, int n_cols, int row0, long t_begin,
                            long t_end, const PartDst& to, int wv, bool run, char* lds) {
   constexpr bool LO = Lo<T>::value, Q = std::is_same<T, Q8>::value;
-  const int lane = threadIdx.x & 63, li = lane & 15, lk = lane >> 4;
   const int hk = a.kv_lo + h;
   const long last = t_end - 1;
   float m_run[NB], l_run[NB];
@@ -456,7 +471,36 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
     for (int b = 0; b < 8; ++b) o[n][b] = f32x4{};
   }
   const int n_tiles = run ? (int)((t_end - t_begin + 31) >> 5) : 0;
+  f32x4* om = reinterpret_cast<f32x4*>(lds);  // [wave][NB][8][64]
+  float* sums = reinterpret_cast<float*>(lds + NW * NB * 32 * 64 * 4);  // [wave][NB][2][64]
+  // The wave's own part of both holds the sums that it has put aside.
+  bool aside = false;
+  // The running sums and those put aside, joined: piece(n, b, value) for each.
+  const auto join = [&](int lane, const auto& piece) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const int at = wv * NB + n;
+      const float unscale = LO ? range.undo(m_run[n], l_run[n]) : 1.f;
+      float f1 = 1.f, f2 = 0.f;
+      if (WALK && aside) {
+        const float m2 = sums[2 * at * 64 + lane], l2 = sums[(2 * at + 1) * 64 + lane];
+        const float mn = fmaxf(m_run[n], m2), ms = mn == -INFINITY ? 0.f : mn;
+        f1 = __builtin_amdgcn_exp2f(m_run[n] - ms);
+        f2 = __builtin_amdgcn_exp2f(m2 - ms);
+        m_run[n] = mn;
+        l_run[n] = l_run[n] * f1 + l2 * f2;
+      }
+#pragma unroll
+      for (int b = 0; b < 8; ++b) {
+        f32x4 v = o[n][b];
+        if constexpr (LO) v *= unscale;
+        if (WALK && aside) v = v * f1 + om[(at * 8 + b) * 64 + lane] * f2;
+        piece(n, b, v);
+      }
+    }
+  };
   if (wv < n_tiles) {
+    const int lane = threadIdx.x & 63, li = lane & 15, lk = lane >> 4;
     float q_up[NB], m_sub[NB];
     long limit[NB];
     f32x4 qv[NB][8];
@@ -612,23 +656,31 @@ __device__ void run_narrow(const RowsArgs& a, const KvView& w, int h, int col0, 
         if (K_LATE && u == 0 && tile + NW < n_tiles) load_raw_k<T>(x, w, hk, p0 + 32 * NW, last, li, lk);
       }
       if (tile + NW < n_tiles) load_raw_v<T>(x, w, hk, p0 + 32 * NW, last, li, lk);
+      if (WALK && (tile / NW + 1) % (kWalkNarrow / 32) == 0 && tile + NW < n_tiles) {
+        const int lane = here(threadIdx.x & 63);
+        join(lane, [&](int n, int b, f32x4 v) { om[((wv * NB + n) * 8 + b) * 64 + lane] = v; });
+        aside = true;
+        range = VRange{};
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+          sums[2 * (wv * NB + n) * 64 + lane] = m_run[n];
+          sums[(2 * (wv * NB + n) + 1) * 64 + lane] = l_run[n];
+          m_run[n] = -INFINITY;  // (the first maximum above it clears the outputs)
+          l_run[n] = 0.f;
+        }
+      }
     }
   }
+  const int lane = WALK ? here(threadIdx.x & 63) : threadIdx.x & 63, li = lane & 15, lk = lane >> 4;
+  if (LO || WALK) join(lane, [&](int n, int b, f32x4 v) { o[n][b] = v; });
   // The waves' partials meet in LDS, and each wave folds its share of the values,
   // in wave order. A lane's 16 bytes i are dims 32 lk + 4 i .. + 3 of column li.
   const int used = min(NW, n_tiles);
-  f32x4* om = reinterpret_cast<f32x4*>(lds);
-  float* sums = reinterpret_cast<float*>(lds + NW * NB * 32 * 64 * 4);  // [wave][NB][2][64]
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
     // Each lane summed its own rows: the other quarters of the column's.
     l_run[n] = swap_sum<16>(l_run[n]);
     l_run[n] = swap_sum<32>(l_run[n]);
-    if constexpr (LO)
-      range.undo(m_run[n], l_run[n], [&](float f) {
-#pragma unroll
-        for (int b = 0; b < 8; ++b) o[n][b] *= f;
-      });
     if (Q && CAUSAL && (taint & (1u << n))) {
 #pragma unroll
       for (int b = 0; b < 8; ++b) o[n][b] *= __builtin_nanf("");
@@ -1066,6 +1118,30 @@ __device__ void run_wide(const RowsArgs& a, const KvView& w, int h, int col0, in
   float m_run = -INFINITY, m_sub = 0.f, l_run = 0.f;
   uint32_t taint = 0;  // Q8_0: this lane's dims met a NaN block in a row its column sees
   int buf = 0, n3 = 0;
+  // The sums put aside: o by lane, then (m, l).
+  const auto place = [&] { return a.aside + (size_t)(blockIdx.x * 8 + wave) * (17 * 64) + here(threadIdx.x & 63); };
+  bool aside = false;
+  // The running sums and those put aside, joined: piece(i, registers 4 i ..) for each.
+  const auto join = [&](f32x4* store, const auto& piece) {
+    const float unscale = LO ? range.undo(m_run, l_run) : 1.f;
+    float f1 = 1.f, f2 = 0.f;
+    if (aside) {
+      const f32x4 s2 = store[16 * 64];
+      const float mn = fmaxf(m_run, s2[0]), ms = mn == -INFINITY ? 0.f : mn;
+      f1 = __builtin_amdgcn_exp2f(m_run - ms);
+      f2 = __builtin_amdgcn_exp2f(s2[0] - ms);
+      m_run = mn;
+      l_run = l_run * f1 + s2[1] * f2;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);  // (few registers are left for the loads in flight)
+      f32x4 v = {o[i >> 2][4 * (i & 3)], o[i >> 2][4 * (i & 3) + 1], o[i >> 2][4 * (i & 3) + 2], o[i >> 2][4 * (i & 3) + 3]};
+      if constexpr (LO) v *= unscale;
+      if (aside) v = v * f1 + store[64 * i] * f2;
+      piece(i, v);
+    }
+  };
   for (long t0 = t_begin; t0 < t_end; t0 += S) {
     const bool more = t0 + S < t_end;
     if (more && !LO) load_share<T, S>(sh, w, hk, t0 + S, last, is_v, tt);
@@ -1144,6 +1220,15 @@ __device__ void run_wide(const RowsArgs& a, const KvView& w, int h, int col0, in
         }
       }
     }
+    if (more && (int)(t0 + S - t_begin) % kWalkWide == 0) {
+      f32x4* const store = place();
+      join(store, [&](int i, f32x4 v) { store[64 * i] = v; });
+      store[16 * 64] = f32x4{m_run, l_run, 0.f, 0.f};
+      aside = true;
+      range = VRange{};
+      m_run = -INFINITY;  // (the first maximum above it clears the outputs)
+      l_run = 0.f;
+    }
     buf ^= 1;
     n3 = n3 == 2 ? 0 : n3 + 1;
     if constexpr (LO) {
@@ -1155,13 +1240,13 @@ __device__ void run_wide(const RowsArgs& a, const KvView& w, int h, int col0, in
     if (more) store_share<T, S>(sh, lds + buf * kStage, t0 + S, last, is_v, tt, Q ? nan_rows[n3] : nullptr);
     __syncthreads();
   }
+  if (LO || aside)
+    join(place(), [&](int i, f32x4 v) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i >> 2][4 * (i & 3) + e] = v[e];
+    });
   // Each lane summed its own rows: the other half of the column's.
   l_run = swap_sum<32>(l_run);
-  if constexpr (LO)
-    range.undo(m_run, l_run, [&](float f) {
-#pragma unroll
-      for (int d = 0; d < 4; ++d) o[d] *= f;
-    });
   if constexpr (Q) {
     if (taint) {
 #pragma unroll
@@ -1229,7 +1314,7 @@ __device__ __forceinline__ bool device_positions(const uint32_t* d_pos, int plan
 
 // A tail item by the four waves `wv` counts: sequence, column block of 16,
 // split (b past them: none, the waves only keep the barriers).
-template <typename T>
+template <typename T, bool WALK>
 __device__ void tail_item(const RowsArgs& a, const TailLens& lens, int b, int wv, char* lds) {
   const int split = b % a.t_splits;
   b /= a.t_splits;
@@ -1245,8 +1330,8 @@ __device__ void tail_item(const RowsArgs& a, const TailLens& lens, int b, int wv
   PartDst to;
   to.part = a.part + a.t_base + split * a.t_slot_floats + ((size_t)seq * a.n_heads + h) * a.t_cb * (16 * kD);
   to.ml = a.ml + 2 * (((size_t)(a.n_splits + split) * a.n_heads + h) * a.rows + seq) * a.group;
-  run_narrow<T, 1, false>(a, w, h, cb * 16, a.group, seq, t_begin, min(len, t_begin + a.t_split_len), to, wv,
-                             t_begin < len, lds);
+  run_narrow<T, 1, false, WALK>(a, w, h, cb * 16, a.group, seq, t_begin, min(len, t_begin + a.t_split_len), to, wv,
+                                t_begin < len, lds);
 }
 
 // Workgroup b of the main items. Those of one XCD (b mod 8) are consecutive in
@@ -1263,13 +1348,14 @@ __device__ __forceinline__ bool main_item(const RowsArgs& a, int b, int& h, int&
   return true;
 }
 
+// Workgroups of narrow items that a CU's registers are to hold.
 template <typename T>
-constexpr int narrow_waves(int nb) {
-  return nb == 2 && Lo<T>::value ? 1 : 2;
+constexpr int narrow_waves(int nb, bool walk) {
+  return nb == 2 && (Lo<T>::value || (walk && !std::is_same<T, Q8>::value)) ? 1 : 2;
 }
 
-template <typename T, int NB, bool TAILS, bool CAUSAL>
-__global__ __launch_bounds__(256, narrow_waves<T>(NB)) void rows_narrow_kernel(RowsArgs a,
+template <typename T, int NB, bool TAILS, bool CAUSAL, bool WALK>
+__global__ __launch_bounds__(256, narrow_waves<T>(NB, WALK)) void rows_narrow_kernel(RowsArgs a,
                                                               std::conditional_t<TAILS, TailLens, NoLens> lens) {
   __shared__ __attribute__((aligned(16))) char lds[narrow_lds(NB)];
   const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -1282,7 +1368,7 @@ __global__ __launch_bounds__(256, narrow_waves<T>(NB)) void rows_narrow_kernel(R
   int split, h, cb = 0;
   if constexpr (TAILS) {
     if ((int)blockIdx.x >= a.main_items) {
-      tail_item<T>(a, lens, (int)blockIdx.x - a.main_items, wv, lds);
+      tail_item<T, WALK>(a, lens, (int)blockIdx.x - a.main_items, wv, lds);
       return;
     }
     if (!main_item(a, blockIdx.x, h, split, cb)) return;
@@ -1311,7 +1397,7 @@ __global__ __launch_bounds__(256, narrow_waves<T>(NB)) void rows_narrow_kernel(R
     to.part += split * a.slot_floats;
     to.ml += split * ml_slot;
   }
-  run_narrow<T, NB, CAUSAL>(a, a.main, h, col0, n_cols, 0, t_begin, t_end, to, wv, true, lds);
+  run_narrow<T, NB, CAUSAL, WALK>(a, a.main, h, col0, n_cols, 0, t_begin, t_end, to, wv, true, lds);
 }
 
 template <typename T, int WC, bool HL, bool TAILS>
@@ -1337,7 +1423,7 @@ __global__ __launch_bounds__(512) void rows_wide_kernel(RowsArgs a, std::conditi
     run_wide<T, WC, HL>(a, a.main, h, col0, n_cols, t_begin, t_end, a.causal != 0, split, lds);
   } else if constexpr (TAILS) {  // two items, four waves each
     const int half = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8);
-    tail_item<T>(a, lens, 2 * (b - a.main_items) + half, __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6) & 3),
+    tail_item<T, true>(a, lens, 2 * (b - a.main_items) + half, __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6) & 3),
                  lds + half * narrow_lds(1));
   }
 }
@@ -1438,26 +1524,29 @@ __global__ __launch_bounds__(64 * (G < 4 ? 4 : G)) void rows_merge_kernel(
 
 // ---- any head size up to 512 --------------------------------------------------------
 // One workgroup a column; each wave walks every fourth row (one row at a time,
-// the head's values over the lanes), f32 arithmetic, the waves' sums joined in
+// the head's values over the lanes), f32 products, the sums over rows in f64 (one
+// term a row: an f32 sum would drop those below 2^-24 of it), the waves' joined in
 // LDS. For geometries no model of this library's path has; it is right, not fast.
 template <typename T, bool TAILS>
 __global__ __launch_bounds__(256) void rows_generic_kernel(RowsArgs a, int hd,
                                                            std::conditional_t<TAILS, TailLens, NoLens> lens) {
   constexpr int kPer = 8;
-  __shared__ float sm_o[3][64 * kPer], sm_m[3], sm_l[3];
+  __shared__ double sm_o[3][64 * kPer], sm_l[3];
+  __shared__ float sm_m[3];
   int positions = a.positions;
   if (!device_positions(a.d_pos, a.positions, positions)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int n_q = a.n_heads * a.group;
   const int row = blockIdx.x / n_q, hq = blockIdx.x % n_q, h = a.kv_lo + hq / a.group;
   const float* qp = a.q + ((size_t)row * a.n_q_heads + (size_t)a.kv_lo * a.group + hq) * hd;
-  float q[kPer], o[kPer];
+  float q[kPer];
+  double o[kPer], l = 0.0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     q[i] = lane + 64 * i < hd ? qp[lane + 64 * i] * a.qscale : 0.f;
-    o[i] = 0.f;
+    o[i] = 0.0;
   }
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY;
   auto walk = [&](const KvView& w, long len) {
     for (long t = wave; t < len; t += 4) {
       float x = 0.f;
@@ -1467,12 +1556,12 @@ __global__ __launch_bounds__(256) void rows_generic_kernel(RowsArgs a, int hd,
       x = group_sum<32>(x);
       x = swap_sum<32>(x);
       const float mn = fmaxf(m, x), ms = mn == -INFINITY ? 0.f : mn;
-      const float f = __builtin_amdgcn_exp2f(m - ms), p = __builtin_amdgcn_exp2f(x - ms);
+      const double f = __builtin_amdgcn_exp2f(m - ms), p = __builtin_amdgcn_exp2f(x - ms);
       m = mn;
       l = l * f + p;
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
-        if (lane + 64 * i < hd) o[i] = o[i] * f + p * kv_value<T, true>(w, hd, h, t, lane + 64 * i);
+        if (lane + 64 * i < hd) o[i] = o[i] * f + p * (double)kv_value<T, true>(w, hd, h, t, lane + 64 * i);
     }
   };
   long limit = positions;
@@ -1498,7 +1587,7 @@ __global__ __launch_bounds__(256) void rows_generic_kernel(RowsArgs a, int hd,
   if (wave > 0) return;
   for (int p = 0; p < 3; ++p) {
     const float mn = fmaxf(m, sm_m[p]), ms = mn == -INFINITY ? 0.f : mn;
-    const float f1 = __builtin_amdgcn_exp2f(m - ms), f2 = __builtin_amdgcn_exp2f(sm_m[p] - ms);
+    const double f1 = __builtin_amdgcn_exp2f(m - ms), f2 = __builtin_amdgcn_exp2f(sm_m[p] - ms);
     m = mn;
     l = l * f1 + sm_l[p] * f2;
 #pragma unroll
@@ -1507,7 +1596,7 @@ __global__ __launch_bounds__(256) void rows_generic_kernel(RowsArgs a, int hd,
   float* dst = a.out + ((size_t)row * n_q + hq) * hd;
 #pragma unroll
   for (int i = 0; i < kPer; ++i)
-    if (lane + 64 * i < hd) dst[lane + 64 * i] = o[i] / l;
+    if (lane + 64 * i < hd) dst[lane + 64 * i] = (float)(o[i] / l);
 }
 
 // ---- plans ------------------------------------------------------------------------
@@ -1687,11 +1776,20 @@ size_t main_floats(const RowsPlan& p, size_t n, size_t group, size_t heads) {
 }
 size_t tail_floats(const RowsPlan& p, size_t n, size_t heads) { return n * heads * p.t_cb * 16 * kD; }
 
+// A launch's workgroups of main items.
+size_t main_items(const RowsPlan& p, size_t heads) { return (heads * p.n_splits * p.n_cb + 7) / 8 * 8; }
+
+// Floats that its wide items' sums are put aside in.
+size_t aside_floats(const RowsPlan& p, size_t heads) {
+  return p.wc && p.split_len > kWalkWide ? main_items(p, heads) * 8 * 17 * 64 * 4 : 0;
+}
+
 size_t plan_floats(const RowsPlan& p, const RowsCall& c) {
-  if (p.generic || p.slots() <= 1) return 0;
+  if (p.generic) return 0;
   const rv_kv* g = c.main ? c.main : c.tails;
   const size_t group = c.n_q_heads / g->n_kv_heads, heads = c.kv_hi - c.kv_lo;
-  return p.n_splits * main_floats(p, p.rows, group, heads) + p.t_splits * tail_floats(p, p.rows, heads) +
+  if (p.slots() <= 1) return aside_floats(p, heads);
+  return aside_floats(p, heads) + p.n_splits * main_floats(p, p.rows, group, heads) + p.t_splits * tail_floats(p, p.rows, heads) +
          2 * p.slots() * p.rows * group * heads;
 }
 
@@ -1705,25 +1803,35 @@ void launch_merge_g(const RowsArgs& a, int items, bool narrow, const TailLens* l
     hipLaunchKernelGGL((rows_merge_kernel<G, false>), grid, block, 0, s, a, (int)narrow, NoLens{});
 }
 
+template <typename T, bool TAILS, bool WALK, typename L>
+void launch_narrow(const RowsPlan& p, const TimedPair& tp, const RowsArgs& a, unsigned tail_items, hipStream_t s,
+                   const L& lens) {
+  if constexpr (TAILS) {
+    const dim3 grid((unsigned)a.main_items + tail_items);
+    if (p.nb == 1)
+      launch_timed(tp, rows_narrow_kernel<T, 1, true, false, WALK>, grid, dim3(256), s, a, lens);
+    else
+      launch_timed(tp, rows_narrow_kernel<T, 2, true, false, WALK>, grid, dim3(256), s, a, lens);
+  } else {
+    const dim3 grid((unsigned)a.n_splits, (unsigned)a.n_heads, (unsigned)a.n_cb);
+    if (a.causal)
+      launch_timed(tp, rows_narrow_kernel<T, 2, false, true, WALK>, grid, dim3(256), s, a, lens);
+    else if (p.nb == 2)
+      launch_timed(tp, rows_narrow_kernel<T, 2, false, false, WALK>, grid, dim3(256), s, a, lens);
+    else
+      launch_timed(tp, rows_narrow_kernel<T, 1, false, false, WALK>, grid, dim3(256), s, a, lens);
+  }
+}
+
 template <typename T, bool HL, bool TAILS, typename L>
 void launch_plan(const RowsPlan& p, const TimedPair& tp, const RowsArgs& a, unsigned tail_items, hipStream_t s,
                  const L& lens) {
   if (p.nb) {
-    if constexpr (TAILS) {
-      const dim3 grid((unsigned)a.main_items + tail_items);
-      if (p.nb == 1)
-        launch_timed(tp, rows_narrow_kernel<T, 1, true, false>, grid, dim3(256), s, a, lens);
-      else
-        launch_timed(tp, rows_narrow_kernel<T, 2, true, false>, grid, dim3(256), s, a, lens);
-    } else {
-      const dim3 grid((unsigned)a.n_splits, (unsigned)a.n_heads, (unsigned)a.n_cb);
-      if (a.causal)
-        launch_timed(tp, rows_narrow_kernel<T, 2, false, true>, grid, dim3(256), s, a, lens);
-      else if (p.nb == 2)
-        launch_timed(tp, rows_narrow_kernel<T, 2, false, false>, grid, dim3(256), s, a, lens);
-      else
-        launch_timed(tp, rows_narrow_kernel<T, 1, false, false>, grid, dim3(256), s, a, lens);
-    }
+    // (the longer form costs short items 2 to 7 %, f16 ones of 32 columns 24 %)
+    if (std::max(p.split_len, p.t_split_len) > NW * kWalkNarrow)
+      launch_narrow<T, TAILS, true>(p, tp, a, tail_items, s, lens);
+    else
+      launch_narrow<T, TAILS, false>(p, tp, a, tail_items, s, lens);
     return;
   }
   const dim3 grid((unsigned)a.main_items + (tail_items + 1) / 2);
@@ -1804,18 +1912,19 @@ HipStatus launch_rows(rv_kv* owner, const RowsCall& c, hipStream_t s, const Work
       }
 #undef RV_GENERIC
     } else {
-      a.part = base;
+      a.aside = (f32x4*)base;
+      a.part = base ? base + aside_floats(p, a.n_heads) : nullptr;
       a.slot_floats = main_floats(p, n, group, a.n_heads);
       a.t_base = p.n_splits * a.slot_floats;
       a.t_slot_floats = tail_floats(p, n, a.n_heads);
-      a.ml = base ? base + a.t_base + p.t_splits * a.t_slot_floats : nullptr;
+      a.ml = base ? a.part + a.t_base + p.t_splits * a.t_slot_floats : nullptr;
       a.n_cb = (int)((n * group + p.columns() - 1) / p.columns());
       a.n_splits = p.n_splits;
       a.split_len = p.split_len;
       a.t_cb = p.t_cb;
       a.t_splits = p.t_splits;
       a.t_split_len = p.t_split_len;
-      a.main_items = (a.n_heads * a.n_splits * a.n_cb + 7) / 8 * 8;
+      a.main_items = (int)((a.n_heads * a.n_splits * a.n_cb + 7) / 8 * 8);
       a.single = p.slots() == 1;
       a.tickets = p.fold ? xcd_tickets(owner) : nullptr;
       const unsigned tail_items = (unsigned)(n * a.n_heads * a.t_cb * a.t_splits);
