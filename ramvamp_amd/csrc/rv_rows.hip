@@ -1723,7 +1723,9 @@ RowsPlan plan_rows(const RowsCall& c, const rv_kv* owner) {
   p.generic = g->head_dim != (size_t)kD;
   p.rows = c.tails ? std::min<size_t>(c.rows, kMaxEach) : c.rows;
   if (p.generic) return p;
-  const long group = (long)(c.n_q_heads / g->n_kv_heads), heads = (long)(c.kv_hi - c.kv_lo);
+  // Planned for all kv heads, so that a range of them takes the whole call's splits
+  // and its outputs are that part of the whole call's, bit for bit.
+  const long group = (long)(c.n_q_heads / g->n_kv_heads), heads = (long)g->n_kv_heads;
   const long cols = (long)p.rows * group;
   const long positions = c.main ? (long)c.positions : 0;
   const bool causal = c.causal && c.rows > 1;  // (one row: its limit is `positions`)

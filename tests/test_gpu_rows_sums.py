@@ -1,7 +1,7 @@
 """What the row attention's sums keep: many small weights behind one that towers
-over them, and scores so large that their last bits weigh. Scores are exact here: a
-query has one or two nonzero values, and SCALE times log2 e is one in f32, so that
-a weight is 2^score."""
+over them, scores so large that their last bits weigh, and a kv head's splits in a
+call of its range alone. Scores of the first two are exact: a query has one or two
+nonzero values, and SCALE times log2 e is one in f32, so that a weight is 2^score."""
 import numpy as np
 import pytest
 
@@ -277,3 +277,29 @@ def test_large_scores_and_large_values_meet_across_splits(base, rest, last, sign
     out = torch.full(q.shape, float("nan"), device="cuda")
     rv.decode_attention_shared(dev(q), p, 0, 300, t, 0, SCALE, out)
     check(host(out), np.tile(want, (n, heads)), 0.0, w * np.abs(v[0]).max(), "splits")
+
+
+@pytest.mark.parametrize("n_kv,group,n", [(4, 8, 4097), (4, 8, 20000), (8, 4, 9000), (2, 40, 5000), (4, 20, 4500)])
+def test_kv_ranges_join_to_the_whole_call_s_bits(n_kv, group, n):
+    """A range's splits are the whole call's, so each head's sums are taken in the
+    same order (as f16 and f32 caches have it)."""
+    torch = torch_cuda()
+    say(f"case q8 kv ranges {(n_kv, group, n)}")
+    rng = np.random.default_rng(n)
+    k, v = (rng.standard_normal((n, n_kv * 128)).astype(np.float32) for _ in range(2))
+    kv = rv.KvCache(1, n_kv, 128, n, "q8_0")
+    kv.append_rows(0, dev(k), dev(v))
+    q = dev(rng.standard_normal(n_kv * group * 128))
+    scale = float(np.float32(128 ** -0.5))
+    whole = torch.full_like(q, float("nan"))
+    rv.decode_attention(q, kv, 0, scale, None, whole)
+    width = group * 128
+    for units in (1, 2, n_kv):
+        got = torch.full_like(q, float("nan"))
+        for u in range(units):
+            heads = range(u * n_kv // units, (u + 1) * n_kv // units)
+            rv.decode_attention_kv_range_in(q, kv, 0, scale, heads, 1 << 40,
+                                            got[heads.start * width:heads.stop * width])
+        assert np.array_equal(host(got).view(np.uint32), host(whole).view(np.uint32)), units
+    want, a = attend(host(q), stored(k, "q8_0"), stored(v, "q8_0"), n_kv, 128, scale)
+    check(host(whole), want, a, np.abs(v).max() * 1.01, "whole")
