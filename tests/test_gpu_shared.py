@@ -399,3 +399,53 @@ def test_refusals():
         rv.decode_step_shared(p, 0, 4, t, 0, q, x[:3], x[:3], w[:5], w, EPS, THETA, 1.0, out)
     with pytest.raises(ValueError):
         rv.decode_step_shared(p, 0, 4, t, 0, q, x[:2], x[:2], w, w, EPS, THETA, 1.0, out)
+
+
+@pytest.mark.parametrize("elem", ["f16", "f32", "q8_0"])
+@pytest.mark.parametrize("prefix,tails", [(70, [0, 3, 17, 1]), (700, [40, 0, 129, 7, 1])])
+def test_step_s_output_is_each_sequence_s_own(elem, prefix, tails):
+    """The same float rows given to the batch's caches and to one cache a sequence, so
+    that the stored blocks are the same for every element type: decode_step_shared's
+    outputs are decode_step's but for the order of the sums, each within
+    rows_util.check's bound of the exact ones."""
+    torch = torch_cuda()
+    say(f"case shared step's output {(elem, prefix, tails)}")
+    rng = np.random.default_rng(prefix)
+    n_kv, group, hd = 2, 8, 128
+    qd, kvd = n_kv * group * hd, n_kv * hd
+    ks, vs = rows(rng, prefix, kvd), rows(rng, prefix, kvd)
+    own = [(rows(rng, n, kvd), rows(rng, n, kvd)) for n in tails]
+    p, t = rv.KvCache(1, n_kv, hd, prefix, elem), rv.KvCache(len(tails), n_kv, hd, max(tails) + 3, elem)
+    p.append_rows(0, dev(ks), dev(vs))
+    single = []
+    for i, (k, v) in enumerate(own):
+        kv = rv.KvCache(1, n_kv, hd, prefix + tails[i] + 3, elem)
+        kv.append_rows(0, dev(ks), dev(vs))
+        if tails[i]:
+            t.append_rows(i, dev(k), dev(v))
+            kv.append_rows(0, dev(k), dev(v))
+        single.append(kv)
+    wq, wk = (rng.uniform(0.9, 1.1, hd).astype(np.float32) for _ in range(2))
+    for step in range(3):
+        q, k, v = (rng.standard_normal((len(tails), d)).astype(np.float32) for d in (qd, kvd, kvd))
+        out = torch.full((len(tails), qd), float("nan"), device="cuda")
+        rv.decode_step_shared(p, 0, prefix, t, 0, dev(q), dev(k), dev(v), dev(wq), dev(wk), EPS, THETA, scale_of(hd),
+                              out)
+        got = host(out)
+        for i, kv in enumerate(single):
+            pos = prefix + tails[i] + step
+            one = torch.full((qd,), float("nan"), device="cuda")
+            rv.decode_step(kv, 0, dev(q[i]), dev(k[i]), dev(v[i]), dev(wq), dev(wk), EPS, THETA, pos, scale_of(hd), one)
+            kk, vv = (host(x) for x in kv.read_rows(0, 0, pos + 1))
+            for whole, first, mine in zip((kk, vv), p.read_rows(0, 0, prefix), t.read_rows(i, 0, tails[i] + step + 1)):
+                assert np.array_equal(whole, np.concatenate([host(first), host(mine)]))
+            h = q[i].astype(np.float64).reshape(-1, hd)
+            y = h / np.sqrt((h * h).mean(-1, keepdims=True) + EPS) * wq
+            ang = pos * np.power(THETA, -2.0 * np.arange(hd // 2) / hd)
+            c, s = np.cos(ang), np.sin(ang)
+            y = np.concatenate([y[:, :64] * c - y[:, 64:] * s, y[:, :64] * s + y[:, 64:] * c], 1)
+            want, a = attend(y.reshape(-1), kk, vv, n_kv, hd, scale_of(hd))
+            # (2 a: the query's own five f32 roundings)
+            check(got[i], want, 2 * a, np.abs(vv).max(), f"shared step {step} sequence {i}")
+            bound = 2 * np.abs(vv).max() * (2 * (np.log(2.0) * 37 * EPS32 * a + 2.0 ** -22) + 96 * EPS32)
+            assert np.abs(got[i].astype(np.float64) - host(one)).max() <= bound, (step, i)
