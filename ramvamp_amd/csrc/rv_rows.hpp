@@ -62,14 +62,6 @@ __device__ __forceinline__ void q8_widen(uint32_t w, f16x2& a, f16x2& b) {
   b = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) + off;
 }
 
-// The same for byte D of two rows' words: (row a's, row b's).
-template <int D>
-__device__ __forceinline__ f16x2 q8_widen_pair(uint32_t a, uint32_t b) {
-  const f16x2 off = {(_Float16)-1152.f, (_Float16)-1152.f};
-  const uint32_t x = __builtin_amdgcn_perm(b, a, 0x0c000c00u | (uint32_t)D | ((uint32_t)(4 + D) << 16)) | 0x64006400u;
-  return __builtin_bit_cast(f16x2, x) + off;
-}
-
 __device__ __forceinline__ float q8_value(uint8_t code, uint16_t scale) {
   return (float)((_Float16)(float)((int)code - 128) * __builtin_bit_cast(_Float16, scale));
 }
