@@ -267,7 +267,10 @@ int32_t rv_attention_at_rows(const rv_kv* kv, const float* q_rows, size_t rows, 
  * Checks, in order: the two caches' geometry, element type, device and stream
  * (RV_ERR_UNSUPPORTED where they differ), q_dim, the prefix's layer and
  * positions, the tails' layers, empty sequences. Work is queued on that
- * stream; `tails`' workspace is used. F32 planes take any finite values: they
+ * stream; `tails`' workspace is used. The prefix is in use as any cache of a call
+ * is: batches of several host threads or streams over one prefix take turns, each
+ * binding it to its stream (rv_kv_set_stream orders them) and calling before the
+ * next one does. F32 planes take any finite values: they
  * pass through f16 hi + lo operands, rows scaled by powers of two, to 2^-22 of
  * themselves or 2^-34 of the largest row's. */
 int32_t rv_decode_attention_shared(const rv_kv* prefix, size_t prefix_layer, size_t prefix_positions,

@@ -21,6 +21,7 @@ reference read the same here. Differences, all forced by the device:
 from __future__ import annotations
 
 import ctypes
+import threading
 from ctypes import byref, c_double, c_int32, c_size_t, c_uint64, c_void_p
 
 import numpy as np
@@ -199,6 +200,7 @@ class KvCache:
         self._kv_dim = n_kv_heads * head_dim
         self._capacity = capacity
         self._torch_device = None
+        self._sharing = threading.Lock()
 
     new = classmethod(lambda cls, *a, **k: cls(*a, **k))
 
@@ -503,7 +505,8 @@ def attention_at_rows(q_rows, cache: KvCache, layer: int, start: int, scale: flo
 
 def _same_stream(prefix: KvCache, tails: KvCache):
     """Both caches of a batch on torch's current stream (host arrays too: the two
-    have to agree)."""
+    have to agree). Called with the prefix's lock held until the call is queued:
+    batches of several threads take turns at binding a prefix to their streams."""
     prefix._bind_stream()
     tails._bind_stream()
 
@@ -518,11 +521,13 @@ def decode_attention_shared(q_rows, prefix: KvCache, prefix_layer: int, prefix_p
     if oa.n != qa.n:
         raise ValueError("out must have the shape of q_rows")
     err = L.RvError()
-    _same_stream(prefix, tails)
-    flags = _flags(tails, (qa, oa))
-    _check(_lib().rv_decode_attention_shared(prefix.handle, prefix_layer, prefix_positions, tails.handle, tail_layer,
-                                             qa.ptr, qa.n // q_dim if q_dim else 0, q_dim, scale, oa.ptr, flags,
-                                             byref(err)), err)
+    with prefix._sharing:
+        _same_stream(prefix, tails)
+        flags = _flags(tails, (qa, oa))
+        rc = _lib().rv_decode_attention_shared(prefix.handle, prefix_layer, prefix_positions, tails.handle, tail_layer,
+                                               qa.ptr, qa.n // q_dim if q_dim else 0, q_dim, scale, oa.ptr, flags,
+                                               byref(err))
+    _check(rc, err)
     return out
 
 
@@ -541,11 +546,13 @@ def decode_step_shared(prefix: KvCache, prefix_layer: int, prefix_positions: int
     if oa.n != qa.n:
         raise ValueError("out must have the shape of q_rows")
     err = L.RvError()
-    _same_stream(prefix, tails)
-    flags = _flags(tails, (qa, ka, va, wq, wk, oa))
-    _check(_lib().rv_decode_step_shared(prefix.handle, prefix_layer, prefix_positions, tails.handle, tail_layer, n,
-                                        qa.ptr, ka.ptr, va.ptr, q_dim, wq.ptr, wq.n, wk.ptr, wk.n, eps, theta, scale,
-                                        oa.ptr, flags, byref(err)), err)
+    with prefix._sharing:
+        _same_stream(prefix, tails)
+        flags = _flags(tails, (qa, ka, va, wq, wk, oa))
+        rc = _lib().rv_decode_step_shared(prefix.handle, prefix_layer, prefix_positions, tails.handle, tail_layer, n,
+                                          qa.ptr, ka.ptr, va.ptr, q_dim, wq.ptr, wq.n, wk.ptr, wk.n, eps, theta,
+                                          scale, oa.ptr, flags, byref(err))
+    _check(rc, err)
     return out
 
 

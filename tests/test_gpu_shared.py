@@ -449,3 +449,71 @@ def test_step_s_output_is_each_sequence_s_own(elem, prefix, tails):
             check(got[i], want, 2 * a, np.abs(vv).max(), f"shared step {step} sequence {i}")
             bound = 2 * np.abs(vv).max() * (2 * (np.log(2.0) * 37 * EPS32 * a + 2.0 ** -22) + 96 * EPS32)
             assert np.abs(got[i].astype(np.float64) - host(one)).max() <= bound, (step, i)
+
+
+def test_one_prefix_for_the_batches_of_two_threads(monkeypatch):
+    """Each thread on a stream of its own: the other's call waits where it would
+    bind the prefix to its stream between this one's binding and its call."""
+    import threading
+
+    from ramvamp_amd import attention as A
+
+    torch = torch_cuda()
+    say("case shared two threads")
+    rng = np.random.default_rng(50)
+    n_kv, group, hd, prefix = 2, 8, 128, 500
+    p = rv.KvCache(1, n_kv, hd, prefix, "f16")
+    pk, pv = rows(rng, prefix, n_kv * hd), rows(rng, prefix, n_kv * hd)
+    p.append_rows(0, dev(pk), dev(pv))
+    torch.cuda.synchronize()
+    flags, entered, done, failed = A._flags, threading.Event(), threading.Event(), []
+
+    def batch_of(seqs, seed):
+        g = np.random.default_rng(seed)
+        t = rv.KvCache(seqs, n_kv, hd, 8, "f16")
+        own = [(rows(g, 3, n_kv * hd), rows(g, 3, n_kv * hd)) for _ in range(seqs)]
+        for i, (k, v) in enumerate(own):
+            t.append_rows(i, dev(k), dev(v))
+        q = g.standard_normal((seqs, n_kv * group * hd)).astype(np.float32)
+        want = expect(q, (stored(pk, "f16"), stored(pv, "f16")),
+                      [(stored(k, "f16"), stored(v, "f16")) for k, v in own], n_kv, hd)
+        return t, q, want
+
+    def call(batch):
+        t, q, _ = batch
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            d = torch.from_numpy(q).cuda()
+            out = torch.full_like(d, float("nan"))
+            rv.decode_attention_shared(d, p, 0, prefix, t, 0, scale_of(hd), out)
+            s.synchronize()
+            return out.cpu().numpy()
+
+    first, second = batch_of(5, 1), batch_of(9, 2)
+    torch.cuda.synchronize()
+    got = {}
+
+    def other():
+        try:
+            entered.wait(30)
+            got["second"] = call(second)
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+        done.set()
+
+    def between(cache, args):
+        r = flags(cache, args)
+        if cache is first[0]:
+            entered.set()
+            done.wait(0.5)
+        return r
+
+    monkeypatch.setattr(A, "_flags", between)
+    th = threading.Thread(target=other)
+    th.start()
+    got["first"] = call(first)
+    th.join(30)
+    assert not failed and not th.is_alive()
+    for name, b in (("first", first), ("second", second)):
+        want, a, vmax = b[2]
+        check(got[name], want, a, vmax, name)
