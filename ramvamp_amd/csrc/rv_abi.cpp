@@ -1164,7 +1164,10 @@ int32_t rv_decode_step(rv_kv* kv, size_t layer, const float* q, size_t q_len, co
   if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
   kv->lens[layer] = len + 1;
   hs = rv::launch_decode(kv, kv->qbuf, n_q, layer, len + 1, scale, 0, kv->n_kv_heads, dout, kv->stream);
-  if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
+  if (hs.e != hipSuccess) {
+    kv->lens[layer] = len;  // (the row is as if never appended: the step can be called again)
+    return hip_fail(err, hs.e, hs.what);
+  }
   return finish(kv, flags, dout, out, q_len, err);
 }
 
@@ -1398,7 +1401,10 @@ int32_t rv_prefill_chunk(rv_kv* kv, size_t layer, const float* q_rows, const flo
     if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
     kv->lens[layer] = len + rows;
     rc = run_rows(kv, kv->qbuf, rows, q_dim, layer, start, p, scale, dout, flags, err);
-    if (rc) return rc;
+    if (rc) {
+      kv->lens[layer] = len;
+      return rc;
+    }
   }
   return finish(kv, flags, dout, out, nq, err);
 }

@@ -635,3 +635,44 @@ def test_bookkeeping_and_refusals():
     with pytest.raises(rv.AttentionError):
         rv.decode_attention(torch.zeros(4 * 64, device="cuda"), kv, 1, 1.0, None, out)
     assert (host(out) == 5.0).all()
+
+
+@pytest.mark.parametrize("call", ["step", "chunk"])
+def test_a_step_refused_for_its_workspace_appends_nothing(call):
+    """Under capture a workspace cannot grow; the same call uncaptured then succeeds."""
+    torch = torch_cuda()
+    say(f"case q8 refused {call}")
+    rng = np.random.default_rng(60)
+    n_kv, group, hd, n = 2, 72, 128, 5000
+    kvd, qd = n_kv * hd, n_kv * group * hd
+    m = 1 if call == "step" else 20
+    kv, held = cache(rng, 2, n_kv, hd, n, cap=n + m)
+    q, k, v = (dev(rng.standard_normal((m, d))) for d in (qd, kvd, kvd))
+    w = torch.ones(hd, device="cuda")
+
+    def run(layer, out):
+        if call == "step":
+            rv.decode_step(kv, layer, q[0], k[0], v[0], w, w, EPS, THETA, n, scale_of(hd), out[0])
+        else:
+            rv.prefill_chunk(kv, layer, q, k, v, w, w, EPS, THETA, n, scale_of(hd), out)
+
+    first, second = (torch.full((m, qd), float("nan"), device="cuda") for _ in range(2))
+    # One split: the query's buffer is there afterwards, no more workspace.
+    kv.set_tuning(rv.RV_TUNE_DECODE_SPLIT_LEN, 8192)
+    run(0, first)
+    torch.cuda.synchronize()
+    # As many as there can be.
+    kv.set_tuning(rv.RV_TUNE_DECODE_SPLIT_LEN, 128)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(rv.DeviceError):
+            run(1, second)
+    assert kv.len(1) == n and np.isnan(host(second)).all()
+    run(1, second)
+    assert kv.len(1) == n + m
+    kk, vv = (host(x) for x in kv.read_rows(1, 0, n + m))
+    got = host(second)
+    for r in (0, m - 1):
+        qr = _norm_rope64(host(q[r]), np.ones(hd), hd, n + r)
+        want, a = attend(qr, kk[:n + r + 1], vv[:n + r + 1], n_kv, hd, scale_of(hd))
+        check(got[r], want, 2 * a, np.abs(vv).max(), f"row {r}")
