@@ -184,7 +184,9 @@ int32_t rv_kv_v_layer(const rv_kv* kv, size_t layer, const void** dev, size_t* n
                       rv_error* err);
 /* kv/mod.rs:428-441 `k_row` / `v_row`, copied to host memory: `dst` gets
  * kv_dim elements of the plane's type (u16 f16 bits or f32); of a Q8_0 cache
- * the row's kv_dim / 32 blocks of 34 bytes, f16 scale then 32 int8 codes. */
+ * the row's kv_dim / 32 blocks of 34 bytes, f16 scale then 32 int8 codes
+ * (attention reads f16(scale * code) of them, as rv_kv_read_rows gives it; the
+ * f32 product differs from that by up to 2^-11 of itself). */
 int32_t rv_kv_read_row(const rv_kv* kv, int plane_v, size_t layer, size_t pos, void* dst,
                        rv_error* err);
 
@@ -270,9 +272,9 @@ int32_t rv_attention_at_rows(const rv_kv* kv, const float* q_rows, size_t rows, 
  * stream; `tails`' workspace is used. The prefix is in use as any cache of a call
  * is: batches of several host threads or streams over one prefix take turns, each
  * binding it to its stream (rv_kv_set_stream orders them) and calling before the
- * next one does. F32 planes take any finite values: they
- * pass through f16 hi + lo operands, rows scaled by powers of two, to 2^-22 of
- * themselves or 2^-34 of the largest row's. */
+ * next one does. F32 planes take any finite values: they pass through f16 hi + lo
+ * operands, rows scaled by powers of two, to 2^-22 of themselves or 2^-34 of the
+ * largest row's. An f16 value below 2^-14 counts to 2^-24 of that. */
 int32_t rv_decode_attention_shared(const rv_kv* prefix, size_t prefix_layer, size_t prefix_positions,
                                    const rv_kv* tails, size_t tail_layer, const float* q_rows, size_t n_seqs,
                                    size_t q_dim, float scale, float* out, uint32_t flags, rv_error* err);

@@ -55,7 +55,7 @@ struct RowsArgs {
   // Partials, a 16-column block's (narrow and tail items) or a 32-column
   // block's (wide items) rows in the order of its wave's registers, so that
   // stores and the merge's loads are whole lines: [slot][block][16 bytes i][64
-  // lanes]. ml: maximum and sum by [slot][column].
+  // lanes]. ml: base and sum by [slot][column].
   float* part;
   float* ml;
   f32x4* aside;           // wide main items longer than kWalkWide: [item][wave][17 x 16 bytes][64 lanes]
@@ -1635,7 +1635,8 @@ void split_positions(long positions, long units, long want, int* n_splits, int* 
 // of columns 21.2, 22.4, 23.8; 200 at 4000, four caches, narrow 60.9, wide with 4, 8
 // waves 49.8, 47.1; 512 at 1000, narrow 35.6, wide 57.9, 46.2, 43.7; 1000
 // at 12000, narrow 485, wide 539, 449, 386; 64 x 4000 Q8_0, narrow 26.8, wide 32.9,
-// 31.9, 34.3; 64 x 16000 f16 55.5, and 62.8, 53.8, 52.4.
+// 31.9, 34.3; 64 x 16000 f16 56.4, and 66.3, 57.6, 53.6 (four caches in turn 62.3,
+// and 70.9, 59.1, 55.1): there the model picks the narrow form, 13 % off.
 // A wide item takes a CU for 7.4 (starting, loading its queries, storing) and `c`
 // per 128 positions. A narrow one takes 5.4 and `n1` alone on its CU, 7.0 and `n2`
 // beside another (f32's registers leave no room for one). What the card does not
