@@ -16,6 +16,9 @@ const SOURCES: &[&str] = &[
         "rv_gemv_abi.cpp",
         "rv_block_abi.cpp",
         "rv_router.hip",
+        "rv_paged.hip",
+        "rv_paged_attn.hip",
+        "rv_paged_abi.cpp",
         "rv_floors.hip",
 ];
 const FLAGS: &[&str] = &["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"];

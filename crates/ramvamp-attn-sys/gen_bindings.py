@@ -21,7 +21,8 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
 INCLUDE = os.path.join(ROOT, "include")
-HEADERS = ["ramvamp_attn.h", "ramvamp_gemv.h", "ramvamp_block.h", "ramvamp_router.h", "ramvamp_floors.h"]
+HEADERS = ["ramvamp_attn.h", "ramvamp_gemv.h", "ramvamp_block.h", "ramvamp_router.h", "ramvamp_paged.h",
+           "ramvamp_floors.h"]
 
 SCALARS = {"void": "()", "int": "c_int", "char": "c_char", "float": "f32", "double": "f64", "size_t": "usize",
            "int8_t": "i8", "uint8_t": "u8", "int16_t": "i16", "uint16_t": "u16", "int32_t": "i32",
@@ -107,7 +108,7 @@ def gen_lib_rs() -> str:
     out = ["// Generated by gen_bindings.py from include/*.h; do not edit by hand.",
            "//! Raw bindings to libramvamp_attn (the MI355X attention hot path's C ABI):",
            "//! one declaration per symbol of include/ramvamp_attn.h, ramvamp_gemv.h,",
-           "//! ramvamp_block.h, ramvamp_router.h and ramvamp_floors.h. The safe wrapper",
+           "//! ramvamp_block.h, ramvamp_router.h, ramvamp_paged.h and ramvamp_floors.h. The safe wrapper",
            "//! that keeps the reference's signatures is crates/ramvamp-attn.",
            "#![allow(non_camel_case_types, clippy::missing_safety_doc)]",
            "use std::os::raw::{c_char, c_int, c_void};", ""]

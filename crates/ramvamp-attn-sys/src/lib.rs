@@ -1,7 +1,7 @@
 // Generated by gen_bindings.py from include/*.h; do not edit by hand.
 //! Raw bindings to libramvamp_attn (the MI355X attention hot path's C ABI):
 //! one declaration per symbol of include/ramvamp_attn.h, ramvamp_gemv.h,
-//! ramvamp_block.h, ramvamp_router.h and ramvamp_floors.h. The safe wrapper
+//! ramvamp_block.h, ramvamp_router.h, ramvamp_paged.h and ramvamp_floors.h. The safe wrapper
 //! that keeps the reference's signatures is crates/ramvamp-attn.
 #![allow(non_camel_case_types, clippy::missing_safety_doc)]
 use std::os::raw::{c_char, c_int, c_void};
@@ -59,6 +59,15 @@ pub const RV_QUANT_BLOCK_COUNT_MISMATCH: i32 = 42;
 pub const RV_QUANT_QUANTIZE_LEN_MISMATCH: i32 = 43;
 pub const RV_QUANT_UNSUPPORTED_FORMAT: i32 = 44;
 pub const RV_FWD_INVALID_TOP_K: i32 = 48;
+pub const RV_PAGED_PAGE_OUT_OF_RANGE: i32 = 56;
+pub const RV_PAGED_SEQUENCE_OUT_OF_RANGE: i32 = 57;
+pub const RV_PAGED_POSITION_OUT_OF_RANGE: i32 = 58;
+pub const RV_ROPE_HALF: u32 = 0;
+pub const RV_ROPE_INTERLEAVED: u32 = 1;
+pub const RV_ROPE_UNSCALED: u32 = 0;
+pub const RV_ROPE_LINEAR: u32 = 1;
+pub const RV_ROPE_NTK: u32 = 2;
+pub const RV_ROPE_YARN: u32 = 3;
 pub const RV_FLOOR_MFMA_F16_16X16X32: i32 = 0;
 pub const RV_FLOOR_MFMA_F16_32X32X16: i32 = 1;
 pub const RV_FLOOR_MFMA_F32_16X16X4: i32 = 2;
@@ -68,6 +77,14 @@ pub const RV_FLOOR_VALU_EXP: i32 = 1;
 pub type rv_elem = i32;
 #[repr(C)]
 pub struct rv_kv {
+    _private: [u8; 0],
+}
+#[repr(C)]
+pub struct rv_rope {
+    _private: [u8; 0],
+}
+#[repr(C)]
+pub struct rv_paged {
     _private: [u8; 0],
 }
 #[repr(C)]
@@ -112,6 +129,14 @@ pub struct rv_attn_block_weights {
     pub wo_len: usize,
     pub q_norm_len: usize,
     pub k_norm_len: usize,
+}
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct rv_page_table {
+    pub ids: *const i32,
+    pub n_seqs: usize,
+    pub pages: usize,
+    pub stride: usize,
 }
 
 extern "C" {
@@ -188,6 +213,20 @@ extern "C" {
     pub fn rv_attn_block_prefill_scratch_bytes(n_rows: usize, hidden: usize, q_dim: usize, kv_dim: usize) -> usize;
     pub fn rv_attn_block_prefill(kv: *mut rv_kv, layer: usize, residual_rows: *mut f32, n_rows: usize, hidden: usize, q_dim: usize, w: *const rv_attn_block_weights, eps: f32, theta: f32, start: usize, scale: f32, scratch: *mut c_void, scratch_len: usize, flags: u32, err: *mut rv_error) -> i32;
     pub fn rv_router_topk(x: *const f32, n_rows: usize, hidden: usize, router: *const f32, router_len: usize, n_experts: usize, top_k: usize, norm_topk_prob: c_int, experts: *mut u32, weights: *mut f32, stream: *mut c_void, flags: u32, err: *mut rv_error) -> i32;
+    pub fn rv_rope_new(head_dim: usize, rotary_dim: usize, layout: u32, theta: f64, scaling: u32, factor: f64, trained_positions: usize, beta_fast: f64, beta_slow: f64, out: *mut *mut rv_rope, err: *mut rv_error) -> i32;
+    pub fn rv_rope_free(rope: *mut rv_rope);
+    pub fn rv_rope_frequencies(rope: *const rv_rope, freq: *mut f64, n: usize, gain: *mut f64, err: *mut rv_error) -> i32;
+    pub fn rv_rope_rows(rope: *const rv_rope, x: *const f32, x_stride: usize, rows: usize, width: usize, positions: *const i32, out: *mut f32, out_stride: usize, stream: *mut c_void, flags: u32, err: *mut rv_error) -> i32;
+    pub fn rv_paged_projected_bytes(n_layers: usize, n_kv_heads: usize, head_dim: usize, n_pages: usize, page_rows: usize, elem: rv_elem, bytes: *mut u64, err: *mut rv_error) -> i32;
+    pub fn rv_paged_new(n_layers: usize, n_kv_heads: usize, head_dim: usize, n_pages: usize, page_rows: usize, elem: rv_elem, device: c_int, out: *mut *mut rv_paged, err: *mut rv_error) -> i32;
+    pub fn rv_paged_free(pg: *mut rv_paged);
+    pub fn rv_paged_set_stream(pg: *mut rv_paged, hip_stream: *mut c_void, err: *mut rv_error) -> i32;
+    pub fn rv_paged_synchronize(pg: *mut rv_paged, err: *mut rv_error) -> i32;
+    pub fn rv_paged_device_status(pg: *mut rv_paged, err: *mut rv_error) -> i32;
+    pub fn rv_paged_append_rows(pg: *mut rv_paged, layer: usize, rope: *const rv_rope, k: *const f32, k_stride: usize, v: *const f32, v_stride: usize, rows: usize, positions: *const i32, seqs: *const i32, table: *const rv_page_table, k_norm_w: *const f32, k_norm_len: usize, eps: f32, flags: u32, err: *mut rv_error) -> i32;
+    pub fn rv_paged_read_rows(pg: *mut rv_paged, layer: usize, rows: usize, positions: *const i32, seqs: *const i32, table: *const rv_page_table, k: *mut c_void, v: *mut c_void, flags: u32, err: *mut rv_error) -> i32;
+    pub fn rv_paged_attention(pg: *mut rv_paged, layer: usize, q: *const f32, q_stride: usize, n_seqs: usize, q_dim: usize, table: *const rv_page_table, lens: *const i32, scale: f32, out: *mut f32, out_stride: usize, flags: u32, err: *mut rv_error) -> i32;
+    pub fn rv_paged_decode_step(pg: *mut rv_paged, layer: usize, rope: *const rv_rope, q: *const f32, q_stride: usize, k: *const f32, k_stride: usize, v: *const f32, v_stride: usize, n_seqs: usize, q_dim: usize, q_norm_w: *const f32, q_norm_len: usize, k_norm_w: *const f32, k_norm_len: usize, eps: f32, table: *const rv_page_table, positions: *const i32, scale: f32, out: *mut f32, out_stride: usize, flags: u32, err: *mut rv_error) -> i32;
     pub fn rv_floor_empty(stream: *mut c_void, err: *mut rv_error) -> i32;
     pub fn rv_floor_stream_read(src: *const c_void, bytes: usize, n_wg: u32, sink: *mut f32, stream: *mut c_void, err: *mut rv_error) -> i32;
     pub fn rv_floor_mfma(form: i32, chains: u32, iters: u32, n_wg: u32, sink: *mut f32, stream: *mut c_void, err: *mut rv_error) -> i32;

@@ -6,8 +6,10 @@ builds it (``build``), loads it (``_lib``), mirrors the reference's Rust
 attention API (``attention``) and quantized projections (``projections``)
 over it, one layer's attention block as a single device call (``block``),
 and makes seeded synthetic inputs (``synth``). Beyond the reference, a cache may
-hold its rows in Q8_0 blocks (``KvCache(..., "q8_0")``), and a batch of sequences
-may decode over a prefix held once (``decode_step_shared``).
+hold its rows in Q8_0 blocks (``KvCache(..., "q8_0")``), a batch of sequences
+may decode over a prefix held once (``decode_step_shared``), and a batch of
+independent sequences over one pool of pages (``PagedKvCache``,
+``paged_decode_step``), its rows rotated by any rotary layout (``Rope``).
 """
 from .attention import (  # noqa: F401
     AttentionError,
@@ -45,5 +47,12 @@ from ._lib import (  # noqa: F401  (knobs of KvCache.set_tuning)
     RV_TUNE_PREFILL_KV_SPLIT,
     RV_TUNE_PREFILL_ROWS,
     RV_TUNE_ROWS_COLUMNS,
+)
+from .paged import (  # noqa: F401
+    PagedKvCache,
+    Rope,
+    paged_attention,
+    paged_decode_step,
+    rope_rows,
 )
 from . import block, projections, router  # noqa: F401,E402

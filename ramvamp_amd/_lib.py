@@ -38,6 +38,13 @@ RV_QF_Q5_K = 2
 RV_QF_Q6_K = 3
 RV_QF_Q8_0 = 4
 RV_QF_Q8_K = 5
+# include/ramvamp_paged.h
+RV_ROPE_HALF = 0
+RV_ROPE_INTERLEAVED = 1
+RV_ROPE_UNSCALED = 0
+RV_ROPE_LINEAR = 1
+RV_ROPE_NTK = 2
+RV_ROPE_YARN = 3
 # include/ramvamp_floors.h
 RV_FLOOR_MFMA_F16_16X16X32 = 0
 RV_FLOOR_MFMA_F16_32X32X16 = 1
@@ -57,6 +64,11 @@ class RvAttnBlockWeights(ctypes.Structure):
                 ("wk", c_void_p), ("wk_len", c_size_t), ("v_format", c_uint32), ("wv", c_void_p),
                 ("wv_len", c_size_t), ("q_norm", c_void_p), ("k_norm", c_void_p), ("o_format", c_uint32),
                 ("wo", c_void_p), ("wo_len", c_size_t), ("q_norm_len", c_size_t), ("k_norm_len", c_size_t)]
+
+
+class RvPageTable(ctypes.Structure):
+    """rv_page_table (include/ramvamp_paged.h)."""
+    _fields_ = [("ids", c_void_p), ("n_seqs", c_size_t), ("pages", c_size_t), ("stride", c_size_t)]
 
 
 # Every symbol include/*.h declares: name -> (restype, argtypes).
@@ -158,6 +170,28 @@ SIGNATURES = {
                                        c_float, c_size_t, c_float, _P, c_size_t, c_uint32, _E]),
     "rv_attn_block_decode_dev": (c_int32, [_P, c_size_t, _P, c_size_t, c_size_t, POINTER(RvAttnBlockWeights),
                                            c_float, c_float, _P, c_size_t, c_float, _P, c_size_t, c_uint32, _E]),
+    # include/ramvamp_paged.h
+    "rv_rope_new": (c_int32, [c_size_t, c_size_t, c_uint32, c_double, c_uint32, c_double, c_size_t, c_double, c_double,
+                              POINTER(c_void_p), _E]),
+    "rv_rope_free": (None, [_P]),
+    "rv_rope_frequencies": (c_int32, [_P, POINTER(c_double), c_size_t, POINTER(c_double), _E]),
+    "rv_rope_rows": (c_int32, [_P, _P, c_size_t, c_size_t, c_size_t, _P, _P, c_size_t, _P, c_uint32, _E]),
+    "rv_paged_projected_bytes": (c_int32, [c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, c_int, POINTER(c_uint64),
+                                           _E]),
+    "rv_paged_new": (c_int32, [c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, c_int, c_int, POINTER(c_void_p),
+                               _E]),
+    "rv_paged_free": (None, [_P]),
+    "rv_paged_set_stream": (c_int32, [_P, _P, _E]),
+    "rv_paged_synchronize": (c_int32, [_P, _E]),
+    "rv_paged_device_status": (c_int32, [_P, _E]),
+    "rv_paged_append_rows": (c_int32, [_P, c_size_t, _P, _P, c_size_t, _P, c_size_t, c_size_t, _P, _P,
+                                       POINTER(RvPageTable), _P, c_size_t, c_float, c_uint32, _E]),
+    "rv_paged_read_rows": (c_int32, [_P, c_size_t, c_size_t, _P, _P, POINTER(RvPageTable), _P, _P, c_uint32, _E]),
+    "rv_paged_attention": (c_int32, [_P, c_size_t, _P, c_size_t, c_size_t, c_size_t, POINTER(RvPageTable), _P, c_float,
+                                     _P, c_size_t, c_uint32, _E]),
+    "rv_paged_decode_step": (c_int32, [_P, c_size_t, _P, _P, c_size_t, _P, c_size_t, _P, c_size_t, c_size_t, c_size_t,
+                                       _P, c_size_t, _P, c_size_t, c_float, POINTER(RvPageTable), _P, c_float, _P,
+                                       c_size_t, c_uint32, _E]),
     # include/ramvamp_floors.h
     "rv_floor_empty": (c_int32, [_P, _E]),
     "rv_floor_stream_read": (c_int32, [_P, c_size_t, c_uint32, _P, _P, _E]),

@@ -55,6 +55,9 @@ _VARIANTS = {
     42: ("KernelError", "BlockCountMismatch", ("weight_blocks", "activation_blocks")),
     43: ("KernelError", "QuantizeLenMismatch", ("format", "floats", "out_blocks")),
     44: ("KernelError", "UnsupportedFormat", ("format",)),
+    56: ("KvError", "PageOutOfRange", ("layer", "row", "page", "n_pages")),
+    57: ("KvError", "SequenceOutOfRange", ("layer", "row", "sequence", "n_seqs")),
+    58: ("KvError", "PositionOutOfTable", ("layer", "row", "position", "positions")),
     48: ("ForwardError", "InvalidTopK", ("top_k", "n_experts")),
 }
 

@@ -41,44 +41,6 @@ struct DstArgs {
   uint32_t layer;
 };
 
-constexpr float kMaxScale = 515.5f;  // 127 * 515.5 rounds to 65472; the next f16, 516, to infinity
-
-// Eight values of a block held by 4 lanes: their codes (+ 128) and the scale.
-struct Oct {
-  f32x4 a, b;
-  __device__ __forceinline__ float operator[](int e) const { return e < 4 ? a[e] : b[e - 4]; }
-};
-
-__device__ __forceinline__ u32x2 q8_oct(const Oct& x, uint16_t& scale) {
-#pragma clang fp contract(off)
-  // The largest magnitude's bits order as integers, and a NaN or an infinity has
-  // larger bits than any finite value.
-  uint32_t m = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(x[e]) & 0x7FFFFFFFu);
-  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, DPP_QUAD_XOR1, 0xF, 0xF, false));
-  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, DPP_QUAD_XOR2, 0xF, 0xF, false));
-  const bool finite = m < 0x7F800000u;
-  float d = finite ? __uint_as_float(m) / 127.f : 0.f;
-  if (d >= 515.75f) d = kMaxScale;  // (halfway to 516, the even one of the two)
-  // Below the smallest normal float the reciprocal may overflow; the f16 scale
-  // is zero there and the codes stand for nothing.
-  const float id = d >= 1.17549435e-38f ? 1.f / d : 0.f;
-  scale = finite ? __builtin_bit_cast(uint16_t, (_Float16)d) : (uint16_t)0x7E00;
-  uint32_t w[2] = {0, 0};
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    // Half away from zero: the conversion truncates, and adding the float below
-    // one half rounds up to the next whole number from exactly one half on.
-    const float y = __builtin_amdgcn_fmed3f(x[e] * id, -127.f, 127.f);
-    const int c = finite ? (int)(y + __builtin_copysignf(0x1.fffffep-2f, y)) : 0;
-    w[e >> 2] |= (uint32_t)(c + 128) << (8 * (e & 3));
-  }
-  return u32x2{w[0], w[1]};
-}
-
-typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
-
 // Quantizes eight values [d, d + 8) of kv head h and stores them at row t of the
 // layer `w` (+ its offsets). The 4 lanes that hold a block call it together.
 template <bool V>

@@ -66,6 +66,50 @@ __device__ __forceinline__ float q8_value(uint8_t code, uint16_t scale) {
   return (float)((_Float16)(float)((int)code - 128) * __builtin_bit_cast(_Float16, scale));
 }
 
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr float kMaxScale = 515.5f;  // 127 * 515.5 rounds to 65472; the next f16, 516, to infinity
+
+struct Oct {
+  f32x4 a, b;
+  __device__ __forceinline__ float operator[](int e) const { return e < 4 ? a[e] : b[e - 4]; }
+  __device__ __forceinline__ void set(int e, float x) {
+    if (e < 4)
+      a[e] = x;
+    else
+      b[e - 4] = x;
+  }
+};
+
+// Eight values of a block held by 4 lanes: their codes (+ 128) and the scale.
+__device__ __forceinline__ u32x2 q8_oct(const Oct& x, uint16_t& scale) {
+#pragma clang fp contract(off)
+  // The largest magnitude's bits order as integers, and a NaN or an infinity has
+  // larger bits than any finite value.
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, DPP_QUAD_XOR1, 0xF, 0xF, false));
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, DPP_QUAD_XOR2, 0xF, 0xF, false));
+  const bool finite = m < 0x7F800000u;
+  float d = finite ? __uint_as_float(m) / 127.f : 0.f;
+  if (d >= 515.75f) d = kMaxScale;  // (halfway to 516, the even one of the two)
+  // Below the smallest normal float the reciprocal may overflow; the f16 scale
+  // is zero there and the codes stand for nothing.
+  const float id = d >= 1.17549435e-38f ? 1.f / d : 0.f;
+  scale = finite ? __builtin_bit_cast(uint16_t, (_Float16)d) : (uint16_t)0x7E00;
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    // Half away from zero: the conversion truncates, and adding the float below
+    // one half rounds up to the next whole number from exactly one half on.
+    const float y = __builtin_amdgcn_fmed3f(x[e] * id, -127.f, 127.f);
+    const int c = finite ? (int)(y + __builtin_copysignf(0x1.fffffep-2f, y)) : 0;
+    w[e >> 2] |= (uint32_t)(c + 128) << (8 * (e & 3));
+  }
+  return u32x2{w[0], w[1]};
+}
+
 // Element `d` of kv head `h` at position `t`, as the readers see it.
 template <typename T, bool V>
 __device__ __forceinline__ float kv_value(const KvView& w, int hd, int h, long t, int d) {

@@ -1,0 +1,174 @@
+"""Rotary frequencies, the paged cache's refusals on the host, and the paged
+kernels' integer arithmetic (tests/paged_deal.cpp), without a GPU."""
+import ctypes
+import math
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+import ramvamp_amd as rv
+from ramvamp_amd import _lib as L
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+def test_dealing_and_places_on_the_host(tmp_path):
+    exe = str(tmp_path / "paged_deal")
+    subprocess.run([os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"), "-x", "hip", "--offload-host-only", "-O1",
+                    "-std=c++17", "-o", exe, os.path.join(HERE, "paged_deal.cpp")], check=True, capture_output=True)
+    out = subprocess.run([exe], capture_output=True, text=True, timeout=100)
+    assert out.returncode == 0 and not out.stdout, out.stdout
+
+
+def frequencies(d, theta, scaling, factor, trained, fast=32.0, slow=1.0):
+    """Pair by pair, as the definition is written."""
+    f, gain = [], 1.0
+    if scaling == "ntk":
+        theta = theta * factor ** (d / (d - 2))
+    if scaling == "yarn":
+        at = [d * math.log(trained / (2 * math.pi * b)) / (2 * math.log(theta)) for b in (fast, slow)]
+        lo, hi = max(math.floor(at[0]), 0), min(math.ceil(at[1]), d - 1)
+        gain = 0.1 * math.log(factor) + 1
+    for i in range(d // 2):
+        x = theta ** (-2 * i / d)
+        if scaling == "linear":
+            x /= factor
+        if scaling == "yarn":
+            r = min(max((i - lo) / max(hi - lo, 0.001), 0), 1)
+            x = x * (1 - r) + x / factor * r
+        f.append(x)
+    return np.array(f), gain
+
+
+@pytest.mark.parametrize("d,theta,scaling,factor,trained", [
+    (128, 1e6, "none", 1, 0), (128, 1e7, None, 1, 0), (2, 1e4, "none", 1, 0), (512, 0.5, "none", 1, 0),
+    (64, 1e4, "linear", 8, 0), (128, 1e6, "ntk", 4, 0), (4, 1e4, "ntk", 1, 0),
+    (128, 1e6, "yarn", 4, 32768), (32, 1e4, "yarn", 40, 4096), (64, 1e4, "yarn", 1, 1), (6, 1e6, "yarn", 2, 10 ** 9),
+])
+def test_rope_frequencies(d, theta, scaling, factor, trained):
+    f, gain = rv.Rope(512, theta, rotary_dim=d, scaling=scaling, factor=factor, trained_positions=trained).frequencies()
+    want, want_gain = frequencies(d, theta, scaling, factor, trained)
+    # pow, log and a handful of f64 operations, each off by at most an ulp of values
+    # that are no larger than what comes out (times the exponent's size for pow).
+    assert np.all(np.abs(f - want) <= 64 * 2.0 ** -52 * want) and abs(gain - want_gain) <= 4 * 2.0 ** -52
+
+
+def test_yarn_leaves_fast_pairs_and_interpolates_slow_ones():
+    f, _ = rv.Rope(128, 1e6, scaling="yarn", factor=4, trained_positions=32768).frequencies()
+    plain, _ = rv.Rope(128, 1e6).frequencies()
+    assert f[0] == plain[0] and abs(f[-1] * 4 / plain[-1] - 1) < 1e-12
+
+
+def test_other_betas_move_the_ramp():
+    f, _ = rv.Rope(64, 1e4, scaling="yarn", factor=8, trained_positions=4096, beta_fast=16, beta_slow=2).frequencies()
+    want, _ = frequencies(64, 1e4, "yarn", 8, 4096, 16, 2)
+    assert np.allclose(f, want, rtol=1e-13, atol=0)
+
+
+@pytest.mark.parametrize("kw,variant", [
+    (dict(head_dim=0, rotary_dim=2), "InvalidHeadDim"), (dict(rotary_dim=0), "InvalidHeadDim"),
+    (dict(rotary_dim=3), "InvalidHeadDim"), (dict(rotary_dim=130), "InvalidHeadDim"),
+    (dict(head_dim=514), "Unsupported"), (dict(theta=0.0), "Unsupported"), (dict(theta=-1.0), "Unsupported"),
+    (dict(theta=math.inf), "Unsupported"), (dict(theta=math.nan), "Unsupported"),
+    (dict(scaling="linear", factor=0.5), "Unsupported"), (dict(scaling="linear", factor=math.nan), "Unsupported"),
+    (dict(scaling="ntk", factor=math.inf), "Unsupported"), (dict(scaling="ntk", factor=2, rotary_dim=2), "Unsupported"),
+    (dict(scaling="yarn", factor=2), "Unsupported"),
+    (dict(scaling="yarn", factor=2, trained_positions=8, theta=1.0), "Unsupported"),
+    (dict(scaling="yarn", factor=2, trained_positions=8, beta_slow=0.0), "Unsupported"),
+    (dict(scaling="yarn", factor=2, trained_positions=8, beta_fast=1.0), "Unsupported"),
+    (dict(scaling="yarn", factor=2, trained_positions=8, beta_fast=math.inf), "Unsupported"),
+])
+def test_rope_refusals(kw, variant):
+    with pytest.raises(rv.RamvampError) as e:
+        rv.Rope(**{"head_dim": 128, "theta": 1e6, **kw})
+    assert e.value.variant == variant
+
+
+def test_rope_names_are_checked():
+    for kw in (dict(layout="neox"), dict(scaling="dynamic")):
+        with pytest.raises(ValueError):
+            rv.Rope(128, 1e6, **kw)
+    err = L.RvError()
+    h = ctypes.c_void_p()
+    assert L.load().rv_rope_new(128, 128, 2, 1e6, 0, 1.0, 0, 32.0, 1.0, ctypes.byref(h), ctypes.byref(err)) == 33
+    assert L.load().rv_rope_new(128, 128, 0, 1e6, 4, 1.0, 0, 32.0, 1.0, ctypes.byref(h), ctypes.byref(err)) == 33
+    assert L.load().rv_rope_new(128, 128, 0, 1e6, 0, 1.0, 0, 32.0, 1.0, None, ctypes.byref(err)) == 32
+
+
+@pytest.mark.parametrize("x,xs,out,os,rows,width,flags,code", [
+    (4096, 128, 8192, 128, 2, 100, 0, 16), (4096, 128, 8192, 128, 2, 0, 0, 16),
+    (4096, 100, 1 << 20, 128, 2, 128, 0, 25), (4096, 128, 1 << 20, 127, 2, 128, 0, 25),
+    (4096, 128, 1 << 20, 128, 2, 128, 1, 33), (None, 128, 1 << 20, 128, 2, 128, 0, 32),
+    (4096, 128, None, 128, 2, 128, 0, 32),
+    (4096, 128, 4100, 128, 2, 128, 0, 33),             # shifted by a value
+    (4096, 256, 4096, 128, 2, 128, 0, 33),             # x's first row is out's
+    (4096, 256, 4096 + 4 * 64, 256, 8, 128, 0, 33),    # half a row further
+    (4096, 256, 4096 + 4 * 320, 256, 8, 128, 0, 33),   # the next row's second half
+])
+def test_rope_rows_refusals(x, xs, out, os, rows, width, flags, code):
+    """Refused before anything is queued: the addresses are never read."""
+    rope, err = rv.Rope(128, 1e6), L.RvError()
+    rc = L.load().rv_rope_rows(rope._h, x, xs, rows, width, 64, out, os, None, flags, ctypes.byref(err))
+    assert rc == code == err.code
+    assert L.load().rv_rope_rows(None, x, xs, rows, width, 64, out, os, None, 0, ctypes.byref(err)) == 32
+
+
+def test_rope_frequencies_refusals():
+    rope, err = rv.Rope(128, 1e6), L.RvError()
+    buf = (ctypes.c_double * 64)()
+    assert L.load().rv_rope_frequencies(rope._h, buf, 63, None, ctypes.byref(err)) == 25
+    assert L.load().rv_rope_frequencies(None, buf, 64, None, ctypes.byref(err)) == 32
+    assert L.load().rv_rope_frequencies(rope._h, None, 64, None, ctypes.byref(err)) == 32
+
+
+def test_projected_bytes():
+    assert rv.PagedKvCache.projected_bytes(48, 4, 128, 1000, 64, "f16") == 48 * 4 * 128 * 64000 * 2 * 2
+    assert rv.PagedKvCache.projected_bytes(1, 4, 128, 3, 8, "f32") == 4 * 128 * 24 * 4 * 2
+    assert rv.PagedKvCache.projected_bytes(2, 1, 96, 5, 1024, "q8_0") == 2 * 3 * 5 * 1024 * 34 * 2
+
+
+@pytest.mark.parametrize("args,variant", [
+    ((0, 4, 128, 8, 64, "f16"), "InvalidDims"), ((1, 0, 128, 8, 64, "f16"), "InvalidDims"),
+    ((1, 4, 0, 8, 64, "f16"), "InvalidDims"), ((1, 4, 128, 0, 64, "f16"), "InvalidDims"),
+    ((1, 4, 128, 8, 4, "f16"), "InvalidDims"), ((1, 4, 128, 8, 48, "f16"), "InvalidDims"),
+    ((1, 4, 128, 8, 2048, "f16"), "InvalidDims"), ((1, 4, 100, 8, 64, "q8_0"), "InvalidDims"),
+    ((1, 4, 513, 8, 64, "f32"), "Unsupported"), ((1, 4, 128, 2 ** 31, 64, "f16"), "Unsupported"),
+    ((1, 2 ** 31, 128, 8, 64, "f16"), "Unsupported"), ((2 ** 60, 4, 128, 8, 64, "f16"), "InvalidDims"),
+    ((2 ** 20, 2 ** 20, 128, 2 ** 30, 1024, "f32"), "InvalidDims"),
+])
+def test_geometry_refusals(args, variant):
+    for call in (rv.PagedKvCache.projected_bytes, rv.PagedKvCache):
+        with pytest.raises(rv.RamvampError) as e:
+            call(*args)
+        assert e.value.variant == variant
+
+
+def test_calls_without_a_cache():
+    lib, err = L.load(), L.RvError()
+    t = L.RvPageTable(None, 0, 0, 0)
+    e, b = ctypes.byref(err), ctypes.byref(t)
+    assert lib.rv_paged_append_rows(None, 0, None, None, 0, None, 0, 0, None, None, b, None, 0, 0.0, 0, e) == 32
+    assert lib.rv_paged_read_rows(None, 0, 0, None, None, b, None, None, 0, e) == 32
+    assert lib.rv_paged_attention(None, 0, None, 0, 0, 0, b, None, 1.0, None, 0, 0, e) == 32
+    assert lib.rv_paged_decode_step(None, 0, None, None, 0, None, 0, None, 0, 0, 0, None, 0, None, 0, 0.0, b, None, 1.0,
+                                    None, 0, 0, e) == 32
+    assert lib.rv_paged_set_stream(None, None, e) == lib.rv_paged_synchronize(None, e) == 32
+    assert lib.rv_paged_device_status(None, e) == 32
+    lib.rv_paged_free(None)
+    lib.rv_rope_free(None)
+
+
+def test_status_names():
+    names = [L.load().rv_status_name(c).decode() for c in (56, 57, 58)]
+    assert names == ["RV_PAGED_PAGE_OUT_OF_RANGE", "RV_PAGED_SEQUENCE_OUT_OF_RANGE", "RV_PAGED_POSITION_OUT_OF_RANGE"]
+
+
+def test_host_tensors_are_refused():
+    torch = pytest.importorskip("torch")
+    x, at = torch.zeros(2, 128), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(TypeError):
+        rv.rope_rows(x, at, rv.Rope(128, 1e6))
+    with pytest.raises(TypeError):
+        rv.rope_rows(np.zeros((2, 128), np.float32), at, rv.Rope(128, 1e6), x)
