@@ -150,8 +150,361 @@ struct Plain {
   }
 };
 
-template <typename Inner>
-__global__ __launch_bounds__(256) void paged_attn_kernel(PagedView w, AttnArgs a) {
+// Heads of whole 16-byte pieces, up to 256 wide (padded to HDP): up to 16 query
+// heads of one kv head are the 16 columns of matrix instructions, a wave takes
+// kRows rows at a time and every fourth such tile of its segment.
+//
+// Scores: S[row][column] = K (A operand: a row a lane, 16 bytes of it straight from
+// memory) times q (B operand, in registers for the whole segment). f16 and Q8_0
+// rows: 16x16x32 f16, q as hi + lo halves scaled by a power of two that puts its
+// largest value in [2^14, 2^15); f32 rows: 16x16x4 f32. A lane then holds four
+// rows of one column (of each 16 rows), which is the A operand of the second
+// product as it stands when the rows are counted in that order: O[column][d] = P
+// times V, for which a lane loads whole 16-byte pieces of those same rows of V and
+// turns the 8 x 8 halves around in registers. P (times 2^15, so that weights down
+// to 2^-38 of the largest count) is hi + lo halves as well.
+//
+// Bound by the rows' bytes: a tile of 32 f16 rows of 128 is 16 KiB and 32 matrix
+// instructions of 16 cycles, and a SIMD's share of the memory rate brings it in
+// some 8000 cycles. So the loads are what is arranged: the next tile's K is asked
+// for as soon as this one's scores are done, its V after this one's product, each
+// into the registers just freed, and page ids a tile ahead of that.
+template <typename T, int HDP, bool FULL>
+struct Tiled {
+  static constexpr bool kF32 = std::is_same<T, float>::value, kQ8 = std::is_same<T, Q8>::value;
+  static constexpr int kRows = kF32 ? 16 : 32, kSub = kRows / 16;
+  static constexpr int VD = kF32 || HDP == 64 ? 4 : 8;  // values of a row of V a lane loads together
+  static constexpr int NH = HDP / (16 * VD);
+  static constexpr int NK = kF32 ? HDP / 16 : kQ8 ? HDP / 64 : HDP / 32;  // 16-byte loads of a row of K a lane
+  static constexpr int NQ = HDP / 32;
+  static constexpr int kBytes = kF32 ? 4 : kQ8 ? 1 : 2;
+  typedef std::conditional_t<kF32, f32x4, u32x4> KReg;
+  typedef std::conditional_t<kF32, f32x4,
+                             std::conditional_t<kQ8, std::conditional_t<VD == 8, u32x2, uint32_t>,
+                                                std::conditional_t<VD == 8, f16x8, f16x4>>> VReg;
+  struct Shared {
+    __attribute__((aligned(16))) float o[4][16][HDP + 4];
+    float m[4][16], l[4][16];
+  };
+  struct Tile {
+    KReg k[kSub][NK];
+    uint16_t ks[kSub][NK];
+    VReg v[4 * kSub][NH];
+    f16x4 vs[kSub][NH];
+  };
+
+  // The first of the eight (f32: four) values of a head that lane group g holds in
+  // operand i.
+  static __device__ __forceinline__ int q_dim(int i, int g) {
+    return kF32 ? 16 * i + 4 * g : kQ8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g;
+  }
+
+  // Values past a head's width are loaded from its start and then cleared, rows
+  // past the last one are rows of the last page, cleared before they count: no
+  // lane goes another way than the others while the operands are in registers.
+  template <typename V>
+  static __device__ __forceinline__ V keep(V x, bool in) {
+    static_assert(sizeof(V) % 4 == 0, "whole words");
+    struct Words {
+      uint32_t w[sizeof(V) / 4];
+    };
+    Words y = __builtin_bit_cast(Words, x);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(V) / 4; ++i) y.w[i] &= in ? 0xFFFFFFFFu : 0u;
+    return __builtin_bit_cast(V, y);
+  }
+
+  static __device__ __forceinline__ void load_k(const PagedView& w, const size_t (&at)[kSub], int g, Tile& t) {
+#pragma unroll
+    for (int j = 0; j < kSub; ++j) {
+      const char* row = w.k + at[j] * w.hd * kBytes;
+#pragma unroll
+      for (int i = 0; i < NK; ++i) {
+        const int d = kF32 ? 16 * i + 4 * g : kQ8 ? 64 * i + 16 * g : 32 * i + 8 * g;
+        const bool in = FULL || d < w.hd;
+        const int dd = in ? d : 0;
+        t.k[j][i] = *reinterpret_cast<const KReg*>(row + dd * kBytes);
+        if constexpr (kQ8)  // (the codes of a scale of zero stand for nothing)
+          t.ks[j][i] = w.ks[at[j] * (w.hd / 32) + dd / 32] & (in ? 0xFFFFu : 0u);
+        else if (!FULL)
+          t.k[j][i] = keep(t.k[j][i], in);
+      }
+    }
+  }
+
+  // hp: page * kv heads + head of the rows.
+  static __device__ __forceinline__ void load_v(const PagedView& w, const size_t (&hp)[kSub],
+                                                const uint32_t (&row)[kSub], int n, Tile& t) {
+#pragma unroll
+    for (int j = 0; j < kSub; ++j) {
+      const char* p = w.v + ((hp[j] << w.t.shift) + row[j]) * w.hd * kBytes;
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        const int d = 16 * VD * h + VD * n;
+        const bool in = FULL || d < w.hd;
+        const int dd = in ? d : 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          t.v[4 * j + i][h] = *reinterpret_cast<const VReg*>(p + ((size_t)i * w.hd + dd) * kBytes);
+          if constexpr (!FULL && !kQ8) t.v[4 * j + i][h] = keep(t.v[4 * j + i][h], in);
+        }
+        if constexpr (kQ8)
+          t.vs[j][h] = keep(*reinterpret_cast<const f16x4*>(
+                                w.vs + ((hp[j] * (w.hd / 32) + dd / 32) << w.t.shift) + row[j]),
+                            in);
+      }
+    }
+  }
+
+  static __device__ __forceinline__ f16x8 widen8(uint32_t a, uint32_t b, _Float16 s) {
+    f16x2 p[4];
+    q8_widen(a, p[0], p[1]);
+    q8_widen(b, p[2], p[3]);
+    f16x8 y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = p[e >> 1][e & 1] * s;
+    return y;
+  }
+
+  static __device__ __forceinline__ void segment(const PagedView& w, const AttnArgs& a, Shared& sh, uint32_t s, int h,
+                                                 int qh, int ncols, long p0, long p1l, bool whole, float* part) {
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t p1 = (uint32_t)p1l, mask = (1u << w.t.shift) - 1;
+    const int32_t* ids = w.t.ids + (long)s * w.t.stride;
+    uint32_t no_page = 0;  // a page id that names no page
+    auto fetch = [&](uint32_t b, uint32_t (&id)[kSub]) {
+#pragma unroll
+      for (int j = 0; j < kSub; ++j) id[j] = (uint32_t)ids[min(b + 16 * j + n, p1 - 1) >> w.t.shift];
+    };
+    size_t k_at[kSub], v_hp[kSub];
+    uint32_t v_row[kSub];
+    auto locate = [&](uint32_t b, const uint32_t (&id)[kSub]) {
+#pragma unroll
+      for (int j = 0; j < kSub; ++j) {
+        const bool is = id[j] < w.t.n_pages;
+        no_page = is ? no_page : id[j];
+        const uint32_t page = is ? id[j] : 0;
+        k_at[j] = (((size_t)page * w.n_kv + h) << w.t.shift) + ((b + 16 * j + n) & mask);
+        v_hp[j] = (size_t)(uint32_t)__shfl((int)page, 4 * g, 64) * w.n_kv + h;
+        v_row[j] = (b + 16 * j + 4 * g) & mask;
+      }
+    };
+    uint32_t b = (uint32_t)p0 + wv * kRows;
+    const bool any = b < p1;
+    Tile t;
+    uint32_t id[kSub];
+    f32x4 acc[NH * VD];
+#pragma unroll
+    for (int i = 0; i < NH * VD; ++i) acc[i] = f32x4{};
+    float m = -INFINITY, l = 0.f;
+    if (any) {
+      fetch(b, id);
+      const float* q = a.q + s * a.q_stride + (long)(qh + min(n, ncols - 1)) * w.hd;
+      f32x4 x[kF32 ? NK : 2 * NQ];
+#pragma unroll
+      for (int i = 0; i < (kF32 ? NK : 2 * NQ); ++i) {
+        const int d = kF32 ? q_dim(i, g) : q_dim(i >> 1, g) + 4 * (i & 1);
+        const bool in = n < ncols && (FULL || d < w.hd);
+        x[i] = keep<f32x4>(*reinterpret_cast<const f32x4u*>(q + (FULL || d < w.hd ? d : 0)), in);
+      }
+      locate(b, id);
+      load_k(w, k_at, g, t);
+      load_v(w, v_hp, v_row, n, t);
+      fetch(b + 4 * kRows, id);
+      float mul = a.scale * kLog2e;
+      f16x8 q_hi[NQ], q_lo[NQ];
+      if constexpr (!kF32) {
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2 * NQ; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(x[i][e]));
+        top = swap_max<32>(swap_max<16>(top));
+        // 2^(14 - its exponent), in two steps where that passes the floats' range.
+        const int ex = top > 0.f && top < INFINITY ? 14 - ilogbf(top) : 0;
+        mul = ldexpf(mul, -ex);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float y = ldexpf(x[2 * i + (e >> 2)][e & 3], ex);
+            q_hi[i][e] = (_Float16)y;
+            q_lo[i][e] = (_Float16)(y - (float)q_hi[i][e]);
+          }
+      }
+      for (;;) {
+        f32x4 sc[kSub];
+#pragma unroll
+        for (int j = 0; j < kSub; ++j) {
+          f32x4 c{};
+          if constexpr (kF32) {
+#pragma unroll
+            for (int i = 0; i < NK; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(t.k[j][i][e], x[i][e], c, 0, 0, 0);
+          } else {
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+              f16x8 k;
+              if constexpr (kQ8)
+                k = widen8(t.k[j][i >> 1][2 * (i & 1)], t.k[j][i >> 1][2 * (i & 1) + 1],
+                           __builtin_bit_cast(_Float16, t.ks[j][i >> 1]));
+              else
+                k = __builtin_bit_cast(f16x8, t.k[j][i]);
+              c = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q_lo[i], c, 0, 0, 0);
+              c = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q_hi[i], c, 0, 0, 0);
+            }
+          }
+          sc[j] = c;
+        }
+        const uint32_t nb = b + 4 * kRows;
+        const bool more = nb < p1, tail = b + kRows > p1;
+        if (more) {
+          locate(nb, id);
+          load_k(w, k_at, g, t);
+          fetch(nb + 4 * kRows, id);
+        }
+        float y[4 * kSub], top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4 * kSub; ++i) {
+          y[i] = sc[i >> 2][i & 3] * mul;
+          if (tail && b + 16 * (i >> 2) + 4 * g + (i & 3) >= p1) y[i] = -INFINITY;
+          top = fmaxf(top, y[i]);
+        }
+        top = fmaxf(m, swap_max<32>(swap_max<16>(top)));
+        if (__any(top > m)) {
+          const float c = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
+          l *= c;
+          m = top;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float f = __shfl(c, 4 * g + r, 64);
+#pragma unroll
+            for (int i = 0; i < NH * VD; ++i) acc[i][r] *= f;
+          }
+        }
+        float p[4 * kSub];
+#pragma unroll
+        for (int i = 0; i < 4 * kSub; ++i) {
+          p[i] = __builtin_amdgcn_exp2f(y[i] - m + (kF32 ? 0.f : 15.f));
+          l += p[i];
+        }
+        if (tail) {  // (what lies behind the last row may be anything)
+#pragma unroll
+          for (int i = 0; i < 4 * kSub; ++i) {
+            const bool in = b + 16 * (i >> 2) + 4 * g + (i & 3) < p1;
+#pragma unroll
+            for (int hh = 0; hh < NH; ++hh) {
+              if constexpr (kQ8)
+                t.vs[i >> 2][hh][i & 3] = in ? t.vs[i >> 2][hh][i & 3] : (_Float16)0.f;
+              else
+                t.v[i][hh] = keep(t.v[i][hh], in);
+            }
+          }
+        }
+        if constexpr (kF32) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int hh = 0; hh < NH; ++hh)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                acc[4 * hh + e] =
+                    __builtin_amdgcn_mfma_f32_16x16x4f32(p[r], t.v[r][hh][e], acc[4 * hh + e], 0, 0, 0);
+        } else {
+          f16x8 p_hi, p_lo;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            p_hi[i] = (_Float16)p[i];
+            p_lo[i] = (_Float16)(p[i] - (float)p_hi[i]);
+          }
+#pragma unroll
+          for (int hh = 0; hh < NH; ++hh) {
+            _Float16 v[8][VD];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if constexpr (kQ8) {
+                const _Float16 vs = t.vs[i >> 2][hh][i & 3];
+                f16x2 c[VD / 2];
+                if constexpr (VD == 8) {
+                  q8_widen(t.v[i][hh][0], c[0], c[1]);
+                  q8_widen(t.v[i][hh][1], c[2], c[3]);
+                } else {
+                  q8_widen(t.v[i][hh], c[0], c[1]);
+                }
+#pragma unroll
+                for (int e = 0; e < VD; ++e) v[i][e] = c[e >> 1][e & 1] * vs;
+              } else {
+#pragma unroll
+                for (int e = 0; e < VD; ++e) v[i][e] = t.v[i][hh][e];
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < VD; ++e) {
+              const f16x8 o = {v[0][e], v[1][e], v[2][e], v[3][e], v[4][e], v[5][e], v[6][e], v[7][e]};
+              f32x4& c = acc[VD * hh + e];
+              c = __builtin_amdgcn_mfma_f32_16x16x32_f16(p_lo, o, c, 0, 0, 0);
+              c = __builtin_amdgcn_mfma_f32_16x16x32_f16(p_hi, o, c, 0, 0, 0);
+            }
+          }
+        }
+        if (!more) break;
+        load_v(w, v_hp, v_row, n, t);
+        b = nb;
+      }
+      l = swap_sum<32>(swap_sum<16>(l));
+    }
+    if (__any(no_page >= w.t.n_pages)) {
+      l = NAN;
+      if (no_page >= w.t.n_pages) paged_refuse(w, RV_PAGED_PAGE_OUT_OF_RANGE, s, no_page, w.t.n_pages);
+    }
+    __syncthreads();
+    if (lane < 16) sh.m[wv][n] = m, sh.l[wv][n] = l;
+    __syncthreads();
+    float f[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int c = 4 * g + r;
+      const float top = fmaxf(fmaxf(sh.m[0][c], sh.m[1][c]), fmaxf(sh.m[2][c], sh.m[3][c]));
+      f[r] = any ? __builtin_amdgcn_exp2f(sh.m[wv][c] - top) : 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (4 * g + r < ncols) {
+#pragma unroll
+        for (int hh = 0; hh < NH; ++hh)
+#pragma unroll
+          for (int e = 0; e < VD; e += 4)
+            *reinterpret_cast<f32x4*>(&sh.o[wv][4 * g + r][16 * VD * hh + VD * n + e]) =
+                f32x4{acc[VD * hh + e][r] * f[r], acc[VD * hh + e + 1][r] * f[r], acc[VD * hh + e + 2][r] * f[r],
+                      acc[VD * hh + e + 3][r] * f[r]};
+      }
+    __syncthreads();
+    for (int i = threadIdx.x; i < ncols * (HDP / 4); i += 256) {
+      const int c = i / (HDP / 4), d = 4 * (i % (HDP / 4));
+      if (!FULL && d >= w.hd) continue;
+      const float top = fmaxf(fmaxf(sh.m[0][c], sh.m[1][c]), fmaxf(sh.m[2][c], sh.m[3][c]));
+      f32x4 o{};
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        o += *reinterpret_cast<const f32x4*>(&sh.o[k][c][d]);
+        // (a wave without rows has no sum)
+        if (sh.l[k][c] != 0.f) sum += __builtin_amdgcn_exp2f(sh.m[k][c] - top) * sh.l[k][c];
+      }
+      if (whole) {
+        *reinterpret_cast<f32x4u*>(a.out + s * a.out_stride + (long)(qh + c) * w.hd + d) = o / sum;
+      } else {
+        *reinterpret_cast<f32x4u*>(part + 2 * a.cols + (long)c * w.hd + d) = o;
+        if (d == 0) part[c] = top, part[a.cols + c] = sum;
+      }
+    }
+  }
+};
+
+template <typename Inner, int WAVES>
+__global__ __launch_bounds__(256, WAVES) void paged_attn_kernel(PagedView w, AttnArgs a) {
   __shared__ typename Inner::Shared sh;
   __shared__ long sums[4];
   __shared__ long found[2];
@@ -221,17 +574,46 @@ __global__ __launch_bounds__(128) void paged_join_kernel(PagedView w, AttnArgs a
   }
 }
 
+// The matrix-instruction kernel takes heads of whole 16-byte pieces (in any type)
+// up to 256 wide; the others one position at a time.
+bool tiled(int hd) { return hd % 8 == 0 && hd <= 256; }
+
+int cols_of(int hd, int group) { return tiled(hd) ? std::min(group, 16) : 1; }
+
 // Workgroups that deal the work of any lengths.
-unsigned ranges(const rv_paged*, size_t n, size_t n_q) {
-  return (unsigned)std::min<size_t>(2048, std::max<size_t>(2 * kCUs, n * n_q));
+unsigned ranges(size_t items) {
+  return (unsigned)std::min<size_t>(2048, std::max<size_t>(2 * kCUs, items));
 }
 
 size_t plan_bytes(size_t n) { return ((n + 1) * sizeof(long) + 255) / 256 * 256; }
 
+template <typename T>
+void launch_attn(const PagedView& w, const AttnArgs& a, dim3 grid, hipStream_t s) {
+#define RV_TILED(HDP, FULL, WAVES) \
+  hipLaunchKernelGGL((paged_attn_kernel<Tiled<T, HDP, FULL>, WAVES>), grid, dim3(256), 0, s, w, a)
+  if (!tiled(w.hd))
+    hipLaunchKernelGGL((paged_attn_kernel<Plain<T>, 1>), grid, dim3(256), 0, s, w, a);
+  else if (w.hd == 64)
+    RV_TILED(64, true, 2);
+  else if (w.hd < 64)
+    RV_TILED(64, false, 2);
+  else if (w.hd == 128)
+    RV_TILED(128, true, 2);
+  else if (w.hd < 128)
+    RV_TILED(128, false, 2);
+  else if (w.hd == 256)
+    RV_TILED(256, true, 1);
+  else
+    RV_TILED(256, false, 1);
+#undef RV_TILED
+}
+
 }  // namespace
 
 size_t paged_attn_ws(const rv_paged* pg, size_t n, size_t n_q) {
-  return plan_bytes(n) + (size_t)ranges(pg, n, n_q) * 2 * (pg->head_dim + 2) * sizeof(float);
+  const size_t group = n_q / pg->n_kv_heads, cols = cols_of((int)pg->head_dim, (int)group);
+  const size_t items = n * pg->n_kv_heads * ((group + cols - 1) / cols);
+  return plan_bytes(n) + (size_t)ranges(items) * 2 * cols * (pg->head_dim + 2) * sizeof(float);
 }
 
 HipStatus launch_paged_attn(const rv_paged* pg, const PagedView& w, const PagedAttn& p, hipStream_t s) {
@@ -242,21 +624,21 @@ HipStatus launch_paged_attn(const rv_paged* pg, const PagedView& w, const PagedA
   a.n = (uint32_t)p.n;
   a.step = p.step;
   a.group = p.n_q / w.n_kv;
-  a.cols = 1;
+  a.cols = cols_of(w.hd, a.group);
   a.blocks = (a.group + a.cols - 1) / a.cols;
   a.scale = p.scale;
   a.out = p.out;
   a.out_stride = (long)p.out_stride;
   a.plan = (long*)pg->ws;
   a.part = (float*)((char*)pg->ws + plan_bytes(p.n));
-  const dim3 grid(ranges(pg, p.n, p.n_q));
+  const dim3 grid(ranges(p.n * w.n_kv * a.blocks));
   HipStatus st;
   if (pg->elem == RV_ELEM_F32)
-    hipLaunchKernelGGL(paged_attn_kernel<Plain<float>>, grid, dim3(256), 0, s, w, a);
+    launch_attn<float>(w, a, grid, s);
   else if (pg->elem == RV_ELEM_F16)
-    hipLaunchKernelGGL(paged_attn_kernel<Plain<_Float16>>, grid, dim3(256), 0, s, w, a);
+    launch_attn<_Float16>(w, a, grid, s);
   else
-    hipLaunchKernelGGL(paged_attn_kernel<Plain<Q8>>, grid, dim3(256), 0, s, w, a);
+    launch_attn<Q8>(w, a, grid, s);
   st.e = hipGetLastError();
   if (st.e != hipSuccess) {
     st.what = "paged attention launch";
