@@ -36,8 +36,10 @@ struct rv_paged {
   unsigned* status = nullptr;  // [0] code, [1] layer, [2] row, [3] what it read, [4] the bound
   // Grown on first need; a replaced buffer is kept until the cache is freed,
   // since a graph captured earlier may still address it.
-  void* ws = nullptr;  // attention: the batch's plan and the split partials
+  void* ws = nullptr;  // attention's partials
   size_t ws_bytes = 0;
+  unsigned* tickets = nullptr;  // and their tickets, zero between calls
+  size_t ticket_bytes = 0;
   float* qbuf = nullptr;  // a step's normed and rotated q rows
   size_t qbuf_bytes = 0;
   std::vector<void*> retired;
@@ -138,7 +140,12 @@ struct PagedAttn {
   float* out;
   size_t out_stride;
 };
-size_t paged_attn_ws(const rv_paged* pg, size_t n, size_t n_q);
-HipStatus launch_paged_attn(const rv_paged* pg, const PagedView& w, const PagedAttn& a, hipStream_t s);
+struct PagedAttnPlan {
+  size_t units;  // of work at most, by what the tables can hold (below 2^31)
+  size_t ws_bytes, ticket_bytes;
+};
+PagedAttnPlan paged_attn_plan(const rv_paged* pg, const rv_page_table& t, size_t n, size_t n_q);
+HipStatus launch_paged_attn(const rv_paged* pg, const PagedView& w, const PagedAttn& a, const PagedAttnPlan& plan,
+                            hipStream_t s);
 
 }  // namespace rv

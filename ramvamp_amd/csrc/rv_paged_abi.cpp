@@ -121,6 +121,27 @@ rv::HipStatus grow(rv_paged* pg, void** buf, size_t* have, size_t bytes, const c
   return st;
 }
 
+// What attention needs of the cache; the units it deals are counted in 32 bits.
+int32_t ready_attn(rv_paged* pg, const rv_page_table& t, size_t n, size_t n_q, rv::PagedAttnPlan* plan,
+                   rv_error* err) {
+  *plan = rv::paged_attn_plan(pg, t, n, n_q);
+  if (plan->units > 0x7FFFFFFFu)
+    return fail(err, RV_ERR_UNSUPPORTED, plan->units, 0, 0, 0, "rows of the tables (128 a unit, for each kv head)");
+  rv::HipStatus st = grow(pg, &pg->ws, &pg->ws_bytes, plan->ws_bytes, "hipMalloc workspace");
+  const size_t had = pg->ticket_bytes;
+  if (st.e == hipSuccess)
+    st = grow(pg, (void**)&pg->tickets, &pg->ticket_bytes, plan->ticket_bytes, "hipMalloc tickets");
+  if (st.e == hipSuccess && pg->ticket_bytes != had) {
+    st.e = hipMemset(pg->tickets, 0, pg->ticket_bytes);
+    if (st.e == hipSuccess) st.e = hipDeviceSynchronize();
+    if (st.e != hipSuccess) {
+      st.what = "clear the tickets";
+      pg->ticket_bytes = 0;  // (the next call makes them anew)
+    }
+  }
+  return st.e == hipSuccess ? RV_OK : hip_fail(err, st);
+}
+
 int32_t check_layer(const rv_paged* pg, size_t layer, rv_error* err) {
   if (layer >= pg->n_layers) return fail(err, RV_KV_LAYER_OUT_OF_RANGE, layer, pg->n_layers);
   return RV_OK;
@@ -318,7 +339,7 @@ void rv_paged_free(rv_paged* pg) {
   {
     DeviceGuard dg(pg->device);
     (void)hipDeviceSynchronize();
-    for (void* p : {pg->k, pg->v, (void*)pg->status, pg->ws, (void*)pg->qbuf})
+    for (void* p : {pg->k, pg->v, (void*)pg->status, pg->ws, (void*)pg->tickets, (void*)pg->qbuf})
       if (p) (void)hipFree(p);
     for (void* p : pg->retired) (void)hipFree(p);
     if (pg->order_ev) (void)hipEventDestroy(pg->order_ev);
@@ -432,10 +453,11 @@ int32_t rv_paged_attention(rv_paged* pg, size_t layer, const float* q, size_t q_
   if (n_seqs == 1) q_stride = out_stride = q_dim;
   if (overlap(q, q_stride, out, out_stride, n_seqs, q_dim)) return unsupported(err, 0, "out overlaps q");
   const size_t n_q = q_dim / pg->head_dim;
-  rv::HipStatus st = grow(pg, &pg->ws, &pg->ws_bytes, rv::paged_attn_ws(pg, n_seqs, n_q), "hipMalloc workspace");
-  if (st.e != hipSuccess) return hip_fail(err, st);
+  rv::PagedAttnPlan plan;
+  if ((rc = ready_attn(pg, *table, n_seqs, n_q, &plan, err))) return rc;
   const rv::PagedAttn a{q, q_stride, n_seqs, (int)n_q, lens, false, scale, out, out_stride};
-  return finish(pg->stream, flags, rv::launch_paged_attn(pg, rv::paged_view(pg, layer, *table), a, pg->stream), err);
+  return finish(pg->stream, flags, rv::launch_paged_attn(pg, rv::paged_view(pg, layer, *table), a, plan, pg->stream),
+                err);
 }
 
 int32_t rv_paged_decode_step(rv_paged* pg, size_t layer, const rv_rope* rope, const float* q, size_t q_stride,
@@ -462,9 +484,9 @@ int32_t rv_paged_decode_step(rv_paged* pg, size_t layer, const rv_rope* rope, co
   for (const auto& p : {std::pair<const void*, const char*>{q, "q"}, {k, "k"}, {v, "v"}, {positions, "positions"}, {out, "out"}})
     if (!p.first) return null_arg(err, p.second);
   const size_t n_q = q_dim / pg->head_dim;
-  rv::HipStatus st = grow(pg, &pg->ws, &pg->ws_bytes, rv::paged_attn_ws(pg, n_seqs, n_q), "hipMalloc workspace");
-  if (st.e == hipSuccess)
-    st = grow(pg, (void**)&pg->qbuf, &pg->qbuf_bytes, n_seqs * q_dim * sizeof(float), "hipMalloc q buffer");
+  rv::PagedAttnPlan plan;
+  if ((rc = ready_attn(pg, *table, n_seqs, n_q, &plan, err))) return rc;
+  rv::HipStatus st = grow(pg, (void**)&pg->qbuf, &pg->qbuf_bytes, n_seqs * q_dim * sizeof(float), "hipMalloc q buffer");
   if (st.e != hipSuccess) return hip_fail(err, st);
   rv::PagedRows r{};
   r.q = q;
@@ -484,7 +506,7 @@ int32_t rv_paged_decode_step(rv_paged* pg, size_t layer, const rv_rope* rope, co
   st = rv::launch_paged_append(pg, w, rope_args(rope), r, pg->stream);
   if (st.e == hipSuccess) {
     const rv::PagedAttn a{pg->qbuf, q_dim, n_seqs, (int)n_q, positions, true, scale, out, out_stride};
-    st = rv::launch_paged_attn(pg, w, a, pg->stream);
+    st = rv::launch_paged_attn(pg, w, a, plan, pg->stream);
   }
   return finish(pg->stream, flags, st, err);
 }

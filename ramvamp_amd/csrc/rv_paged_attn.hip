@@ -5,13 +5,15 @@
 // the rows with the running maximum m.
 //
 // The lengths are on the device and ragged, so the work is dealt there: a unit is
-// kUnitRows positions of one item (a sequence's kv head, or a part of its query
+// kUnitRows rows of one item (a sequence's kv head, or a part of its query
 // heads), the units of the batch in order are cut into equal ranges, one a
-// workgroup, and every workgroup finds its own range by a prefix sum over the
+// workgroup, and every wave finds its workgroup's range by a prefix sum over the
 // lengths. An item inside one range is finished there; one that is cut leaves a
-// partial (maximum, sum, weighted sum of v) per range, at most two a workgroup
-// (its first item and its last), and a second launch joins them in order, so
-// that results do not depend on which workgroup ends first.
+// partial (weighted sum of v, maximum, sum) per range, at most two a workgroup
+// (its first item and its last). The workgroup that leaves an item's last partial
+// joins them all, in order, so that results do not depend on which that is.
+// Partials are stored and loaded at device scope (the XCDs' L2s do not see each
+// other's lines), and counted by tickets that are zero between calls.
 #include "rv_paged.hpp"
 
 #include <algorithm>
@@ -31,37 +33,131 @@ struct AttnArgs {
   float scale;
   float* out;
   long out_stride;
-  long* plan;   // [0] units a range, [1 + s] units before sequence s
-  float* part;  // [workgroup][2][cols * (hd + 2)]: maxima, sums, rows
+  unsigned* tickets;  // one a range (its group's), then one an item
+  float* part;        // [range][2][cols * (hd + 2)]: rows, then (maximum, sum) of each column
+  uint32_t part_bytes;
 };
 
-// Rows sequence s attends; negative: refused.
-__device__ __forceinline__ long seq_rows(const PagedView& w, const AttnArgs& a, uint32_t s, bool say) {
-  const int len = a.lens[s];
-  const long rows = attended_rows(w.t, len, a.step);
-  if (rows < 0 && say)
-    paged_refuse(w, RV_PAGED_POSITION_OUT_OF_RANGE, s, (uint32_t)len, (uint32_t)min(table_rows(w.t), 0xFFFFFFFFl));
-  return rows;
+constexpr uint32_t kMaxRanges = 2048;
+constexpr uint32_t kRefused = 0xFFFFFFFFu;
+
+// Rows a sequence of this length attends, kRefused where the table has not so many.
+__device__ __forceinline__ uint32_t rows_of_len(const PagedView& w, const AttnArgs& a, int len) {
+  return (uint32_t)attended_rows(w.t, len, a.step);
 }
 
-// Sum over the workgroup, and of the threads before this one.
-__device__ __forceinline__ long block_scan(long x, long& before, long* sums) {
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  long inc = x;
-  for (int o = 1; o < 64; o <<= 1) {
-    const long y = __shfl_up(inc, o, 64);
-    if (lane >= o) inc += y;
+__device__ __forceinline__ uint32_t units_of_rows(uint32_t rows) { return rows == kRefused ? 0 : units_of(rows); }
+
+// Sum of the lanes up to and including this one.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+#define RV_SHIFTED(CTRL, ROWS) (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, false)
+  x += RV_SHIFTED(0x111, 0xF);  // row_shr:1, 2, 4, 8: within 16 lanes
+  x += RV_SHIFTED(0x112, 0xF);
+  x += RV_SHIFTED(0x114, 0xF);
+  x += RV_SHIFTED(0x118, 0xF);
+  x += RV_SHIFTED(0x142, 0xA);  // row_bcast:15 into the odd rows
+  x += RV_SHIFTED(0x143, 0xC);  // row_bcast:31 into the upper half
+#undef RV_SHIFTED
+  return x;
+}
+
+// ---- partials ---------------------------------------------------------------------
+
+constexpr int kDeviceScope = 16;  // the sc1 bit of a buffer instruction's cache policy
+
+struct Partials {
+  __amdgpu_buffer_rsrc_t rs;
+  int cols, hd;
+  __device__ __forceinline__ Partials(const AttnArgs& a, int hd_)
+      : rs(__builtin_amdgcn_make_buffer_rsrc(a.part, (short)0, (int)a.part_bytes, 0x00020000)), cols(a.cols), hd(hd_) {}
+  // Byte offset of a partial; of column c's (maximum, sum) in it.
+  __device__ __forceinline__ uint32_t at(uint32_t range, int which) const {
+    return (range * 2 + which) * (uint32_t)(cols * (hd + 2)) * 4u;
+  }
+  __device__ __forceinline__ uint32_t stat(int c) const { return (uint32_t)(cols * hd + 2 * c) * 4u; }
+  __device__ __forceinline__ void put_stat(uint32_t p, int c, float m, float l) const {
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, m), rs, p + stat(c), 0, kDeviceScope);
+    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, l), rs, p + stat(c) + 4, 0, kDeviceScope);
+  }
+  __device__ __forceinline__ float word(uint32_t o) const {
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, o, 0, kDeviceScope));
+  }
+};
+
+// Joins `count` partials, of ranges first, first + step, .. (which(i): the one of
+// range i's two), in order: into `out` (ncols rows of hd), or into the first's place.
+// A thread has one column's VEC values, and kBatch partials in flight.
+template <int VEC, typename Which>
+__device__ __forceinline__ void join(const Partials& p, uint32_t first, uint32_t step, uint32_t count, Which which,
+                                     int ncols, float* out) {
+  constexpr int kBatch = 16;
+  typedef float Row __attribute__((ext_vector_type(VEC)));
+  const int pieces = p.hd / VEC;
+  for (int j = threadIdx.x; j < ncols * pieces; j += 256) {
+    const int c = j / pieces, d = (j - c * pieces) * VEC;
+    float m = -INFINITY, l = 0.f;
+    Row o = (Row)0.f;
+    for (uint32_t b0 = 0; b0 < count; b0 += kBatch) {
+      Row x[kBatch];
+      float mx[kBatch], lx[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const uint32_t r = first + step * min(b0 + i, count - 1), at = p.at(r, which(r));
+        if constexpr (VEC == 4)
+          x[i] = __builtin_bit_cast(Row, __builtin_amdgcn_raw_buffer_load_b128(
+                                             p.rs, at + (uint32_t)(c * p.hd + d) * 4u, 0, kDeviceScope));
+        else
+          x[i] = p.word(at + (uint32_t)(c * p.hd + d) * 4u);
+        mx[i] = p.word(at + p.stat(c));
+        lx[i] = p.word(at + p.stat(c) + 4);
+      }
+      float top = m;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) top = fmaxf(top, mx[i]);  // (repeats of the last change nothing)
+      // Where every score so far is minus infinity or NaN nothing is scaled, and the
+      // sums carry what there is.
+      const float f = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
+      o *= f;
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (b0 + i < count) {
+          const float g = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx[i] - top);
+          o += x[i] * g;
+          l += lx[i] * g;
+        }
+      m = top;
+    }
+    if (out) {
+      const Row y = o / l;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) out[(long)c * p.hd + d + e] = y[e];
+    } else {
+      const uint32_t at = p.at(first, which(first));
+      if constexpr (VEC == 4) {
+        __builtin_amdgcn_raw_buffer_store_b128(o, p.rs, at + (uint32_t)(c * p.hd + d) * 4u, 0, kDeviceScope);
+      } else {
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, (float)o[0]), p.rs,
+                                              at + (uint32_t)(c * p.hd + d) * 4u, 0, kDeviceScope);
+      }
+      if (d == 0) p.put_stat(at, c, m, l);
+    }
+  }
+}
+
+// Whether this workgroup is the last of `n` to come here, its stores of partials
+// complete; the last leaves the ticket zero for the next call.
+__device__ __forceinline__ bool last_of(unsigned* ticket, uint32_t n, unsigned& drawn) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    drawn = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (drawn == n - 1) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
-  if (lane == 63) sums[wv] = inc;
-  __syncthreads();
-  long total = 0, skip = 0;
-  for (int i = 0; i < 4; ++i) {
-    if (i < wv) skip += sums[i];
-    total += sums[i];
-  }
-  before = skip + inc - x;
-  return total;
+  const bool last = drawn == n - 1;
+  __syncthreads();  // (the next draw writes it)
+  return last;
 }
 
 template <typename T>
@@ -82,13 +178,16 @@ __device__ __forceinline__ float paged_value(const PagedView& w, bool is_v, size
 template <typename T>
 struct Plain {
   static constexpr int kPer = kMaxHalf * 2 / 64;
+  static constexpr int kVec = 1;
   struct Shared {
     float o[4][kMaxHalf * 2];
     float m[4], l[4];
   };
-  // Positions [p0, p1) of sequence s, kv head h, query head qh (of the whole).
+  // Rows [p0, p1) of sequence s, kv head h, query head qh (of the whole): the
+  // output where `whole`, else the partial at `part`.
   static __device__ __forceinline__ void segment(const PagedView& w, const AttnArgs& a, Shared& sh, uint32_t s, int h,
-                                                 int qh, int, long p0, long p1, bool whole, float* part) {
+                                                 int qh, int, uint32_t p0, uint32_t p1, bool whole,
+                                                 const Partials& pt, uint32_t part) {
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const float* q = a.q + s * a.q_stride + (long)qh * w.hd;
     const float scale = a.scale * kLog2e;
@@ -100,7 +199,7 @@ struct Plain {
       o[j] = 0.f;
     }
     float m = -INFINITY, l = 0.f;
-    for (long p = p0 + wv; p < p1; p += 4) {
+    for (uint32_t p = p0 + wv; p < p1; p += 4) {
       uint32_t page = (uint32_t)w.t.ids[(long)s * w.t.stride + (p >> w.t.shift)];
       if (page >= w.t.n_pages) {
         if (lane == 0) paged_refuse(w, RV_PAGED_PAGE_OUT_OF_RANGE, s, page, w.t.n_pages);
@@ -108,7 +207,7 @@ struct Plain {
         continue;
       }
       const size_t hp = (size_t)page * w.n_kv + h;
-      const uint32_t row = (uint32_t)p & ((1u << w.t.shift) - 1);
+      const uint32_t row = p & ((1u << w.t.shift) - 1);
       float dot = 0.f;
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
@@ -144,9 +243,9 @@ struct Plain {
       if (whole)
         a.out[s * a.out_stride + (long)qh * w.hd + d] = y / sum;
       else
-        part[2 + d] = y;
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, y), pt.rs, part + 4u * d, 0, kDeviceScope);
     }
-    if (!whole && threadIdx.x == 0) part[0] = top, part[1] = sum;
+    if (!whole && threadIdx.x == 0) pt.put_stat(part, 0, top, sum);
   }
 };
 
@@ -178,6 +277,7 @@ struct Tiled {
   static constexpr int NK = kF32 ? HDP / 16 : kQ8 ? HDP / 64 : HDP / 32;  // 16-byte loads of a row of K a lane
   static constexpr int NQ = HDP / 32;
   static constexpr int kBytes = kF32 ? 4 : kQ8 ? 1 : 2;
+  static constexpr int kVec = 4;
   typedef std::conditional_t<kF32, f32x4, u32x4> KReg;
   typedef std::conditional_t<kF32, f32x4,
                              std::conditional_t<kQ8, std::conditional_t<VD == 8, u32x2, uint32_t>,
@@ -267,10 +367,11 @@ struct Tiled {
   }
 
   static __device__ __forceinline__ void segment(const PagedView& w, const AttnArgs& a, Shared& sh, uint32_t s, int h,
-                                                 int qh, int ncols, long p0, long p1l, bool whole, float* part) {
+                                                 int qh, int ncols, uint32_t p0, uint32_t p1, bool whole,
+                                                 const Partials& pt, uint32_t part) {
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const uint32_t p1 = (uint32_t)p1l, mask = (1u << w.t.shift) - 1;
+    const uint32_t mask = (1u << w.t.shift) - 1;
     const int32_t* ids = w.t.ids + (long)s * w.t.stride;
     uint32_t no_page = 0;  // a page id that names no page
     auto fetch = [&](uint32_t b, uint32_t (&id)[kSub]) {
@@ -290,7 +391,7 @@ struct Tiled {
         v_row[j] = (b + 16 * j + 4 * g) & mask;
       }
     };
-    uint32_t b = (uint32_t)p0 + wv * kRows;
+    uint32_t b = p0 + wv * kRows;
     const bool any = b < p1;
     Tile t;
     uint32_t id[kSub];
@@ -496,8 +597,8 @@ struct Tiled {
       if (whole) {
         *reinterpret_cast<f32x4u*>(a.out + s * a.out_stride + (long)(qh + c) * w.hd + d) = o / sum;
       } else {
-        *reinterpret_cast<f32x4u*>(part + 2 * a.cols + (long)c * w.hd + d) = o;
-        if (d == 0) part[c] = top, part[a.cols + c] = sum;
+        __builtin_amdgcn_raw_buffer_store_b128(o, pt.rs, part + (uint32_t)(c * w.hd + d) * 4u, 0, kDeviceScope);
+        if (d == 0) pt.put_stat(part, c, top, sum);
       }
     }
   }
@@ -506,71 +607,72 @@ struct Tiled {
 template <typename Inner, int WAVES>
 __global__ __launch_bounds__(256, WAVES) void paged_attn_kernel(PagedView w, AttnArgs a) {
   __shared__ typename Inner::Shared sh;
-  __shared__ long sums[4];
-  __shared__ long found[2];
-  const int tid = threadIdx.x;
-  const bool planner = blockIdx.x == 0;
-  const long items = (long)w.n_kv * a.blocks;
-  long mine = 0, before;
-  for (uint32_t s = tid; s < a.n; s += 256) mine += units_of(seq_rows(w, a, s, planner)) * items;
-  const long total = block_scan(mine, before, sums);
-  const long per = units_per_range(total, gridDim.x);
-  const long start = blockIdx.x * per, end = min(total, start + per);
-  if (tid == 0) found[0] = -1;
-  long base = 0;
-  for (uint32_t s0 = 0; s0 < a.n; s0 += 256) {
-    const uint32_t s = s0 + tid;
-    const long u = s < a.n ? units_of(seq_rows(w, a, s, false)) * items : 0;
-    const long sum = block_scan(u, before, sums);
-    if (planner && s < a.n) a.plan[1 + s] = base + before;
-    if (start >= base + before && start < base + before + u) found[0] = s, found[1] = base + before;
-    base += sum;
-    if (!planner && start < base) break;
-  }
-  if (planner && tid == 0) a.plan[0] = per;
-  if (start >= end) return;
-  __syncthreads();
-  walk_units(
-      (uint32_t)found[0], start - found[1], start, end, items, [&](uint32_t s) { return seq_rows(w, a, s, false); },
-      [&](uint32_t s, long rows, long item, long u0, long u1, long at) {
-        const int h = (int)(item / a.blocks), c0 = (int)(item % a.blocks) * a.cols;
-        float* part = a.part + ((long)blockIdx.x * 2 + partial_of(blockIdx.x, per, at)) * a.cols * (w.hd + 2);
-        Inner::segment(w, a, sh, s, h, h * a.group + c0, min(a.cols, a.group - c0), u0 * kUnitRows,
-                       min(rows, u1 * kUnitRows), u0 == 0 && u1 == units_of(rows), part);
-      });
-}
-
-// grid (sequences, query heads): joins the partials of items that were cut; a
-// sequence without rows gets zeros, a refused one NaN.
-__global__ __launch_bounds__(128) void paged_join_kernel(PagedView w, AttnArgs a) {
-  const uint32_t s = blockIdx.x, qh = blockIdx.y;
-  float* out = a.out + s * a.out_stride + (long)qh * w.hd;
-  const long rows = seq_rows(w, a, s, false), units = units_of(rows);
-  if (rows <= 0) {
-    for (int d = threadIdx.x; d < w.hd; d += 128) out[d] = rows < 0 ? NAN : 0.f;
-    return;
-  }
-  const long per = a.plan[0], h = qh / a.group, g = qh % a.group;
-  const long start = a.plan[1 + s] + (h * a.blocks + g / a.cols) * units, end = start + units;
-  const long w0 = start / per, w1 = (end - 1) / per;
-  if (w0 == w1) return;
-  const int c = (int)(g % a.cols);
-  const long step = (long)a.cols * (w.hd + 2);
-  auto part = [&](long i) { return a.part + (i * 2 + partial_of(i, per, start)) * step; };
-  float top = -INFINITY;
-  for (long i = w0; i <= w1; ++i) top = fmaxf(top, part(i)[c]);
-  float sum = 0.f;
-  for (long i = w0; i <= w1; ++i) {
-    const float m = part(i)[c], l = part(i)[a.cols + c];
-    sum += m == -INFINITY ? l : exp2f(m - top) * l;
-  }
-  for (int d = threadIdx.x; d < w.hd; d += 128) {
-    float y = 0.f;
-    for (long i = w0; i <= w1; ++i) {
-      const float m = part(i)[c];
-      if (m != -INFINITY) y += exp2f(m - top) * part(i)[2 * a.cols + (long)c * w.hd + d];
+  __shared__ unsigned drawn;
+  const int lane = threadIdx.x & 63;
+  const uint32_t r = blockIdx.x, items = (uint32_t)(w.n_kv * a.blocks);
+  // Sequence i's rows, for the 64 from s0 on a lane each.
+  auto chunk = [&](uint32_t s0) {
+    return s0 + lane < a.n ? rows_of_len(w, a, a.lens[s0 + lane]) : 0u;
+  };
+  uint32_t rows = chunk(0), sum = wave_scan(units_of_rows(rows) * items), base = 0;
+  uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+  for (uint32_t s0 = 64; s0 < a.n; s0 += 64)
+    total += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(units_of_rows(chunk(s0)) * items), 63);
+  const uint32_t per = units_per_range(total, (uint32_t)gridDim.x);
+  const uint32_t start = r * per, end = min(total, start + per);
+  if (start < end) {
+    uint32_t s0 = 0;
+    for (;;) {  // the chunk that holds the range's first unit
+      const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+      if (start < base + all) break;
+      base += all;
+      s0 += 64;
+      rows = chunk(s0);
+      sum = wave_scan(units_of_rows(rows) * items);
     }
-    out[d] = y / sum;
+    const int at0 = __builtin_ctzll(__ballot(start < base + sum));
+    const uint32_t before = base + (at0 ? (uint32_t)__builtin_amdgcn_readlane((int)sum, at0 - 1) : 0u);
+    const Partials pt(a, w.hd);
+    walk_units(
+        s0 + at0, start - before, start, end, items,
+        [&](uint32_t s) -> uint32_t {
+          const uint32_t n = s - s0 < 64 ? (uint32_t)__builtin_amdgcn_readlane((int)rows, (int)(s - s0))
+                                         : rows_of_len(w, a, a.lens[s]);
+          return n == kRefused ? 0 : n;
+        },
+        [&](uint32_t s, uint32_t n, uint32_t item, uint32_t u0, uint32_t u1, uint32_t at) {
+          const uint32_t units = units_of(n), first = at - u0;
+          const int h = (int)item / a.blocks, c0 = ((int)item - h * a.blocks) * a.cols;
+          const int qh = h * a.group + c0, ncols = min(a.cols, a.group - c0);
+          const bool whole = u0 == 0 && u1 == units;
+          Inner::segment(w, a, sh, s, h, qh, ncols, u0 * kUnitRows, min(n, u1 * kUnitRows), whole, pt,
+                         pt.at(r, partial_of(r, per, at)));
+          if (whole) return;
+          const uint32_t w0 = first / per, pieces = (first + units - 1) / per - w0 + 1;
+          auto which = [&](uint32_t i) { return partial_of(i, per, first); };
+          float* out = a.out + s * a.out_stride + (long)qh * w.hd;
+          unsigned* ticket = a.tickets + kMaxRanges + s * items + item;
+          const uint32_t groups = groups_of(pieces);
+          if (groups == 1) {
+            if (last_of(ticket, pieces, drawn)) join<Inner::kVec>(pt, w0, 1, pieces, which, ncols, out);
+            return;
+          }
+          const uint32_t g0 = w0 + (r - w0) / kGroup * kGroup, mine = min((uint32_t)kGroup, w0 + pieces - g0);
+          if (mine > 1) {  // (two items' groups may open at one range, but only one of more than a piece)
+            if (!last_of(a.tickets + g0, mine, drawn)) return;
+            join<Inner::kVec>(pt, g0, 1, mine, which, ncols, (float*)nullptr);
+          }
+          if (last_of(ticket, groups, drawn)) join<Inner::kVec>(pt, w0, kGroup, groups, which, ncols, out);
+        });
+  }
+  // Sequences without rows: zeros; refused ones: NaN.
+  for (uint32_t s = r; s < a.n; s += gridDim.x) {
+    const int len = a.lens[s];
+    const uint32_t n = rows_of_len(w, a, len);
+    if (n != 0 && n != kRefused) continue;
+    if (n == kRefused && threadIdx.x == 0)
+      paged_refuse(w, RV_PAGED_POSITION_OUT_OF_RANGE, s, (uint32_t)len, (uint32_t)min(table_rows(w.t), 0xFFFFFFFFl));
+    for (int d = threadIdx.x; d < w.n_kv * a.group * w.hd; d += 256) a.out[s * a.out_stride + d] = n ? NAN : 0.f;
   }
 }
 
@@ -580,12 +682,16 @@ bool tiled(int hd) { return hd % 8 == 0 && hd <= 256; }
 
 int cols_of(int hd, int group) { return tiled(hd) ? std::min(group, 16) : 1; }
 
-// Workgroups that deal the work of any lengths.
-unsigned ranges(size_t items) {
-  return (unsigned)std::min<size_t>(2048, std::max<size_t>(2 * kCUs, items));
+// Workgroups that deal the work of `units` units at most: two a CU, which is what
+// is resident, or one an item where there are more.
+uint32_t ranges(size_t items, size_t units) {
+  return (uint32_t)std::max<size_t>(1, std::min(units, std::min<size_t>(kMaxRanges, std::max<size_t>(2 * kCUs, items))));
 }
 
-size_t plan_bytes(size_t n) { return ((n + 1) * sizeof(long) + 255) / 256 * 256; }
+size_t items_per_seq(const rv_paged* pg, size_t n_q) {
+  const size_t group = n_q / pg->n_kv_heads, cols = cols_of((int)pg->head_dim, (int)group);
+  return pg->n_kv_heads * ((group + cols - 1) / cols);
+}
 
 template <typename T>
 void launch_attn(const PagedView& w, const AttnArgs& a, dim3 grid, hipStream_t s) {
@@ -610,13 +716,18 @@ void launch_attn(const PagedView& w, const AttnArgs& a, dim3 grid, hipStream_t s
 
 }  // namespace
 
-size_t paged_attn_ws(const rv_paged* pg, size_t n, size_t n_q) {
-  const size_t group = n_q / pg->n_kv_heads, cols = cols_of((int)pg->head_dim, (int)group);
-  const size_t items = n * pg->n_kv_heads * ((group + cols - 1) / cols);
-  return plan_bytes(n) + (size_t)ranges(items) * 2 * cols * (pg->head_dim + 2) * sizeof(float);
+PagedAttnPlan paged_attn_plan(const rv_paged* pg, const rv_page_table& t, size_t n, size_t n_q) {
+  PagedAttnPlan p;
+  const size_t items = n * items_per_seq(pg, n_q), rows = t.pages * pg->page_rows;
+  const size_t cols = cols_of((int)pg->head_dim, (int)(n_q / pg->n_kv_heads));
+  p.units = items * ((rows + kUnitRows - 1) / kUnitRows);  // (both below 2^42: no overflow that matters below)
+  p.ws_bytes = (size_t)ranges(items, SIZE_MAX) * 2 * cols * (pg->head_dim + 2) * sizeof(float);
+  p.ticket_bytes = (kMaxRanges + items) * sizeof(unsigned);
+  return p;
 }
 
-HipStatus launch_paged_attn(const rv_paged* pg, const PagedView& w, const PagedAttn& p, hipStream_t s) {
+HipStatus launch_paged_attn(const rv_paged* pg, const PagedView& w, const PagedAttn& p, const PagedAttnPlan& plan,
+                            hipStream_t s) {
   AttnArgs a{};
   a.q = p.q;
   a.q_stride = (long)p.q_stride;
@@ -629,9 +740,10 @@ HipStatus launch_paged_attn(const rv_paged* pg, const PagedView& w, const PagedA
   a.scale = p.scale;
   a.out = p.out;
   a.out_stride = (long)p.out_stride;
-  a.plan = (long*)pg->ws;
-  a.part = (float*)((char*)pg->ws + plan_bytes(p.n));
-  const dim3 grid(ranges(p.n * w.n_kv * a.blocks));
+  a.tickets = pg->tickets;
+  a.part = (float*)pg->ws;
+  a.part_bytes = (uint32_t)plan.ws_bytes;
+  const dim3 grid(ranges(p.n * w.n_kv * a.blocks, plan.units));
   HipStatus st;
   if (pg->elem == RV_ELEM_F32)
     launch_attn<float>(w, a, grid, s);
@@ -640,13 +752,7 @@ HipStatus launch_paged_attn(const rv_paged* pg, const PagedView& w, const PagedA
   else
     launch_attn<Q8>(w, a, grid, s);
   st.e = hipGetLastError();
-  if (st.e != hipSuccess) {
-    st.what = "paged attention launch";
-    return st;
-  }
-  hipLaunchKernelGGL(paged_join_kernel, dim3((unsigned)p.n, (unsigned)p.n_q), dim3(128), 0, s, w, a);
-  st.e = hipGetLastError();
-  if (st.e != hipSuccess) st.what = "paged join launch";
+  if (st.e != hipSuccess) st.what = "paged attention launch";
   return st;
 }
 

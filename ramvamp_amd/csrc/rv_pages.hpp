@@ -57,35 +57,52 @@ RV_HD long attended_rows(const Pages& t, int len, bool step) {
 // cut into ranges of `per` units, one a workgroup.
 constexpr int kUnitRows = 128;
 
-RV_HD long units_of(long rows) { return rows > 0 ? (rows + kUnitRows - 1) / kUnitRows : 0; }
+template <typename I>
+RV_HD I units_of(I rows) {
+  return rows > 0 ? (rows + (kUnitRows - 1)) / kUnitRows : 0;
+}
 
-RV_HD long units_per_range(long total, long ranges) {
-  const long per = (total + ranges - 1) / ranges;
+template <typename I>
+RV_HD I units_per_range(I total, I ranges) {
+  const I per = (total + ranges - 1) / ranges;
   return per > 1 ? per : 1;
 }
 
 // Which of its range's two partials a cut item's piece is kept in: the first when
 // it opens the range (the item may have begun before), else the second (it runs on
 // past the range's end).
-RV_HD int partial_of(long range, long per, long item_start) { return item_start > range * per ? 1 : 0; }
+template <typename I>
+RV_HD int partial_of(I range, I per, I item_start) {
+  return item_start > range * per ? 1 : 0;
+}
 
 // Walks the units [start, end), the first of which is unit `off` of sequence s:
-// visit(sequence, its rows, item, first unit, last unit + 1 of the item).
-template <typename Rows, typename Visit>
-RV_HD void walk_units(uint32_t s, long off, long start, long end, long items, Rows rows_of, Visit visit) {
-  for (long at = start; at < end;) {
-    const long rows = rows_of(s), units = units_of(rows);
+// visit(sequence, its rows, item, first unit, last unit + 1 of the item, the first
+// unit's place in the line).
+template <typename I, typename Rows, typename Visit>
+RV_HD void walk_units(uint32_t s, I off, I start, I end, I items, Rows rows_of, Visit visit) {
+  for (I at = start; at < end;) {
+    const I rows = rows_of(s), units = units_of(rows);
     if (off >= units * items) {
       off -= units * items;
       ++s;
       continue;
     }
-    const long item = off / units, u0 = off - item * units;
-    const long u1 = units < u0 + (end - at) ? units : u0 + (end - at);
+    const I item = off / units, u0 = off - item * units;
+    const I u1 = units < u0 + (end - at) ? units : u0 + (end - at);
     visit(s, rows, item, u0, u1, at);
     off += u1 - u0;
     at += u1 - u0;
   }
+}
+
+// The partials of an item cut into `pieces` are joined by whoever leaves the last
+// of them; past kFlat pieces first in groups of kGroup, whose partials the last of
+// a group replaces by one.
+constexpr int kFlat = 32, kGroup = 16;
+
+RV_HD uint32_t groups_of(uint32_t pieces) {
+  return pieces > (uint32_t)kFlat ? (pieces + kGroup - 1) / kGroup : 1;
 }
 
 }  // namespace rv
