@@ -39,7 +39,8 @@ struct Turns {
 };
 
 // Cosines and sines of a row's pairs, by the threads of a workgroup.
-__device__ __forceinline__ void fill_turns(const RopeArgs& rope, int pos, Turns& t) {
+template <int N>
+__device__ __forceinline__ void fill_turns(const RopeArgs<N>& rope, int pos, Turns& t) {
   for (int i = threadIdx.x; i < rope.pairs; i += blockDim.x) {
     double sd, cd;
     sincos((double)pos * rope.freq[i], &sd, &cd);
@@ -141,8 +142,8 @@ __device__ __forceinline__ void store_piece(const RopeShape& sh, const Turns& t,
 // grid (rows, parts of a row). A thread takes whole pairs, so x and out may be
 // the same rows; its next piece is in flight while the last is turned, and its
 // first while the angles are.
-template <bool INTER>
-__global__ __launch_bounds__(256) void rope_rows_kernel(RopeArgs rope, RopeShape sh, const float* x, long x_stride,
+template <int N, bool INTER>
+__global__ __launch_bounds__(256) void rope_rows_kernel(RopeArgs<N> rope, RopeShape sh, const float* x, long x_stride,
                                                         const int32_t* __restrict__ positions, float* out,
                                                         long out_stride) {
   __shared__ Turns turns;
@@ -227,8 +228,8 @@ __device__ __forceinline__ void store_row(const PagedView& w, bool is_v, int h, 
 // side by side, eight consecutive values each. Normed values pass through LDS,
 // where a thread finds the other halves of its pairs, and come out in the order
 // the pages hold them.
-template <typename T>
-__global__ __launch_bounds__(256) void paged_append_kernel(PagedView w, RopeArgs rope, AppendArgs a) {
+template <typename T, int N>
+__global__ __launch_bounds__(256) void paged_append_kernel(PagedView w, RopeArgs<N> rope, AppendArgs a) {
 #pragma clang fp contract(off)
   __shared__ __attribute__((aligned(16))) float row[256 * 8];
   __shared__ Turns turns;
@@ -371,53 +372,81 @@ constexpr size_t kMaxGridRows = (size_t)1 << 23;  // rows x 256 threads within 3
 
 }  // namespace
 
-HipStatus launch_rope_rows(const RopeArgs& rope, int hd, const float* x, size_t x_stride, size_t rows, size_t width,
+namespace {
+
+template <int N>
+RopeArgs<N> rope_args(const rv_rope* rope) {
+  RopeArgs<N> a;
+  if (!rope) return a;
+  a.pairs = (int)(rope->rotary_dim / 2);
+  a.interleaved = rope->layout == RV_ROPE_INTERLEAVED;
+  a.gain = rope->gain;
+  for (int i = 0; i < a.pairs; ++i) a.freq[i] = rope->freq[i];
+  return a;
+}
+
+// f(arguments) with the smaller of the two sizes that holds the pairs.
+template <typename F>
+HipStatus with_rope(const rv_rope* rope, F f) {
+  if (!rope || rope->rotary_dim <= 2 * kFewPairs) return f(rope_args<kFewPairs>(rope));
+  return f(rope_args<kMaxHalf>(rope));
+}
+
+}  // namespace
+
+HipStatus launch_rope_rows(const rv_rope& rope, const float* x, size_t x_stride, size_t rows, size_t width,
                            const int32_t* positions, float* out, size_t out_stride, hipStream_t s) {
-  HipStatus st;
   RopeShape sh;
-  sh.hd = hd;
-  sh.pairs = rope.pairs;
-  sh.pair_groups = (rope.pairs + 3) / 4;
+  sh.hd = (int)rope.head_dim;
+  sh.pairs = (int)rope.rotary_dim / 2;
+  sh.pair_groups = (sh.pairs + 3) / 4;
   // What passes through is copied, unless it is there already.
-  sh.groups = sh.pair_groups + (x == out ? 0 : (hd - 2 * rope.pairs + 7) / 8);
-  sh.pieces = (uint32_t)(width / hd * sh.groups);
+  sh.groups = sh.pair_groups + (x == out ? 0 : (sh.hd - 2 * sh.pairs + 7) / 8);
+  sh.pieces = (uint32_t)(width / sh.hd * sh.groups);
   const unsigned block = std::min(256u, (sh.pieces + 63) / 64 * 64);
   unsigned parts = (sh.pieces + block - 1) / block;
   // One piece a thread while the launch is small; a whole row per workgroup, its
   // angles computed once, when rows alone fill the CUs.
   if (rows * parts > 8 * (size_t)kCUs) parts = (unsigned)std::max<size_t>(1, std::min<size_t>(parts, 8 * kCUs / rows));
-  for (size_t r0 = 0; r0 < rows; r0 += kMaxGridRows) {
-    const dim3 grid((unsigned)std::min(rows - r0, kMaxGridRows), parts);
-    if (rope.interleaved)
-      hipLaunchKernelGGL(rope_rows_kernel<true>, grid, dim3(block), 0, s, rope, sh, x + r0 * x_stride, (long)x_stride,
-                         positions + r0, out + r0 * out_stride, (long)out_stride);
-    else
-      hipLaunchKernelGGL(rope_rows_kernel<false>, grid, dim3(block), 0, s, rope, sh, x + r0 * x_stride,
-                         (long)x_stride, positions + r0, out + r0 * out_stride, (long)out_stride);
-    if ((st = launched("rope launch")).e != hipSuccess) return st;
-  }
-  return st;
+  return with_rope(&rope, [&](const auto& ra) {
+    constexpr int N = sizeof(ra.freq) / sizeof(double);
+    HipStatus st;
+    for (size_t r0 = 0; r0 < rows; r0 += kMaxGridRows) {
+      const dim3 grid((unsigned)std::min(rows - r0, kMaxGridRows), parts);
+      if (ra.interleaved)
+        hipLaunchKernelGGL((rope_rows_kernel<N, true>), grid, dim3(block), 0, s, ra, sh, x + r0 * x_stride,
+                           (long)x_stride, positions + r0, out + r0 * out_stride, (long)out_stride);
+      else
+        hipLaunchKernelGGL((rope_rows_kernel<N, false>), grid, dim3(block), 0, s, ra, sh, x + r0 * x_stride,
+                           (long)x_stride, positions + r0, out + r0 * out_stride, (long)out_stride);
+      if ((st = launched("rope launch")).e != hipSuccess) return st;
+    }
+    return st;
+  });
 }
 
-HipStatus launch_paged_append(const rv_paged* pg, const PagedView& w, const RopeArgs& rope, const PagedRows& r,
+HipStatus launch_paged_append(const rv_paged* pg, const PagedView& w, const rv_rope* rope, const PagedRows& r,
                               hipStream_t s) {
-  HipStatus st;
   AppendArgs a{r.q,        r.k,     r.v,    r.q_w,       r.k_w,    (long)r.q_stride, (long)r.k_stride, (long)r.v_stride,
                r.q_out,    r.n_q,   r.positions, r.seqs, r.eps,    0, 0};
   while ((8 << a.lanes_log) < w.hd) ++a.lanes_log;
   const unsigned slots = (unsigned)(r.n_q + 2 * w.n_kv) << a.lanes_log;
   const unsigned block = std::min(256u, (slots + 63) / 64 * 64);
-  for (a.r0 = 0; a.r0 < r.rows; a.r0 += kMaxGridRows) {
-    const dim3 grid((unsigned)std::min(r.rows - a.r0, kMaxGridRows), (slots + block - 1) / block);
-    if (pg->elem == RV_ELEM_F32)
-      hipLaunchKernelGGL(paged_append_kernel<float>, grid, dim3(block), 0, s, w, rope, a);
-    else if (pg->elem == RV_ELEM_F16)
-      hipLaunchKernelGGL(paged_append_kernel<_Float16>, grid, dim3(block), 0, s, w, rope, a);
-    else
-      hipLaunchKernelGGL(paged_append_kernel<Q8>, grid, dim3(block), 0, s, w, rope, a);
-    if ((st = launched("paged append launch")).e != hipSuccess) return st;
-  }
-  return st;
+  return with_rope(rope, [&](const auto& ra) {
+    constexpr int N = sizeof(ra.freq) / sizeof(double);
+    HipStatus st;
+    for (a.r0 = 0; a.r0 < r.rows; a.r0 += kMaxGridRows) {
+      const dim3 grid((unsigned)std::min(r.rows - a.r0, kMaxGridRows), (slots + block - 1) / block);
+      if (pg->elem == RV_ELEM_F32)
+        hipLaunchKernelGGL((paged_append_kernel<float, N>), grid, dim3(block), 0, s, w, ra, a);
+      else if (pg->elem == RV_ELEM_F16)
+        hipLaunchKernelGGL((paged_append_kernel<_Float16, N>), grid, dim3(block), 0, s, w, ra, a);
+      else
+        hipLaunchKernelGGL((paged_append_kernel<Q8, N>), grid, dim3(block), 0, s, w, ra, a);
+      if ((st = launched("paged append launch")).e != hipSuccess) return st;
+    }
+    return st;
+  });
 }
 
 HipStatus launch_paged_read(const rv_paged* pg, const PagedView& w, size_t rows, const int32_t* positions,

@@ -29,6 +29,7 @@ struct rv_paged {
   size_t n_layers = 0, n_kv_heads = 0, head_dim = 0, n_pages = 0, page_rows = 0, kv_dim = 0;
   int elem = RV_ELEM_F16;
   int device = 0;
+  bool xcd_ok = false;  // xcd_dealing_ok of the device
   void* k = nullptr;
   void* v = nullptr;
   hipStream_t stream = nullptr;
@@ -66,13 +67,16 @@ struct PagedView {
 };
 PagedView paged_view(const rv_paged* pg, size_t layer, const rv_page_table& t);
 
-// The rotation as the kernels take it: frequencies by value.
+// The rotation as the kernels take it: frequencies by value, of up to N pairs (a
+// launch's arguments cost the host by their size: 64 pairs in place of 256 ...).
+template <int N>
 struct RopeArgs {
   int pairs = 0;  // 0: none
   int interleaved = 0;
   double gain = 1.0;
-  double freq[kMaxHalf];
+  double freq[N];
 };
+constexpr int kFewPairs = 64;
 
 // Records a refusal: the first since the last read stays.
 __device__ __forceinline__ void paged_refuse(const PagedView& w, uint32_t code, uint32_t row, uint32_t got,
@@ -103,7 +107,7 @@ __device__ __forceinline__ bool paged_place(const PagedView& w, uint32_t r, int 
   return false;
 }
 
-HipStatus launch_rope_rows(const RopeArgs& rope, int hd, const float* x, size_t x_stride, size_t rows, size_t width,
+HipStatus launch_rope_rows(const rv_rope& rope, const float* x, size_t x_stride, size_t rows, size_t width,
                            const int32_t* positions, float* out, size_t out_stride, hipStream_t s);
 // k and v rows into the pages and, with n_q heads a row, q rows normed and
 // rotated into q_out (contiguous).
@@ -123,7 +127,7 @@ struct PagedRows {
   const float* k_w;
   float eps;
 };
-HipStatus launch_paged_append(const rv_paged* pg, const PagedView& w, const RopeArgs& rope, const PagedRows& r,
+HipStatus launch_paged_append(const rv_paged* pg, const PagedView& w, const rv_rope* rope, const PagedRows& r,
                               hipStream_t s);
 HipStatus launch_paged_read(const rv_paged* pg, const PagedView& w, size_t rows, const int32_t* positions,
                             const int32_t* seqs, void* k, void* v, hipStream_t s);

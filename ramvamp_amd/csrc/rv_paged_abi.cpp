@@ -176,16 +176,6 @@ int32_t check_rope(const rv_paged* pg, const rv_rope* rope, rv_error* err) {
   return RV_OK;
 }
 
-rv::RopeArgs rope_args(const rv_rope* rope) {
-  rv::RopeArgs a;
-  if (!rope) return a;
-  a.pairs = (int)(rope->rotary_dim / 2);
-  a.interleaved = rope->layout == RV_ROPE_INTERLEAVED;
-  a.gain = rope->gain;
-  for (int i = 0; i < a.pairs; ++i) a.freq[i] = rope->freq[i];
-  return a;
-}
-
 int32_t finish(hipStream_t s, uint32_t flags, const rv::HipStatus& st, rv_error* err) {
   if (st.e != hipSuccess) return hip_fail(err, st);
   if (flags & RV_SYNC) {
@@ -285,7 +275,7 @@ int32_t rv_rope_rows(const rv_rope* rope, const float* x, size_t x_stride, size_
   if (rows == 1) x_stride = out_stride = width;
   if (!(x == out && x_stride == out_stride) && overlap(x, x_stride, out, out_stride, rows, width))
     return unsupported(err, 0, "out overlaps x");
-  const rv::HipStatus st = rv::launch_rope_rows(rope_args(rope), (int)hd, x, x_stride, rows, width, positions, out,
+  const rv::HipStatus st = rv::launch_rope_rows(*rope, x, x_stride, rows, width, positions, out,
                                                 out_stride, (hipStream_t)stream);
   return finish((hipStream_t)stream, flags, st, err);
 }
@@ -326,6 +316,7 @@ int32_t rv_paged_new(size_t n_layers, size_t n_kv_heads, size_t head_dim, size_t
   if (e == hipSuccess) e = hipMalloc((void**)&pg->status, 256);
   if (e == hipSuccess) e = hipMemset(pg->status, 0, 256);
   if (e == hipSuccess) e = hipDeviceSynchronize();
+  if (e == hipSuccess) pg->xcd_ok = rv::xcd_dealing_ok(device);
   if (e != hipSuccess) {
     rv_paged_free(pg);
     return hip_fail(err, e, "hipMalloc pages");
@@ -415,7 +406,7 @@ int32_t rv_paged_append_rows(rv_paged* pg, size_t layer, const rv_rope* rope, co
   r.k_w = k_norm_w;
   r.eps = eps;
   return finish(pg->stream, flags,
-                rv::launch_paged_append(pg, rv::paged_view(pg, layer, *table), rope_args(rope), r, pg->stream), err);
+                rv::launch_paged_append(pg, rv::paged_view(pg, layer, *table), rope, r, pg->stream), err);
 }
 
 int32_t rv_paged_read_rows(rv_paged* pg, size_t layer, size_t rows, const int32_t* positions, const int32_t* seqs,
@@ -503,7 +494,7 @@ int32_t rv_paged_decode_step(rv_paged* pg, size_t layer, const rv_rope* rope, co
   r.k_w = k_norm_w;
   r.eps = eps;
   const rv::PagedView w = rv::paged_view(pg, layer, *table);
-  st = rv::launch_paged_append(pg, w, rope_args(rope), r, pg->stream);
+  st = rv::launch_paged_append(pg, w, rope, r, pg->stream);
   if (st.e == hipSuccess) {
     const rv::PagedAttn a{pg->qbuf, q_dim, n_seqs, (int)n_q, positions, true, scale, out, out_stride};
     st = rv::launch_paged_attn(pg, w, a, plan, pg->stream);

@@ -11,9 +11,12 @@
 // lengths. An item inside one range is finished there; one that is cut leaves a
 // partial (weighted sum of v, maximum, sum) per range, at most two a workgroup
 // (its first item and its last). The workgroup that leaves an item's last partial
-// joins them all, in order, so that results do not depend on which that is.
-// Partials are stored and loaded at device scope (the XCDs' L2s do not see each
-// other's lines), and counted by tickets that are zero between calls.
+// joins them all, in order, so that results do not depend on which that is. Where
+// they are all of a group (up to 16 workgroups of one XCD) they pass through its L2,
+// where they are many first those of each group do (loads at device scope bring a CU
+// some 12 bytes a cycle, loads from its L2 several times that), and else, and across
+// groups, they are stored and loaded at device scope, since the XCDs' L2s do not see
+// each other's lines. Partials are counted by tickets that are zero between calls.
 #include "rv_paged.hpp"
 
 #include <algorithm>
@@ -33,12 +36,15 @@ struct AttnArgs {
   float scale;
   float* out;
   long out_stride;
-  unsigned* tickets;  // one a range (its group's), then one an item
-  float* part;        // [range][2][cols * (hd + 2)]: rows, then (maximum, sum) of each column
+  int slots;          // log2 of the XCDs that workgroups are known to be dealt to in turn
+  int most, few;      // log2 of the ranges there may be (cut_units)
+  unsigned* tickets;  // [group][2], then one an item
+  // [range][2], then [group][2]: rows [cols][hd], then (maximum, sum) of each column.
+  float* part;
   uint32_t part_bytes;
 };
 
-constexpr uint32_t kMaxRanges = 2048;
+constexpr uint32_t kMaxRanges = 2 * kCUs, kGroups = kMaxRanges / kGroup;
 constexpr uint32_t kRefused = 0xFFFFFFFFu;
 
 // Rows a sequence of this length attends, kRefused where the table has not so many.
@@ -63,84 +69,127 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 
 // ---- partials ---------------------------------------------------------------------
 
-constexpr int kDeviceScope = 16;  // the sc1 bit of a buffer instruction's cache policy
+// Cache policies of the buffer instructions: the sc1 bit, device scope; the sc0 bit
+// of a load, past the CU's L1 to its XCD's L2.
+constexpr int kDeviceScope = 16, kXcdScope = 1;
 
 struct Partials {
   __amdgpu_buffer_rsrc_t rs;
   int cols, hd;
   __device__ __forceinline__ Partials(const AttnArgs& a, int hd_)
       : rs(__builtin_amdgcn_make_buffer_rsrc(a.part, (short)0, (int)a.part_bytes, 0x00020000)), cols(a.cols), hd(hd_) {}
-  // Byte offset of a partial; of column c's (maximum, sum) in it.
-  __device__ __forceinline__ uint32_t at(uint32_t range, int which) const {
-    return (range * 2 + which) * (uint32_t)(cols * (hd + 2)) * 4u;
-  }
+  // Byte offset of a partial (2 * range + which; the slots' behind them); of column
+  // c's (maximum, sum) in it.
+  __device__ __forceinline__ uint32_t at(uint32_t i) const { return i * (uint32_t)(cols * (hd + 2)) * 4u; }
   __device__ __forceinline__ uint32_t stat(int c) const { return (uint32_t)(cols * hd + 2 * c) * 4u; }
-  __device__ __forceinline__ void put_stat(uint32_t p, int c, float m, float l) const {
-    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, m), rs, p + stat(c), 0, kDeviceScope);
-    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, l), rs, p + stat(c) + 4, 0, kDeviceScope);
+  // Stores to be seen on this XCD, or on all.
+  __device__ __forceinline__ void put(uint32_t o, float x, bool here) const {
+    if (here)
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, x), rs, o, 0, 0);
+    else
+      __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, x), rs, o, 0, kDeviceScope);
   }
+  __device__ __forceinline__ void put(uint32_t o, f32x4 x, bool here) const {
+    if (here)
+      __builtin_amdgcn_raw_buffer_store_b128(x, rs, o, 0, 0);
+    else
+      __builtin_amdgcn_raw_buffer_store_b128(x, rs, o, 0, kDeviceScope);
+  }
+  __device__ __forceinline__ void put_stat(uint32_t p, int c, float m, float l, bool here) const {
+    put(p + stat(c), m, here);
+    put(p + stat(c) + 4, l, here);
+  }
+  template <int POLICY>
   __device__ __forceinline__ float word(uint32_t o) const {
-    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, o, 0, kDeviceScope));
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, o, 0, POLICY));
   }
 };
 
-// Joins `count` partials, of ranges first, first + step, .. (which(i): the one of
-// range i's two), in order: into `out` (ncols rows of hd), or into the first's place.
-// A thread has one column's VEC values, and kBatch partials in flight.
-template <int VEC, typename Which>
-__device__ __forceinline__ void join(const Partials& p, uint32_t first, uint32_t step, uint32_t count, Which which,
-                                     int ncols, float* out) {
-  constexpr int kBatch = 16;
+constexpr uint32_t kMostPieces = 64;  // that are joined at once
+
+// Joins `count` partials (at most kMostPieces), in order, partial `first` and then
+// rest, rest + 2, ..: into `out` (ncols rows of hd), or into partial `to` for all
+// XCDs. What a load costs the CU's address unit is by the instruction: LANES lanes
+// have a column, VEC of its values each, load its partials' (maximum, sum) one a lane,
+// and pass their factors on by lane permutes; 16 partials' values are in flight.
+template <int VEC, int LANES, int POLICY>
+__device__ __forceinline__ void join(const Partials& p, uint32_t first, uint32_t rest, uint32_t count, int ncols,
+                                     float* out, uint32_t to) {
   typedef float Row __attribute__((ext_vector_type(VEC)));
-  const int pieces = p.hd / VEC;
-  for (int j = threadIdx.x; j < ncols * pieces; j += 256) {
-    const int c = j / pieces, d = (j - c * pieces) * VEC;
-    float m = -INFINITY, l = 0.f;
-    Row o = (Row)0.f;
-    for (uint32_t b0 = 0; b0 < count; b0 += kBatch) {
-      Row x[kBatch];
-      float mx[kBatch], lx[kBatch];
+  constexpr uint32_t kBatch = 16;
+  constexpr int kStats = (int)kMostPieces / LANES, kColumns = 256 / LANES;  // a lane's; of the workgroup at once
+  const int lane = threadIdx.x & 63, mine = lane & (LANES - 1);
+  const uint32_t one = p.at(1);
+  auto place = [&](uint32_t i) { return (i ? rest + 2 * (i - 1) : first) * one; };
+  for (int c0 = 0; c0 < ncols; c0 += kColumns) {
+    const int cc = c0 + (int)threadIdx.x / LANES, c = min(cc, ncols - 1);
+    float m[kStats], l[kStats], top = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const uint32_t r = first + step * min(b0 + i, count - 1), at = p.at(r, which(r));
-        if constexpr (VEC == 4)
-          x[i] = __builtin_bit_cast(Row, __builtin_amdgcn_raw_buffer_load_b128(
-                                             p.rs, at + (uint32_t)(c * p.hd + d) * 4u, 0, kDeviceScope));
-        else
-          x[i] = p.word(at + (uint32_t)(c * p.hd + d) * 4u);
-        mx[i] = p.word(at + p.stat(c));
-        lx[i] = p.word(at + p.stat(c) + 4);
-      }
-      float top = m;
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) top = fmaxf(top, mx[i]);  // (repeats of the last change nothing)
-      // Where every score so far is minus infinity or NaN nothing is scaled, and the
-      // sums carry what there is.
-      const float f = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
-      o *= f;
-      l *= f;
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i)
-        if (b0 + i < count) {
-          const float g = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mx[i] - top);
-          o += x[i] * g;
-          l += lx[i] * g;
-        }
-      m = top;
+    for (int i = 0; i < kStats; ++i) {
+      const uint32_t k = mine + LANES * i, at = place(min(k, count - 1)) + p.stat(c);
+      m[i] = p.word<POLICY>(at);
+      l[i] = p.word<POLICY>(at + 4);
     }
-    if (out) {
-      const Row y = o / l;
+    for (int d = mine * VEC; d < (p.hd + LANES * VEC - 1) / (LANES * VEC) * (LANES * VEC); d += LANES * VEC) {
+      const uint32_t row = (uint32_t)(c * p.hd + min(d, p.hd - VEC)) * 4u;
+      Row o = (Row)0.f;
+      for (uint32_t b0 = 0; b0 < count; b0 += kBatch) {
+        Row x[kBatch];
+        uint32_t at = place(b0) + row;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) out[(long)c * p.hd + d + e] = y[e];
-    } else {
-      const uint32_t at = p.at(first, which(first));
-      if constexpr (VEC == 4) {
-        __builtin_amdgcn_raw_buffer_store_b128(o, p.rs, at + (uint32_t)(c * p.hd + d) * 4u, 0, kDeviceScope);
-      } else {
-        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, (float)o[0]), p.rs,
-                                              at + (uint32_t)(c * p.hd + d) * 4u, 0, kDeviceScope);
+        for (uint32_t i = 0; i < kBatch; ++i) {
+          if (i % 4 == 0 && b0 + i >= count) break;  // (past the last, up to three: it again, not counted)
+          if constexpr (VEC == 4)
+            x[i] = __builtin_bit_cast(Row, __builtin_amdgcn_raw_buffer_load_b128(p.rs, at, 0, POLICY));
+          else
+            x[i] = p.word<POLICY>(at);
+          if (b0 + i + 1 < count) at = b0 + i ? at + 2 * one : rest * one + row;
+        }
+        if (b0 == 0 && d == mine * VEC) {
+#pragma unroll
+          for (int i = 0; i < kStats; ++i) {
+            const bool in = mine + LANES * i < (int)count;
+            m[i] = in ? m[i] : -INFINITY;
+            l[i] = in ? l[i] : 0.f;
+            top = fmaxf(top, m[i]);
+          }
+          top = group_max<16>(top);
+          if (LANES >= 32) top = swap_max<16>(top);
+          if (LANES >= 64) top = swap_max<32>(top);
+          // (Where every score is minus infinity or NaN nothing is scaled, and the sums
+          // carry what there is.)
+#pragma unroll
+          for (int i = 0; i < kStats; ++i) {
+            m[i] = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[i] - top);
+            sum += m[i] * l[i];
+          }
+          sum = group_sum<16>(sum);
+          if (LANES >= 32) sum = swap_sum<16>(sum);
+          if (LANES >= 64) sum = swap_sum<32>(sum);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kBatch; ++i) {
+          if (i % 4 == 0 && b0 + i >= count) break;
+          const uint32_t k = b0 + i;
+          float f = m[0];
+#pragma unroll
+          for (int s = 1; s < kStats; ++s) f = k / LANES == (uint32_t)s ? m[s] : f;
+          f = __shfl(f, (lane & ~(LANES - 1)) + (int)(k & (LANES - 1)), 64);
+          o += x[i] * (k < count ? f : 0.f);
+        }
       }
-      if (d == 0) p.put_stat(at, c, m, l);
+      if (cc >= ncols || d >= p.hd) continue;
+      if (out) {
+        const float inv = 1.f / sum;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) out[(long)c * p.hd + d + e] = o[e] * inv;
+      } else {
+        if constexpr (VEC == 4)
+          p.put(p.at(to) + row, o, false);
+        else
+          p.put(p.at(to) + row, o[0], false);
+        if (d == 0) p.put_stat(p.at(to), c, top, sum, false);
+      }
     }
   }
 }
@@ -178,16 +227,17 @@ __device__ __forceinline__ float paged_value(const PagedView& w, bool is_v, size
 template <typename T>
 struct Plain {
   static constexpr int kPer = kMaxHalf * 2 / 64;
-  static constexpr int kVec = 1;
+  static constexpr int kVec = 1, kLanes = 64;
   struct Shared {
     float o[4][kMaxHalf * 2];
     float m[4], l[4];
   };
   // Rows [p0, p1) of sequence s, kv head h, query head qh (of the whole): the
-  // output where `whole`, else the partial at `part`.
+  // output where `whole`, else the partial that where() names.
+  template <typename Where>
   static __device__ __forceinline__ void segment(const PagedView& w, const AttnArgs& a, Shared& sh, uint32_t s, int h,
                                                  int qh, int, uint32_t p0, uint32_t p1, bool whole,
-                                                 const Partials& pt, uint32_t part) {
+                                                 const Partials& pt, Where where) {
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const float* q = a.q + s * a.q_stride + (long)qh * w.hd;
     const float scale = a.scale * kLog2e;
@@ -230,6 +280,8 @@ struct Plain {
 #pragma unroll
     for (int j = 0; j < kPer; ++j) sh.o[wv][lane + 64 * j] = o[j];
     __syncthreads();
+    bool here = false;
+    const uint32_t part = whole ? 0 : where(here);
     const float top = fmaxf(fmaxf(sh.m[0], sh.m[1]), fmaxf(sh.m[2], sh.m[3]));
     float f[4], sum = 0.f;
     for (int i = 0; i < 4; ++i) {
@@ -243,9 +295,9 @@ struct Plain {
       if (whole)
         a.out[s * a.out_stride + (long)qh * w.hd + d] = y / sum;
       else
-        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, y), pt.rs, part + 4u * d, 0, kDeviceScope);
+        pt.put(part + 4u * d, y, here);
     }
-    if (!whole && threadIdx.x == 0) pt.put_stat(part, 0, top, sum);
+    if (!whole && threadIdx.x == 0) pt.put_stat(part, 0, top, sum, here);
   }
 };
 
@@ -268,16 +320,18 @@ struct Plain {
 // some 8000 cycles. So the loads are what is arranged: the next tile's K is asked
 // for as soon as this one's scores are done, its V after this one's product, each
 // into the registers just freed, and page ids a tile ahead of that.
-template <typename T, int HDP, bool FULL>
+template <typename T, int HDP, bool FULL, int D>
 struct Tiled {
   static constexpr bool kF32 = std::is_same<T, float>::value, kQ8 = std::is_same<T, Q8>::value;
   static constexpr int kRows = kF32 ? 16 : 32, kSub = kRows / 16;
+  static constexpr int kStep = 4 * kRows;  // from one of a wave's tiles to its next
   static constexpr int VD = kF32 || HDP == 64 ? 4 : 8;  // values of a row of V a lane loads together
   static constexpr int NH = HDP / (16 * VD);
   static constexpr int NK = kF32 ? HDP / 16 : kQ8 ? HDP / 64 : HDP / 32;  // 16-byte loads of a row of K a lane
   static constexpr int NQ = HDP / 32;
   static constexpr int kBytes = kF32 ? 4 : kQ8 ? 1 : 2;
-  static constexpr int kVec = 4;
+  static constexpr int kVec = 4, kLanes = HDP / 4;
+  static __device__ __forceinline__ int width(const PagedView& w) { return FULL ? HDP : w.hd; }
   typedef std::conditional_t<kF32, f32x4, u32x4> KReg;
   typedef std::conditional_t<kF32, f32x4,
                              std::conditional_t<kQ8, std::conditional_t<VD == 8, u32x2, uint32_t>,
@@ -299,6 +353,17 @@ struct Tiled {
     return kF32 ? 16 * i + 4 * g : kQ8 ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) : 32 * i + 8 * g;
   }
 
+  // Loads past the caches (every row is read once): 64 sequences of up to 16000 f16
+  // rows 229 -> 203 us. Not of rows below a line of 128 bytes, which would be brought
+  // twice: 32 of up to 8000 Q8_0 rows of 64 23.0 us so, 25.2 past the caches.
+  template <typename V>
+  static __device__ __forceinline__ V stream(const char* p) {
+    if constexpr (HDP * kBytes >= 128)
+      return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+    else
+      return *reinterpret_cast<const V*>(p);
+  }
+
   // Values past a head's width are loaded from its start and then cleared, rows
   // past the last one are rows of the last page, cleared before they count: no
   // lane goes another way than the others while the operands are in registers.
@@ -315,17 +380,18 @@ struct Tiled {
   }
 
   static __device__ __forceinline__ void load_k(const PagedView& w, const size_t (&at)[kSub], int g, Tile& t) {
+    const int hd = width(w);
 #pragma unroll
     for (int j = 0; j < kSub; ++j) {
-      const char* row = w.k + at[j] * w.hd * kBytes;
+      const char* row = w.k + at[j] * hd * kBytes;
 #pragma unroll
       for (int i = 0; i < NK; ++i) {
         const int d = kF32 ? 16 * i + 4 * g : kQ8 ? 64 * i + 16 * g : 32 * i + 8 * g;
-        const bool in = FULL || d < w.hd;
+        const bool in = FULL || d < hd;
         const int dd = in ? d : 0;
-        t.k[j][i] = *reinterpret_cast<const KReg*>(row + dd * kBytes);
+        t.k[j][i] = stream<KReg>(row + dd * kBytes);
         if constexpr (kQ8)  // (the codes of a scale of zero stand for nothing)
-          t.ks[j][i] = w.ks[at[j] * (w.hd / 32) + dd / 32] & (in ? 0xFFFFu : 0u);
+          t.ks[j][i] = w.ks[at[j] * (hd / 32) + dd / 32] & (in ? 0xFFFFu : 0u);
         else if (!FULL)
           t.k[j][i] = keep(t.k[j][i], in);
       }
@@ -335,22 +401,23 @@ struct Tiled {
   // hp: page * kv heads + head of the rows.
   static __device__ __forceinline__ void load_v(const PagedView& w, const size_t (&hp)[kSub],
                                                 const uint32_t (&row)[kSub], int n, Tile& t) {
+    const int hd = width(w);
 #pragma unroll
     for (int j = 0; j < kSub; ++j) {
-      const char* p = w.v + ((hp[j] << w.t.shift) + row[j]) * w.hd * kBytes;
+      const char* p = w.v + ((hp[j] << w.t.shift) + row[j]) * hd * kBytes;
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
         const int d = 16 * VD * h + VD * n;
-        const bool in = FULL || d < w.hd;
+        const bool in = FULL || d < hd;
         const int dd = in ? d : 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          t.v[4 * j + i][h] = *reinterpret_cast<const VReg*>(p + ((size_t)i * w.hd + dd) * kBytes);
+          t.v[4 * j + i][h] = stream<VReg>(p + ((size_t)i * hd + dd) * kBytes);
           if constexpr (!FULL && !kQ8) t.v[4 * j + i][h] = keep(t.v[4 * j + i][h], in);
         }
         if constexpr (kQ8)
           t.vs[j][h] = keep(*reinterpret_cast<const f16x4*>(
-                                w.vs + ((hp[j] * (w.hd / 32) + dd / 32) << w.t.shift) + row[j]),
+                                w.vs + ((hp[j] * (hd / 32) + dd / 32) << w.t.shift) + row[j]),
                             in);
       }
     }
@@ -366,9 +433,10 @@ struct Tiled {
     return y;
   }
 
+  template <typename Where>
   static __device__ __forceinline__ void segment(const PagedView& w, const AttnArgs& a, Shared& sh, uint32_t s, int h,
                                                  int qh, int ncols, uint32_t p0, uint32_t p1, bool whole,
-                                                 const Partials& pt, uint32_t part) {
+                                                 const Partials& pt, Where where) {
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const uint32_t mask = (1u << w.t.shift) - 1;
@@ -393,7 +461,7 @@ struct Tiled {
     };
     uint32_t b = p0 + wv * kRows;
     const bool any = b < p1;
-    Tile t;
+    Tile t[D];
     uint32_t id[kSub];
     f32x4 acc[NH * VD];
 #pragma unroll
@@ -409,10 +477,15 @@ struct Tiled {
         const bool in = n < ncols && (FULL || d < w.hd);
         x[i] = keep<f32x4>(*reinterpret_cast<const f32x4u*>(q + (FULL || d < w.hd ? d : 0)), in);
       }
-      locate(b, id);
-      load_k(w, k_at, g, t);
-      load_v(w, v_hp, v_row, n, t);
-      fetch(b + 4 * kRows, id);
+#pragma unroll
+      for (int i = 0; i < D; ++i) {
+        if (i == 0 || b + i * kStep < p1) {
+          locate(b + i * kStep, id);
+          load_k(w, k_at, g, t[i]);
+          load_v(w, v_hp, v_row, n, t[i]);
+        }
+        fetch(b + (i + 1) * kStep, id);
+      }
       float mul = a.scale * kLog2e;
       f16x8 q_hi[NQ], q_lo[NQ];
       if constexpr (!kF32) {
@@ -434,37 +507,45 @@ struct Tiled {
             q_lo[i][e] = (_Float16)(y - (float)q_hi[i][e]);
           }
       }
-      for (;;) {
-        f32x4 sc[kSub];
+      // One tile: its scores, then the K of the one D tiles on in its place, its part of
+      // the output, and the V of that; whether there is another tile.
+      auto step = [&](Tile& t, bool first) {
+        // (Every chain of dependent matrix instructions is as short as it can be: hi and
+        // lo apart, the two 16 rows in turn.)
+        f32x4 sc[kSub], sl[kSub];
 #pragma unroll
-        for (int j = 0; j < kSub; ++j) {
-          f32x4 c{};
-          if constexpr (kF32) {
+        for (int j = 0; j < kSub; ++j) sc[j] = sl[j] = f32x4{};
+        if constexpr (kF32) {
 #pragma unroll
-            for (int i = 0; i < NK; ++i)
+          for (int i = 0; i < NK; ++i)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(t.k[j][i][e], x[i][e], c, 0, 0, 0);
-          } else {
+            for (int e = 0; e < 4; ++e) {
+              f32x4& c = i & 1 ? sl[0] : sc[0];
+              c = __builtin_amdgcn_mfma_f32_16x16x4f32(t.k[0][i][e], x[i][e], c, 0, 0, 0);
+            }
+        } else {
 #pragma unroll
-            for (int i = 0; i < NQ; ++i) {
+          for (int i = 0; i < NQ; ++i)
+#pragma unroll
+            for (int j = 0; j < kSub; ++j) {
               f16x8 k;
               if constexpr (kQ8)
                 k = widen8(t.k[j][i >> 1][2 * (i & 1)], t.k[j][i >> 1][2 * (i & 1) + 1],
                            __builtin_bit_cast(_Float16, t.ks[j][i >> 1]));
               else
                 k = __builtin_bit_cast(f16x8, t.k[j][i]);
-              c = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q_lo[i], c, 0, 0, 0);
-              c = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q_hi[i], c, 0, 0, 0);
+              sl[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q_lo[i], sl[j], 0, 0, 0);
+              sc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q_hi[i], sc[j], 0, 0, 0);
             }
-          }
-          sc[j] = c;
         }
-        const uint32_t nb = b + 4 * kRows;
+#pragma unroll
+        for (int j = 0; j < kSub; ++j) sc[j] += sl[j];
+        const uint32_t nb = b + D * kStep;
         const bool more = nb < p1, tail = b + kRows > p1;
         if (more) {
           locate(nb, id);
           load_k(w, k_at, g, t);
-          fetch(nb + 4 * kRows, id);
+          fetch(nb + kStep, id);
         }
         float y[4 * kSub], top = -INFINITY;
 #pragma unroll
@@ -478,6 +559,7 @@ struct Tiled {
           const float c = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
           l *= c;
           m = top;
+          if (!first)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float f = __shfl(c, 4 * g + r, 64);
@@ -550,9 +632,14 @@ struct Tiled {
             }
           }
         }
-        if (!more) break;
-        load_v(w, v_hp, v_row, n, t);
-        b = nb;
+        if (more) load_v(w, v_hp, v_row, n, t);
+        b += kStep;
+        return b < p1;
+      };
+      for (bool on = true, first = true; on; first = false) {
+#pragma unroll
+        for (int i = 0; i < D; ++i)
+          if (on) on = step(t[i], first && i == 0);
       }
       l = swap_sum<32>(swap_sum<16>(l));
     }
@@ -560,16 +647,8 @@ struct Tiled {
       l = NAN;
       if (no_page >= w.t.n_pages) paged_refuse(w, RV_PAGED_PAGE_OUT_OF_RANGE, s, no_page, w.t.n_pages);
     }
-    __syncthreads();
+    __syncthreads();  // (the last segment's reads)
     if (lane < 16) sh.m[wv][n] = m, sh.l[wv][n] = l;
-    __syncthreads();
-    float f[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int c = 4 * g + r;
-      const float top = fmaxf(fmaxf(sh.m[0][c], sh.m[1][c]), fmaxf(sh.m[2][c], sh.m[3][c]));
-      f[r] = any ? __builtin_amdgcn_exp2f(sh.m[wv][c] - top) : 0.f;
-    }
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       if (4 * g + r < ncols) {
@@ -578,9 +657,10 @@ struct Tiled {
 #pragma unroll
           for (int e = 0; e < VD; e += 4)
             *reinterpret_cast<f32x4*>(&sh.o[wv][4 * g + r][16 * VD * hh + VD * n + e]) =
-                f32x4{acc[VD * hh + e][r] * f[r], acc[VD * hh + e + 1][r] * f[r], acc[VD * hh + e + 2][r] * f[r],
-                      acc[VD * hh + e + 3][r] * f[r]};
+                f32x4{acc[VD * hh + e][r], acc[VD * hh + e + 1][r], acc[VD * hh + e + 2][r], acc[VD * hh + e + 3][r]};
       }
+    bool here = false;
+    const uint32_t part = whole ? 0 : where(here);
     __syncthreads();
     for (int i = threadIdx.x; i < ncols * (HDP / 4); i += 256) {
       const int c = i / (HDP / 4), d = 4 * (i % (HDP / 4));
@@ -590,15 +670,16 @@ struct Tiled {
       float sum = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        o += *reinterpret_cast<const f32x4*>(&sh.o[k][c][d]);
-        // (a wave without rows has no sum)
-        if (sh.l[k][c] != 0.f) sum += __builtin_amdgcn_exp2f(sh.m[k][c] - top) * sh.l[k][c];
+        // (A wave without rows has a sum of zero and a maximum of minus infinity.)
+        const float lk = sh.l[k][c], f = lk != 0.f ? __builtin_amdgcn_exp2f(sh.m[k][c] - top) : 0.f;
+        o += *reinterpret_cast<const f32x4*>(&sh.o[k][c][d]) * f;
+        sum += f * lk;
       }
       if (whole) {
-        *reinterpret_cast<f32x4u*>(a.out + s * a.out_stride + (long)(qh + c) * w.hd + d) = o / sum;
+        *reinterpret_cast<f32x4u*>(a.out + s * a.out_stride + (long)(qh + c) * w.hd + d) = o * (1.f / sum);
       } else {
-        __builtin_amdgcn_raw_buffer_store_b128(o, pt.rs, part + (uint32_t)(c * w.hd + d) * 4u, 0, kDeviceScope);
-        if (d == 0) pt.put_stat(part, c, top, sum);
+        pt.put(part + (uint32_t)(c * w.hd + d) * 4u, o, here);
+        if (d == 0) pt.put_stat(part, c, top, sum, here);
       }
     }
   }
@@ -609,7 +690,7 @@ __global__ __launch_bounds__(256, WAVES) void paged_attn_kernel(PagedView w, Att
   __shared__ typename Inner::Shared sh;
   __shared__ unsigned drawn;
   const int lane = threadIdx.x & 63;
-  const uint32_t r = blockIdx.x, items = (uint32_t)(w.n_kv * a.blocks);
+  const uint32_t items = (uint32_t)(w.n_kv * a.blocks);
   // Sequence i's rows, for the 64 from s0 on a lane each.
   auto chunk = [&](uint32_t s0) {
     return s0 + lane < a.n ? rows_of_len(w, a, a.lens[s0 + lane]) : 0u;
@@ -618,8 +699,11 @@ __global__ __launch_bounds__(256, WAVES) void paged_attn_kernel(PagedView w, Att
   uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
   for (uint32_t s0 = 64; s0 < a.n; s0 += 64)
     total += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(units_of_rows(chunk(s0)) * items), 63);
-  const uint32_t per = units_per_range(total, (uint32_t)gridDim.x);
-  const uint32_t start = r * per, end = min(total, start + per);
+  const auto divide = [](uint32_t x, uint32_t y) { return quotient(x, y, __builtin_amdgcn_rcpf((float)y)); };
+  const Cut cut = cut_units(total, a.most, a.few, a.slots, divide);
+  const uint32_t per = cut.per, in_slot = cut.in_slot, slot = slot_of(blockIdx.x, a.slots);
+  const uint32_t ranges = in_slot << a.slots, r = range_of(blockIdx.x, a.slots, in_slot);
+  const uint32_t start = r * per, end = blockIdx.x < ranges ? min(total, start + per) : 0;
   if (start < end) {
     uint32_t s0 = 0;
     for (;;) {  // the chunk that holds the range's first unit
@@ -642,31 +726,49 @@ __global__ __launch_bounds__(256, WAVES) void paged_attn_kernel(PagedView w, Att
         },
         [&](uint32_t s, uint32_t n, uint32_t item, uint32_t u0, uint32_t u1, uint32_t at) {
           const uint32_t units = units_of(n), first = at - u0;
-          const int h = (int)item / a.blocks, c0 = ((int)item - h * a.blocks) * a.cols;
+          const int h = a.blocks == 1 ? (int)item : (int)divide(item, (uint32_t)a.blocks);
+          const int c0 = ((int)item - h * a.blocks) * a.cols;
           const int qh = h * a.group + c0, ncols = min(a.cols, a.group - c0);
           const bool whole = u0 == 0 && u1 == units;
-          Inner::segment(w, a, sh, s, h, qh, ncols, u0 * kUnitRows, min(n, u1 * kUnitRows), whole, pt,
-                         pt.at(r, partial_of(r, per, at)));
+          Pieces ps{};
+          uint32_t of_group = 0;
+          bool once = false;   // joined at once, at device scope
+          bool alone = false;  // the group's only piece of many: its partial as it is
+          Inner::segment(w, a, sh, s, h, qh, ncols, u0 * kUnitRows, min(n, u1 * kUnitRows), whole, pt, [&](bool& here) {
+            const Group g = group_of(r, slot, in_slot);
+            ps = pieces_of(g, divide(first, per), divide(first + units - 1, per), first, per, in_slot, divide);
+            of_group = group_partial(g, first, per);
+            once = a.slots == 0 || (ps.groups > 1 && ps.all <= kGroup);
+            alone = !once && ps.groups > 1 && ps.count == 1;
+            here = !once && !alone;
+            return pt.at(alone ? 2 * ranges + of_group : 2 * r + partial_of(r, per, at));
+          });
           if (whole) return;
-          const uint32_t w0 = first / per, pieces = (first + units - 1) / per - w0 + 1;
-          auto which = [&](uint32_t i) { return partial_of(i, per, first); };
-          float* out = a.out + s * a.out_stride + (long)qh * w.hd;
-          unsigned* ticket = a.tickets + kMaxRanges + s * items + item;
-          const uint32_t groups = groups_of(pieces);
-          if (groups == 1) {
-            if (last_of(ticket, pieces, drawn)) join<Inner::kVec>(pt, w0, 1, pieces, which, ncols, out);
-            return;
+          unsigned* const ticket = a.tickets + 2 * kGroups + s * items + item;
+          float* const out = a.out + s * a.out_stride + (long)qh * w.hd;
+          uint32_t piece0 = 2 * ps.first + partial_of(ps.first, per, first), rest = 2 * (ps.first + 1), count = ps.groups;
+          if (once) {
+            piece0 = 2 * ps.w0 + partial_of(ps.w0, per, first);
+            rest = 2 * (ps.w0 + 1);
+            count = ps.all;
+          } else {
+            const bool only = ps.groups == 1;
+            if (!alone) {
+              if (!last_of(only ? ticket : a.tickets + of_group, ps.count, drawn)) return;
+              join<Inner::kVec, Inner::kLanes, kXcdScope>(pt, piece0, rest, ps.count, ncols, only ? out : nullptr,
+                                                          2 * ranges + of_group);
+            }
+            if (only) return;
+            piece0 = 2 * ranges + ps.group0;
+            rest = (piece0 & ~1u) + 2;
           }
-          const uint32_t g0 = w0 + (r - w0) / kGroup * kGroup, mine = min((uint32_t)kGroup, w0 + pieces - g0);
-          if (mine > 1) {  // (two items' groups may open at one range, but only one of more than a piece)
-            if (!last_of(a.tickets + g0, mine, drawn)) return;
-            join<Inner::kVec>(pt, g0, 1, mine, which, ncols, (float*)nullptr);
-          }
-          if (last_of(ticket, groups, drawn)) join<Inner::kVec>(pt, w0, kGroup, groups, which, ncols, out);
-        });
+          if (last_of(ticket, count, drawn))
+            join<Inner::kVec, Inner::kLanes, kDeviceScope>(pt, piece0, rest, count, ncols, out, 0);
+        },
+        divide);
   }
   // Sequences without rows: zeros; refused ones: NaN.
-  for (uint32_t s = r; s < a.n; s += gridDim.x) {
+  for (uint32_t s = blockIdx.x; s < a.n; s += gridDim.x) {
     const int len = a.lens[s];
     const uint32_t n = rows_of_len(w, a, len);
     if (n != 0 && n != kRefused) continue;
@@ -682,10 +784,24 @@ bool tiled(int hd) { return hd % 8 == 0 && hd <= 256; }
 
 int cols_of(int hd, int group) { return tiled(hd) ? std::min(group, 16) : 1; }
 
-// Workgroups that deal the work of `units` units at most: two a CU, which is what
-// is resident, or one an item where there are more.
-uint32_t ranges(size_t items, size_t units) {
-  return (uint32_t)std::max<size_t>(1, std::min(units, std::min<size_t>(kMaxRanges, std::max<size_t>(2 * kCUs, items))));
+// Bytes of K and V that a wave has in flight.
+size_t tile_bytes(const rv_paged* pg) {
+  const size_t wide = pg->head_dim <= 64 ? 64 : pg->head_dim <= 128 ? 128 : 256;
+  return 2 * wide * (pg->elem == RV_ELEM_F32 ? 64 : pg->elem == RV_ELEM_F16 ? 64 : 34);
+}
+
+// log2 of the ranges the work is cut into: two a CU (what is resident), and where it
+// is long one a CU if a wave's tile is 16 KiB and the items are no more than the CUs,
+// or if one is what is resident. f16, 128 wide, us at 256 | 512 ranges: 64 sequences of
+// up to 16000 rows 191 | 198, but 128 of 300 21.2 | 18.4; Q8_0, 32 of up to 8192: 50.6 |
+// 39.3; f16, 64 wide, 64 of up to 8000: 120 | 116. With more some wait for others to end.
+// Where the XCDs are not known apart an item has at most kMostPieces.
+void set_ranges(const rv_paged* pg, size_t items, size_t units, AttnArgs& a) {
+  const bool wide = pg->head_dim > 128;
+  a.slots = pg->xcd_ok ? 3 : 0;
+  a.most = a.slots == 0 ? 6 : wide ? 8 : 9;
+  while (a.most > 3 && units <= ((size_t)1 << a.most) / 2) --a.most;  // (never so many units)
+  a.few = a.most == 9 && tile_bytes(pg) >= 16384 && items <= (size_t)kCUs ? 8 : a.most;
 }
 
 size_t items_per_seq(const rv_paged* pg, size_t n_q) {
@@ -696,7 +812,7 @@ size_t items_per_seq(const rv_paged* pg, size_t n_q) {
 template <typename T>
 void launch_attn(const PagedView& w, const AttnArgs& a, dim3 grid, hipStream_t s) {
 #define RV_TILED(HDP, FULL, WAVES) \
-  hipLaunchKernelGGL((paged_attn_kernel<Tiled<T, HDP, FULL>, WAVES>), grid, dim3(256), 0, s, w, a)
+  hipLaunchKernelGGL((paged_attn_kernel<Tiled<T, HDP, FULL, 1>, WAVES>), grid, dim3(256), 0, s, w, a)
   if (!tiled(w.hd))
     hipLaunchKernelGGL((paged_attn_kernel<Plain<T>, 1>), grid, dim3(256), 0, s, w, a);
   else if (w.hd == 64)
@@ -721,8 +837,8 @@ PagedAttnPlan paged_attn_plan(const rv_paged* pg, const rv_page_table& t, size_t
   const size_t items = n * items_per_seq(pg, n_q), rows = t.pages * pg->page_rows;
   const size_t cols = cols_of((int)pg->head_dim, (int)(n_q / pg->n_kv_heads));
   p.units = items * ((rows + kUnitRows - 1) / kUnitRows);  // (both below 2^42: no overflow that matters below)
-  p.ws_bytes = (size_t)ranges(items, SIZE_MAX) * 2 * cols * (pg->head_dim + 2) * sizeof(float);
-  p.ticket_bytes = (kMaxRanges + items) * sizeof(unsigned);
+  p.ws_bytes = (size_t)2 * (kMaxRanges + kGroups) * cols * (pg->head_dim + 2) * sizeof(float);
+  p.ticket_bytes = (2 * kGroups + items) * sizeof(unsigned);
   return p;
 }
 
@@ -743,7 +859,8 @@ HipStatus launch_paged_attn(const rv_paged* pg, const PagedView& w, const PagedA
   a.tickets = pg->tickets;
   a.part = (float*)pg->ws;
   a.part_bytes = (uint32_t)plan.ws_bytes;
-  const dim3 grid(ranges(p.n * w.n_kv * a.blocks, plan.units));
+  set_ranges(pg, p.n * w.n_kv * a.blocks, plan.units, a);
+  const dim3 grid(1u << a.most);
   HipStatus st;
   if (pg->elem == RV_ELEM_F32)
     launch_attn<float>(w, a, grid, s);

@@ -62,6 +62,19 @@ RV_HD I units_of(I rows) {
   return rows > 0 ? (rows + (kUnitRows - 1)) / kUnitRows : 0;
 }
 
+// x / y for a quotient below 2^21, by a float reciprocal of y that is off by at
+// most 2^-22 of itself (x and y round by 2^-24, the product by 2^-24: the estimate
+// is less than one off).
+RV_HD uint32_t quotient(uint32_t x, uint32_t y, float reciprocal_y) {
+  uint32_t q = (uint32_t)((float)x * reciprocal_y);
+  const uint32_t r = x - q * y;
+  if ((int32_t)r < 0)
+    --q;
+  else if (r >= y)
+    ++q;
+  return q;
+}
+
 template <typename I>
 RV_HD I units_per_range(I total, I ranges) {
   const I per = (total + ranges - 1) / ranges;
@@ -76,11 +89,19 @@ RV_HD int partial_of(I range, I per, I item_start) {
   return item_start > range * per ? 1 : 0;
 }
 
+struct PlainQuotient {
+  template <typename I>
+  RV_HD I operator()(I x, I y) const {
+    return x / y;
+  }
+};
+
 // Walks the units [start, end), the first of which is unit `off` of sequence s:
 // visit(sequence, its rows, item, first unit, last unit + 1 of the item, the first
 // unit's place in the line).
-template <typename I, typename Rows, typename Visit>
-RV_HD void walk_units(uint32_t s, I off, I start, I end, I items, Rows rows_of, Visit visit) {
+template <typename I, typename Rows, typename Visit, typename Quotient = PlainQuotient>
+RV_HD void walk_units(uint32_t s, I off, I start, I end, I items, Rows rows_of, Visit visit,
+                      Quotient divide = Quotient()) {
   for (I at = start; at < end;) {
     const I rows = rows_of(s), units = units_of(rows);
     if (off >= units * items) {
@@ -88,7 +109,7 @@ RV_HD void walk_units(uint32_t s, I off, I start, I end, I items, Rows rows_of, 
       ++s;
       continue;
     }
-    const I item = off / units, u0 = off - item * units;
+    const I item = divide(off, units), u0 = off - item * units;
     const I u1 = units < u0 + (end - at) ? units : u0 + (end - at);
     visit(s, rows, item, u0, u1, at);
     off += u1 - u0;
@@ -96,13 +117,74 @@ RV_HD void walk_units(uint32_t s, I off, I start, I end, I items, Rows rows_of, 
   }
 }
 
-// The partials of an item cut into `pieces` are joined by whoever leaves the last
-// of them; past kFlat pieces first in groups of kGroup, whose partials the last of
-// a group replaces by one.
-constexpr int kFlat = 32, kGroup = 16;
+// Workgroups are dealt to the XCDs in turn, so with 2^slots of them, in_slot ranges to
+// each, workgroup b takes a range such that consecutive ones share an XCD: range r is
+// of slot r / in_slot. A slot's ranges make groups of kGroup. An item's pieces (ranges
+// w0 .. w1) are joined by whoever leaves the last of them, or, where they are many and
+// of several groups, first within each group, then across groups.
+constexpr uint32_t kGroup = 16;
 
-RV_HD uint32_t groups_of(uint32_t pieces) {
-  return pieces > (uint32_t)kFlat ? (pieces + kGroup - 1) / kGroup : 1;
+RV_HD uint32_t slot_of(uint32_t b, int slots) { return b & ((1u << slots) - 1); }
+
+RV_HD uint32_t range_of(uint32_t b, int slots, uint32_t in_slot) { return slot_of(b, slots) * in_slot + (b >> slots); }
+
+struct Group {
+  uint32_t id, lo, hi;  // its number, first and last range
+};
+
+RV_HD Group group_of(uint32_t r, uint32_t slot, uint32_t in_slot) {
+  const uint32_t k = (r - slot * in_slot) / kGroup, last = slot * in_slot + in_slot - 1;
+  Group g;
+  g.id = slot * ((in_slot + kGroup - 1) / kGroup) + k;
+  g.lo = slot * in_slot + k * kGroup;
+  g.hi = g.lo + kGroup - 1 < last ? g.lo + kGroup - 1 : last;
+  return g;
+}
+
+// Of the two partials a group keeps for items that other groups have ranges of too:
+// the first is the item's that is there from the group's first unit on.
+RV_HD uint32_t group_partial(const Group& g, uint32_t item_start, uint32_t per) {
+  return 2 * g.id + (item_start > g.lo * per ? 1 : 0);
+}
+
+struct Pieces {
+  uint32_t first, count;    // of the group: its ranges of the item
+  uint32_t w0, all;         // of the item: its first range, and how many
+  uint32_t group0, groups;  // and its first group's partial, and how many groups
+};
+
+template <typename Quotient = PlainQuotient>
+RV_HD Pieces pieces_of(const Group& g, uint32_t w0, uint32_t w1, uint32_t item_start, uint32_t per, uint32_t in_slot,
+                       Quotient divide = Quotient()) {
+  Pieces p;
+  p.first = w0 > g.lo ? w0 : g.lo;
+  p.count = (w1 < g.hi ? w1 : g.hi) - p.first + 1;
+  p.w0 = w0;
+  p.all = w1 - w0 + 1;
+  const Group a = w0 >= g.lo ? g : group_of(w0, divide(w0, in_slot), in_slot);
+  const Group z = w1 <= g.hi ? g : group_of(w1, divide(w1, in_slot), in_slot);
+  p.group0 = group_partial(a, item_start, per);
+  p.groups = z.id - a.id + 1;
+  return p;
+}
+
+// How `total` units are cut: units a range, and the ranges of a slot (so that every
+// slot has as many to do). At most 2^most ranges; 2^few where that makes eight units
+// or more a range.
+struct Cut {
+  uint32_t per, in_slot;
+};
+
+template <typename Quotient = PlainQuotient>
+RV_HD Cut cut_units(uint32_t total, int most, int few, int slots, Quotient divide = Quotient()) {
+  const int n = total >> (few + 3) ? few : most;
+  Cut c;
+  c.per = (total + (1u << n) - 1) >> n;
+  if (c.per < 1) c.per = 1;
+  const uint32_t used = c.per == 1 ? total : divide(total + c.per - 1, c.per);
+  c.in_slot = (used + (1u << slots) - 1) >> slots;
+  if (c.in_slot < 1) c.in_slot = 1;
+  return c;
 }
 
 }  // namespace rv

@@ -26,21 +26,32 @@ from .attention import _check, _elem_code, _lib, _raw_stream
 _LAYOUTS = {"half": L.RV_ROPE_HALF, "interleaved": L.RV_ROPE_INTERLEAVED}
 _SCALINGS = {"none": L.RV_ROPE_UNSCALED, "linear": L.RV_ROPE_LINEAR, "ntk": L.RV_ROPE_NTK, "yarn": L.RV_ROPE_YARN}
 
-_torch = None
+_torch = _F32 = _I32 = _current_device = None
 
 
 def _t():
-    global _torch
+    global _torch, _F32, _I32, _current_device
     if _torch is None:
         import torch
 
+        _F32, _I32 = torch.float32, torch.int32
+        _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
         _torch = torch
     return _torch
 
 
+# The checks below are most of a small call's time on the host, so the ordinary
+# arguments (contiguous, of the right type, on the call's device) pass on few
+# attribute reads; what does not is looked at one property at a time.
+
+
 def _rows(x, what, device):
     """(address, rows, width, stride) of a float32 matrix whose rows lie in one piece each."""
-    torch = _t()
+    torch = _torch or _t()
+    if type(x) is torch.Tensor and x.dtype is _F32 and x.get_device() == device >= 0 and x.is_contiguous():
+        shape = x.shape
+        if len(shape) == 2:
+            return x.data_ptr(), shape[0], shape[1], shape[1]
     if not isinstance(x, torch.Tensor) or x.dtype is not torch.float32 or not x.is_cuda:
         raise TypeError(f"{what} must be a float32 torch tensor on the GPU")
     if x.dim() != 2:
@@ -55,7 +66,11 @@ def _rows(x, what, device):
 
 
 def _ints(x, n, what, device) -> int:
-    torch = _t()
+    torch = _torch or _t()
+    if type(x) is torch.Tensor and x.dtype is _I32 and x.get_device() == device >= 0 and x.is_contiguous():
+        shape = x.shape
+        if len(shape) == 1 and shape[0] == n:
+            return x.data_ptr()
     if not isinstance(x, torch.Tensor) or x.dtype is not torch.int32 or not x.is_cuda:
         raise TypeError(f"{what} must be an int32 torch tensor on the GPU")
     if x.dim() != 1 or x.shape[0] != n or (n > 1 and x.stride(0) != 1):
@@ -68,7 +83,7 @@ def _ints(x, n, what, device) -> int:
 def _weight(x, what, device):
     if x is None:
         return None, 0
-    torch = _t()
+    torch = _torch or _t()
     if not isinstance(x, torch.Tensor) or x.dtype is not torch.float32 or not x.is_cuda or not x.is_contiguous():
         raise TypeError(f"{what} must be a contiguous float32 torch tensor on the GPU")
     if x.get_device() != device:
@@ -77,7 +92,11 @@ def _weight(x, what, device):
 
 
 def _table(x, device) -> L.RvPageTable:
-    torch = _t()
+    torch = _torch or _t()
+    if type(x) is torch.Tensor and x.dtype is _I32 and x.get_device() == device >= 0 and x.is_contiguous():
+        shape = x.shape
+        if len(shape) == 2:
+            return L.RvPageTable(x.data_ptr(), shape[0], shape[1], shape[1])
     if not isinstance(x, torch.Tensor) or x.dtype is not torch.int32 or not x.is_cuda or x.dim() != 2:
         raise TypeError("table must be a 2-D int32 torch tensor on the GPU: sequences x pages")
     n, pages = x.shape
@@ -132,16 +151,16 @@ class Rope:
 def rope_rows(x, positions, rope: Rope, out=None):
     """rv_rope_rows: the heads of row r of x rotated at positions[r], into out
     (a new tensor by default; x itself rotates in place). Returns out."""
-    torch = _t()
+    torch = _torch or _t()
     if out is None:
         out = torch.empty(x.shape, dtype=torch.float32, device=x.device)
     device = x.get_device() if isinstance(x, torch.Tensor) else -1
     xp, rows, width, xs = _rows(x, "x", device)
     op, out_rows, out_width, os = _rows(out, "out", device)
-    if (out_rows, out_width) != (rows, width):
+    if out_rows != rows or out_width != width:
         raise ValueError("out must have the shape of x")
     pos = _ints(positions, rows, "positions", device)
-    if torch.cuda.current_device() != device:
+    if _current_device() != device:
         with torch.cuda.device(device):
             return rope_rows(x, positions, rope, out)
     err = L.RvError()
@@ -216,7 +235,7 @@ class PagedKvCache:
         position writes nothing."""
         kp, rows, width, ks = _rows(k_rows, "k_rows", self.device)
         vp, v_n, v_width, vs = _rows(v_rows, "v_rows", self.device)
-        if width != self.kv_dim or (v_n, v_width) != (rows, width):
+        if width != self.kv_dim or v_n != rows or v_width != width:
             raise ValueError("k_rows and v_rows must both be rows x kv_dim")
         wp, wn = _weight(k_norm_w, "k_norm_w", self.device)
         self._call(_lib().rv_paged_append_rows, layer, rope._h if rope else None, kp, ks, vp, vs, rows,
@@ -229,27 +248,31 @@ class PagedKvCache:
         sequence seqs[r] as attention reads them: float32 of an f32 cache, else
         float16; zeros for a negative position or one refused. Into the tensors
         given, else into new ones."""
-        torch = _t()
+        torch = _torch or _t()
         rows = positions.shape[0] if isinstance(positions, torch.Tensor) and positions.dim() == 1 else 0
         pos = _ints(positions, rows, "positions", self.device)
         dtype = torch.float32 if self.elem == "f32" else torch.float16
         if k is None and v is None:
-            k = torch.empty_strided((rows, self.kv_dim), (self.kv_dim, 1), dtype=dtype, device=positions.device)
-            v = torch.empty_like(k)
-        for x, what in ((k, "k"), (v, "v")):
-            if x is None:
-                continue
-            if not isinstance(x, torch.Tensor) or x.dtype is not dtype or not x.is_cuda or not x.is_contiguous():
-                raise TypeError(f"{what} must be a contiguous {dtype} torch tensor on the GPU")
-            if x.numel() != rows * self.kv_dim:
-                raise ValueError(f"{what} must be rows x kv_dim")
-            if x.get_device() != self.device:
-                raise ValueError(f"{what} is on another device than the call's")
+            n = rows * self.kv_dim
+            k, v = torch.empty_strided((2, rows, self.kv_dim), (n, self.kv_dim, 1), dtype=dtype,
+                                       device=positions.device).unbind(0)
+            kp = k.data_ptr()
+            vp = kp + n * k.element_size()
+        else:
+            kp, vp = (None if x is None else self._row_buffer(x, what, dtype, rows) for x, what in ((k, "k"), (v, "v")))
         self._call(_lib().rv_paged_read_rows, layer, rows, pos,
                    None if seqs is None else _ints(seqs, rows, "seqs", self.device),
-                   byref(_table(table, self.device)), None if k is None else k.data_ptr(),
-                   None if v is None else v.data_ptr(), 0)
+                   byref(_table(table, self.device)), kp, vp, 0)
         return k, v
+
+    def _row_buffer(self, x, what, dtype, rows) -> int:
+        if not isinstance(x, _torch.Tensor) or x.dtype is not dtype or not x.is_cuda or not x.is_contiguous():
+            raise TypeError(f"{what} must be a contiguous {dtype} torch tensor on the GPU")
+        if x.numel() != rows * self.kv_dim:
+            raise ValueError(f"{what} must be rows x kv_dim")
+        if x.get_device() != self.device:
+            raise ValueError(f"{what} is on another device than the call's")
+        return x.data_ptr()
 
 
 def paged_attention(q_rows, cache: PagedKvCache, layer: int, table, lens, scale: float, out):
@@ -257,7 +280,7 @@ def paged_attention(q_rows, cache: PagedKvCache, layer: int, table, lens, scale:
     sequence i of the table; length 0 gives zeros."""
     qp, n, width, qs = _rows(q_rows, "q_rows", cache.device)
     op, out_n, out_width, os = _rows(out, "out", cache.device)
-    if (out_n, out_width) != (n, width):
+    if out_n != n or out_width != width:
         raise ValueError("out must have the shape of q_rows")
     cache._call(_lib().rv_paged_attention, layer, qp, qs, n, width, byref(_table(table, cache.device)),
                 _ints(lens, n, "lens", cache.device), scale, op, os, 0)
@@ -275,9 +298,9 @@ def paged_decode_step(cache: PagedKvCache, layer: int, q_rows, k_rows, v_rows, q
     kp, k_n, k_width, ks = _rows(k_rows, "k_rows", d)
     vp, v_n, v_width, vs = _rows(v_rows, "v_rows", d)
     op, out_n, out_width, os = _rows(out, "out", d)
-    if (out_n, out_width) != (n, width):
+    if out_n != n or out_width != width:
         raise ValueError("out must have the shape of q_rows")
-    if (k_n, k_width) != (n, cache.kv_dim) or (v_n, v_width) != (n, cache.kv_dim):
+    if k_n != n or v_n != n or k_width != cache.kv_dim or v_width != cache.kv_dim:
         raise ValueError("k_rows and v_rows must be rows x kv_dim with q_rows' rows")
     wqp, wqn = _weight(q_norm_w, "q_norm_w", d)
     wkp, wkn = _weight(k_norm_w, "k_norm_w", d)

@@ -66,8 +66,79 @@ static void deal(const std::vector<long>& rows, long items, long ranges) {
   CHECK(joined == kept.size(), "%zu pieces of %zu joined", joined, kept.size());
 }
 
+// The joins within and across groups: every piece is kept where its group's last
+// workgroup, or the item's, looks for it, and no place is used twice.
+static void join_groups(const std::vector<uint32_t>& units, int log_slots, int most, int few) {
+  uint32_t total = 0;
+  for (uint32_t u : units) total += u;
+  const Cut cut = cut_units(total, most, few, log_slots);
+  const uint32_t slots = 1u << log_slots, per = cut.per, in_slot = cut.in_slot, ranges = slots * in_slot;
+  CHECK(ranges <= std::max(1u << most, slots), "%u ranges", ranges);
+  CHECK((uint64_t)per * ranges >= total, "units left over");
+  std::vector<int> dealt(ranges, 0);
+  for (uint32_t b = 0; b < ranges; ++b) {
+    const uint32_t r = range_of(b, log_slots, in_slot);
+    CHECK(r < ranges && r / in_slot == b % slots && slot_of(b, log_slots) == b % slots, "workgroup %u", b);
+    const Group g = group_of(r, b % slots, in_slot);
+    CHECK(g.lo <= r && r <= g.hi && g.hi - g.lo < kGroup && g.hi / in_slot == b % slots, "group of %u", r);
+    CHECK(r == 0 || g.id == group_of(r - 1, (r - 1) / in_slot, in_slot).id + (r == g.lo ? 1 : 0), "number of %u's", r);
+    ++dealt[r];
+  }
+  for (int d : dealt) CHECK(d == 1, "a range dealt %d times", d);
+  std::map<uint32_t, int> pieces_at, groups_at;  // partial -> item
+  uint32_t first = 0;
+  for (size_t item = 0; item < units.size(); first += units[item++]) {
+    const uint32_t w0 = first / per, w1 = (first + units[item] - 1) / per;
+    if (!units[item] || w0 == w1) continue;
+    uint32_t seen = 0, seen_groups = 0, group0 = 0;
+    for (uint32_t r = w0; r <= w1; ++r) {
+      const Group g = group_of(r, r / in_slot, in_slot);
+      const Pieces p = pieces_of(g, w0, w1, first, per, in_slot);
+      CHECK(p.first <= r && r < p.first + p.count && p.count <= kGroup && p.w0 == w0 && p.all == w1 - w0 + 1, "range %u", r);
+      const uint32_t at = std::max(first, r * per), mine = 2 * r + partial_of(r, per, at);
+      const uint32_t of_group = group_partial(g, first, per);
+      // Where the group's join, and one of all pieces, look for this piece.
+      const uint32_t looked = r == p.first ? 2 * p.first + partial_of(p.first, per, first)
+                                           : 2 * (p.first + 1) + 2 * (r - p.first - 1);
+      const uint32_t flat = r == w0 ? 2 * w0 + partial_of(w0, per, first) : 2 * (w0 + 1) + 2 * (r - w0 - 1);
+      CHECK(looked == mine && flat == mine, "range %u's piece", r);
+      CHECK(!pieces_at.count(mine), "partial %u twice", mine);
+      pieces_at[mine] = (int)item;
+      if (r == w0) group0 = of_group;
+      CHECK(p.group0 == group0, "first group");
+      if (r == p.first) {
+        if (p.groups > 1) {
+          CHECK(of_group == (seen_groups ? (group0 & ~1u) + 2 + 2 * (seen_groups - 1) : group0), "group %u", g.id);
+          CHECK(of_group < 2 * 32 && !groups_at.count(of_group), "group partial %u twice", of_group);
+          groups_at[of_group] = (int)item;
+        }
+        ++seen_groups;
+        seen += p.count;
+      }
+    }
+    const Pieces p = pieces_of(group_of(w0, w0 / in_slot, in_slot), w0, w1, first, per, in_slot);
+    CHECK(seen == p.all && seen_groups == p.groups, "%u pieces, %u groups", seen, seen_groups);
+  }
+}
+
 int main() {
   std::mt19937 g(7);
+  for (int i = 0; i < 4000; ++i) {
+    std::vector<uint32_t> units(1 + g() % 60);
+    const uint32_t most = 1 + (i % 2 ? g() % 40 : g() % 2000);
+    for (auto& u : units) u = g() % (most + 1);
+    if (i % 7 == 0) units.resize(1);
+    const int slots = i % 5 ? 3 : 0, cut = slots + (int)(g() % 7);
+    join_groups(units, slots, cut, cut && i % 3 ? cut - 1 : cut);
+  }
+  // Quotients by a reciprocal two steps off either way.
+  for (int i = 0; i < 2000000; ++i) {
+    const uint32_t y = 1 + (g() >> (g() % 32)), q = g() % (1u << (g() % 21));
+    const uint64_t x = (uint64_t)q * y + (i % 3 == 0 ? 0 : i % 3 == 1 ? y - 1 : g() % y);
+    if (x >= 0x80000000u || y >= 0x80000000u) continue;
+    const float rcp = (float)(1.0 / y) * (1.f + ((int)(g() % 5) - 2) * 5.96e-8f);
+    CHECK(quotient((uint32_t)x, y, rcp) == q, "%u / %u", (uint32_t)x, y);
+  }
   deal({1}, 1, 512);
   deal({0, 0, 0}, 4, 512);
   deal({131000}, 4, 512);
