@@ -185,9 +185,14 @@ class PagedKvCache:
         self.n_pages, self.page_rows, self.kv_dim = n_pages, page_rows, n_kv_heads * head_dim
         self.elem = {L.RV_ELEM_F16: "f16", L.RV_ELEM_F32: "f32", L.RV_ELEM_Q8_0: "q8_0"}[_elem_code(elem)]
         self.device = device
+        torch = _t()
+        self._dtype = torch.float32 if self.elem == "f32" else torch.float16  # of rows read back
+        self._torch_device = torch.device("cuda", device)
         self._stream = None
-        # One call at a time binds the stream and queues its work.
+        # One call at a time binds the stream, queues its work and has the error's place.
         self._lock = threading.Lock()
+        self._lib, self._err = _lib(), err
+        self._err_ref = byref(err)
 
     def __del__(self):
         h = getattr(self, "_h", None)
@@ -209,23 +214,21 @@ class PagedKvCache:
         return int(out.value)
 
     def _call(self, fn, *args):
-        err = L.RvError()
         with self._lock:
             s = _raw_stream(self.device)
             if s != self._stream:
-                _check(_lib().rv_paged_set_stream(self._h, s, byref(err)), err)
+                _check(self._lib.rv_paged_set_stream(self._h, s, self._err_ref), self._err)
                 self._stream = s
-            rc = fn(self._h, *args, byref(err))
-        if rc:
-            _check(rc, err)
+            if fn(self._h, *args, self._err_ref):
+                _check(self._err.code, self._err)
 
     def synchronize(self):
-        self._call(_lib().rv_paged_synchronize)
+        self._call(self._lib.rv_paged_synchronize)
 
     def device_status(self):
         """Waits for the stream; raises KvError (PageOutOfRange, SequenceOutOfRange or
         PositionOutOfTable) when the device refused a row since the last read."""
-        self._call(_lib().rv_paged_device_status)
+        self._call(self._lib.rv_paged_device_status)
 
     def append_rows(self, layer: int, k_rows, v_rows, table, positions, seqs=None, rope: Rope | None = None,
                     k_norm_w=None, eps: float = 0.0):
@@ -238,7 +241,7 @@ class PagedKvCache:
         if width != self.kv_dim or v_n != rows or v_width != width:
             raise ValueError("k_rows and v_rows must both be rows x kv_dim")
         wp, wn = _weight(k_norm_w, "k_norm_w", self.device)
-        self._call(_lib().rv_paged_append_rows, layer, rope._h if rope else None, kp, ks, vp, vs, rows,
+        self._call(self._lib.rv_paged_append_rows, layer, rope._h if rope else None, kp, ks, vp, vs, rows,
                    _ints(positions, rows, "positions", self.device),
                    None if seqs is None else _ints(seqs, rows, "seqs", self.device),
                    byref(_table(table, self.device)), wp, wn, eps, 0)
@@ -248,26 +251,25 @@ class PagedKvCache:
         sequence seqs[r] as attention reads them: float32 of an f32 cache, else
         float16; zeros for a negative position or one refused. Into the tensors
         given, else into new ones."""
-        torch = _torch or _t()
-        rows = positions.shape[0] if isinstance(positions, torch.Tensor) and positions.dim() == 1 else 0
+        rows = positions.shape[0] if isinstance(positions, _torch.Tensor) and positions.dim() == 1 else 0
         pos = _ints(positions, rows, "positions", self.device)
-        dtype = torch.float32 if self.elem == "f32" else torch.float16
         if k is None and v is None:
-            n = rows * self.kv_dim
-            k, v = torch.empty_strided((2, rows, self.kv_dim), (n, self.kv_dim, 1), dtype=dtype,
-                                       device=positions.device).unbind(0)
-            kp = k.data_ptr()
-            vp = kp + n * k.element_size()
+            d = self.kv_dim
+            k, v = _torch.empty_strided((2, rows, d), (rows * d, d, 1), dtype=self._dtype,
+                                        device=self._torch_device).unbind(0)
+            kp, vp = k.data_ptr(), v.data_ptr()
         else:
-            kp, vp = (None if x is None else self._row_buffer(x, what, dtype, rows) for x, what in ((k, "k"), (v, "v")))
-        self._call(_lib().rv_paged_read_rows, layer, rows, pos,
+            kp, vp = self._row_buffer(k, "k", rows), self._row_buffer(v, "v", rows)
+        self._call(self._lib.rv_paged_read_rows, layer, rows, pos,
                    None if seqs is None else _ints(seqs, rows, "seqs", self.device),
                    byref(_table(table, self.device)), kp, vp, 0)
         return k, v
 
-    def _row_buffer(self, x, what, dtype, rows) -> int:
-        if not isinstance(x, _torch.Tensor) or x.dtype is not dtype or not x.is_cuda or not x.is_contiguous():
-            raise TypeError(f"{what} must be a contiguous {dtype} torch tensor on the GPU")
+    def _row_buffer(self, x, what, rows):
+        if x is None:
+            return None
+        if not isinstance(x, _torch.Tensor) or x.dtype is not self._dtype or not x.is_cuda or not x.is_contiguous():
+            raise TypeError(f"{what} must be a contiguous {self._dtype} torch tensor on the GPU")
         if x.numel() != rows * self.kv_dim:
             raise ValueError(f"{what} must be rows x kv_dim")
         if x.get_device() != self.device:
@@ -282,7 +284,7 @@ def paged_attention(q_rows, cache: PagedKvCache, layer: int, table, lens, scale:
     op, out_n, out_width, os = _rows(out, "out", cache.device)
     if out_n != n or out_width != width:
         raise ValueError("out must have the shape of q_rows")
-    cache._call(_lib().rv_paged_attention, layer, qp, qs, n, width, byref(_table(table, cache.device)),
+    cache._call(cache._lib.rv_paged_attention, layer, qp, qs, n, width, byref(_table(table, cache.device)),
                 _ints(lens, n, "lens", cache.device), scale, op, os, 0)
     return out
 
@@ -304,6 +306,6 @@ def paged_decode_step(cache: PagedKvCache, layer: int, q_rows, k_rows, v_rows, q
         raise ValueError("k_rows and v_rows must be rows x kv_dim with q_rows' rows")
     wqp, wqn = _weight(q_norm_w, "q_norm_w", d)
     wkp, wkn = _weight(k_norm_w, "k_norm_w", d)
-    cache._call(_lib().rv_paged_decode_step, layer, rope._h if rope else None, qp, qs, kp, ks, vp, vs, n, width, wqp,
+    cache._call(cache._lib.rv_paged_decode_step, layer, rope._h if rope else None, qp, qs, kp, ks, vp, vs, n, width, wqp,
                 wqn, wkp, wkn, eps, byref(_table(table, d)), _ints(positions, n, "positions", d), scale, op, os, 0)
     return out
