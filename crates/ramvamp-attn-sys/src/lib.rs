@@ -68,6 +68,7 @@ pub const RV_ROPE_UNSCALED: u32 = 0;
 pub const RV_ROPE_LINEAR: u32 = 1;
 pub const RV_ROPE_NTK: u32 = 2;
 pub const RV_ROPE_YARN: u32 = 3;
+pub const RV_TUNE_PAGED_JOIN: i32 = 1;
 pub const RV_FLOOR_MFMA_F16_16X16X32: i32 = 0;
 pub const RV_FLOOR_MFMA_F16_32X32X16: i32 = 1;
 pub const RV_FLOOR_MFMA_F32_16X16X4: i32 = 2;
@@ -220,6 +221,7 @@ extern "C" {
     pub fn rv_paged_projected_bytes(n_layers: usize, n_kv_heads: usize, head_dim: usize, n_pages: usize, page_rows: usize, elem: rv_elem, bytes: *mut u64, err: *mut rv_error) -> i32;
     pub fn rv_paged_new(n_layers: usize, n_kv_heads: usize, head_dim: usize, n_pages: usize, page_rows: usize, elem: rv_elem, device: c_int, out: *mut *mut rv_paged, err: *mut rv_error) -> i32;
     pub fn rv_paged_free(pg: *mut rv_paged);
+    pub fn rv_paged_set_tuning(pg: *mut rv_paged, knob: i32, value: i64, err: *mut rv_error) -> i32;
     pub fn rv_paged_set_stream(pg: *mut rv_paged, hip_stream: *mut c_void, err: *mut rv_error) -> i32;
     pub fn rv_paged_synchronize(pg: *mut rv_paged, err: *mut rv_error) -> i32;
     pub fn rv_paged_device_status(pg: *mut rv_paged, err: *mut rv_error) -> i32;

@@ -106,8 +106,8 @@ typedef struct rv_page_table {
 
 /* Bytes of both planes (Q8_0: 34 per 32 elements). RV_KV_INVALID_DIMS as
  * rv_kv_projected_bytes (d = n_pages), also for page_rows not a power of two
- * from 8 to 1024; RV_ERR_UNSUPPORTED: head_dim above 512, n_pages or kv heads
- * times head_dim past 2^31 - 1. */
+ * from 8 to 1024; RV_ERR_UNSUPPORTED: head_dim above 512, n_kv_heads above
+ * 65535, n_pages past 2^31 - 1. */
 int32_t rv_paged_projected_bytes(size_t n_layers, size_t n_kv_heads, size_t head_dim, size_t n_pages,
                                  size_t page_rows, rv_elem elem, uint64_t* bytes, rv_error* err);
 /* Zeroed pages on `device`. */
@@ -115,6 +115,12 @@ int32_t rv_paged_new(size_t n_layers, size_t n_kv_heads, size_t head_dim, size_t
                      rv_elem elem, int device, rv_paged** out, rv_error* err);
 /* Waits for the device's queued work before it frees the pages. */
 void rv_paged_free(rv_paged* pg);
+/* As rv_kv_set_tuning. RV_TUNE_PAGED_JOIN: how workgroups that share a
+ * sequence's kv head join what they have: 0 within each XCD's L2 first where the
+ * device deals workgroups to its XCDs in turn (checked when the cache is made),
+ * else across them at once, 2 always so. */
+#define RV_TUNE_PAGED_JOIN 1
+int32_t rv_paged_set_tuning(rv_paged* pg, int32_t knob, int64_t value, rv_error* err);
 /* As rv_kv_set_stream: later calls are queued on it, behind what the old one
  * holds. Calls on one cache share its workspace: one stream at a time, and so
  * two graphs captured over one cache are replayed one after the other. */
@@ -154,9 +160,14 @@ int32_t rv_paged_read_rows(rv_paged* pg, size_t layer, size_t rows, const int32_
  * Q8_0 rows are matrix operands as stored, q and probabilities f16 hi + lo
  * halves scaled by powers of two (to 2^-22 of themselves, or 2^-38 of the
  * largest of a head's), sums in f32. An infinity or NaN in a row that is
- * attended makes that head's output NaN; what lies in rows past lens[i] never
- * counts. Checks, in order: q_dim, layer, the strides, the table, n_seqs, out
- * overlapping q (RV_ERR_UNSUPPORTED). */
+ * attended reaches the outputs of that kv head's query heads alone: NaN, but for
+ * an infinity of K that may, where it makes a score minus infinity, leave its row
+ * without weight. What lies in rows past lens[i] never counts.
+ * RV_ERR_UNSUPPORTED: n_seqs past 2^23, query heads past 65535, and tables whose
+ * rows are more than 2^31 - 1 units (n_seqs * the tables' rows / 128 for each 16
+ * query heads of a kv head; of every query head where head_dim is no multiple of
+ * 8 or above 256). Checks, in order: q_dim, layer, the strides, the table, n_seqs,
+ * out overlapping q (RV_ERR_UNSUPPORTED), the units. */
 int32_t rv_paged_attention(rv_paged* pg, size_t layer, const float* q, size_t q_stride, size_t n_seqs, size_t q_dim,
                            const rv_page_table* table, const int32_t* lens, float scale, float* out,
                            size_t out_stride, uint32_t flags, rv_error* err);

@@ -46,6 +46,7 @@ from ._lib import (  # noqa: F401  (knobs of KvCache.set_tuning)
     RV_TUNE_KERNEL_TIMING,
     RV_TUNE_PREFILL_KV_SPLIT,
     RV_TUNE_PREFILL_ROWS,
+    RV_TUNE_PAGED_JOIN,
     RV_TUNE_ROWS_COLUMNS,
 )
 from .paged import (  # noqa: F401

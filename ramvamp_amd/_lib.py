@@ -31,6 +31,7 @@ RV_TUNE_KERNEL_TIMING = 7
 RV_TUNE_DECODE_DEPTH = 9
 RV_TUNE_DECODE_MERGE = 11
 RV_TUNE_ROWS_COLUMNS = 12
+RV_TUNE_PAGED_JOIN = 1  # of a paged cache
 RV_NOALLOC_SCRATCH_BYTES = 8 << 20
 # include/ramvamp_gemv.h
 RV_QF_Q4_K = 1
@@ -182,6 +183,7 @@ SIGNATURES = {
                                _E]),
     "rv_paged_free": (None, [_P]),
     "rv_paged_set_stream": (c_int32, [_P, _P, _E]),
+    "rv_paged_set_tuning": (c_int32, [_P, c_int32, c_int64, _E]),
     "rv_paged_synchronize": (c_int32, [_P, _E]),
     "rv_paged_device_status": (c_int32, [_P, _E]),
     "rv_paged_append_rows": (c_int32, [_P, c_size_t, _P, _P, c_size_t, _P, c_size_t, c_size_t, _P, _P,

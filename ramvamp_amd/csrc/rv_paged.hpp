@@ -30,6 +30,7 @@ struct rv_paged {
   int elem = RV_ELEM_F16;
   int device = 0;
   bool xcd_ok = false;  // xcd_dealing_ok of the device
+  int64_t tune_join = 0;
   void* k = nullptr;
   void* v = nullptr;
   hipStream_t stream = nullptr;
@@ -67,8 +68,8 @@ struct PagedView {
 };
 PagedView paged_view(const rv_paged* pg, size_t layer, const rv_page_table& t);
 
-// The rotation as the kernels take it: frequencies by value, of up to N pairs (a
-// launch's arguments cost the host by their size: 64 pairs in place of 256 ...).
+// The rotation as the kernels take it: frequencies by value, of up to N pairs (the
+// most that a head has would make every launch's arguments 2 KiB).
 template <int N>
 struct RopeArgs {
   int pairs = 0;  // 0: none
@@ -145,7 +146,7 @@ struct PagedAttn {
   size_t out_stride;
 };
 struct PagedAttnPlan {
-  size_t units;  // of work at most, by what the tables can hold (below 2^31)
+  size_t units;  // of work at most, by what the tables can hold
   size_t ws_bytes, ticket_bytes;
 };
 PagedAttnPlan paged_attn_plan(const rv_paged* pg, const rv_page_table& t, size_t n, size_t n_q);

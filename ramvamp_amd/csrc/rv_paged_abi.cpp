@@ -83,7 +83,7 @@ int32_t geometry(size_t n_layers, size_t n_kv_heads, size_t head_dim, size_t n_p
   if (head_dim > 512) return unsupported(err, head_dim, "head_dim above 512");
   if (elem == RV_ELEM_Q8_0 && head_dim % 32) return invalid("Q8_0 rows need a head_dim that is a multiple of 32");
   if (n_pages > 0x7FFFFFFFu) return unsupported(err, n_pages, "pages past 2^31 - 1");
-  if (n_kv_heads > 0x7FFFFFFFu / head_dim) return unsupported(err, n_kv_heads, "row width past 2^31 - 1");
+  if (n_kv_heads > 65535) return unsupported(err, n_kv_heads, "kv heads past 65535");
   size_t n = n_kv_heads * head_dim;
   if (__builtin_mul_overflow(n, page_rows * n_pages, &n) || __builtin_mul_overflow(n, n_layers, &n))
     return invalid("total size overflows usize");
@@ -112,6 +112,7 @@ rv::HipStatus grow(rv_paged* pg, void** buf, size_t* have, size_t bytes, const c
   }
   st.e = hipMalloc(&p, want);
   if (st.e != hipSuccess) {
+    (void)hipGetLastError();
     st.what = what;
     return st;
   }
@@ -298,6 +299,10 @@ int32_t rv_paged_new(size_t n_layers, size_t n_kv_heads, size_t head_dim, size_t
   size_t bytes;
   int32_t rc = geometry(n_layers, n_kv_heads, head_dim, n_pages, page_rows, elem, &bytes, err);
   if (rc) return rc;
+  int devices = 0;
+  hipError_t e = hipGetDeviceCount(&devices);
+  if (e == hipSuccess && (device < 0 || device >= devices)) e = hipErrorInvalidDevice;
+  if (e != hipSuccess) return hip_fail(err, e, "device");
   rv_paged* pg = new (std::nothrow) rv_paged();
   if (!pg) return fail(err, RV_ERR_HIP, (uint64_t)hipErrorOutOfMemory, 0, 0, 0, "host allocation");
   pg->n_layers = n_layers;
@@ -309,7 +314,7 @@ int32_t rv_paged_new(size_t n_layers, size_t n_kv_heads, size_t head_dim, size_t
   pg->elem = elem;
   pg->device = device;
   DeviceGuard dg(device);
-  hipError_t e = hipMalloc(&pg->k, pg->plane_bytes());
+  e = hipMalloc(&pg->k, pg->plane_bytes());
   if (e == hipSuccess) e = hipMalloc(&pg->v, pg->plane_bytes());
   if (e == hipSuccess) e = hipMemset(pg->k, 0, pg->plane_bytes());
   if (e == hipSuccess) e = hipMemset(pg->v, 0, pg->plane_bytes());
@@ -319,6 +324,7 @@ int32_t rv_paged_new(size_t n_layers, size_t n_kv_heads, size_t head_dim, size_t
   if (e == hipSuccess) pg->xcd_ok = rv::xcd_dealing_ok(device);
   if (e != hipSuccess) {
     rv_paged_free(pg);
+    (void)hipGetLastError();  // (reported here, not by the next call to ask)
     return hip_fail(err, e, "hipMalloc pages");
   }
   *out = pg;
@@ -336,6 +342,13 @@ void rv_paged_free(rv_paged* pg) {
     if (pg->order_ev) (void)hipEventDestroy(pg->order_ev);
   }
   delete pg;
+}
+
+int32_t rv_paged_set_tuning(rv_paged* pg, int32_t knob, int64_t value, rv_error* err) {
+  if (!pg) return null_arg(err, "pg");
+  if (knob != RV_TUNE_PAGED_JOIN) return unsupported(err, (uint64_t)knob, "tuning knob");
+  pg->tune_join = value;
+  return ok(err);
 }
 
 int32_t rv_paged_set_stream(rv_paged* pg, void* hip_stream, rv_error* err) {

@@ -105,7 +105,7 @@ struct Partials {
   }
 };
 
-constexpr uint32_t kMostPieces = 64;  // that are joined at once
+constexpr uint32_t kMostPieces = 32;  // that are joined at once
 
 // Joins `count` partials (at most kMostPieces), in order, partial `first` and then
 // rest, rest + 2, ..: into `out` (ncols rows of hd), or into partial `to` for all
@@ -117,7 +117,7 @@ __device__ __forceinline__ void join(const Partials& p, uint32_t first, uint32_t
                                      float* out, uint32_t to) {
   typedef float Row __attribute__((ext_vector_type(VEC)));
   constexpr uint32_t kBatch = 16;
-  constexpr int kStats = (int)kMostPieces / LANES, kColumns = 256 / LANES;  // a lane's; of the workgroup at once
+  constexpr int kStats = LANES < (int)kMostPieces ? (int)kMostPieces / LANES : 1, kColumns = 256 / LANES;  // a lane's; of the workgroup at once
   const int lane = threadIdx.x & 63, mine = lane & (LANES - 1);
   const uint32_t one = p.at(1);
   auto place = [&](uint32_t i) { return (i ? rest + 2 * (i - 1) : first) * one; };
@@ -167,15 +167,15 @@ __device__ __forceinline__ void join(const Partials& p, uint32_t first, uint32_t
           if (LANES >= 32) sum = swap_sum<16>(sum);
           if (LANES >= 64) sum = swap_sum<32>(sum);
         }
+        float fs = m[0];  // (a batch's factors are all in one register)
+#pragma unroll
+        for (int s = 1; s < kStats; ++s) fs = b0 / LANES == (uint32_t)s ? m[s] : fs;
+        const int from = (lane & ~(LANES - 1)) + (int)(b0 & (LANES - 1));
 #pragma unroll
         for (uint32_t i = 0; i < kBatch; ++i) {
           if (i % 4 == 0 && b0 + i >= count) break;
-          const uint32_t k = b0 + i;
-          float f = m[0];
-#pragma unroll
-          for (int s = 1; s < kStats; ++s) f = k / LANES == (uint32_t)s ? m[s] : f;
-          f = __shfl(f, (lane & ~(LANES - 1)) + (int)(k & (LANES - 1)), 64);
-          o += x[i] * (k < count ? f : 0.f);
+          const float f = __shfl(fs, from + (int)i, 64);
+          o += x[i] * (b0 + i < count ? f : 0.f);
         }
       }
       if (cc >= ncols || d >= p.hd) continue;
@@ -320,7 +320,7 @@ struct Plain {
 // some 8000 cycles. So the loads are what is arranged: the next tile's K is asked
 // for as soon as this one's scores are done, its V after this one's product, each
 // into the registers just freed, and page ids a tile ahead of that.
-template <typename T, int HDP, bool FULL, int D>
+template <typename T, int HDP, bool FULL>
 struct Tiled {
   static constexpr bool kF32 = std::is_same<T, float>::value, kQ8 = std::is_same<T, Q8>::value;
   static constexpr int kRows = kF32 ? 16 : 32, kSub = kRows / 16;
@@ -461,7 +461,7 @@ struct Tiled {
     };
     uint32_t b = p0 + wv * kRows;
     const bool any = b < p1;
-    Tile t[D];
+    Tile t;
     uint32_t id[kSub];
     f32x4 acc[NH * VD];
 #pragma unroll
@@ -477,15 +477,10 @@ struct Tiled {
         const bool in = n < ncols && (FULL || d < w.hd);
         x[i] = keep<f32x4>(*reinterpret_cast<const f32x4u*>(q + (FULL || d < w.hd ? d : 0)), in);
       }
-#pragma unroll
-      for (int i = 0; i < D; ++i) {
-        if (i == 0 || b + i * kStep < p1) {
-          locate(b + i * kStep, id);
-          load_k(w, k_at, g, t[i]);
-          load_v(w, v_hp, v_row, n, t[i]);
-        }
-        fetch(b + (i + 1) * kStep, id);
-      }
+      locate(b, id);
+      load_k(w, k_at, g, t);
+      load_v(w, v_hp, v_row, n, t);
+      fetch(b + kStep, id);
       float mul = a.scale * kLog2e;
       f16x8 q_hi[NQ], q_lo[NQ];
       if constexpr (!kF32) {
@@ -507,9 +502,10 @@ struct Tiled {
             q_lo[i][e] = (_Float16)(y - (float)q_hi[i][e]);
           }
       }
-      // One tile: its scores, then the K of the one D tiles on in its place, its part of
-      // the output, and the V of that; whether there is another tile.
-      auto step = [&](Tile& t, bool first) {
+      // A tile: its scores, then the next one's K in the place of its own, its part of
+      // the output, and the next one's V.
+      bool first = true;
+      do {
         // (Every chain of dependent matrix instructions is as short as it can be: hi and
         // lo apart, the two 16 rows in turn.)
         f32x4 sc[kSub], sl[kSub];
@@ -540,7 +536,7 @@ struct Tiled {
         }
 #pragma unroll
         for (int j = 0; j < kSub; ++j) sc[j] += sl[j];
-        const uint32_t nb = b + D * kStep;
+        const uint32_t nb = b + kStep;
         const bool more = nb < p1, tail = b + kRows > p1;
         if (more) {
           locate(nb, id);
@@ -634,13 +630,8 @@ struct Tiled {
         }
         if (more) load_v(w, v_hp, v_row, n, t);
         b += kStep;
-        return b < p1;
-      };
-      for (bool on = true, first = true; on; first = false) {
-#pragma unroll
-        for (int i = 0; i < D; ++i)
-          if (on) on = step(t[i], first && i == 0);
-      }
+        first = false;
+      } while (b < p1);
       l = swap_sum<32>(swap_sum<16>(l));
     }
     if (__any(no_page >= w.t.n_pages)) {
@@ -697,8 +688,12 @@ __global__ __launch_bounds__(256, WAVES) void paged_attn_kernel(PagedView w, Att
   };
   uint32_t rows = chunk(0), sum = wave_scan(units_of_rows(rows) * items), base = 0;
   uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
-  for (uint32_t s0 = 64; s0 < a.n; s0 += 64)
-    total += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(units_of_rows(chunk(s0)) * items), 63);
+  if (a.n > 64) {
+    uint32_t mine = 0;
+#pragma unroll 8
+    for (uint32_t s0 = 64; s0 < a.n; s0 += 64) mine += units_of_rows(chunk(s0));
+    total += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(mine * items), 63);
+  }
   const auto divide = [](uint32_t x, uint32_t y) { return quotient(x, y, __builtin_amdgcn_rcpf((float)y)); };
   const Cut cut = cut_units(total, a.most, a.few, a.slots, divide);
   const uint32_t per = cut.per, in_slot = cut.in_slot, slot = slot_of(blockIdx.x, a.slots);
@@ -719,10 +714,17 @@ __global__ __launch_bounds__(256, WAVES) void paged_attn_kernel(PagedView w, Att
     const Partials pt(a, w.hd);
     walk_units(
         s0 + at0, start - before, start, end, items,
+        [&](uint32_t s) -> uint32_t { return (uint32_t)__builtin_amdgcn_readlane((int)rows, (int)(s - s0)); },
         [&](uint32_t s) -> uint32_t {
-          const uint32_t n = s - s0 < 64 ? (uint32_t)__builtin_amdgcn_readlane((int)rows, (int)(s - s0))
-                                         : rows_of_len(w, a, a.lens[s]);
-          return n == kRefused ? 0 : n;
+          for (;;) {
+            if (s - s0 >= 64) {
+              s0 = s;
+              rows = chunk(s0);
+            }
+            const uint64_t live = __ballot(units_of_rows(rows) != 0) >> (s - s0);
+            if (live) return s + (uint32_t)__builtin_ctzll(live);
+            s = s0 + 64;
+          }
         },
         [&](uint32_t s, uint32_t n, uint32_t item, uint32_t u0, uint32_t u1, uint32_t at) {
           const uint32_t units = units_of(n), first = at - u0;
@@ -795,11 +797,11 @@ size_t tile_bytes(const rv_paged* pg) {
 // or if one is what is resident. f16, 128 wide, us at 256 | 512 ranges: 64 sequences of
 // up to 16000 rows 191 | 198, but 128 of 300 21.2 | 18.4; Q8_0, 32 of up to 8192: 50.6 |
 // 39.3; f16, 64 wide, 64 of up to 8000: 120 | 116. With more some wait for others to end.
-// Where the XCDs are not known apart an item has at most kMostPieces.
+// Where the XCDs are not known apart, an item has at most kMostPieces.
 void set_ranges(const rv_paged* pg, size_t items, size_t units, AttnArgs& a) {
   const bool wide = pg->head_dim > 128;
-  a.slots = pg->xcd_ok ? 3 : 0;
-  a.most = a.slots == 0 ? 6 : wide ? 8 : 9;
+  a.slots = pg->xcd_ok && pg->tune_join != 2 ? 3 : 0;
+  a.most = a.slots == 0 ? 5 : wide ? 8 : 9;
   while (a.most > 3 && units <= ((size_t)1 << a.most) / 2) --a.most;  // (never so many units)
   a.few = a.most == 9 && tile_bytes(pg) >= 16384 && items <= (size_t)kCUs ? 8 : a.most;
 }
@@ -812,7 +814,7 @@ size_t items_per_seq(const rv_paged* pg, size_t n_q) {
 template <typename T>
 void launch_attn(const PagedView& w, const AttnArgs& a, dim3 grid, hipStream_t s) {
 #define RV_TILED(HDP, FULL, WAVES) \
-  hipLaunchKernelGGL((paged_attn_kernel<Tiled<T, HDP, FULL, 1>, WAVES>), grid, dim3(256), 0, s, w, a)
+  hipLaunchKernelGGL((paged_attn_kernel<Tiled<T, HDP, FULL>, WAVES>), grid, dim3(256), 0, s, w, a)
   if (!tiled(w.hd))
     hipLaunchKernelGGL((paged_attn_kernel<Plain<T>, 1>), grid, dim3(256), 0, s, w, a);
   else if (w.hd == 64)
@@ -836,7 +838,7 @@ PagedAttnPlan paged_attn_plan(const rv_paged* pg, const rv_page_table& t, size_t
   PagedAttnPlan p;
   const size_t items = n * items_per_seq(pg, n_q), rows = t.pages * pg->page_rows;
   const size_t cols = cols_of((int)pg->head_dim, (int)(n_q / pg->n_kv_heads));
-  p.units = items * ((rows + kUnitRows - 1) / kUnitRows);  // (both below 2^42: no overflow that matters below)
+  if (__builtin_mul_overflow(items, (rows + kUnitRows - 1) / kUnitRows, &p.units)) p.units = SIZE_MAX;
   p.ws_bytes = (size_t)2 * (kMaxRanges + kGroups) * cols * (pg->head_dim + 2) * sizeof(float);
   p.ticket_bytes = (2 * kGroups + items) * sizeof(unsigned);
   return p;

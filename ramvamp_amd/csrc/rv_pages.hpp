@@ -75,12 +75,6 @@ RV_HD uint32_t quotient(uint32_t x, uint32_t y, float reciprocal_y) {
   return q;
 }
 
-template <typename I>
-RV_HD I units_per_range(I total, I ranges) {
-  const I per = (total + ranges - 1) / ranges;
-  return per > 1 ? per : 1;
-}
-
 // Which of its range's two partials a cut item's piece is kept in: the first when
 // it opens the range (the item may have begun before), else the second (it runs on
 // past the range's end).
@@ -98,15 +92,15 @@ struct PlainQuotient {
 
 // Walks the units [start, end), the first of which is unit `off` of sequence s:
 // visit(sequence, its rows, item, first unit, last unit + 1 of the item, the first
-// unit's place in the line).
-template <typename I, typename Rows, typename Visit, typename Quotient = PlainQuotient>
-RV_HD void walk_units(uint32_t s, I off, I start, I end, I items, Rows rows_of, Visit visit,
+// unit's place in the line). next_of(s): the first sequence from s on that has rows.
+template <typename I, typename Rows, typename Next, typename Visit, typename Quotient = PlainQuotient>
+RV_HD void walk_units(uint32_t s, I off, I start, I end, I items, Rows rows_of, Next next_of, Visit visit,
                       Quotient divide = Quotient()) {
   for (I at = start; at < end;) {
     const I rows = rows_of(s), units = units_of(rows);
     if (off >= units * items) {
       off -= units * items;
-      ++s;
+      s = next_of(s + 1);
       continue;
     }
     const I item = divide(off, units), u0 = off - item * units;

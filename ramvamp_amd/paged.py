@@ -222,6 +222,12 @@ class PagedKvCache:
             if fn(self._h, *args, self._err_ref):
                 _check(self._err.code, self._err)
 
+    def set_tuning(self, knob: int, value: int):
+        """rv_paged_set_tuning: ``RV_TUNE_PAGED_JOIN``, 0 or 2."""
+        with self._lock:
+            if self._lib.rv_paged_set_tuning(self._h, knob, value, self._err_ref):
+                _check(self._err.code, self._err)
+
     def synchronize(self):
         self._call(self._lib.rv_paged_synchronize)
 

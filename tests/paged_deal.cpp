@@ -28,7 +28,7 @@ using namespace rv;
 static void deal(const std::vector<long>& rows, long items, long ranges) {
   std::vector<long> before(rows.size() + 1, 0);
   for (size_t s = 0; s < rows.size(); ++s) before[s + 1] = before[s] + units_of(rows[s]) * items;
-  const long total = before.back(), per = units_per_range(total, ranges);
+  const long total = before.back(), per = std::max((total + ranges - 1) / ranges, 1l);
   CHECK(per * ranges >= total, "units left over");
   std::vector<int> seen(total, 0);
   std::map<std::pair<long, int>, std::pair<size_t, long>> kept;  // (range, partial) -> (sequence, item)
@@ -38,6 +38,10 @@ static void deal(const std::vector<long>& rows, long items, long ranges) {
     size_t s = 0;
     while (!(start >= before[s] && start < before[s + 1])) ++s;
     walk_units((uint32_t)s, start - before[s], start, end, items, [&](uint32_t i) { return rows[i]; },
+               [&](uint32_t i) {
+                 while (units_of(rows[i]) == 0) ++i;
+                 return i;
+               },
                [&](uint32_t i, long n, long item, long u0, long u1, long at) {
                  CHECK(n == rows[i] && item >= 0 && item < items, "sequence %u item %ld", i, item);
                  CHECK(u0 < u1 && u1 <= units_of(n), "units %ld..%ld", u0, u1);

@@ -393,6 +393,64 @@ def test_many_ragged_sequences(elem):
 
 
 @pytest.mark.parametrize("elem", ["f16", "f32", "q8_0"])
+@pytest.mark.parametrize("n_kv,group,hd,page,lens", [
+    (4, 8, 128, 64, [9000, 1, 300]), (1, 4, 128, 64, [40000]), (2, 17, 64, 16, [5000, 70]), (1, 2, 192, 16, [6000]),
+    (1, 2, 512, 16, [700, 90])])
+def test_joins_across_xcds_alone(elem, n_kv, group, hd, page, lens):
+    """The joins of a device that does not deal workgroups to its XCDs in turn."""
+    torch = torch_cuda()
+    say(f"case joins {(elem, n_kv, group, hd, lens)}")
+    rng = np.random.default_rng(hd + lens[0])
+    c, table, own = filled(rng, elem, n_kv, hd, page, lens)
+    q = rng.standard_normal((len(lens), n_kv * group * hd)).astype(np.float32)
+    want, a, vmax = expect(q, own, n_kv, hd)
+    got = []
+    for join in (2, 0, 2):
+        c.set_tuning(rv.RV_TUNE_PAGED_JOIN, join)
+        out = torch.full(q.shape, 9.0, device="cuda")
+        rv.paged_attention(dev(q), c, 1, ints(table), ints(lens), scale_of(hd), out)
+        got.append(host(out))
+        for i in range(len(lens)):
+            check(got[-1][i], want[i], a, vmax, f"join {join} sequence {i}")
+    assert np.array_equal(got[0].view(np.uint32), got[2].view(np.uint32))
+    with pytest.raises(rv.RamvampError):
+        c.set_tuning(2, 0)
+
+
+@pytest.mark.parametrize("hd", [64, 20])
+def test_mostly_empty_batches(hd):
+    """Few sequences with rows between many without, refused ones among those."""
+    torch = torch_cuda()
+    say(f"case mostly empty {hd}")
+    rng = np.random.default_rng(13)
+    n, n_kv, group = 1500, 2, 4
+    for live in ([0], [1499], [63, 64], [5, 128, 700, 1100, 1498], []):
+        lens = np.zeros(n, int)
+        lens[live] = rng.integers(1, 700, len(live))
+        refused = [i for i in (2, 66, 900, 1497) if i not in live]
+        c, table, own = filled(rng, "f16", n_kv, hd, 16, lens[live] if live else [1], junk=False)
+        wide = np.full((n, table.shape[1]), -7)
+        wide[live] = table[:len(live)]
+        asked = lens.copy()
+        asked[refused] = -3
+        q = rng.standard_normal((n, n_kv * group * hd)).astype(np.float32)
+        out = torch.full(q.shape, 9.0, device="cuda")
+        rv.paged_attention(dev(q), c, 1, ints(wide), ints(asked), scale_of(hd), out)
+        with pytest.raises(rv.KvError) as e:
+            c.device_status()
+        assert e.value.variant == "PositionOutOfTable"
+        got = host(out)
+        assert np.isnan(got[refused]).all()
+        if live:
+            want, a, vmax = expect(q[live], own, n_kv, hd)
+            for j, i in enumerate(live):
+                check(got[i], want[j], a, vmax, f"sequence {i}")
+        rest = np.ones(n, bool)
+        rest[live] = rest[refused] = False
+        assert not got[rest].any()
+
+
+@pytest.mark.parametrize("elem", ["f16", "f32", "q8_0"])
 @pytest.mark.parametrize("hd", [128, 20])
 def test_long_split_keeps_small_weights(elem, hd):
     """A first row far above the rest, whose weights are small and many: each counts."""
@@ -705,6 +763,95 @@ def test_captured_step_follows_positions_and_tables(elem):
         assert np.array_equal(a, b, equal_nan=True)
 
 
+def test_graphs_over_one_cache_in_turn_while_its_workspace_grows():
+    """Two captured batches, replayed alternately; then larger eager calls, which take
+    new workspaces, and the graphs again."""
+    torch = torch_cuda()
+    say("case two graphs")
+    rng = np.random.default_rng(51)
+    lens = [9000, 700, 40, 3, 0]
+    c, table, own = filled(rng, "f16", 2, 128, 16, lens)
+    q = rng.standard_normal((5, 2 * 4 * 128)).astype(np.float32)
+    t, n, qd = ints(table), ints(lens), dev(q)
+    outs, graphs = [torch.empty(5, 1024, device="cuda") for _ in range(2)], []
+    want, a, vmax = expect(q, own, 2, 128)
+    torch.cuda.synchronize()
+    call = lambda o, k: rv.paged_attention(qd[:k], c, 1, t[:k], n[:k], scale_of(128), o[:k])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(outs[0], 5)
+    torch.cuda.current_stream().wait_stream(side)
+    for o, k in zip(outs, (5, 1)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(o, k)
+        graphs.append(g)
+    for rep in range(4):
+        for o in outs:
+            o.fill_(float("nan"))
+        for g in graphs:
+            g.replay()
+        if rep:
+            # Sixteen heads a kv head, then a batch ten times as large.
+            big = dev(rng.standard_normal((5, 2 * 16 * 128)))
+            rv.paged_attention(big, c, 1, t, n, scale_of(128), torch.empty_like(big))
+            many = ints(np.tile(table, (10 * rep, 1)))
+            wide = qd.repeat(10 * rep, 1)
+            o2 = rv.paged_attention(wide, c, 1, many, n.repeat(10 * rep), scale_of(128), torch.empty_like(wide))
+            for i in range(50 * rep):
+                check(host(o2)[i], want[i % 5], a, vmax, f"batch {i}")
+        for i in range(5):
+            check(host(outs[0])[i], want[i], a, vmax, f"replay {rep} sequence {i}")
+        check(host(outs[1])[0], want[0], a, vmax, f"replay {rep} of one")
+        assert torch.isnan(outs[1][1:]).all()
+
+
+def test_rows_of_one_call_that_name_one_place():
+    """Of two rows for one place it holds values of both; no other place changes."""
+    say("case one place twice")
+    rng = np.random.default_rng(52)
+    c = rv.PagedKvCache(1, 2, 64, 2, 8, "f16")
+    k, v = rows(rng, 6, 128), rows(rng, 6, 128)
+    at = [3, 3, 3, 4, 3, 3]
+    c.append_rows(0, dev(k), dev(v), ints([[1]]), ints(at), ints([0] * 6))
+    (gk, gv) = (host(x) for x in c.read_rows(0, ints([[1]]), ints(range(8)), ints([0] * 8)))
+    for got, x in ((gk, k), (gv, v)):
+        x = x.astype(np.float16)
+        assert np.array_equal(got[4], x[3]) and not got[[0, 1, 2, 5, 6, 7]].any()
+        assert np.all(np.any(got[3] == x[[0, 1, 2, 4, 5]], axis=0))
+    kp, _ = c.read_rows(0, ints([[0]]), ints(range(8)), ints([0] * 8))
+    assert not host(kp).any()
+
+
+def test_step_of_a_large_padded_batch():
+    """More sequences than a wave has lanes, a third of them padding, into strided out."""
+    torch = torch_cuda()
+    say("case large step")
+    rng = np.random.default_rng(53)
+    n, n_kv, group, hd = 150, 2, 4, 64
+    lens = rng.integers(0, 200, n)
+    off = rng.random(n) < 0.3
+    c, table, own = filled(rng, "q8_0", n_kv, hd, 16, lens, extra=1)
+    q, k, v, _ = step_inputs(rng, n, n_kv, group, hd)
+    wide = torch.full((n, q.shape[1] + 8), 9.0, device="cuda")
+    out = wide[:, 4:4 + q.shape[1]]
+    rv.paged_decode_step(c, 1, dev(q), dev(k), dev(v), None, None, EPS, None, ints(table), ints(np.where(off, -1, lens)),
+                         scale_of(hd), out)
+    c.device_status()
+    new = [(np.concatenate([o[0], stored(k[i:i + 1], "q8_0")]), np.concatenate([o[1], stored(v[i:i + 1], "q8_0")]))
+           for i, o in enumerate(own)]
+    want, a, vmax = expect(q, new, n_kv, hd)
+    got = host(out)
+    for i in range(n):
+        if off[i]:
+            assert not got[i].any()
+        else:
+            check(got[i], want[i], a, vmax, f"sequence {i}")
+    w = host(wide)
+    assert np.all(w[:, :4] == 9) and np.all(w[:, -4:] == 9)
+
+
 def test_a_captured_call_that_would_allocate_is_refused():
     torch = torch_cuda()
     say("case capture refused")
@@ -817,6 +964,16 @@ def test_host_refusals():
         with pytest.raises(rv.RamvampError) as e:
             call()
         assert e.value.variant == variant
+    with pytest.raises(rv.DeviceError):
+        rv.PagedKvCache(1, 2, 64, 4, 16, "f16", device=torch.cuda.device_count())
+    with pytest.raises(rv.DeviceError):
+        rv.PagedKvCache(1, 64, 128, 2 ** 20, 1024, "f32")  # 64 TiB
+    # 2^21 pages of 1024 rows for each of 128 kv heads: 2^31 units.
+    many = rv.PagedKvCache(1, 128, 8, 1, 1024, "f16")
+    with pytest.raises(rv.RamvampError) as e:
+        rv.paged_attention(f(1, 1024), many, 0, torch.zeros(1, 2 ** 21, dtype=torch.int32, device="cuda"), ints([1]), 1.0,
+                           f(1, 1024))
+    assert e.value.variant == "Unsupported"
     for call in [
             lambda: rv.paged_attention(f(2, 256).double(), c, 0, t, one, 1.0, out),
             lambda: rv.paged_attention(f(256, 2).T, c, 0, t, one, 1.0, out),

@@ -3,6 +3,7 @@ kernels' integer arithmetic (tests/paged_deal.cpp), without a GPU."""
 import ctypes
 import math
 import os
+import re
 import subprocess
 
 import numpy as np
@@ -10,6 +11,7 @@ import pytest
 
 import ramvamp_amd as rv
 from ramvamp_amd import _lib as L
+from ramvamp_amd import build as B
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 
@@ -20,6 +22,45 @@ def test_dealing_and_places_on_the_host(tmp_path):
                     "-std=c++17", "-o", exe, os.path.join(HERE, "paged_deal.cpp")], check=True, capture_output=True)
     out = subprocess.run([exe], capture_output=True, text=True, timeout=100)
     assert out.returncode == 0 and not out.stdout, out.stdout
+
+
+def partial_saves(asm):
+    """Labels of blocks that save vector registers before they restore the exec mask
+    there: of the lanes that went another way the copy holds nothing, yet it is read
+    back for all of them."""
+    found = []
+    for body in re.findall(r"^_Z\S+:\s.*?\.Lfunc_end", asm, re.M | re.S):
+        loops = set(re.findall(r"s_cbranch_execnz (\.LBB\d+_\d+)", body))
+        lines = [l.strip() for l in body.splitlines()]
+        for i, l in enumerate(lines):
+            if not re.match(r"\.LBB\d+_\d+:", l) or l.split(":")[0] in loops:
+                continue
+            saves = False
+            for t in lines[i + 1:i + 40]:
+                if t.startswith(("s_or_b64 exec", "s_or_saveexec", "s_andn2_saveexec")):
+                    if saves:
+                        found.append(l.split(":")[0])
+                    break
+                if re.match(r"s_cbranch|s_branch|\.LBB|s_and_saveexec|s_endpgm", t):
+                    break
+                saves |= t.startswith(("v_accvgpr", "scratch_", "buffer_"))
+    return found
+
+
+def test_no_register_is_saved_under_a_partial_mask(tmp_path):
+    """The attention kernels keep whole tiles in registers, more than 256 with the
+    widest heads, and every value has to be kept for every lane."""
+    planted = ("_Zk: ; @k\n s_and_saveexec_b64 s[0:1], vcc\n s_cbranch_execz .LBB0_2\n; %bb.1:\n v_mov_b32_e32 v1, 0\n"
+               ".LBB0_2:\n{} s_or_b64 exec, exec, s[0:1]\n s_endpgm\n.Lfunc_end0:\n")
+    assert partial_saves(planted.format(" v_accvgpr_write_b32 a0, v0\n")) == [".LBB0_2"]
+    assert not partial_saves(planted.format(""))
+    out = str(tmp_path / "attn.s")
+    subprocess.run([B.HIPCC, *B.FLAGS, "--offload-device-only", "-S", "-o", out,
+                    os.path.join(os.path.dirname(HERE), "ramvamp_amd", "csrc", "rv_paged_attn.hip")], check=True,
+                   capture_output=True)
+    with open(out) as f:
+        asm = f.read()
+    assert asm.count("paged_attn_kernel") > 20 and not partial_saves(asm)
 
 
 def frequencies(d, theta, scaling, factor, trained, fast=32.0, slow=1.0):
@@ -135,8 +176,8 @@ def test_projected_bytes():
     ((1, 4, 128, 8, 4, "f16"), "InvalidDims"), ((1, 4, 128, 8, 48, "f16"), "InvalidDims"),
     ((1, 4, 128, 8, 2048, "f16"), "InvalidDims"), ((1, 4, 100, 8, 64, "q8_0"), "InvalidDims"),
     ((1, 4, 513, 8, 64, "f32"), "Unsupported"), ((1, 4, 128, 2 ** 31, 64, "f16"), "Unsupported"),
-    ((1, 2 ** 31, 128, 8, 64, "f16"), "Unsupported"), ((2 ** 60, 4, 128, 8, 64, "f16"), "InvalidDims"),
-    ((2 ** 20, 2 ** 20, 128, 2 ** 30, 1024, "f32"), "InvalidDims"),
+    ((1, 2 ** 31, 128, 8, 64, "f16"), "Unsupported"), ((1, 65536, 1, 8, 64, "f16"), "Unsupported"), ((2 ** 60, 4, 128, 8, 64, "f16"), "InvalidDims"),
+    ((2 ** 30, 65535, 128, 2 ** 30, 1024, "f32"), "InvalidDims"),
 ])
 def test_geometry_refusals(args, variant):
     for call in (rv.PagedKvCache.projected_bytes, rv.PagedKvCache):
@@ -155,7 +196,7 @@ def test_calls_without_a_cache():
     assert lib.rv_paged_decode_step(None, 0, None, None, 0, None, 0, None, 0, 0, 0, None, 0, None, 0, 0.0, b, None, 1.0,
                                     None, 0, 0, e) == 32
     assert lib.rv_paged_set_stream(None, None, e) == lib.rv_paged_synchronize(None, e) == 32
-    assert lib.rv_paged_device_status(None, e) == 32
+    assert lib.rv_paged_device_status(None, e) == lib.rv_paged_set_tuning(None, 1, 2, e) == 32
     lib.rv_paged_free(None)
     lib.rv_rope_free(None)
 
