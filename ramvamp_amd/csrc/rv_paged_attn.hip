@@ -303,7 +303,9 @@ struct Plain {
 
 // Heads of whole 16-byte pieces, up to 256 wide (padded to HDP): up to 16 query
 // heads of one kv head are the 16 columns of matrix instructions, a wave takes
-// kRows rows at a time and every fourth such tile of its segment.
+// kRows rows at a time and every fourth such tile of its segment (16 rows of f32, and
+// where 32 of 256 values would leave registers for one wave a SIMD only: f16, 128
+// sequences of 300 45.4 -> 41.0 us; Q8_0, 32 of up to 4000 57.7 -> 53.5).
 //
 // Scores: S[row][column] = K (A operand: a row a lane, 16 bytes of it straight from
 // memory) times q (B operand, in registers for the whole segment). f16 and Q8_0
@@ -323,7 +325,7 @@ struct Plain {
 template <typename T, int HDP, bool FULL>
 struct Tiled {
   static constexpr bool kF32 = std::is_same<T, float>::value, kQ8 = std::is_same<T, Q8>::value;
-  static constexpr int kRows = kF32 ? 16 : 32, kSub = kRows / 16;
+  static constexpr int kRows = kF32 || (HDP == 256 && FULL) ? 16 : 32, kSub = kRows / 16;
   static constexpr int kStep = 4 * kRows;  // from one of a wave's tiles to its next
   static constexpr int VD = kF32 || HDP == 64 ? 4 : 8;  // values of a row of V a lane loads together
   static constexpr int NH = HDP / (16 * VD);
@@ -336,6 +338,13 @@ struct Tiled {
   typedef std::conditional_t<kF32, f32x4,
                              std::conditional_t<kQ8, std::conditional_t<VD == 8, u32x2, uint32_t>,
                                                 std::conditional_t<VD == 8, f16x8, f16x4>>> VReg;
+  typedef std::conditional_t<kSub == 2, f16x8, f16x4> PReg;  // a lane's rows of one column of P, or of V
+  static __device__ __forceinline__ f32x4 weigh(PReg p, PReg v, f32x4 c) {
+    if constexpr (kSub == 2)
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(p, v, c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x16f16(p, v, c, 0, 0, 0);
+  }
   struct Shared {
     __attribute__((aligned(16))) float o[4][16][HDP + 4];
     float m[4][16], l[4][16];
@@ -592,17 +601,17 @@ struct Tiled {
                 acc[4 * hh + e] =
                     __builtin_amdgcn_mfma_f32_16x16x4f32(p[r], t.v[r][hh][e], acc[4 * hh + e], 0, 0, 0);
         } else {
-          f16x8 p_hi, p_lo;
+          PReg p_hi, p_lo;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+          for (int i = 0; i < 4 * kSub; ++i) {
             p_hi[i] = (_Float16)p[i];
             p_lo[i] = (_Float16)(p[i] - (float)p_hi[i]);
           }
 #pragma unroll
           for (int hh = 0; hh < NH; ++hh) {
-            _Float16 v[8][VD];
+            _Float16 v[4 * kSub][VD];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 4 * kSub; ++i) {
               if constexpr (kQ8) {
                 const _Float16 vs = t.vs[i >> 2][hh][i & 3];
                 f16x2 c[VD / 2];
@@ -621,10 +630,12 @@ struct Tiled {
             }
 #pragma unroll
             for (int e = 0; e < VD; ++e) {
-              const f16x8 o = {v[0][e], v[1][e], v[2][e], v[3][e], v[4][e], v[5][e], v[6][e], v[7][e]};
+              PReg o;
+#pragma unroll
+              for (int i = 0; i < 4 * kSub; ++i) o[i] = v[i][e];
               f32x4& c = acc[VD * hh + e];
-              c = __builtin_amdgcn_mfma_f32_16x16x32_f16(p_lo, o, c, 0, 0, 0);
-              c = __builtin_amdgcn_mfma_f32_16x16x32_f16(p_hi, o, c, 0, 0, 0);
+              c = weigh(p_lo, o, c);
+              c = weigh(p_hi, o, c);
             }
           }
         }
@@ -786,24 +797,22 @@ bool tiled(int hd) { return hd % 8 == 0 && hd <= 256; }
 
 int cols_of(int hd, int group) { return tiled(hd) ? std::min(group, 16) : 1; }
 
-// Bytes of K and V that a wave has in flight.
-size_t tile_bytes(const rv_paged* pg) {
-  const size_t wide = pg->head_dim <= 64 ? 64 : pg->head_dim <= 128 ? 128 : 256;
-  return 2 * wide * (pg->elem == RV_ELEM_F32 ? 64 : pg->elem == RV_ELEM_F16 ? 64 : 34);
-}
-
-// log2 of the ranges the work is cut into: two a CU (what is resident), and where it
-// is long one a CU if a wave's tile is 16 KiB and the items are no more than the CUs,
-// or if one is what is resident. f16, 128 wide, us at 256 | 512 ranges: 64 sequences of
-// up to 16000 rows 191 | 198, but 128 of 300 21.2 | 18.4; Q8_0, 32 of up to 8192: 50.6 |
-// 39.3; f16, 64 wide, 64 of up to 8000: 120 | 116. With more some wait for others to end.
-// Where the XCDs are not known apart, an item has at most kMostPieces.
+// log2 of the ranges the work is cut into: two a CU (what is resident), or one where
+// the registers hold one (f32 256 wide, and widths between 128 and 256). Long f16 work
+// above 64 wide takes one a CU where the items are no more than the CUs: with more,
+// some wait for others to end. us at 256 | 512 ranges: f16, 128 wide, 64 sequences of up
+// to 16000 rows 191 | 198, but 128 of 300 21.2 | 18.4; f16, 256 wide, 32 of up to 4000
+// 81.6 | 87.4; not of f16 64 wide, 64 of up to 8000 120 | 116; Q8_0 128 wide, 32 of up to
+// 8192 50.6 | 39.3; Q8_0 256 wide, 32 of up to 4000 55.9 | 53.5; f32 128 wide, 64 of up to
+// 4000 116 | 105.6 (of up to 16000 376 | 387). Where the XCDs are not known apart, an
+// item has at most kMostPieces.
 void set_ranges(const rv_paged* pg, size_t items, size_t units, AttnArgs& a) {
-  const bool wide = pg->head_dim > 128;
+  const bool f16 = pg->elem == RV_ELEM_F16;
+  const bool wide = pg->head_dim > 128 && (pg->head_dim != 256 || pg->elem == RV_ELEM_F32);
   a.slots = pg->xcd_ok && pg->tune_join != 2 ? 3 : 0;
   a.most = a.slots == 0 ? 5 : wide ? 8 : 9;
   while (a.most > 3 && units <= ((size_t)1 << a.most) / 2) --a.most;  // (never so many units)
-  a.few = a.most == 9 && tile_bytes(pg) >= 16384 && items <= (size_t)kCUs ? 8 : a.most;
+  a.few = a.most == 9 && f16 && pg->head_dim > 64 && items <= (size_t)kCUs ? 8 : a.most;
 }
 
 size_t items_per_seq(const rv_paged* pg, size_t n_q) {
@@ -826,7 +835,7 @@ void launch_attn(const PagedView& w, const AttnArgs& a, dim3 grid, hipStream_t s
   else if (w.hd < 128)
     RV_TILED(128, false, 2);
   else if (w.hd == 256)
-    RV_TILED(256, true, 1);
+    RV_TILED(256, true, (std::is_same<T, float>::value ? 1 : 2));
   else
     RV_TILED(256, false, 1);
 #undef RV_TILED
