@@ -17,6 +17,12 @@
 // some 12 bytes a cycle, loads from its L2 several times that), and else, and across
 // groups, they are stored and loaded at device scope, since the XCDs' L2s do not see
 // each other's lines. Partials are counted by tickets that are zero between calls.
+//
+// Bound by the pages' bytes where there are many: f16, 32 query heads over 4 of 128, 64
+// sequences of up to 16000 rows 188 us, 6.6 TB/s (a streaming read's rate); one of 131000
+// 47, 5.7 TB/s. Q8_0 is bound by issue (32 of up to 8192 rows 39 us, 3.7 TB/s, vector
+// instructions 54 % of the cycles); few rows by one phase after the other: 100 rows 5.8,
+// 4096 11.5 us, a third of it the joins.
 #include "rv_paged.hpp"
 
 #include <algorithm>
@@ -78,7 +84,7 @@ struct Partials {
   int cols, hd;
   __device__ __forceinline__ Partials(const AttnArgs& a, int hd_)
       : rs(__builtin_amdgcn_make_buffer_rsrc(a.part, (short)0, (int)a.part_bytes, 0x00020000)), cols(a.cols), hd(hd_) {}
-  // Byte offset of a partial (2 * range + which; the slots' behind them); of column
+  // Byte offset of a partial (2 * range + which; the groups' behind them); of column
   // c's (maximum, sum) in it.
   __device__ __forceinline__ uint32_t at(uint32_t i) const { return i * (uint32_t)(cols * (hd + 2)) * 4u; }
   __device__ __forceinline__ uint32_t stat(int c) const { return (uint32_t)(cols * hd + 2 * c) * 4u; }
@@ -222,8 +228,11 @@ __device__ __forceinline__ float paged_value(const PagedView& w, bool is_v, size
   }
 }
 
-// Any head width: one query head an item, a wave one position at a time, the
-// head's values over its lanes.
+// Any head width: one query head an item, a wave four rows at a time, the head's
+// values over its lanes, so that a row is read again for every query head of its
+// group: for the widths that tiles do not take. 16 sequences of 2000
+// f16 rows, 4 kv heads of 8 query heads of 100: 182 us (791 a row at a time; 22 the
+// tiles at 104).
 template <typename T>
 struct Plain {
   static constexpr int kPer = kMaxHalf * 2 / 64;
@@ -249,30 +258,48 @@ struct Plain {
       o[j] = 0.f;
     }
     float m = -INFINITY, l = 0.f;
-    for (uint32_t p = p0 + wv; p < p1; p += 4) {
-      uint32_t page = (uint32_t)w.t.ids[(long)s * w.t.stride + (p >> w.t.shift)];
+    // Four rows of one page at a time; past the last row it again, without weight.
+    for (uint32_t b = p0 + 4 * wv; b < p1; b += 16) {
+      const uint32_t page = (uint32_t)w.t.ids[(long)s * w.t.stride + (b >> w.t.shift)];
       if (page >= w.t.n_pages) {
         if (lane == 0) paged_refuse(w, RV_PAGED_PAGE_OUT_OF_RANGE, s, page, w.t.n_pages);
         l = NAN;
         continue;
       }
       const size_t hp = (size_t)page * w.n_kv + h;
-      const uint32_t row = p & ((1u << w.t.shift) - 1);
-      float dot = 0.f;
+      const uint32_t mask = (1u << w.t.shift) - 1;
+      uint32_t row[4];
+      float y[4] = {}, v[4][kPer];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) row[r] = min(b + r, p1 - 1) & mask;
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
-        const int d = lane + 64 * j;
-        if (d < w.hd) dot += x[j] * paged_value<T>(w, false, hp, row, d);
+        if (64 * j >= w.hd) break;
+        const int d = min(lane + 64 * j, w.hd - 1);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          y[r] += x[j] * paged_value<T>(w, false, hp, row[r], d);
+          v[r][j] = paged_value<T>(w, true, hp, row[r], d);
+        }
       }
-      dot = swap_sum<32>(swap_sum<16>(group_sum<16>(dot)));
-      const float y = dot * scale, mn = fmaxf(m, y);
-      const float c = mn == -INFINITY ? 1.f : exp2f(m - mn), e = mn == -INFINITY ? 0.f : exp2f(y - mn);
-      m = mn;
-      l = l * c + e;
+      float mn = m;
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const int d = lane + 64 * j;
-        if (d < w.hd) o[j] = o[j] * c + e * paged_value<T>(w, true, hp, row, d);
+      for (int r = 0; r < 4; ++r) {
+        y[r] = b + r < p1 ? swap_sum<32>(swap_sum<16>(group_sum<16>(y[r]))) * scale : -INFINITY;
+        mn = fmaxf(mn, y[r]);
+      }
+      const float c = mn == -INFINITY ? 1.f : exp2f(m - mn);
+      m = mn;
+      l *= c;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) o[j] *= c;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float e = y[r] == -INFINITY ? 0.f : exp2f(y[r] - mn);  // (NaN of a NaN)
+        l += e;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+          if (64 * j < w.hd) o[j] += e * v[r][j];
       }
     }
     __syncthreads();

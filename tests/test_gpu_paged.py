@@ -550,6 +550,31 @@ def test_a_nonfinite_row_stays_in_its_head_and_sequence():
 
 
 @pytest.mark.parametrize("elem", ["f16", "f32", "q8_0"])
+@pytest.mark.parametrize("hd", [128, 64, 20, 512])
+@pytest.mark.parametrize("n,at", [(1, 0), (200, 0), (200, 4), (200, 16), (200, 199), (6000, 3000)])
+def test_a_nan_anywhere_reaches_the_output(elem, hd, n, at):
+    """A row of NaN, the first that a wave sees or its last, in K or in V."""
+    torch = torch_cuda()
+    if elem == "q8_0" and hd % 32:
+        pytest.skip("Q8_0 rows are blocks of 32")
+    say(f"case NaN {(elem, hd, n, at)}")
+    rng = np.random.default_rng(n + at)
+    c, table, own = filled(rng, elem, 2, hd, 16, [n, 90])
+    q = rng.standard_normal((2, 4 * hd)).astype(np.float32)
+    row = np.full((1, 2 * hd), np.nan, np.float32)
+    row[:, hd:] = 1.0  # kv head 1 stays sound
+    for bad_k in (True, False):
+        fine = np.ones((1, 2 * hd), np.float32)
+        c.append_rows(1, dev(row if bad_k else fine), dev(fine if bad_k else row), ints(table), ints([at]), ints([0]))
+        out = torch.empty(2, 4 * hd, device="cuda")
+        rv.paged_attention(dev(q), c, 1, ints(table), ints([n, 90]), scale_of(hd), out)
+        got = host(out)
+        assert np.isnan(got[0, :2 * hd]).all() and np.isfinite(got[0, 2 * hd:]).all()
+        want, a, vmax = expect(q[1:], own[1:], 2, hd)
+        check(got[1], want[0], a, vmax, "the sequence beside it")
+
+
+@pytest.mark.parametrize("elem", ["f16", "f32", "q8_0"])
 @pytest.mark.parametrize("hd", [128, 32])
 def test_refused_sequences(elem, hd):
     """Bad pages and lengths: NaN for their sequence, recorded, the others as without them."""
