@@ -231,8 +231,8 @@ __device__ __forceinline__ float paged_value(const PagedView& w, bool is_v, size
 // Any head width: one query head an item, a wave four rows at a time, the head's
 // values over its lanes, so that a row is read again for every query head of its
 // group: for the widths that tiles do not take. 16 sequences of 2000
-// f16 rows, 4 kv heads of 8 query heads of 100: 182 us (791 a row at a time; 22 the
-// tiles at 104).
+// f16 rows, 4 kv heads of 8 query heads of 100: 232 us (791 a row at a time; 182 with
+// sums of f32; 20 the tiles at 104).
 template <typename T>
 struct Plain {
   static constexpr int kPer = kMaxHalf * 2 / 64;
@@ -250,14 +250,16 @@ struct Plain {
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const float* q = a.q + s * a.q_stride + (long)qh * w.hd;
     const float scale = a.scale * kLog2e;
-    float x[kPer], o[kPer];
+    float x[kPer];
+    double o[kPer];  // (in f32 many small weights behind a large one would be dropped)
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int d = lane + 64 * j;
       x[j] = d < w.hd ? q[d] : 0.f;
-      o[j] = 0.f;
+      o[j] = 0.0;
     }
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY;
+    double l = 0.0;
     // Four rows of one page at a time; past the last row it again, without weight.
     for (uint32_t b = p0 + 4 * wv; b < p1; b += 16) {
       const uint32_t page = (uint32_t)w.t.ids[(long)s * w.t.stride + (b >> w.t.shift)];
@@ -299,13 +301,13 @@ struct Plain {
         l += e;
 #pragma unroll
         for (int j = 0; j < kPer; ++j)
-          if (64 * j < w.hd) o[j] += e * v[r][j];
+          if (64 * j < w.hd) o[j] += (double)e * v[r][j];
       }
     }
     __syncthreads();
-    if (lane == 0) sh.m[wv] = m, sh.l[wv] = l;
+    if (lane == 0) sh.m[wv] = m, sh.l[wv] = (float)l;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) sh.o[wv][lane + 64 * j] = o[j];
+    for (int j = 0; j < kPer; ++j) sh.o[wv][lane + 64 * j] = (float)o[j];
     __syncthreads();
     bool here = false;
     const uint32_t part = whole ? 0 : where(here);
@@ -354,6 +356,11 @@ struct Tiled {
   static constexpr bool kF32 = std::is_same<T, float>::value, kQ8 = std::is_same<T, Q8>::value;
   static constexpr int kRows = kF32 || (HDP == 256 && FULL) ? 16 : 32, kSub = kRows / 16;
   static constexpr int kStep = 4 * kRows;  // from one of a wave's tiles to its next
+  // A sum of f32 drops what is below 2^-24 of it, the many small weights behind a large
+  // one whole: a wave's sums are put aside (in LDS) and begun again after so many tiles.
+  // So at most 2^-18 of the largest value is lost: a product's rows (32, 16, of f32 4)
+  // count down to 2^-25 together.
+  static constexpr uint32_t kAside = kF32 ? 32 : 64;
   static constexpr int VD = kF32 || HDP == 64 ? 4 : 8;  // values of a row of V a lane loads together
   static constexpr int NH = HDP / (16 * VD);
   static constexpr int NK = kF32 ? HDP / 16 : kQ8 ? HDP / 64 : HDP / 32;  // 16-byte loads of a row of K a lane
@@ -503,6 +510,29 @@ struct Tiled {
 #pragma unroll
     for (int i = 0; i < NH * VD; ++i) acc[i] = f32x4{};
     float m = -INFINITY, l = 0.f;
+    float m_aside = -INFINITY, l_aside = 0.f;
+    bool aside = false;
+    auto place = [&](int r, int i) { return reinterpret_cast<f32x4*>(&sh.o[wv][4 * g + r][16 * VD * (i / VD) + VD * n + i % VD]); };
+    auto put_aside = [&] {
+      const float c = m_aside == m ? 1.f : __builtin_amdgcn_exp2f(m_aside - m);
+      l_aside = l_aside * c + l;
+      m_aside = m;
+      l = 0.f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float f = __shfl(c, 4 * g + r, 64);
+#pragma unroll
+        for (int i = 0; i < NH * VD; i += 4) {
+          f32x4 x = {acc[i][r], acc[i + 1][r], acc[i + 2][r], acc[i + 3][r]};
+          if (aside) x += *place(r, i) * f;
+          *place(r, i) = x;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NH * VD; ++i) acc[i] = f32x4{};
+      aside = true;
+    };
+    if (p1 - p0 > kAside * kStep) __syncthreads();  // (the last segment's reads)
     if (any) {
       fetch(b, id);
       const float* q = a.q + s * a.q_stride + (long)(qh + min(n, ncols - 1)) * w.hd;
@@ -541,6 +571,7 @@ struct Tiled {
       // A tile: its scores, then the next one's K in the place of its own, its part of
       // the output, and the next one's V.
       bool first = true;
+      uint32_t left = kAside;
       do {
         // (Every chain of dependent matrix instructions is as short as it can be: hi and
         // lo apart, the two 16 rows in turn.)
@@ -599,12 +630,13 @@ struct Tiled {
             for (int i = 0; i < NH * VD; ++i) acc[i][r] *= f;
           }
         }
-        float p[4 * kSub];
+        float p[4 * kSub], lt[kSub];
 #pragma unroll
         for (int i = 0; i < 4 * kSub; ++i) {
           p[i] = __builtin_amdgcn_exp2f(y[i] - m + (kF32 ? 0.f : 15.f));
-          l += p[i];
+          lt[i >> 2] = i & 3 ? lt[i >> 2] + p[i] : p[i];
         }
+        l += kSub == 2 ? lt[0] + lt[kSub - 1] : lt[0];
         if (tail) {  // (what lies behind the last row may be anything)
 #pragma unroll
           for (int i = 0; i < 4 * kSub; ++i) {
@@ -669,7 +701,15 @@ struct Tiled {
         if (more) load_v(w, v_hp, v_row, n, t);
         b += kStep;
         first = false;
+        if (--left == 0 && b < p1) {
+          put_aside();
+          left = kAside;
+        }
       } while (b < p1);
+      if (aside) {
+        put_aside();
+        l = l_aside;
+      }
       l = swap_sum<32>(swap_sum<16>(l));
     }
     if (__any(no_page >= w.t.n_pages)) {
@@ -678,16 +718,15 @@ struct Tiled {
     }
     __syncthreads();  // (the last segment's reads)
     if (lane < 16) sh.m[wv][n] = m, sh.l[wv][n] = l;
+    if (!aside) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (4 * g + r < ncols) {
+      for (int r = 0; r < 4; ++r)
+        if (4 * g + r < ncols) {
 #pragma unroll
-        for (int hh = 0; hh < NH; ++hh)
-#pragma unroll
-          for (int e = 0; e < VD; e += 4)
-            *reinterpret_cast<f32x4*>(&sh.o[wv][4 * g + r][16 * VD * hh + VD * n + e]) =
-                f32x4{acc[VD * hh + e][r], acc[VD * hh + e + 1][r], acc[VD * hh + e + 2][r], acc[VD * hh + e + 3][r]};
-      }
+          for (int i = 0; i < NH * VD; i += 4)
+            *place(r, i) = f32x4{acc[i][r], acc[i + 1][r], acc[i + 2][r], acc[i + 3][r]};
+        }
+    }
     bool here = false;
     const uint32_t part = whole ? 0 : where(here);
     __syncthreads();

@@ -483,6 +483,39 @@ def test_long_split_keeps_small_weights(elem, hd):
 
 
 @pytest.mark.parametrize("elem", ["f16", "f32", "q8_0"])
+@pytest.mark.parametrize("hd", [64, 128, 256, 192, 20])
+def test_long_sums_keep_small_weights(elem, hd):
+    """As above where a workgroup has whole sequences: 300 over one's pages. Of the two kv
+    heads' values one has the first row apart, the other the rest."""
+    torch = torch_cuda()
+    if elem == "q8_0" and hd % 32:
+        pytest.skip("Q8_0 rows are blocks of 32")
+    say(f"case long sums {(elem, hd)}")
+    n, seqs = 130000, 300
+    c = rv.PagedKvCache(1, 2, hd, -(-n // 64), 64, elem)
+    k, v = torch.zeros(n, 2 * hd, device="cuda"), torch.ones(n, 2 * hd, device="cuda")
+    k[0, 0] = k[0, hd] = 1.0
+    v[0, :hd] = 0.0
+    v[1:, hd:] = 0.0
+    table = ints(np.random.default_rng(0).permutation(-(-n // 64))[None])
+    c.append_rows(0, k, v, table, ints(np.arange(n)), ints(np.zeros(n)))
+    gaps = np.array([24.5, 27.5, 29.5, 31.5]) * np.log(2)  # the first row's score above the others'
+    q = np.zeros((2, 4, hd), np.float32)
+    q[:, :, 0] = gaps / scale_of(hd)
+    q = np.tile(q.reshape(1, -1), (seqs, 1))
+    out = torch.empty(seqs, 8 * hd, device="cuda")
+    rv.paged_attention(dev(q), c, 0, table.repeat(seqs, 1), ints([n] * seqs), scale_of(hd), out)
+    one = stored(np.ones((1, 32), np.float32), elem)[0, 0].astype(np.float64)
+    first = one * np.float32(gaps / scale_of(hd)).astype(np.float64) * scale_of(hd)
+    rest = (n - 1) * np.exp(-first)
+    want = np.stack([one * rest / (1 + rest), one / (1 + rest)])
+    # The weights as in the test above, and check()'s 96 half steps of the largest value.
+    bound = rest / (1 + rest) * (2 * gaps + 1) * 2.0 ** -21 + 96 * EPS32
+    err = np.abs(host(out).reshape(seqs, 2, 4, hd) - want[None, :, :, None]).max((0, 3))
+    assert np.all(err <= bound), (err, bound)
+
+
+@pytest.mark.parametrize("elem", ["f16", "f32", "q8_0"])
 @pytest.mark.parametrize("mag", [1e-20, 1e-6, 1e6, 1e15])
 def test_queries_of_any_magnitude(elem, mag):
     """q times mag, the scale divided by it: the same output."""
