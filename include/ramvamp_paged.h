@@ -8,7 +8,7 @@
  * what it does they round as it does.
  *
  * Conventions of ramvamp_attn.h, and:
- *  - Tensor pointers are device pointers, 4-byte aligned, on the cache's
+ *  - Tensor pointers are device pointers, aligned to an element, on the cache's
  *    device; RV_HOST_PTRS is RV_ERR_UNSUPPORTED. Rows of f32 inputs and outputs
  *    may lie further apart than their width: `*_stride` is the elements from one
  *    row to the next, at least the width (RV_PRIM_LENGTH_MISMATCH, a = width,

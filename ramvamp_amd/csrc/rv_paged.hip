@@ -357,6 +357,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedView w, RopeArgs
 
 // ---- and back ----------------------------------------------------------------------
 
+typedef _Float16 f16x8u __attribute__((ext_vector_type(8), aligned(2)));  // a caller's rows
+
 // Eight values a thread of one plane (blockIdx.y: K, V), as attention reads them: f16
 // pages' 5734 rows of 4 heads of 128 7.1 us, 3.3 TB/s (the position and the page id come
 // first); one row 2.6.
@@ -391,16 +393,16 @@ __global__ __launch_bounds__(256) void paged_read_kernel(PagedView w, const int3
     f16x8 y;
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = (_Float16)(p[e >> 1][e & 1] * s);
-    *reinterpret_cast<f16x8*>(o) = y;
+    *reinterpret_cast<f16x8u*>(o) = y;
   } else {
     const O* p = reinterpret_cast<const O*>(base) + at * w.hd + d;
     const int n = min(8, w.hd - (int)d);
     if (w.hd % 8 == 0) {
       if constexpr (sizeof(O) == 4) {
-        *reinterpret_cast<f32x4*>(o) = *reinterpret_cast<const f32x4*>(p);
-        *reinterpret_cast<f32x4*>(o + 4) = *reinterpret_cast<const f32x4*>(p + 4);
+        *reinterpret_cast<f32x4u*>(o) = *reinterpret_cast<const f32x4*>(p);
+        *reinterpret_cast<f32x4u*>(o + 4) = *reinterpret_cast<const f32x4*>(p + 4);
       } else {
-        *reinterpret_cast<f16x8*>(o) = *reinterpret_cast<const f16x8*>(p);
+        *reinterpret_cast<f16x8u*>(o) = *reinterpret_cast<const f16x8*>(p);
       }
     } else {
       for (int e = 0; e < n; ++e) o[e] = p[e];

@@ -187,6 +187,32 @@ def test_rows_come_back_as_stored_and_nothing_else_changes(elem, n_kv, hd, page)
     assert np.array_equal(host(only).astype(np.float32), wv, equal_nan=True)
 
 
+@pytest.mark.parametrize("elem", ["f16", "f32", "q8_0"])
+@pytest.mark.parametrize("skip", [1, 2, 3])
+def test_rows_into_tensors_at_any_element(elem, skip):
+    """k and v views that begin at an element's boundary alone; then V alone."""
+    torch = torch_cuda()
+    say(f"case rows at any element {(elem, skip)}")
+    rng = np.random.default_rng(skip)
+    c = rv.PagedKvCache(1, 2, 32, 3, 8, elem)
+    k, v = rows(rng, 5, 64), rows(rng, 5, 64)
+    t, at, seq = ints([[2, 0]]), ints([3, 9, 0, 12, 7]), ints([0] * 5)
+    wide = torch.full((2 * 5 * 64 + 16,), 9.0, device="cuda")
+    kin, vin = wide[skip:skip + 320].view(5, 64), wide[skip + 320:skip + 640].view(5, 64)
+    kin.copy_(dev(k)), vin.copy_(dev(v))
+    c.append_rows(0, kin, vin, t, at, seq)
+    dt = torch.float32 if elem == "f32" else torch.float16
+    buf = torch.full((2 * 320 + 16,), 9.0, device="cuda", dtype=dt)
+    gk, gv = buf[skip:skip + 320].view(5, 64), buf[skip + 320:skip + 640].view(5, 64)
+    c.read_rows(0, t, at, seq, k=gk, v=gv)
+    assert np.array_equal(host(gk).astype(np.float32), stored(k, elem))
+    assert np.array_equal(host(gv).astype(np.float32), stored(v, elem))
+    assert torch.all(buf[:skip] == 9) and torch.all(buf[skip + 640:] == 9)
+    gk.fill_(5)
+    got = c.read_rows(0, t, at, seq, v=gv)
+    assert got[0] is None and torch.all(gk == 5) and np.array_equal(host(gv).astype(np.float32), stored(v, elem))
+
+
 def test_padding_and_refused_rows_write_nothing_and_are_recorded():
     torch = torch_cuda()
     say("case refused rows")
@@ -971,6 +997,45 @@ def test_streams_take_turns_and_caches_do_not_meet():
     for i in range(2):
         want, a, vmax = expect(q, two[i][2], 4, 128)
         check(host(res[i]), want, a, vmax, f"thread {i}")
+
+
+def test_threads_take_turns_at_one_cache():
+    """Two threads on streams of their own, one cache and one workspace; each appends to
+    its own sequence and attends both."""
+    torch = torch_cuda()
+    say("case threads at one cache")
+    rng = np.random.default_rng(42)
+    lens = [5000, 3000]
+    c, table, own = filled(rng, "f16", 4, 128, 64, lens)
+    q = [rng.standard_normal((2, 4096)).astype(np.float32) for _ in range(2)]
+    want = [expect(x, own, 4, 128) for x in q]
+    t, n, qd = ints(table), ints(lens), [dev(x) for x in q]
+    new = [(dev(own[i][0][-1:]), dev(own[i][1][-1:])) for i in range(2)]  # the last rows again
+    last, seq = [ints([m - 1]) for m in lens], [ints([i]) for i in range(2)]
+    torch.cuda.synchronize()
+    outs, errs = [[], []], []
+
+    def work(i):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(30):
+                    c.append_rows(1, *new[i], t, last[i], seq[i])
+                    outs[i].append(rv.paged_attention(qd[i], c, 1, t, n, scale_of(128),
+                                                      torch.empty(2, 4096, device="cuda")))
+            s.synchronize()
+        except Exception as e:  # noqa: BLE001
+            errs.append(e)
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [x.start() for x in ts]
+    [x.join() for x in ts]
+    assert not errs
+    c.device_status()
+    for i in range(2):
+        for o in outs[i]:
+            assert np.array_equal(host(o).view(np.uint32), host(outs[i][0]).view(np.uint32))
+        check(host(outs[i][0]), *want[i], f"thread {i}")
 
 
 def test_empty_calls():
