@@ -398,18 +398,23 @@ struct Tiled {
 
   // Loads past the caches (every row is read once): 64 sequences of up to 16000 f16
   // rows 229 -> 203 us. Not of rows below a line of 128 bytes, which would be brought
-  // twice: 32 of up to 8000 Q8_0 rows of 64 23.0 us so, 25.2 past the caches.
+  // twice: 32 of up to 8000 Q8_0 rows of 64 23.0 us so, 25.2 past the caches. Nor where
+  // a narrower head's first values are loaded twice, but for f16: 32 of up to 4000 rows
+  // of 96, through the caches | past them: f32 65 | 69, Q8_0 28 | 30, f16 40 | 36.
   template <typename V>
   static __device__ __forceinline__ V stream(const char* p) {
-    if constexpr (HDP * kBytes >= 128)
+    if constexpr (HDP * kBytes >= 128 && (FULL || (!kF32 && !kQ8 && HDP > 64)))
       return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
     else
       return *reinterpret_cast<const V*>(p);
   }
 
-  // Values past a head's width are loaded from its start and then cleared, rows
-  // past the last one are rows of the last page, cleared before they count: no
-  // lane goes another way than the others while the operands are in registers.
+  // Past a head's width its first values are loaded again: of K they meet a q of zero
+  // (and are no less finite than their row), of V they make outputs that nobody takes.
+  // Rows past the last one are rows of the last page, cleared before they count. So no
+  // lane goes another way than the others while the operands are in registers, and
+  // nothing waits for a load before its tile's turn (with masks at the loads 32 sequences
+  // of up to 4000 f32 rows of 96 109 us, so 65; f16 47, so 36).
   template <typename V>
   static __device__ __forceinline__ V keep(V x, bool in) {
     static_assert(sizeof(V) % 4 == 0, "whole words");
@@ -430,13 +435,9 @@ struct Tiled {
 #pragma unroll
       for (int i = 0; i < NK; ++i) {
         const int d = kF32 ? 16 * i + 4 * g : kQ8 ? 64 * i + 16 * g : 32 * i + 8 * g;
-        const bool in = FULL || d < hd;
-        const int dd = in ? d : 0;
+        const int dd = FULL || d < hd ? d : 0;
         t.k[j][i] = stream<KReg>(row + dd * kBytes);
-        if constexpr (kQ8)  // (the codes of a scale of zero stand for nothing)
-          t.ks[j][i] = w.ks[at[j] * (hd / 32) + dd / 32] & (in ? 0xFFFFu : 0u);
-        else if (!FULL)
-          t.k[j][i] = keep(t.k[j][i], in);
+        if constexpr (kQ8) t.ks[j][i] = w.ks[at[j] * (hd / 32) + dd / 32];
       }
     }
   }
@@ -450,18 +451,12 @@ struct Tiled {
       const char* p = w.v + ((hp[j] << w.t.shift) + row[j]) * hd * kBytes;
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
-        const int d = 16 * VD * h + VD * n;
-        const bool in = FULL || d < hd;
-        const int dd = in ? d : 0;
+        const int d = 16 * VD * h + VD * n, dd = FULL || d < hd ? d : 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          t.v[4 * j + i][h] = stream<VReg>(p + ((size_t)i * hd + dd) * kBytes);
-          if constexpr (!FULL && !kQ8) t.v[4 * j + i][h] = keep(t.v[4 * j + i][h], in);
-        }
+        for (int i = 0; i < 4; ++i) t.v[4 * j + i][h] = stream<VReg>(p + ((size_t)i * hd + dd) * kBytes);
         if constexpr (kQ8)
-          t.vs[j][h] = keep(*reinterpret_cast<const f16x4*>(
-                                w.vs + ((hp[j] * (hd / 32) + dd / 32) << w.t.shift) + row[j]),
-                            in);
+          t.vs[j][h] =
+              *reinterpret_cast<const f16x4*>(w.vs + ((hp[j] * (hd / 32) + dd / 32) << w.t.shift) + row[j]);
       }
     }
   }
