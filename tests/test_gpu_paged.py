@@ -999,6 +999,33 @@ def test_streams_take_turns_and_caches_do_not_meet():
         check(host(res[i]), want, a, vmax, f"thread {i}")
 
 
+@pytest.mark.parametrize("elem", ["f16", "f32", "q8_0"])
+def test_step_of_a_fused_matrix(elem):
+    """q, k and v as columns of one matrix, out over q: the bits of rows apart."""
+    torch = torch_cuda()
+    say(f"case fused matrix {elem}")
+    rng = np.random.default_rng(54)
+    lens, n_kv, group, hd = [70, 0, 300], 2, 4, 96
+    two = [filled(np.random.default_rng(1), elem, n_kv, hd, 16, lens, extra=1) for _ in range(2)]
+    (c, table, _), (d, _, _) = two
+    q, k, v, (wq, wk) = step_inputs(rng, 3, n_kv, group, hd)
+    rope = rv.Rope(hd, THETA, 48, "interleaved")
+    args = (dev(wq), dev(wk), EPS, rope, ints(table), ints(lens), scale_of(hd))
+    want = rv.paged_decode_step(c, 1, dev(q), dev(k), dev(v), *args, torch.empty(q.shape, device="cuda"))
+    a, b = q.shape[1], k.shape[1]
+    fused = torch.full((3, a + 2 * b + 3), 9.0, device="cuda")
+    parts = [fused[:, 1:1 + a], fused[:, 1 + a:1 + a + b], fused[:, 1 + a + b:1 + a + 2 * b]]
+    for x, y in zip(parts, (q, k, v)):
+        x.copy_(dev(y))
+    rv.paged_decode_step(d, 1, *parts, *args, parts[0])
+    assert np.array_equal(host(parts[0]).copy().view(np.uint32), host(want).view(np.uint32))
+    w = host(fused)
+    assert np.all(w[:, 0] == 9) and np.all(w[:, -2:] == 9)
+    assert np.array_equal(w[:, 1 + a:1 + a + b], k) and np.array_equal(w[:, 1 + a + b:-2], v)
+    for x, y in zip(everything(c, 1), everything(d, 1)):
+        assert np.array_equal(x, y, equal_nan=True)
+
+
 def test_threads_take_turns_at_one_cache():
     """Two threads on streams of their own, one cache and one workspace; each appends to
     its own sequence and attends both."""
