@@ -859,21 +859,21 @@ bool tiled(int hd) { return hd % 8 == 0 && hd <= 256; }
 int cols_of(int hd, int group) { return tiled(hd) ? std::min(group, 16) : 1; }
 
 // log2 of the ranges the work is cut into: two a CU (what is resident), or one where
-// the registers hold one (f32 256 wide, and widths between 128 and 256). Long f16 work
-// above 64 wide takes one a CU where the items are no more than the CUs: with more,
-// some wait for others to end. us at 256 | 512 ranges: f16, 128 wide, 64 sequences of up
-// to 16000 rows 191 | 198, but 128 of 300 21.2 | 18.4; f16, 256 wide, 32 of up to 4000
-// 81.6 | 87.4; not of f16 64 wide, 64 of up to 8000 120 | 116; Q8_0 128 wide, 32 of up to
-// 8192 50.6 | 39.3; Q8_0 256 wide, 32 of up to 4000 55.9 | 53.5; f32 128 wide, 64 of up to
-// 4000 116 | 105.6 (of up to 16000 376 | 387). Where the XCDs are not known apart, an
-// item has at most kMostPieces.
+// the registers hold one (f32 256 wide, and widths between 128 and 256). f16 and f32
+// above 64 wide take one a CU from two units a range on, where the items are no more
+// than the CUs (f32: half the CUs): with more, some wait for others to end. us at 256 |
+// 512 ranges: f16, 128 wide, 64 sequences of up to 16000 rows 191 | 198, 8 of 4000 17.8 |
+// 18.4, but 128 of 300 22.7 | 20.1; f16, 256 wide, 32 of up to 4000 81.6 | 87.4; not of
+// f16 64 wide, 64 of up to 8000 127 | 124; f32, 128 wide, 8 of 7000 44.7 | 47.4, but 64 of
+// up to 4000 112 | 105; Q8_0, 128 wide, 32 of up to 8192 51 | 39. Where the XCDs are not
+// known apart, an item has at most kMostPieces.
 void set_ranges(const rv_paged* pg, size_t items, size_t units, AttnArgs& a) {
-  const bool f16 = pg->elem == RV_ELEM_F16;
   const bool wide = pg->head_dim > 128 && (pg->head_dim != 256 || pg->elem == RV_ELEM_F32);
   a.slots = pg->xcd_ok && pg->tune_join != 2 ? 3 : 0;
   a.most = a.slots == 0 ? 5 : wide ? 8 : 9;
   while (a.most > 3 && units <= ((size_t)1 << a.most) / 2) --a.most;  // (never so many units)
-  a.few = a.most == 9 && f16 && pg->head_dim > 64 && items <= (size_t)kCUs ? 8 : a.most;
+  const size_t even = pg->elem == RV_ELEM_F16 ? kCUs : pg->elem == RV_ELEM_F32 ? kCUs / 2 : 0;
+  a.few = a.most == 9 && pg->head_dim > 64 && items <= even ? 8 : a.most;
 }
 
 size_t items_per_seq(const rv_paged* pg, size_t n_q) {

@@ -163,15 +163,15 @@ RV_HD Pieces pieces_of(const Group& g, uint32_t w0, uint32_t w1, uint32_t item_s
 }
 
 // How `total` units are cut: units a range, and the ranges of a slot (so that every
-// slot has as many to do). At most 2^most ranges; 2^few where that makes eight units
-// or more a range.
+// slot has as many to do). At most 2^most ranges; 2^few where that makes two units or
+// more a range.
 struct Cut {
   uint32_t per, in_slot;
 };
 
 template <typename Quotient = PlainQuotient>
 RV_HD Cut cut_units(uint32_t total, int most, int few, int slots, Quotient divide = Quotient()) {
-  const int n = total >> (few + 3) ? few : most;
+  const int n = total >> (few + 1) ? few : most;
   Cut c;
   c.per = (total + (1u << n) - 1) >> n;
   if (c.per < 1) c.per = 1;
