@@ -540,8 +540,10 @@ struct Tiled {
       }
       locate(b, id);
       load_k(w, k_at, g, t);
-      load_v(w, v_hp, v_row, n, t);
       fetch(b + kStep, id);
+      __builtin_amdgcn_sched_barrier(0);  // (loads in the order in which they are waited for)
+      load_v(w, v_hp, v_row, n, t);
+      __builtin_amdgcn_sched_barrier(0);
       float mul = a.scale * kLog2e;
       f16x8 q_hi[NQ], q_lo[NQ];
       if constexpr (!kF32) {
@@ -565,9 +567,12 @@ struct Tiled {
       }
       // A tile: its scores, then the next one's K in the place of its own, its part of
       // the output, and the next one's V.
-      bool first = true;
-      uint32_t left = kAside;
-      do {
+      // A wave's last tile is another instance of the step: in the others every load is
+      // unconditional, so that the wait for one is not for those after it as well that
+      // another path would not have, and no row is past the last (f16, 8 sequences of 7000
+      // 28.5 -> 26.9 us; f32 45.8 -> 43.1; f16, 1000 of 100 74 -> 68).
+      auto step = [&](auto is_last, bool first) {
+        constexpr bool kLast = decltype(is_last)::value;
         // (Every chain of dependent matrix instructions is as short as it can be: hi and
         // lo apart, the two 16 rows in turn.)
         f32x4 sc[kSub], sl[kSub];
@@ -599,8 +604,8 @@ struct Tiled {
 #pragma unroll
         for (int j = 0; j < kSub; ++j) sc[j] += sl[j];
         const uint32_t nb = b + kStep;
-        const bool more = nb < p1, tail = b + kRows > p1;
-        if (more) {
+        const bool tail = kLast && b + kRows > p1;
+        if constexpr (!kLast) {
           locate(nb, id);
           load_k(w, k_at, g, t);
           fetch(nb + kStep, id);
@@ -693,14 +698,18 @@ struct Tiled {
             }
           }
         }
-        if (more) load_v(w, v_hp, v_row, n, t);
-        b += kStep;
-        first = false;
-        if (--left == 0 && b < p1) {
+        if constexpr (!kLast) load_v(w, v_hp, v_row, n, t);
+      };
+      const bool only = b + kStep >= p1;
+      uint32_t left = kAside;
+      for (; b + kStep < p1; b += kStep) {
+        step(std::false_type{}, false);
+        if (--left == 0) {
           put_aside();
           left = kAside;
         }
-      } while (b < p1);
+      }
+      step(std::true_type{}, only);
       if (aside) {
         put_aside();
         l = l_aside;
