@@ -782,7 +782,7 @@ __global__ __launch_bounds__(256, WAVES) void paged_attn_kernel(PagedView w, Att
   const uint32_t start = r * per, end = blockIdx.x < ranges ? min(total, start + per) : 0;
   if (start < end) {
     uint32_t s0 = 0;
-    for (;;) {  // the chunk that holds the range's first unit
+    while (s0 < a.n) {  // the chunk that holds the range's first unit (none: the lengths have been changed)
       const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
       if (start < base + all) break;
       base += all;
@@ -790,14 +790,15 @@ __global__ __launch_bounds__(256, WAVES) void paged_attn_kernel(PagedView w, Att
       rows = chunk(s0);
       sum = wave_scan(units_of_rows(rows) * items);
     }
-    const int at0 = __builtin_ctzll(__ballot(start < base + sum));
+    const int at0 = __builtin_ctzll(__ballot(start < base + sum) | 1ull << 63);
     const uint32_t before = base + (at0 ? (uint32_t)__builtin_amdgcn_readlane((int)sum, at0 - 1) : 0u);
     const Partials pt(a, w.hd);
     walk_units(
-        s0 + at0, start - before, start, end, items,
+        s0 + at0, start - before, start, s0 < a.n ? end : start, items,
         [&](uint32_t s) -> uint32_t { return (uint32_t)__builtin_amdgcn_readlane((int)rows, (int)(s - s0)); },
         [&](uint32_t s) -> uint32_t {
           for (;;) {
+            if (s >= a.n) return kNoMore;
             if (s - s0 >= 64) {
               s0 = s;
               rows = chunk(s0);

@@ -92,7 +92,10 @@ struct PlainQuotient {
 
 // Walks the units [start, end), the first of which is unit `off` of sequence s:
 // visit(sequence, its rows, item, first unit, last unit + 1 of the item, the first
-// unit's place in the line). next_of(s): the first sequence from s on that has rows.
+// unit's place in the line). next_of(s): the first sequence from s on that has rows, or
+// kNoMore, where the walk ends (the lengths have been changed under it).
+constexpr uint32_t kNoMore = 0xFFFFFFFFu;
+
 template <typename I, typename Rows, typename Next, typename Visit, typename Quotient = PlainQuotient>
 RV_HD void walk_units(uint32_t s, I off, I start, I end, I items, Rows rows_of, Next next_of, Visit visit,
                       Quotient divide = Quotient()) {
@@ -101,6 +104,7 @@ RV_HD void walk_units(uint32_t s, I off, I start, I end, I items, Rows rows_of, 
     if (off >= units * items) {
       off -= units * items;
       s = next_of(s + 1);
+      if (s == kNoMore) return;
       continue;
     }
     const I item = divide(off, units), u0 = off - item * units;

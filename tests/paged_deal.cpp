@@ -154,6 +154,12 @@ int main() {
     deal(rows, 1 + g() % 9, 1 + g() % 2048);
   }
 
+  // Lengths that shrink under the walk: it ends.
+  int visits = 0;
+  walk_units(0u, 0l, 0l, 10l, 1l, [](uint32_t) { return 100l; },
+             [](uint32_t s) { return s < 3 ? s : kNoMore; }, [&](uint32_t, long, long, long, long, long) { ++visits; });
+  CHECK(visits == 3, "%d visits", visits);
+
   const int32_t ids[3 * 5] = {4, 0, -1, 9, 9, 7, 6, 5, 9, 9, 8, INT32_MIN, INT32_MAX, 9, 9};  // 3 of 5 entries a row
   const Pages t{ids, 5, 3, 3, 9, 4};
   uint32_t page = 99, row = 99, got = 99;
