@@ -178,8 +178,8 @@ int32_t rv_paged_attention(rv_paged* pg, size_t layer, const float* q, size_t q_
  * rv_paged_append_rows and rv_paged_attention one after the other; a negative
  * position gives zeros and writes nothing. Positions and tables are read when
  * the step runs, so a captured step is replayed for every token (advance the
- * positions in the graph, or between replays on its stream); the first call of a batch size
- * may have to allocate and is not captured (RV_ERR_UNSUPPORTED). */
+ * positions in the graph, or between replays on its stream); the first call of
+ * a batch size may have to allocate and is not captured (RV_ERR_UNSUPPORTED). */
 int32_t rv_paged_decode_step(rv_paged* pg, size_t layer, const rv_rope* rope, const float* q, size_t q_stride,
                              const float* k, size_t k_stride, const float* v, size_t v_stride, size_t n_seqs,
                              size_t q_dim, const float* q_norm_w, size_t q_norm_len, const float* k_norm_w,
