@@ -45,7 +45,8 @@ struct AttnArgs {
   int slots;          // log2 of the XCDs that workgroups are known to be dealt to in turn
   int most, few;      // log2 of the ranges there may be (cut_units)
   unsigned* tickets;  // [group][2], then one an item
-  // [range][2], then [group][2]: rows [cols][hd], then (maximum, sum) of each column.
+  // [range][2], then [group][2]: rows [cols][hd], then (maximum, sum) of each column
+  // (partial_floats).
   float* part;
   uint32_t part_bytes;
 };
@@ -75,18 +76,24 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 
 // ---- partials ---------------------------------------------------------------------
 
-// Cache policies of the buffer instructions: the sc1 bit, device scope; the sc0 bit
-// of a load, past the CU's L1 to its XCD's L2.
+// Cache policies of the buffer instructions: the sc1 bit, device scope; the sc0 bit of a
+// load, workgroup scope, which the CU's L1 may serve. That is enough for partials that
+// this XCD wrote: a launch begins with an empty L1, a partial's lines are its own, and
+// they are written once, before the first load of any of them.
 constexpr int kDeviceScope = 16, kXcdScope = 1;
 
 struct Partials {
   __amdgpu_buffer_rsrc_t rs;
   int cols, hd;
+  uint32_t bytes;  // of one
   __device__ __forceinline__ Partials(const AttnArgs& a, int hd_)
-      : rs(__builtin_amdgcn_make_buffer_rsrc(a.part, (short)0, (int)a.part_bytes, 0x00020000)), cols(a.cols), hd(hd_) {}
+      : rs(__builtin_amdgcn_make_buffer_rsrc(a.part, (short)0, (int)a.part_bytes, 0x00020000)),
+        cols(a.cols),
+        hd(hd_),
+        bytes(partial_floats((uint32_t)a.cols, (uint32_t)hd_) * 4u) {}
   // Byte offset of a partial (2 * range + which; the groups' behind them); of column
   // c's (maximum, sum) in it.
-  __device__ __forceinline__ uint32_t at(uint32_t i) const { return i * (uint32_t)(cols * (hd + 2)) * 4u; }
+  __device__ __forceinline__ uint32_t at(uint32_t i) const { return i * bytes; }
   __device__ __forceinline__ uint32_t stat(int c) const { return (uint32_t)(cols * hd + 2 * c) * 4u; }
   // Stores to be seen on this XCD, or on all.
   __device__ __forceinline__ void put(uint32_t o, float x, bool here) const {
@@ -919,7 +926,7 @@ PagedAttnPlan paged_attn_plan(const rv_paged* pg, const rv_page_table& t, size_t
   const size_t items = n * items_per_seq(pg, n_q), rows = t.pages * pg->page_rows;
   const size_t cols = cols_of((int)pg->head_dim, (int)(n_q / pg->n_kv_heads));
   if (__builtin_mul_overflow(items, (rows + kUnitRows - 1) / kUnitRows, &p.units)) p.units = SIZE_MAX;
-  p.ws_bytes = (size_t)2 * (kMaxRanges + kGroups) * cols * (pg->head_dim + 2) * sizeof(float);
+  p.ws_bytes = (size_t)2 * (kMaxRanges + kGroups) * partial_floats((uint32_t)cols, (uint32_t)pg->head_dim) * sizeof(float);
   p.ticket_bytes = (2 * kGroups + items) * sizeof(unsigned);
   return p;
 }

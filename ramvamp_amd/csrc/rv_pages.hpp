@@ -83,6 +83,15 @@ RV_HD int partial_of(I range, I per, I item_start) {
   return item_start > range * per ? 1 : 0;
 }
 
+// Floats of a partial: `cols` rows of hd values, then (maximum, sum) of each column, in
+// whole lines of the caches. Two partials have different writers, and a CU that reads
+// one may keep its lines: none of them may hold a part of another that is still to come.
+constexpr uint32_t kLineFloats = 32;
+
+RV_HD uint32_t partial_floats(uint32_t cols, uint32_t hd) {
+  return (cols * (hd + 2) + kLineFloats - 1) / kLineFloats * kLineFloats;
+}
+
 struct PlainQuotient {
   template <typename I>
   RV_HD I operator()(I x, I y) const {

@@ -213,3 +213,12 @@ def test_host_tensors_are_refused():
         rv.rope_rows(x, at, rv.Rope(128, 1e6))
     with pytest.raises(TypeError):
         rv.rope_rows(np.zeros((2, 128), np.float32), at, rv.Rope(128, 1e6), x)
+
+
+def test_joins_on_the_host(tmp_path):
+    """Partials in lines of their own."""
+    exe = str(tmp_path / "paged_joins")
+    subprocess.run([os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"), "-x", "hip", "--offload-host-only", "-O1",
+                    "-std=c++17", "-o", exe, os.path.join(HERE, "paged_joins.cpp")], check=True, capture_output=True)
+    out = subprocess.run([exe], capture_output=True, text=True, timeout=100)
+    assert out.returncode == 0 and not out.stdout, out.stdout
