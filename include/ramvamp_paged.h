@@ -17,7 +17,9 @@
  *    sequence numbers) is checked on the device: a row or sequence that names
  *    what is not there is refused by itself, as its call says, nothing out of
  *    bounds is touched, and one such refusal is recorded for
- *    rv_paged_device_status.
+ *    rv_paged_device_status. It must not change between the call and the end of
+ *    its work: outputs of a call under which it did are undefined (nothing out of
+ *    bounds is touched all the same, and later calls are as ever).
  */
 #ifndef RAMVAMP_PAGED_H
 #define RAMVAMP_PAGED_H

@@ -40,7 +40,7 @@ struct rv_paged {
   // since a graph captured earlier may still address it.
   void* ws = nullptr;  // attention's partials
   size_t ws_bytes = 0;
-  unsigned* tickets = nullptr;  // and their tickets, zero between calls
+  unsigned* tickets = nullptr;  // and their tickets, behind the words that say whose turn it is
   size_t ticket_bytes = 0;
   float* qbuf = nullptr;  // a step's normed and rotated q rows
   size_t qbuf_bytes = 0;
@@ -147,7 +147,7 @@ struct PagedAttn {
 };
 struct PagedAttnPlan {
   size_t units;  // of work at most, by what the tables can hold
-  size_t ws_bytes, ticket_bytes;
+  size_t ws_bytes, tickets, ticket_bytes;
 };
 PagedAttnPlan paged_attn_plan(const rv_paged* pg, const rv_page_table& t, size_t n, size_t n_q);
 HipStatus launch_paged_attn(const rv_paged* pg, const PagedView& w, const PagedAttn& a, const PagedAttnPlan& plan,

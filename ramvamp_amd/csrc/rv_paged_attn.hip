@@ -16,7 +16,8 @@
 // where they are many first those of each group do (loads at device scope bring a CU
 // some 12 bytes a cycle, loads from its L2 several times that), and else, and across
 // groups, they are stored and loaded at device scope, since the XCDs' L2s do not see
-// each other's lines. Partials are counted by tickets that are zero between calls.
+// each other's lines. Partials are counted by tickets, two sets of them in turn by the
+// launch, each cleared by the launch after its own.
 //
 // Bound by the pages' bytes where there are many: f16, 32 query heads over 4 of 128, 64
 // sequences of up to 16000 rows 188 us, 6.6 TB/s (a streaming read's rate); one of 131000
@@ -44,7 +45,10 @@ struct AttnArgs {
   long out_stride;
   int slots;          // log2 of the XCDs that workgroups are known to be dealt to in turn
   int most, few;      // log2 of the ranges there may be (cut_units)
-  unsigned* tickets;  // [group][2], then one an item
+  Turn* turns;        // a word a workgroup (rv_pages.hpp)
+  unsigned* tickets;  // two sets of [group][2], then one an item; from one set to the other:
+  size_t set_words;
+  uint32_t n_tickets;
   // [range][2], then [group][2]: rows [cols][hd], then (maximum, sum) of each column
   // (partial_floats).
   float* part;
@@ -52,6 +56,7 @@ struct AttnArgs {
 };
 
 constexpr uint32_t kMaxRanges = 2 * kCUs, kGroups = kMaxRanges / kGroup;
+static_assert(kTurns % kMaxRanges == 0, "a turn's word for every workgroup");
 constexpr uint32_t kRefused = 0xFFFFFFFFu;
 
 // Rows a sequence of this length attends, kRefused where the table has not so many.
@@ -208,14 +213,11 @@ __device__ __forceinline__ void join(const Partials& p, uint32_t first, uint32_t
 }
 
 // Whether this workgroup is the last of `n` to come here, its stores of partials
-// complete; the last leaves the ticket zero for the next call.
+// complete.
 __device__ __forceinline__ bool last_of(unsigned* ticket, uint32_t n, unsigned& drawn) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  if (threadIdx.x == 0) {
-    drawn = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (drawn == n - 1) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
+  if (threadIdx.x == 0) drawn = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
   const bool last = drawn == n - 1;
   __syncthreads();  // (the next draw writes it)
@@ -770,6 +772,8 @@ __global__ __launch_bounds__(256, WAVES) void paged_attn_kernel(PagedView w, Att
   __shared__ unsigned drawn;
   const int lane = threadIdx.x & 63;
   const uint32_t items = (uint32_t)(w.n_kv * a.blocks);
+  const Turn turn = a.turns[blockIdx.x];
+  unsigned* const tickets = a.tickets + (turn.set ? a.set_words : 0);
   // Sequence i's rows, for the 64 from s0 on a lane each.
   auto chunk = [&](uint32_t s0) {
     return s0 + lane < a.n ? rows_of_len(w, a, a.lens[s0 + lane]) : 0u;
@@ -835,7 +839,7 @@ __global__ __launch_bounds__(256, WAVES) void paged_attn_kernel(PagedView w, Att
             return pt.at(alone ? 2 * ranges + of_group : 2 * r + partial_of(r, per, at));
           });
           if (whole) return;
-          unsigned* const ticket = a.tickets + 2 * kGroups + s * items + item;
+          unsigned* const ticket = tickets + 2 * kGroups + s * items + item;
           float* const out = a.out + s * a.out_stride + (long)qh * w.hd;
           uint32_t piece0 = 2 * ps.first + partial_of(ps.first, per, first), rest = 2 * (ps.first + 1), count = ps.groups;
           if (once) {
@@ -845,7 +849,7 @@ __global__ __launch_bounds__(256, WAVES) void paged_attn_kernel(PagedView w, Att
           } else {
             const bool only = ps.groups == 1;
             if (!alone) {
-              if (!last_of(only ? ticket : a.tickets + of_group, ps.count, drawn)) return;
+              if (!last_of(only ? ticket : tickets + of_group, ps.count, drawn)) return;
               join<Inner::kVec, Inner::kLanes, kXcdScope>(pt, piece0, rest, ps.count, ncols, only ? out : nullptr,
                                                           2 * ranges + of_group);
             }
@@ -857,6 +861,12 @@ __global__ __launch_bounds__(256, WAVES) void paged_attn_kernel(PagedView w, Att
             join<Inner::kVec, Inner::kLanes, kDeviceScope>(pt, piece0, rest, count, ncols, out, 0);
         },
         divide);
+  }
+  if (threadIdx.x < 64) {  // (the wave that has drawn the tickets)
+    unsigned* const other = a.tickets + (turn.set ? 0 : a.set_words);
+    end_turn(
+        turn, blockIdx.x, gridDim.x, threadIdx.x, 64, a.n_tickets, [&](uint32_t c, Turn next) { a.turns[c] = next; },
+        [&](size_t i) { other[i] = 0; });
   }
   // Sequences without rows: zeros; refused ones: NaN.
   for (uint32_t s = blockIdx.x; s < a.n; s += gridDim.x) {
@@ -927,7 +937,9 @@ PagedAttnPlan paged_attn_plan(const rv_paged* pg, const rv_page_table& t, size_t
   const size_t cols = cols_of((int)pg->head_dim, (int)(n_q / pg->n_kv_heads));
   if (__builtin_mul_overflow(items, (rows + kUnitRows - 1) / kUnitRows, &p.units)) p.units = SIZE_MAX;
   p.ws_bytes = (size_t)2 * (kMaxRanges + kGroups) * partial_floats((uint32_t)cols, (uint32_t)pg->head_dim) * sizeof(float);
-  p.ticket_bytes = (2 * kGroups + items) * sizeof(unsigned);
+  p.tickets = 2 * kGroups + items;
+  if (p.tickets > 0x7FFFFFFFu) p.units = SIZE_MAX;  // (tables without pages)
+  p.ticket_bytes = kTurns * sizeof(Turn) + 2 * set_words(p.tickets) * sizeof(unsigned);
   return p;
 }
 
@@ -945,7 +957,10 @@ HipStatus launch_paged_attn(const rv_paged* pg, const PagedView& w, const PagedA
   a.scale = p.scale;
   a.out = p.out;
   a.out_stride = (long)p.out_stride;
-  a.tickets = pg->tickets;
+  a.turns = (Turn*)pg->tickets;
+  a.tickets = (unsigned*)(a.turns + kTurns);
+  a.set_words = (pg->ticket_bytes - kTurns * sizeof(Turn)) / sizeof(unsigned) / 2 / kLineFloats * kLineFloats;
+  a.n_tickets = (uint32_t)plan.tickets;
   a.part = (float*)pg->ws;
   a.part_bytes = (uint32_t)plan.ws_bytes;
   set_ranges(pg, p.n * w.n_kv * a.blocks, plan.units, a);

@@ -4,6 +4,10 @@
 #include <stdio.h>
 #include <stdlib.h>
 
+#include <algorithm>
+#include <random>
+#include <vector>
+
 #include "../ramvamp_amd/csrc/rv_pages.hpp"
 
 #define CHECK(c, ...)               \
@@ -31,7 +35,44 @@ static void lines() {
     }
 }
 
+// A launch finds its tickets zero, whatever an earlier one left: workgroups come in any
+// order, draw in any number (as where the lengths change under them and they do not
+// agree on the pieces), and launches differ in grid and in tickets.
+static void turns() {
+  std::mt19937 g(11);
+  for (int run = 0; run < 300; ++run) {
+    const size_t words = set_words(1 + g() % 3000);
+    CHECK(words % kLineFloats == 0, "%zu words", words);
+    std::vector<Turn> turn(kTurns, Turn{0, 0});
+    std::vector<uint32_t> tickets(2 * words, 0);
+    for (int launch = 0; launch < 12; ++launch) {
+      const uint32_t grid = 8u << (g() % 7), n = 1 + g() % words;
+      const uint32_t lanes = 1u << (g() % 7);
+      const bool agree = g() % 2;
+      const uint32_t set = turn[0].set;
+      for (size_t i = 0; i < words; ++i) CHECK(tickets[set * words + i] == 0, "run %d launch %d: ticket %zu", run, launch, i);
+      std::vector<uint32_t> order(grid);
+      for (uint32_t b = 0; b < grid; ++b) order[b] = b;
+      std::shuffle(order.begin(), order.end(), g);
+      uint32_t last = 0;
+      for (uint32_t b : order) {
+        const Turn t = turn[b];
+        CHECK(t.set == set && t.used <= words, "run %d launch %d: workgroup %u's turn", run, launch, b);
+        if (agree)
+          last += tickets[t.set * words]++ == grid - 1;  // one item of all workgroups
+        else
+          for (int k = 0; k < 3; ++k) tickets[t.set * words + g() % n] += g() % 3;
+        for (uint32_t lane = 0; lane < lanes; ++lane)
+          end_turn(t, b, grid, lane, lanes, n, [&](uint32_t c, Turn next) { turn.at(c) = next; },
+                   [&](size_t i) { tickets.at((1 - t.set) * words + i) = 0; });
+      }
+      CHECK(!agree || last == 1, "run %d launch %d: %u last", run, launch, last);
+    }
+  }
+}
+
 int main() {
   lines();
+  turns();
   return 0;
 }
