@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "../../include/ramvamp_attn.h"
+#include "rv_order.hpp"
 
 struct rv_kv {
   size_t n_layers = 0, n_kv_heads = 0, head_dim = 0, capacity = 0, kv_dim = 0, plane = 0;
@@ -137,6 +138,33 @@ constexpr long kCUs = 256;
 HipStatus ensure_workspace(rv_kv* kv, size_t bytes, size_t bound = 0);
 // Whether work on s is being captured into a graph.
 bool capturing(hipStream_t s);
+
+// What a cache's StreamOrder asks of HIP; calls are made with its device current.
+struct HipStreams {
+  typedef hipStream_t Stream;
+  typedef hipError_t Error;
+  static constexpr hipError_t kUnsupported = hipErrorStreamCaptureUnsupported;
+  hipEvent_t ev = nullptr;
+
+  static bool capturing(hipStream_t s) { return rv::capturing(s); }
+  static bool recordable(hipStream_t s) {
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    const bool is = hipStreamIsCapturing(s, &cs) == hipSuccess && cs == hipStreamCaptureStatusNone;
+    if (!is) (void)hipGetLastError();
+    return is;
+  }
+  hipError_t record(hipStream_t s) {
+    if (!ev) {
+      const hipError_t e = hipEventCreateWithFlags(&ev, hipEventDisableTiming);
+      if (e != hipSuccess) {
+        ev = nullptr;
+        return e;
+      }
+    }
+    return hipEventRecord(ev, s);
+  }
+  hipError_t wait(hipStream_t s) { return hipStreamWaitEvent(s, ev, 0); }
+};
 // The normalised-q buffer, with the workspace's growth rules.
 HipStatus ensure_qbuf(rv_kv* kv, size_t bytes);
 // RV_ERR_UNSUPPORTED for a call that would have to allocate under graph

@@ -33,8 +33,7 @@ struct rv_paged {
   int64_t tune_join = 0;
   void* k = nullptr;
   void* v = nullptr;
-  hipStream_t stream = nullptr;
-  hipEvent_t order_ev = nullptr;
+  rv::StreamOrder<rv::HipStreams> order;  // order.stream: what calls are queued on
   unsigned* status = nullptr;  // [0] code, [1] layer, [2] row, [3] what it read, [4] the bound
   // Grown on first need; a replaced buffer is kept until the cache is freed,
   // since a graph captured earlier may still address it.

@@ -31,7 +31,7 @@ int32_t hip_fail(rv_error* err, const rv::HipStatus& st) {
 
 int32_t hip_fail(rv_error* err, hipError_t e, const char* what) { return hip_fail(err, rv::HipStatus{e, what}); }
 
-// Makes the cache's device current for the scope of one call.
+// Makes a device current for the scope of one call.
 struct DeviceGuard {
   int prev = -1;
   explicit DeviceGuard(int dev) {
@@ -42,6 +42,13 @@ struct DeviceGuard {
     int cur = -1;
     if (prev >= 0 && hipGetDevice(&cur) == hipSuccess && cur != prev) (void)hipSetDevice(prev);
   }
+};
+
+// A call's scope: the cache's device current, and what it queues behind earlier calls.
+struct Queued {
+  DeviceGuard dg;
+  const hipError_t e;
+  explicit Queued(rv_paged* pg) : dg(pg->device), e(pg->order.settle()) {}
 };
 
 int32_t check_flags(uint32_t flags, rv_error* err) {
@@ -96,7 +103,7 @@ int32_t geometry(size_t n_layers, size_t n_kv_heads, size_t head_dim, size_t n_p
 rv::HipStatus grow(rv_paged* pg, void** buf, size_t* have, size_t bytes, const char* what) {
   rv::HipStatus st;
   if (bytes <= *have) return st;
-  if (rv::capturing(pg->stream)) {
+  if (rv::capturing(pg->order.stream)) {
     st.e = hipErrorStreamCaptureUnsupported;
     st.what = "workspace growth under graph capture (run a call of this shape uncaptured first)";
     return st;
@@ -339,7 +346,7 @@ void rv_paged_free(rv_paged* pg) {
     for (void* p : {pg->k, pg->v, (void*)pg->status, pg->ws, (void*)pg->tickets, (void*)pg->qbuf})
       if (p) (void)hipFree(p);
     for (void* p : pg->retired) (void)hipFree(p);
-    if (pg->order_ev) (void)hipEventDestroy(pg->order_ev);
+    if (pg->order.api.ev) (void)hipEventDestroy(pg->order.api.ev);
   }
   delete pg;
 }
@@ -354,33 +361,26 @@ int32_t rv_paged_set_tuning(rv_paged* pg, int32_t knob, int64_t value, rv_error*
 int32_t rv_paged_set_stream(rv_paged* pg, void* hip_stream, rv_error* err) {
   if (!pg) return null_arg(err, "pg");
   const hipStream_t next = (hipStream_t)hip_stream;
-  if (next == pg->stream) return ok(err);
+  if (next == pg->order.stream) return ok(err);
   DeviceGuard dg(pg->device);
-  if (rv::capturing(next) || rv::capturing(pg->stream)) {
-    pg->stream = next;
-    return ok(err);
-  }
-  hipError_t e = hipSuccess;
-  if (!pg->order_ev) e = hipEventCreateWithFlags(&pg->order_ev, hipEventDisableTiming);
-  if (e == hipSuccess) e = hipEventRecord(pg->order_ev, pg->stream);
-  if (e == hipSuccess) e = hipStreamWaitEvent(next, pg->order_ev, 0);
-  if (e != hipSuccess) return hip_fail(err, e, "stream hand-over");
-  pg->stream = next;
-  return ok(err);
+  const hipError_t e = pg->order.move_to(next);
+  return e == hipSuccess ? ok(err) : hip_fail(err, e, "stream hand-over");
 }
 
 int32_t rv_paged_synchronize(rv_paged* pg, rv_error* err) {
   if (!pg) return null_arg(err, "pg");
-  DeviceGuard dg(pg->device);
-  return finish(pg->stream, RV_SYNC, {}, err);
+  const Queued queued(pg);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
+  return finish(pg->order.stream, RV_SYNC, {}, err);
 }
 
 int32_t rv_paged_device_status(rv_paged* pg, rv_error* err) {
   if (!pg) return null_arg(err, "pg");
-  DeviceGuard dg(pg->device);
-  if (rv::capturing(pg->stream)) return unsupported(err, 0, "device status under graph capture");
+  const Queued queued(pg);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
+  if (rv::capturing(pg->order.stream)) return unsupported(err, 0, "device status under graph capture");
   uint32_t w[5] = {};
-  hipError_t e = hipStreamSynchronize(pg->stream);
+  hipError_t e = hipStreamSynchronize(pg->order.stream);
   if (e == hipSuccess) e = hipMemcpy(w, pg->status, sizeof(w), hipMemcpyDeviceToHost);
   if (e != hipSuccess) return hip_fail(err, e, "read the device status");
   if (w[0] == 0) return ok(err);
@@ -405,8 +405,9 @@ int32_t rv_paged_append_rows(rv_paged* pg, size_t layer, const rv_rope* rope, co
   if ((rc = check_stride(rows, pg->kv_dim, k_stride, "k rows vs their stride", err))) return rc;
   if ((rc = check_stride(rows, pg->kv_dim, v_stride, "v rows vs their stride", err))) return rc;
   if ((rc = check_table(table, rows, !seqs, err))) return rc;
-  DeviceGuard dg(pg->device);
-  if (rows == 0) return finish(pg->stream, flags, {}, err);
+  const Queued queued(pg);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
+  if (rows == 0) return finish(pg->order.stream, flags, {}, err);
   if (!k || !v || !positions) return null_arg(err, !k ? "k" : !v ? "v" : "positions");
   rv::PagedRows r{};
   r.k = k;
@@ -418,8 +419,8 @@ int32_t rv_paged_append_rows(rv_paged* pg, size_t layer, const rv_rope* rope, co
   r.seqs = seqs;
   r.k_w = k_norm_w;
   r.eps = eps;
-  return finish(pg->stream, flags,
-                rv::launch_paged_append(pg, rv::paged_view(pg, layer, *table), rope, r, pg->stream), err);
+  return finish(pg->order.stream, flags,
+                rv::launch_paged_append(pg, rv::paged_view(pg, layer, *table), rope, r, pg->order.stream), err);
 }
 
 int32_t rv_paged_read_rows(rv_paged* pg, size_t layer, size_t rows, const int32_t* positions, const int32_t* seqs,
@@ -429,11 +430,12 @@ int32_t rv_paged_read_rows(rv_paged* pg, size_t layer, size_t rows, const int32_
   if (rc) return rc;
   if ((rc = check_layer(pg, layer, err))) return rc;
   if ((rc = check_table(table, rows, !seqs, err))) return rc;
-  DeviceGuard dg(pg->device);
-  if (rows == 0 || (!k && !v)) return finish(pg->stream, flags, {}, err);
+  const Queued queued(pg);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
+  if (rows == 0 || (!k && !v)) return finish(pg->order.stream, flags, {}, err);
   if (!positions) return null_arg(err, "positions");
-  return finish(pg->stream, flags,
-                rv::launch_paged_read(pg, rv::paged_view(pg, layer, *table), rows, positions, seqs, k, v, pg->stream),
+  return finish(pg->order.stream, flags,
+                rv::launch_paged_read(pg, rv::paged_view(pg, layer, *table), rows, positions, seqs, k, v, pg->order.stream),
                 err);
 }
 
@@ -451,8 +453,9 @@ int32_t rv_paged_attention(rv_paged* pg, size_t layer, const float* q, size_t q_
   if ((rc = check_stride(n_seqs, q_dim, out_stride, "out rows vs their stride", err))) return rc;
   if ((rc = check_table(table, n_seqs, true, err))) return rc;
   if (n_seqs > kMaxSeqs) return unsupported(err, n_seqs, "sequences past 2^23");
-  DeviceGuard dg(pg->device);
-  if (n_seqs == 0) return finish(pg->stream, flags, {}, err);
+  const Queued queued(pg);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
+  if (n_seqs == 0) return finish(pg->order.stream, flags, {}, err);
   if (!q || !lens || !out) return null_arg(err, !q ? "q" : !lens ? "lens" : "out");
   if (n_seqs == 1) q_stride = out_stride = q_dim;
   if (overlap(q, q_stride, out, out_stride, n_seqs, q_dim)) return unsupported(err, 0, "out overlaps q");
@@ -460,7 +463,7 @@ int32_t rv_paged_attention(rv_paged* pg, size_t layer, const float* q, size_t q_
   rv::PagedAttnPlan plan;
   if ((rc = ready_attn(pg, *table, n_seqs, n_q, &plan, err))) return rc;
   const rv::PagedAttn a{q, q_stride, n_seqs, (int)n_q, lens, false, scale, out, out_stride};
-  return finish(pg->stream, flags, rv::launch_paged_attn(pg, rv::paged_view(pg, layer, *table), a, plan, pg->stream),
+  return finish(pg->order.stream, flags, rv::launch_paged_attn(pg, rv::paged_view(pg, layer, *table), a, plan, pg->order.stream),
                 err);
 }
 
@@ -483,8 +486,9 @@ int32_t rv_paged_decode_step(rv_paged* pg, size_t layer, const rv_rope* rope, co
   if ((rc = check_stride(n_seqs, q_dim, out_stride, "out rows vs their stride", err))) return rc;
   if ((rc = check_table(table, n_seqs, true, err))) return rc;
   if (n_seqs > kMaxSeqs) return unsupported(err, n_seqs, "sequences past 2^23");
-  DeviceGuard dg(pg->device);
-  if (n_seqs == 0) return finish(pg->stream, flags, {}, err);
+  const Queued queued(pg);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
+  if (n_seqs == 0) return finish(pg->order.stream, flags, {}, err);
   for (const auto& p : {std::pair<const void*, const char*>{q, "q"}, {k, "k"}, {v, "v"}, {positions, "positions"}, {out, "out"}})
     if (!p.first) return null_arg(err, p.second);
   const size_t n_q = q_dim / pg->head_dim;
@@ -507,12 +511,12 @@ int32_t rv_paged_decode_step(rv_paged* pg, size_t layer, const rv_rope* rope, co
   r.k_w = k_norm_w;
   r.eps = eps;
   const rv::PagedView w = rv::paged_view(pg, layer, *table);
-  st = rv::launch_paged_append(pg, w, rope, r, pg->stream);
+  st = rv::launch_paged_append(pg, w, rope, r, pg->order.stream);
   if (st.e == hipSuccess) {
     const rv::PagedAttn a{pg->qbuf, q_dim, n_seqs, (int)n_q, positions, true, scale, out, out_stride};
-    st = rv::launch_paged_attn(pg, w, a, plan, pg->stream);
+    st = rv::launch_paged_attn(pg, w, a, plan, pg->order.stream);
   }
-  return finish(pg->stream, flags, st, err);
+  return finish(pg->order.stream, flags, st, err);
 }
 
 }  // extern "C"

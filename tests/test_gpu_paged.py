@@ -1149,3 +1149,44 @@ def test_host_refusals():
     assert np.all(host(out) == 3)
     for k, v in (everything(c, 0), everything(c, 1)):
         assert not k.any() and not v.any()
+
+
+@pytest.mark.parametrize("back", [False, True])
+def test_calls_behind_a_capture_wait_for_those_before_it(back):
+    """A call on one stream, held up there, another captured on a second without a wait
+    for the device, then one on a third, or on the second itself."""
+    torch = torch_cuda()
+    say(f"case behind a capture {back}")
+    rng = np.random.default_rng(55)
+    lens, n_kv, hd = [300, 40], 2, 128
+    c, table, _ = filled(rng, "f16", n_kv, hd, 16, lens)
+    k, v = rows(rng, 2, n_kv * hd), rows(rng, 2, n_kv * hd)
+    t, n, last, seq = ints(table), ints(lens), ints([m - 1 for m in lens]), ints([0, 1])
+    kd, vd, q = dev(k), dev(v), dev(rng.standard_normal((2, 2 * 4 * hd)))
+    out = torch.empty(2, 2 * 4 * hd, device="cuda")
+    gk, gv = (torch.zeros(2, n_kv * hd, dtype=torch.float16, device="cuda") for _ in range(2))
+    big = torch.ones(8192, 8192, device="cuda")
+    first, second, third = (torch.cuda.Stream() for _ in range(3))
+    with torch.cuda.stream(second):
+        rv.paged_attention(q, c, 1, t, n, scale_of(hd), out)  # (allocates)
+    with torch.cuda.stream(first):
+        hold = big @ big
+    torch.cuda.synchronize()
+    with torch.cuda.stream(first):
+        for _ in range(8):
+            torch.mm(big, big, out=hold)
+        c.append_rows(1, kd, vd, t, last, seq)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(second):
+        g.capture_begin()
+        rv.paged_attention(q, c, 1, t, n, scale_of(hd), out)
+        g.capture_end()
+    with torch.cuda.stream(second if back else third):
+        c.read_rows(1, t, last, seq, k=gk, v=gv)
+    torch.cuda.synchronize()
+    assert np.array_equal(host(gk), k.astype(np.float16)) and np.array_equal(host(gv), v.astype(np.float16))
+    out.fill_(float("nan"))
+    g.replay()
+    torch.cuda.synchronize()
+    again = rv.paged_attention(q, c, 1, t, n, scale_of(hd), torch.empty_like(out))
+    assert np.array_equal(host(out).view(np.uint32), host(again).view(np.uint32))

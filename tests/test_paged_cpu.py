@@ -222,3 +222,12 @@ def test_joins_on_the_host(tmp_path):
                     "-std=c++17", "-o", exe, os.path.join(HERE, "paged_joins.cpp")], check=True, capture_output=True)
     out = subprocess.run([exe], capture_output=True, text=True, timeout=100)
     assert out.returncode == 0 and not out.stdout, out.stdout
+
+
+def test_a_cache_passes_from_stream_to_stream_on_the_host(tmp_path):
+    """Calls wait for all earlier ones, whatever was captured in between."""
+    exe = str(tmp_path / "stream_order")
+    subprocess.run([os.environ.get("CXX", "g++"), "-O1", "-std=c++17", "-o", exe, os.path.join(HERE, "stream_order.cpp")],
+                   check=True, capture_output=True)
+    out = subprocess.run([exe], capture_output=True, text=True, timeout=100)
+    assert out.returncode == 0 and not out.stdout, out.stdout
