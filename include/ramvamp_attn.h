@@ -130,7 +130,10 @@ int32_t rv_kv_projected_bytes(size_t n_layers, size_t n_kv_heads, size_t head_di
 int32_t rv_kv_new(size_t n_layers, size_t n_kv_heads, size_t head_dim, size_t capacity,
                   rv_elem elem, int device, rv_kv** out, rv_error* err);
 void rv_kv_free(rv_kv* kv);
-/* Stream every later call on this cache is queued on (a hipStream_t). */
+/* Stream every later call on this cache is queued on (a hipStream_t), behind what
+ * the old one holds. A captured call waits for nothing outside its graph, whose
+ * replays are the caller's to order; a call behind a capture waits for what came
+ * before it (RV_ERR_UNSUPPORTED while a stream under capture holds that). */
 int32_t rv_kv_set_stream(rv_kv* kv, void* hip_stream, rv_error* err);
 int32_t rv_kv_synchronize(rv_kv* kv, rv_error* err);
 

@@ -123,12 +123,9 @@ void rv_paged_free(rv_paged* pg);
  * else across them at once, 2 always so. */
 #define RV_TUNE_PAGED_JOIN 1
 int32_t rv_paged_set_tuning(rv_paged* pg, int32_t knob, int64_t value, rv_error* err);
-/* As rv_kv_set_stream: later calls are queued on it, behind what the old one
- * holds. A captured call waits for nothing outside its graph, whose replays are the
- * caller's to order; a call behind a capture waits for what came before it.
- * RV_ERR_UNSUPPORTED where that is still held by a stream under capture. Calls on
- * one cache share its workspace: one stream at a time, and so two graphs captured
- * over one cache are replayed one after the other. */
+/* As rv_kv_set_stream. Calls on one cache share its workspace: one stream at a
+ * time, and so two graphs captured over one cache are replayed one after the
+ * other. */
 int32_t rv_paged_set_stream(rv_paged* pg, void* hip_stream, rv_error* err);
 int32_t rv_paged_synchronize(rv_paged* pg, rv_error* err);
 /* Waits for the stream, then returns and clears what a call recorded when the

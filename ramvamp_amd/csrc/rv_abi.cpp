@@ -53,6 +53,17 @@ struct DeviceGuard {
   }
 };
 
+// A call's scope: the cache's device current, and what it queues behind earlier calls
+// of the cache (of the prefix too, which is on the same stream).
+struct Queued {
+  DeviceGuard dg;
+  hipError_t e;
+  explicit Queued(const rv_kv* kv, const rv_kv* prefix = nullptr)
+      : dg(kv->device), e(const_cast<rv_kv*>(kv)->order.settle()) {
+    if (e == hipSuccess && prefix) e = const_cast<rv_kv*>(prefix)->order.settle();
+  }
+};
+
 size_t sat_mul(size_t a, size_t b) {
   size_t r;
   return __builtin_mul_overflow(a, b, &r) ? SIZE_MAX : r;
@@ -129,7 +140,7 @@ struct Stager {
   hipStream_t s;
   size_t used = 0;
   hipError_t e = hipSuccess;
-  explicit Stager(rv_kv* k) : kv(k), s(k->stream) {}
+  explicit Stager(rv_kv* k) : kv(k), s(k->order.stream) {}
   bool reserve(size_t bytes) {
     if (bytes <= kv->stage_bytes) return true;
     if (rv::capturing(s)) {
@@ -160,12 +171,12 @@ struct Stager {
 
 int32_t finish(rv_kv* kv, uint32_t flags, float* dev_out, float* host_out, size_t n, rv_error* err) {
   if (flags & RV_HOST_PTRS) {
-    hipError_t e = hipMemcpyAsync(host_out, dev_out, n * sizeof(float), hipMemcpyDeviceToHost, kv->stream);
+    hipError_t e = hipMemcpyAsync(host_out, dev_out, n * sizeof(float), hipMemcpyDeviceToHost, kv->order.stream);
     if (e != hipSuccess) return hip_fail(err, e, "hipMemcpyAsync D2H");
-    e = hipStreamSynchronize(kv->stream);
+    e = hipStreamSynchronize(kv->order.stream);
     if (e != hipSuccess) return hip_fail(err, e, "hipStreamSynchronize");
   } else if (flags & RV_SYNC) {
-    hipError_t e = hipStreamSynchronize(kv->stream);
+    hipError_t e = hipStreamSynchronize(kv->order.stream);
     if (e != hipSuccess) return hip_fail(err, e, "hipStreamSynchronize");
   }
   return ok(err);
@@ -176,7 +187,8 @@ int32_t run_attention(rv_kv* kv, const float* q, size_t q_len, size_t layer, con
                       size_t kv_hi, float* out, size_t out_len, uint32_t flags, rv_error* err) {
   if (kv_lo == kv_hi) return ok(err);  // the validated no-op of a surplus shard
   if (!q || !out) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, !q ? "q" : "out");
-  DeviceGuard dg(kv->device);
+  const Queued queued(kv);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
   const float* dq = q;
   float* dout = out;
   if (flags & RV_HOST_PTRS) {
@@ -186,7 +198,7 @@ int32_t run_attention(rv_kv* kv, const float* q, size_t q_len, size_t layer, con
     dout = st.carve(out_len);
     if (st.e != hipSuccess) return hip_fail(err, st.e, "hipMemcpyAsync H2D");
   }
-  rv::HipStatus hs = rv::launch_decode(kv, dq, p.n_q_heads, layer, p.positions, scale, kv_lo, kv_hi, dout, kv->stream);
+  rv::HipStatus hs = rv::launch_decode(kv, dq, p.n_q_heads, layer, p.positions, scale, kv_lo, kv_hi, dout, kv->order.stream);
   if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
   return finish(kv, flags, dout, out, out_len, err);
 }
@@ -257,7 +269,7 @@ int32_t shared_check(const rv_kv* prefix, size_t prefix_layer, size_t prefix_pos
   if (prefix->elem != tails->elem)
     return fail(err, RV_ERR_UNSUPPORTED, (uint64_t)prefix->elem, (uint64_t)tails->elem, 0, 0,
                 "prefix and tails of different element types");
-  if (prefix->device != tails->device || prefix->stream != tails->stream)
+  if (prefix->device != tails->device || prefix->order.stream != tails->order.stream)
     return fail(err, RV_ERR_UNSUPPORTED, (uint64_t)prefix->device, (uint64_t)tails->device, 0, 0,
                 "prefix and tails on different devices or streams");
   if (q_dim == 0 || q_dim % hd) return fail(err, RV_ATTN_Q_LEN_INDIVISIBLE, q_dim, hd);
@@ -377,7 +389,7 @@ TimedPair timing_pair(rv_kv* kv, hipStream_t s) {
 HipStatus ensure_workspace(rv_kv* kv, size_t bytes, size_t bound) {
   HipStatus st;
   if (bytes <= kv->ws_bytes) return st;
-  if (capturing(kv->stream)) {
+  if (capturing(kv->order.stream)) {
     st.e = hipErrorStreamCaptureUnsupported;
     st.what = "workspace growth under graph capture (run a call of this shape uncaptured first)";
     return st;
@@ -398,7 +410,7 @@ HipStatus ensure_workspace(rv_kv* kv, size_t bytes, size_t bound) {
 HipStatus ensure_qbuf(rv_kv* kv, size_t bytes) {
   HipStatus st;
   if (bytes <= kv->qbuf_bytes) return st;
-  if (capturing(kv->stream)) {
+  if (capturing(kv->order.stream)) {
     st.e = hipErrorStreamCaptureUnsupported;
     st.what = "q buffer growth under graph capture (run a call of this shape uncaptured first)";
     return st;
@@ -424,7 +436,7 @@ HipStatus ensure_qbuf(rv_kv* kv, size_t bytes) {
 HipStatus ensure_rope_tab(rv_kv* kv, float theta, size_t n) {
   HipStatus st;
   if (kv->rope_tab && kv->rope_theta == theta && kv->rope_n >= n) return st;
-  if (capturing(kv->stream)) {
+  if (capturing(kv->order.stream)) {
     st.e = hipErrorStreamCaptureUnsupported;
     st.what = "rope table growth under graph capture (run a device-position step uncaptured first)";
     return st;
@@ -609,7 +621,7 @@ void rv_kv_free(rv_kv* kv) {
   if (!kv) return;
   {
     DeviceGuard dg(kv->device);
-    if (kv->stream) (void)hipStreamSynchronize(kv->stream);
+    if (kv->order.stream && !kv->order.pending) (void)hipStreamSynchronize(kv->order.stream);
     else (void)hipDeviceSynchronize();
     for (void* p : {kv->k, kv->v, kv->ws, (void*)kv->qbuf, kv->stage, (void*)kv->tickets, (void*)kv->rope_tab,
                     (void*)kv->pf_tickets})
@@ -618,42 +630,29 @@ void rv_kv_free(rv_kv* kv) {
       if (p) (void)hipFree(p);
     for (void* p : kv->retired) (void)hipFree(p);
     for (hipEvent_t e : kv->ev) (void)hipEventDestroy(e);
-    if (kv->order_ev) (void)hipEventDestroy(kv->order_ev);
+    if (kv->order.api.ev) (void)hipEventDestroy(kv->order.api.ev);
   }
   delete kv;
 }
 
 // The cache's planes, workspace and staged copies are shared by every call,
 // so work queued on the new stream is ordered after what the old one holds.
-// Not across a graph capture: an event recorded outside a capture cannot
-// order work inside it (a capture's work runs when the graph is launched).
+// Not inside a graph capture: an event recorded outside of one cannot order
+// work inside it (a capture's work runs when the graph is launched).
 int32_t rv_kv_set_stream(rv_kv* kv, void* hip_stream, rv_error* err) {
   if (!kv) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, "kv");
   const hipStream_t next = (hipStream_t)hip_stream;
-  if (next == kv->stream) return ok(err);
+  if (next == kv->order.stream) return ok(err);
   DeviceGuard dg(kv->device);
-  if (rv::capturing(next) || rv::capturing(kv->stream)) {
-    kv->stream = next;
-    return ok(err);
-  }
-  if (!kv->order_ev) {
-    const hipError_t e = hipEventCreateWithFlags(&kv->order_ev, hipEventDisableTiming);
-    if (e != hipSuccess) {
-      kv->order_ev = nullptr;
-      return hip_fail(err, e, "hipEventCreate (stream hand-over)");
-    }
-  }
-  hipError_t e = hipEventRecord(kv->order_ev, kv->stream);
-  if (e == hipSuccess) e = hipStreamWaitEvent(next, kv->order_ev, 0);
-  if (e != hipSuccess) return hip_fail(err, e, "stream hand-over");
-  kv->stream = next;
-  return ok(err);
+  const hipError_t e = kv->order.move_to(next);
+  return e == hipSuccess ? ok(err) : hip_fail(err, e, "stream hand-over");
 }
 
 int32_t rv_kv_synchronize(rv_kv* kv, rv_error* err) {
   if (!kv) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, "kv");
-  DeviceGuard dg(kv->device);
-  hipError_t e = hipStreamSynchronize(kv->stream);
+  const Queued queued(kv);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
+  hipError_t e = hipStreamSynchronize(kv->order.stream);
   if (e != hipSuccess) return hip_fail(err, e, "hipStreamSynchronize");
   return ok(err);
 }
@@ -699,7 +698,8 @@ int32_t rv_kv_append_rows(rv_kv* kv, size_t layer, const float* k, const float* 
   if (rows > kv->capacity - len) return fail(err, RV_KV_CAPACITY_EXCEEDED, layer, kv->capacity);
   if (rows == 0) return ok(err);
   if (!k || !v) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, !k ? "k" : "v");
-  DeviceGuard dg(kv->device);
+  const Queued queued(kv);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
   const float* dk = k;
   const float* dv = v;
   if (flags & RV_HOST_PTRS) {
@@ -715,14 +715,14 @@ int32_t rv_kv_append_rows(rv_kv* kv, size_t layer, const float* k, const float* 
     rv::RowDst dst;
     dst.layer = layer;
     dst.row0 = (long)len;
-    hs = rv::launch_append_dst(kv, dst, dk, dv, rows, kv->stream);
+    hs = rv::launch_append_dst(kv, dst, dk, dv, rows, kv->order.stream);
   } else {
-    hs = rv::launch_append(kv, layer, len, dk, dv, rows, kv->stream);
+    hs = rv::launch_append(kv, layer, len, dk, dv, rows, kv->order.stream);
   }
   if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
   kv->lens[layer] = len + rows;
   if (flags & (RV_HOST_PTRS | RV_SYNC)) {
-    hipError_t e = hipStreamSynchronize(kv->stream);
+    hipError_t e = hipStreamSynchronize(kv->order.stream);
     if (e != hipSuccess) return hip_fail(err, e, "hipStreamSynchronize");
   }
   return ok(err);
@@ -781,7 +781,8 @@ int32_t rv_kv_read_rows(const rv_kv* ckv, size_t layer, size_t pos, size_t rows,
     return fail(err, RV_KV_POSITION_OUT_OF_RANGE, layer, sat_add(pos, rows ? rows - 1 : 0), len);
   if (rows == 0) return ok(err);
   if (!k && !v) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, "k and v");
-  DeviceGuard dg(kv->device);
+  const Queued queued(kv);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
   const size_t n = rows * kv->kv_dim;
   float *dk = k, *dv = v;
   if (flags & RV_HOST_PTRS) {
@@ -790,10 +791,10 @@ int32_t rv_kv_read_rows(const rv_kv* ckv, size_t layer, size_t pos, size_t rows,
     dk = k ? st.carve(n) : nullptr;
     dv = v ? st.carve(n) : nullptr;
   }
-  rv::HipStatus hs = rv::launch_read_rows(kv, layer, pos, rows, dk, dv, kv->stream);
+  rv::HipStatus hs = rv::launch_read_rows(kv, layer, pos, rows, dk, dv, kv->order.stream);
   if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
   if ((flags & RV_HOST_PTRS) && k && v) {
-    const hipError_t e = hipMemcpyAsync(k, dk, n * 4, hipMemcpyDeviceToHost, kv->stream);
+    const hipError_t e = hipMemcpyAsync(k, dk, n * 4, hipMemcpyDeviceToHost, kv->order.stream);
     if (e != hipSuccess) return hip_fail(err, e, "hipMemcpyAsync D2H");
   }
   return v ? finish(kv, flags, dv, v, n, err) : finish(kv, flags, dk, k, n, err);
@@ -810,7 +811,8 @@ int32_t rv_kv_append_each(rv_kv* kv, size_t layer0, size_t n, const float* k, co
   if ((rc = check_room(kv, layer0, n, err))) return rc;
   if (kv->capacity > kMaxRows) return fail(err, RV_ERR_UNSUPPORTED, kv->capacity, 0, 0, 0, "position past 2^31");
   if (!k || !v) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, !k ? "k" : "v");
-  DeviceGuard dg(kv->device);
+  const Queued queued(kv);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
   const float *dk = k, *dv = v;
   if (flags & RV_HOST_PTRS) {
     Stager st(kv);
@@ -823,12 +825,12 @@ int32_t rv_kv_append_each(rv_kv* kv, size_t layer0, size_t n, const float* k, co
   for (size_t r0 = 0; r0 < n; r0 += rv::kMaxEach) {
     const size_t m = std::min<size_t>(rv::kMaxEach, n - r0);
     const rv::HipStatus hs = rv::launch_append_dst(kv, each_dst(kv, layer0, r0, m, 0), dk + r0 * kv->kv_dim,
-                                                   dv + r0 * kv->kv_dim, m, kv->stream);
+                                                   dv + r0 * kv->kv_dim, m, kv->order.stream);
     if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
   }
   for (size_t i = 0; i < n; ++i) kv->lens[layer0 + i] += 1;
   if (flags & (RV_HOST_PTRS | RV_SYNC)) {
-    const hipError_t e = hipStreamSynchronize(kv->stream);
+    const hipError_t e = hipStreamSynchronize(kv->order.stream);
     if (e != hipSuccess) return hip_fail(err, e, "hipStreamSynchronize");
   }
   return ok(err);
@@ -844,7 +846,8 @@ int32_t rv_decode_attention_shared(const rv_kv* prefix, size_t prefix_layer, siz
       shared_check(prefix, prefix_layer, prefix_positions, tails, tail_layer, n_seqs, q_dim, false, err);
   if (rc) return rc;
   if (!q_rows || !out) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, !q_rows ? "q_rows" : "out");
-  DeviceGuard dg(tails->device);
+  const Queued queued(tails, prefix);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
   const size_t n = n_seqs * q_dim;
   const float* dq = q_rows;
   float* dout = out;
@@ -857,7 +860,7 @@ int32_t rv_decode_attention_shared(const rv_kv* prefix, size_t prefix_layer, siz
   }
   const rv::HipStatus hs = rv::launch_rows(
       tails, shared_call(prefix, prefix_layer, prefix_positions, tails, tail_layer, dq, n_seqs, q_dim, scale, dout),
-      tails->stream);
+      tails->order.stream);
   if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
   return finish(tails, flags, dout, out, n, err);
 }
@@ -876,7 +879,8 @@ int32_t rv_decode_step_shared(const rv_kv* prefix, size_t prefix_layer, size_t p
     return rc;
   if (!q_rows || !k_rows || !v_rows || !q_norm_w || !k_norm_w || !out)
     return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, "tensor");
-  DeviceGuard dg(tails->device);
+  const Queued queued(tails, prefix);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
   const size_t hd = tails->head_dim, kvd = tails->kv_dim, nq = n_seqs * q_dim, nk = n_seqs * kvd;
   const float *dq = q_rows, *dk = k_rows, *dv = v_rows, *dwq = q_norm_w, *dwk = k_norm_w;
   float* dout = out;
@@ -900,14 +904,14 @@ int32_t rv_decode_step_shared(const rv_kv* prefix, size_t prefix_layer, size_t p
     const size_t m = std::min<size_t>(rv::kMaxEach, n_seqs - r0);
     hs = rv::launch_prologue_dst(tails, each_dst(tails, tail_layer, r0, m, prefix_positions), dq + r0 * q_dim,
                                  tails->qbuf + r0 * q_dim, n_q, dk + r0 * kvd, dv + r0 * kvd, m, dwq, dwk, eps, inv,
-                                 tails->stream);
+                                 tails->order.stream);
   }
   if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
   for (size_t i = 0; i < n_seqs; ++i) tails->lens[tail_layer + i] += 1;
   hs = rv::launch_rows(tails,
                        shared_call(prefix, prefix_layer, prefix_positions, tails, tail_layer, tails->qbuf, n_seqs,
                                    q_dim, scale, dout),
-                       tails->stream);
+                       tails->order.stream);
   if (hs.e != hipSuccess) {
     for (size_t i = 0; i < n_seqs; ++i) tails->lens[tail_layer + i] -= 1;
     return hip_fail(err, hs.e, hs.what);
@@ -939,23 +943,24 @@ int32_t rv_kv_read_row(const rv_kv* kv, int plane_v, size_t layer, size_t pos, v
   if (rc) return rc;
   const size_t len = kv->lens[layer];
   if (pos >= len) return fail(err, RV_KV_POSITION_OUT_OF_RANGE, layer, pos, len);
-  DeviceGuard dg(kv->device);
+  const Queued queued(kv);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
   if (kv->elem == RV_ELEM_Q8_0) {
     rv_kv* m = const_cast<rv_kv*>(kv);
     Stager st(m);
     const size_t bytes = kv->kv_dim / 32 * 34;
     if (!st.reserve(Stager::align(bytes))) return hip_fail(err, st.e, "hipMalloc stage");
-    const rv::HipStatus hs = rv::launch_read_blocks(kv, plane_v, layer, pos, (uint8_t*)m->stage, kv->stream);
+    const rv::HipStatus hs = rv::launch_read_blocks(kv, plane_v, layer, pos, (uint8_t*)m->stage, kv->order.stream);
     if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
-    hipError_t e = hipMemcpyAsync(dst, m->stage, bytes, hipMemcpyDeviceToHost, kv->stream);
-    if (e == hipSuccess) e = hipStreamSynchronize(kv->stream);
+    hipError_t e = hipMemcpyAsync(dst, m->stage, bytes, hipMemcpyDeviceToHost, kv->order.stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(kv->order.stream);
     if (e != hipSuccess) return hip_fail(err, e, "read_row");
     return ok(err);
   }
   const size_t es = kv->elem_size();
   const char* src = (plane_v ? kv->v_layer(layer) : kv->k_layer(layer)) + pos * kv->kv_dim * es;
-  hipError_t e = hipMemcpyAsync(dst, src, kv->kv_dim * es, hipMemcpyDeviceToHost, kv->stream);
-  if (e == hipSuccess) e = hipStreamSynchronize(kv->stream);
+  hipError_t e = hipMemcpyAsync(dst, src, kv->kv_dim * es, hipMemcpyDeviceToHost, kv->order.stream);
+  if (e == hipSuccess) e = hipStreamSynchronize(kv->order.stream);
   if (e != hipSuccess) return hip_fail(err, e, "read_row");
   return ok(err);
 }
@@ -980,15 +985,16 @@ int32_t rv_decode_attention_noalloc(const rv_kv* ckv, const float* q, size_t q_l
   const size_t need = rv::decode_ws_need(kv, p.n_q_heads, p.positions, kv->n_kv_heads);
   if (need > rv::kNoAllocScratchBytes)
     return fail(err, RV_ERR_UNSUPPORTED, need, rv::kNoAllocScratchBytes, 0, 0, "decode scratch above the no-alloc limit");
-  DeviceGuard dg(kv->device);
+  const Queued queued(kv);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
   void* base = nullptr;
   rv::HipStatus hs = rv::noalloc_scratch(kv->device, &base);
   if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
   const rv::Workspace ws{base, rv::kNoAllocScratchBytes};
-  hs = rv::launch_decode(kv, q, p.n_q_heads, layer, p.positions, scale, 0, kv->n_kv_heads, out, kv->stream, &ws);
+  hs = rv::launch_decode(kv, q, p.n_q_heads, layer, p.positions, scale, 0, kv->n_kv_heads, out, kv->order.stream, &ws);
   if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
   if (flags & RV_SYNC) {
-    const hipError_t e = hipStreamSynchronize(kv->stream);
+    const hipError_t e = hipStreamSynchronize(kv->order.stream);
     if (e != hipSuccess) return hip_fail(err, e, "hipStreamSynchronize");
   }
   return ok(err);
@@ -1057,13 +1063,13 @@ static int32_t run_rows(rv_kv* kv, const float* dq, size_t rows, size_t q_dim, s
     c.scale = scale;
     c.out = dout;
     c.split = (flags & RV_PREFILL_MODE_MASK) == RV_PREFILL_EXACT;
-    hs = rv::launch_rows(kv, c, kv->stream);
+    hs = rv::launch_rows(kv, c, kv->order.stream);
   } else if (rv::prefill_supported(kv, p.group, start + rows)) {
-    hs = rv::launch_prefill(kv, dq, rows, p.n_q_heads, layer, start, scale, dout, flags, nullptr, kv->stream);
+    hs = rv::launch_prefill(kv, dq, rows, p.n_q_heads, layer, start, scale, dout, flags, nullptr, kv->order.stream);
   } else {
     for (size_t r = 0; r < rows && hs.e == hipSuccess; ++r)
       hs = rv::launch_decode(kv, dq + r * q_dim, p.n_q_heads, layer, start + r + 1, scale, 0, kv->n_kv_heads,
-                             dout + r * q_dim, kv->stream);
+                             dout + r * q_dim, kv->order.stream);
   }
   if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
   return RV_OK;
@@ -1078,7 +1084,8 @@ int32_t rv_attention_at_rows(const rv_kv* ckv, const float* q_rows, size_t rows,
   int32_t rc = rows_plan(kv, rows, q_dim, layer, start, &p, err);
   if (rc) return rc;
   if (!q_rows || !out) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, !q_rows ? "q_rows" : "out");
-  DeviceGuard dg(kv->device);
+  const Queued queued(kv);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
   const size_t n = rows * q_dim;
   const float* dq = q_rows;
   float* dout = out;
@@ -1114,7 +1121,8 @@ int32_t rv_decode_step(rv_kv* kv, size_t layer, const float* q, size_t q_len, co
   if (out_len != q_len) return fail(err, RV_ATTN_OUT_LEN_MISMATCH, out_len, q_len);
   if (position > 0xFFFFFFFFull) return fail(err, RV_ERR_UNSUPPORTED, position, 0, 0, 0, "position past u32");
   if (!q || !k || !v || !q_norm_w || !k_norm_w || !out) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, "tensor");
-  DeviceGuard dg(kv->device);
+  const Queued queued(kv);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
   const float *dq = q, *dk = k, *dv = v, *dwq = q_norm_w, *dwk = k_norm_w;
   float* dout = out;
   if (flags & RV_HOST_PTRS) {
@@ -1144,7 +1152,7 @@ int32_t rv_decode_step(rv_kv* kv, size_t layer, const float* q, size_t q_len, co
       pro.sn[i] = (float)sd;
     }
     kv->lens[layer] = len + 1;
-    rv::HipStatus hs = rv::launch_decode_pro(kv, dq, n_q, layer, len + 1, scale, pro, dout, kv->stream);
+    rv::HipStatus hs = rv::launch_decode_pro(kv, dq, n_q, layer, len + 1, scale, pro, dout, kv->order.stream);
     if (hs.e != hipSuccess) {
       kv->lens[layer] = len;
       return hip_fail(err, hs.e, hs.what);
@@ -1160,14 +1168,14 @@ int32_t rv_decode_step(rv_kv* kv, size_t layer, const float* q, size_t q_len, co
     dst.layer = layer;
     dst.row0 = (long)len;
     dst.pos0 = (long)position;
-    hs = rv::launch_prologue_dst(kv, dst, dq, kv->qbuf, n_q, dk, dv, 1, dwq, dwk, eps, inv, kv->stream);
+    hs = rv::launch_prologue_dst(kv, dst, dq, kv->qbuf, n_q, dk, dv, 1, dwq, dwk, eps, inv, kv->order.stream);
   } else {
     hs = rv::launch_row_prologue(kv, layer, len, dq, kv->qbuf, n_q, dk, dv, 1, dwq, dwk, eps, inv, position, nullptr,
-                                 nullptr, kv->stream);
+                                 nullptr, kv->order.stream);
   }
   if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
   kv->lens[layer] = len + 1;
-  hs = rv::launch_decode(kv, kv->qbuf, n_q, layer, len + 1, scale, 0, kv->n_kv_heads, dout, kv->stream);
+  hs = rv::launch_decode(kv, kv->qbuf, n_q, layer, len + 1, scale, 0, kv->n_kv_heads, dout, kv->order.stream);
   if (hs.e != hipSuccess) {
     kv->lens[layer] = len;  // (the row is as if never appended: the step can be called again)
     return hip_fail(err, hs.e, hs.what);
@@ -1190,7 +1198,8 @@ int32_t rv_decode_step_dev(rv_kv* kv, size_t layer, const float* q, size_t q_len
   if (!q || !k || !v || !q_norm_w || !k_norm_w || !out || !d_position)
     return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, "tensor");
   if (flags & RV_HOST_PTRS) return fail(err, RV_ERR_UNSUPPORTED, flags, 0, 0, 0, "RV_HOST_PTRS (device pointers only)");
-  DeviceGuard dg(kv->device);
+  const Queued queued(kv);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
   if (kv->elem == RV_ELEM_Q8_0) {
     rv::InvFreq inv;
     rv::fill_inv_freq(inv, kv->head_dim, theta);
@@ -1202,7 +1211,7 @@ int32_t rv_decode_step_dev(rv_kv* kv, size_t layer, const float* q, size_t q_len
     dst.status = rv::dev_status(kv);
     const size_t n_q = q_len / kv->head_dim;
     if (hs.e == hipSuccess)
-      hs = rv::launch_prologue_dst(kv, dst, q, kv->qbuf, n_q, k, v, 1, q_norm_w, k_norm_w, eps, inv, kv->stream);
+      hs = rv::launch_prologue_dst(kv, dst, q, kv->qbuf, n_q, k, v, 1, q_norm_w, k_norm_w, eps, inv, kv->order.stream);
     if (hs.e == hipSuccess) {
       rv::RowsCall c;
       c.main = kv;
@@ -1215,7 +1224,7 @@ int32_t rv_decode_step_dev(rv_kv* kv, size_t layer, const float* q, size_t q_len
       c.scale = scale;
       c.out = out;
       c.d_pos = d_position;
-      hs = rv::launch_rows(kv, c, kv->stream);
+      hs = rv::launch_rows(kv, c, kv->order.stream);
     }
     if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
     return finish(kv, flags, out, out, q_len, err);
@@ -1224,7 +1233,7 @@ int32_t rv_decode_step_dev(rv_kv* kv, size_t layer, const float* q, size_t q_len
   if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
   rv::DecodePro pro{k, v, q_norm_w, k_norm_w, eps, {}, {}, d_position, kv->rope_tab, (int)max_position,
                     rv::dev_status(kv), (uint32_t)layer};
-  hs = rv::launch_decode_pro(kv, q, q_len / kv->head_dim, layer, max_position + 1, scale, pro, out, kv->stream);
+  hs = rv::launch_decode_pro(kv, q, q_len / kv->head_dim, layer, max_position + 1, scale, pro, out, kv->order.stream);
   if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
   return finish(kv, flags, out, out, q_len, err);
 }
@@ -1246,9 +1255,10 @@ int32_t rv_kv_commit(rv_kv* kv, size_t layer, size_t rows, rv_error* err) {
 // [3] the step's max_position + 1. Read after the stream drains, then cleared.
 int32_t rv_kv_device_status(rv_kv* kv, rv_error* err) {
   if (!kv) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, "kv");
-  DeviceGuard dg(kv->device);
+  const Queued queued(kv);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
   uint32_t w[4] = {0, 0, 0, 0};
-  hipError_t e = kv->stream ? hipStreamSynchronize(kv->stream) : hipDeviceSynchronize();
+  hipError_t e = kv->order.stream ? hipStreamSynchronize(kv->order.stream) : hipDeviceSynchronize();
   if (e == hipSuccess) e = hipMemcpy(w, rv::dev_status(kv), sizeof(w), hipMemcpyDeviceToHost);
   if (e != hipSuccess) return hip_fail(err, e, "read the device status");
   if (w[0] == 0) return ok(err);
@@ -1314,8 +1324,9 @@ int32_t rv_kv_xcd_dealing(rv_kv* kv, int32_t* ok_out, rv_error* err) {
 int32_t rv_position_advance(rv_kv* kv, uint32_t* d_position, uint32_t n, rv_error* err) {
   if (!kv) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, "kv");
   if (!d_position) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, "d_position");
-  DeviceGuard dg(kv->device);
-  const rv::HipStatus hs = rv::launch_position_advance(d_position, n, kv->stream);
+  const Queued queued(kv);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
+  const rv::HipStatus hs = rv::launch_position_advance(d_position, n, kv->order.stream);
   if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
   return ok(err);
 }
@@ -1340,7 +1351,8 @@ int32_t rv_prefill_chunk(rv_kv* kv, size_t layer, const float* q_rows, const flo
   if (rows == 0) return ok(err);
   if (!q_rows || !k_rows || !v_rows || !q_norm_w || !k_norm_w || !out)
     return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, "tensor");
-  DeviceGuard dg(kv->device);
+  const Queued queued(kv);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
   const size_t nq = rows * q_dim, nk = rows * kv->kv_dim;
   const float *dq = q_rows, *dk = k_rows, *dv = v_rows, *dwq = q_norm_w, *dwk = k_norm_w;
   float* dout = out;
@@ -1367,7 +1379,7 @@ int32_t rv_prefill_chunk(rv_kv* kv, size_t layer, const float* q_rows, const flo
     // layout; otherwise it writes the rows' (cos, sin) table and the q
     // prologue runs inside the attention kernel's query loads.
     rv::StageDst sd;
-    hs = rv::prepare_prefill_stage(kv, layer, len, rows, flags, kv->stream, &sd);
+    hs = rv::prepare_prefill_stage(kv, layer, len, rows, flags, kv->order.stream, &sd);
     // (The preparation reads q and its norm weight with 16-byte loads.)
     const bool prep = sd.base != nullptr && ((uintptr_t)dq % 16) == 0 && ((uintptr_t)dwq % 16) == 0 &&
                       q_dim % 4 == 0;
@@ -1383,12 +1395,12 @@ int32_t rv_prefill_chunk(rv_kv* kv, size_t layer, const float* q_rows, const flo
     if (hs.e == hipSuccess)
       hs = rv::launch_row_prologue(kv, layer, len, prep ? dq : nullptr, nullptr, prep ? p.n_q_heads : 0, dk, dv, rows,
                                    prep ? dwq : nullptr, dwk, eps, inv, start, prep ? nullptr : kv->qbuf, &sd,
-                                   kv->stream, prep ? &qp : nullptr);
+                                   kv->order.stream, prep ? &qp : nullptr);
     if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
     kv->lens[layer] = len + rows;
     rv::QNorm qn{dwq, eps, kv->qbuf};
     if (prep) qn.prepped = (const char*)kv->qbuf;
-    hs = rv::launch_prefill(kv, dq, rows, p.n_q_heads, layer, start, scale, dout, flags, &qn, kv->stream);
+    hs = rv::launch_prefill(kv, dq, rows, p.n_q_heads, layer, start, scale, dout, flags, &qn, kv->order.stream);
     if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
   } else {
     hs = rv::ensure_qbuf(kv, nq * sizeof(float));
@@ -1397,10 +1409,10 @@ int32_t rv_prefill_chunk(rv_kv* kv, size_t layer, const float* q_rows, const flo
       dst.layer = layer;
       dst.row0 = (long)len;
       dst.pos0 = (long)start;
-      hs = rv::launch_prologue_dst(kv, dst, dq, kv->qbuf, q_dim / hd, dk, dv, rows, dwq, dwk, eps, inv, kv->stream);
+      hs = rv::launch_prologue_dst(kv, dst, dq, kv->qbuf, q_dim / hd, dk, dv, rows, dwq, dwk, eps, inv, kv->order.stream);
     } else if (hs.e == hipSuccess) {
       hs = rv::launch_row_prologue(kv, layer, len, dq, kv->qbuf, q_dim / hd, dk, dv, rows, dwq, dwk, eps, inv, start,
-                                   nullptr, nullptr, kv->stream);
+                                   nullptr, nullptr, kv->order.stream);
     }
     if (hs.e != hipSuccess) return hip_fail(err, hs.e, hs.what);
     kv->lens[layer] = len + rows;
@@ -1434,8 +1446,9 @@ int32_t rv_kv_set_tuning(rv_kv* kv, int32_t knob, int64_t value, rv_error* err) 
 int32_t rv_kv_kernel_time(rv_kv* kv, double* total_ms, uint64_t* launches, rv_error* err) {
   if (!kv) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, "kv");
   if (!total_ms || !launches) return fail(err, RV_ERR_NULL_ARG, 0, 0, 0, 0, !total_ms ? "total_ms" : "launches");
-  DeviceGuard dg(kv->device);
-  const hipError_t e = kv->stream ? hipStreamSynchronize(kv->stream) : hipDeviceSynchronize();
+  const Queued queued(kv);
+  if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
+  const hipError_t e = kv->order.stream ? hipStreamSynchronize(kv->order.stream) : hipDeviceSynchronize();
   if (e != hipSuccess) return hip_fail(err, e, "synchronize before reading kernel times");
   rv::timing_fold(kv);
   *total_ms = kv->timed_ms;

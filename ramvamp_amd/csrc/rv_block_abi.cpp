@@ -95,7 +95,7 @@ static int32_t block_decode(rv_kv* kv, size_t layer, float* residual, size_t hid
   int prev = -1;
   if (hipGetDevice(&prev) != hipSuccess) prev = -1;
   if (prev != kv->device) (void)hipSetDevice(kv->device);
-  const hipStream_t s = kv->stream;
+  const hipStream_t s = kv->order.stream;
   rv::HipStatus st = rv::in_proj_launch(in, s);
   if (st.e != hipSuccess) rc = fail(err, RV_ERR_HIP, (uint64_t)st.e, 0, st.what);
   if (!rc && d_position)
@@ -186,7 +186,7 @@ int32_t rv_attn_block_prefill(rv_kv* kv, size_t layer, float* residual_rows, siz
   int prev = -1;
   if (hipGetDevice(&prev) != hipSuccess) prev = -1;
   if (prev != kv->device) (void)hipSetDevice(kv->device);
-  const hipStream_t s = kv->stream;
+  const hipStream_t s = kv->order.stream;
   rv::HipStatus st = rv::in_proj_rows_launch(in, n, s);
   if (st.e != hipSuccess) rc = fail(err, RV_ERR_HIP, (uint64_t)st.e, 0, st.what);
   if (!rc)

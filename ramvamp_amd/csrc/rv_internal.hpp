@@ -13,6 +13,40 @@
 #include "../../include/ramvamp_attn.h"
 #include "rv_order.hpp"
 
+namespace rv {
+
+// Whether work on s is being captured into a graph.
+bool capturing(hipStream_t s);
+
+// What a cache's StreamOrder asks of HIP; calls are made with its device current.
+struct HipStreams {
+  typedef hipStream_t Stream;
+  typedef hipError_t Error;
+  static constexpr hipError_t kUnsupported = hipErrorStreamCaptureUnsupported;
+  hipEvent_t ev = nullptr;
+
+  static bool capturing(hipStream_t s) { return rv::capturing(s); }
+  static bool recordable(hipStream_t s) {
+    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+    const bool is = hipStreamIsCapturing(s, &cs) == hipSuccess && cs == hipStreamCaptureStatusNone;
+    if (!is) (void)hipGetLastError();
+    return is;
+  }
+  hipError_t record(hipStream_t s) {
+    if (!ev) {
+      const hipError_t e = hipEventCreateWithFlags(&ev, hipEventDisableTiming);
+      if (e != hipSuccess) {
+        ev = nullptr;
+        return e;
+      }
+    }
+    return hipEventRecord(ev, s);
+  }
+  hipError_t wait(hipStream_t s) { return hipStreamWaitEvent(s, ev, 0); }
+};
+
+}  // namespace rv
+
 struct rv_kv {
   size_t n_layers = 0, n_kv_heads = 0, head_dim = 0, capacity = 0, kv_dim = 0, plane = 0;
   int elem = RV_ELEM_F16;
@@ -20,7 +54,7 @@ struct rv_kv {
   void* k = nullptr;  // [n_layers][capacity][kv_dim], elem-sized, device (Q8_0: rv_rows.hpp)
   void* v = nullptr;
   std::vector<size_t> lens;  // per-layer cursors (kv/mod.rs:147), host-side
-  hipStream_t stream = nullptr;
+  rv::StreamOrder<rv::HipStreams> order;  // order.stream: what calls are queued on
 
   // Device workspace, grown on first need and then reused by every call:
   // decode and prefill split partials, normalised q rows / RoPE tables.
@@ -40,9 +74,6 @@ struct rv_kv {
   // arriver resets its own): 9 * n_kv_heads counters, one per 128-byte line;
   // then the device status words (rv_kv_device_status).
   unsigned* tickets = nullptr;
-  // Recorded on the old stream when rv_kv_set_stream moves the cache to a
-  // new one, which then waits for it.
-  hipEvent_t order_ev = nullptr;
   // Prefill's staged copy of each layer's K/V tiles (MFMA type and LDS
   // layout), kept across calls so a reused prefix is converted once:
   // positions [0, staged_pos[layer]) are current for staged_mode[layer].
@@ -136,35 +167,6 @@ constexpr long kCUs = 256;
 // grows it), and the old buffer is retired, not freed. Growth under graph
 // capture is refused with hipErrorStreamCaptureUnsupported.
 HipStatus ensure_workspace(rv_kv* kv, size_t bytes, size_t bound = 0);
-// Whether work on s is being captured into a graph.
-bool capturing(hipStream_t s);
-
-// What a cache's StreamOrder asks of HIP; calls are made with its device current.
-struct HipStreams {
-  typedef hipStream_t Stream;
-  typedef hipError_t Error;
-  static constexpr hipError_t kUnsupported = hipErrorStreamCaptureUnsupported;
-  hipEvent_t ev = nullptr;
-
-  static bool capturing(hipStream_t s) { return rv::capturing(s); }
-  static bool recordable(hipStream_t s) {
-    hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
-    const bool is = hipStreamIsCapturing(s, &cs) == hipSuccess && cs == hipStreamCaptureStatusNone;
-    if (!is) (void)hipGetLastError();
-    return is;
-  }
-  hipError_t record(hipStream_t s) {
-    if (!ev) {
-      const hipError_t e = hipEventCreateWithFlags(&ev, hipEventDisableTiming);
-      if (e != hipSuccess) {
-        ev = nullptr;
-        return e;
-      }
-    }
-    return hipEventRecord(ev, s);
-  }
-  hipError_t wait(hipStream_t s) { return hipStreamWaitEvent(s, ev, 0); }
-};
 // The normalised-q buffer, with the workspace's growth rules.
 HipStatus ensure_qbuf(rv_kv* kv, size_t bytes);
 // RV_ERR_UNSUPPORTED for a call that would have to allocate under graph

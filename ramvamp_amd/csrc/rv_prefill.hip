@@ -1825,7 +1825,7 @@ HipStatus launch_prefill(rv_kv* kv, const float* q_rows, size_t rows, size_t n_q
 HipStatus ensure_prefill_tickets(rv_kv* kv, size_t units) {
   HipStatus st;
   if (units <= kv->pf_ticket_units) return st;
-  if (capturing(kv->stream)) {
+  if (capturing(kv->order.stream)) {
     st.e = hipErrorStreamCaptureUnsupported;
     st.what = "prefill ticket growth under graph capture (run a call of this shape uncaptured first)";
     return st;

@@ -159,3 +159,44 @@ def test_device_bytes_account_for_everything_the_cache_allocates(elem):
     qbuf = rows * hd * 4  # at least the chunk's (cos, sin) rows, or its prepared queries
     assert now2 - now1 >= exact_copy + f16_copy + qbuf, (now2 - now1)
     assert now2 <= bound2 and bound2 >= bound0
+
+
+@pytest.mark.parametrize("back", [False, True])
+def test_calls_behind_a_capture_wait_for_those_before_it(back):
+    """An append on one stream, held up there, a step captured on a second without a wait
+    for the device, then rows read on a third, or on the second itself."""
+    torch = torch_cuda()
+    say(f"case behind a capture {back}")
+    rng = np.random.default_rng(7)
+    kv = rv.KvCache(1, 4, 128, 64, "f16")
+    k, v = (rng.standard_normal((20, 512)).astype(np.float32) for _ in range(2))
+    kd, vd, q, out = dev(k), dev(v), dev(rng.standard_normal(4096)), torch.empty(4096, device="cuda")
+    big = torch.ones(8192, 8192, device="cuda")
+    first, second, third = (torch.cuda.Stream() for _ in range(3))
+    with torch.cuda.stream(second):
+        kv.append_rows(0, kd[:10], vd[:10])
+        rv.decode_attention(q, kv, 0, 128 ** -0.5, None, out)  # (allocates)
+    with torch.cuda.stream(first):
+        hold = big @ big
+    torch.cuda.synchronize()
+    with torch.cuda.stream(first):
+        for _ in range(8):
+            torch.mm(big, big, out=hold)
+        kv.append_rows(0, kd[10:], vd[10:])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(second):
+        g.capture_begin()
+        rv.decode_attention(q, kv, 0, 128 ** -0.5, None, out)
+        g.capture_end()
+    with torch.cuda.stream(second if back else third):
+        gk, gv = kv.read_rows(0, 10, 10)
+    torch.cuda.synchronize()
+    assert np.array_equal(gk.cpu().numpy(), k[10:].astype(np.float16).astype(np.float32))
+    assert np.array_equal(gv.cpu().numpy(), v[10:].astype(np.float16).astype(np.float32))
+    out.fill_(float("nan"))
+    g.replay()
+    want = torch.empty_like(out)
+    torch.cuda.synchronize()
+    rv.decode_attention(q, kv, 0, 128 ** -0.5, None, want)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
