@@ -772,7 +772,7 @@ __global__ __launch_bounds__(256, WAVES) void paged_attn_kernel(PagedView w, Att
   __shared__ unsigned drawn;
   const int lane = threadIdx.x & 63;
   const uint32_t items = (uint32_t)(w.n_kv * a.blocks);
-  const Turn turn = a.turns[blockIdx.x];
+  const Turn turn = a.turns[own_turn(blockIdx.x, gridDim.x)];
   unsigned* const tickets = a.tickets + (turn.set ? a.set_words : 0);
   // Sequence i's rows, for the 64 from s0 on a lane each.
   auto chunk = [&](uint32_t s0) {
@@ -791,6 +791,14 @@ __global__ __launch_bounds__(256, WAVES) void paged_attn_kernel(PagedView w, Att
   const uint32_t per = cut.per, in_slot = cut.in_slot, slot = slot_of(blockIdx.x, a.slots);
   const uint32_t ranges = in_slot << a.slots, r = range_of(blockIdx.x, a.slots, in_slot);
   const uint32_t start = r * per, end = blockIdx.x < ranges ? min(total, start + per) : 0;
+  // By the wave that draws tickets, and here, where nothing waits for its stores: 100 rows
+  // 5.7 us, 6.0 at the end.
+  if (threadIdx.x < 64) {
+    unsigned* const other = a.tickets + (turn.set ? 0 : a.set_words);
+    end_turn(
+        turn, blockIdx.x, gridDim.x, threadIdx.x, 64, a.n_tickets, [&](uint32_t c, Turn next) { a.turns[c] = next; },
+        [&](size_t i) { other[i] = 0; });
+  }
   if (start < end) {
     uint32_t s0 = 0;
     while (s0 < a.n) {  // the chunk that holds the range's first unit (none: the lengths have been changed)
@@ -861,12 +869,6 @@ __global__ __launch_bounds__(256, WAVES) void paged_attn_kernel(PagedView w, Att
             join<Inner::kVec, Inner::kLanes, kDeviceScope>(pt, piece0, rest, count, ncols, out, 0);
         },
         divide);
-  }
-  if (threadIdx.x < 64) {  // (the wave that has drawn the tickets)
-    unsigned* const other = a.tickets + (turn.set ? 0 : a.set_words);
-    end_turn(
-        turn, blockIdx.x, gridDim.x, threadIdx.x, 64, a.n_tickets, [&](uint32_t c, Turn next) { a.turns[c] = next; },
-        [&](size_t i) { other[i] = 0; });
   }
   // Sequences without rows: zeros; refused ones: NaN.
   for (uint32_t s = blockIdx.x; s < a.n; s += gridDim.x) {

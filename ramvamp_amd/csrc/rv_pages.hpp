@@ -180,13 +180,15 @@ RV_HD Pieces pieces_of(const Group& g, uint32_t w0, uint32_t w1, uint32_t item_s
 // cleared. So a launch finds zeros whatever was left of earlier ones, also of one whose
 // lengths were changed while it ran, and whose workgroups did not agree on the pieces.
 // Whose turn it is each workgroup reads from a word of its own, which it alone writes
-// in the launch: of kTurns words, those that are its number modulo the launch's grid (a
-// power of two). All are equal between launches.
+// in the launch: kTurns words are shared out evenly over the launch's grid (a power of
+// two). All are equal between launches.
 constexpr uint32_t kTurns = 512;
 
 struct Turn {
   uint32_t set, used;  // the set that counts, and the tickets of the other to be cleared
 };
+
+RV_HD uint32_t own_turn(uint32_t block, uint32_t grid) { return block * (kTurns / grid); }
 
 RV_HD size_t set_words(size_t tickets) { return (tickets + kLineFloats - 1) / kLineFloats * kLineFloats; }
 
@@ -195,7 +197,7 @@ RV_HD size_t set_words(size_t tickets) { return (tickets + kLineFloats - 1) / kL
 template <typename Pass, typename Clear>
 RV_HD void end_turn(Turn t, uint32_t block, uint32_t grid, uint32_t lane, uint32_t lanes, uint32_t tickets, Pass pass,
                     Clear clear) {
-  for (uint32_t c = block + lane * grid; c < kTurns; c += lanes * grid) pass(c, Turn{1 - t.set, tickets});
+  for (uint32_t c = lane; c < kTurns / grid; c += lanes) pass(own_turn(block, grid) + c, Turn{1 - t.set, tickets});
   for (size_t i = (size_t)block * lanes + lane; i < t.used; i += (size_t)grid * lanes) clear(i);
 }
 

@@ -56,7 +56,7 @@ static void turns() {
       std::shuffle(order.begin(), order.end(), g);
       uint32_t last = 0;
       for (uint32_t b : order) {
-        const Turn t = turn[b];
+        const Turn t = turn[own_turn(b, grid)];
         CHECK(t.set == set && t.used <= words, "run %d launch %d: workgroup %u's turn", run, launch, b);
         if (agree)
           last += tickets[t.set * words]++ == grid - 1;  // one item of all workgroups
