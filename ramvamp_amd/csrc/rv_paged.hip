@@ -201,6 +201,12 @@ __device__ __forceinline__ void store_row(const PagedView& w, bool is_v, int h, 
     }
   } else {
     T* p = reinterpret_cast<T*>(is_v ? w.v : w.k) + at * w.hd + d;
+    if constexpr (std::is_same<T, float>::value) {
+      bool large = false;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) large |= is_v && (__float_as_uint(y[e]) & 0x7FFFFFFFu) - 0x6F800000u < 0x10000000u;
+      if (large) w.status[kLarge] = 1;
+    }
     if (w.hd % 8 == 0) {
       if constexpr (std::is_same<T, float>::value) {
         *reinterpret_cast<f32x4*>(p) = y.a;

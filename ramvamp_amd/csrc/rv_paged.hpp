@@ -34,7 +34,7 @@ struct rv_paged {
   void* k = nullptr;
   void* v = nullptr;
   rv::StreamOrder<rv::HipStreams> order;  // order.stream: what calls are queued on
-  unsigned* status = nullptr;  // [0] code, [1] layer, [2] row, [3] what it read, [4] the bound
+  unsigned* status = nullptr;  // [0] code, [1] layer, [2] row, [3] what it read, [4] the bound, [kLarge]
   // Grown on first need; a replaced buffer is kept until the cache is freed,
   // since a graph captured earlier may still address it.
   void* ws = nullptr;  // attention's partials
@@ -77,6 +77,10 @@ struct RopeArgs {
   double freq[N];
 };
 constexpr int kFewPairs = 64;
+
+// The word beside the status that says whether f32 pages have ever held a finite value of
+// V of 2^96 or more: where none has, no sum of up to 2^31 of them passes the floats' range.
+constexpr int kLarge = 16;
 
 // Records a refusal: the first since the last read stays.
 __device__ __forceinline__ void paged_refuse(const PagedView& w, uint32_t code, uint32_t row, uint32_t got,

@@ -2,7 +2,9 @@
 // over its pages.
 //
 // o = sum_t p_t v_t / sum_t p_t, p_t = exp(scale * (q . k_t) - m), in one pass over
-// the rows with the running maximum m.
+// the rows with the running maximum m. Where f32 pages may hold values of V whose sum
+// over the sequence's n rows passes the floats' range, p_t is times 2^-k < 1 / (2 n)
+// in numerator and denominator alike.
 //
 // The lengths are on the device and ragged, so the work is dealt there: a unit is
 // kUnitRows rows of one item (a sequence's kv head, or a part of its query
@@ -79,6 +81,15 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
   return x;
 }
 
+// A power of two that n weights of at most 1 each times it make less than one half of.
+__device__ __forceinline__ float weight_unit(uint32_t n) { return ldexpf(1.f, __builtin_clz(n) - 33); }
+
+// y, the average that a sum o gives of values that may be `large`: of finite ones finite,
+// whatever its last rounding.
+__device__ __forceinline__ float average(float o, float y, bool large) {
+  return large && __builtin_isinf(y) && !__builtin_isinf(o) ? __builtin_copysignf(0x1.fffffep127f, y) : y;
+}
+
 // ---- partials ---------------------------------------------------------------------
 
 // Cache policies of the buffer instructions: the sc1 bit, device scope; the sc0 bit of a
@@ -132,7 +143,7 @@ constexpr uint32_t kMostPieces = 32;  // that are joined at once
 // and pass their factors on by lane permutes; 16 partials' values are in flight.
 template <int VEC, int LANES, int POLICY>
 __device__ __forceinline__ void join(const Partials& p, uint32_t first, uint32_t rest, uint32_t count, int ncols,
-                                     float* out, uint32_t to) {
+                                     float* out, uint32_t to, bool large) {
   typedef float Row __attribute__((ext_vector_type(VEC)));
   constexpr uint32_t kBatch = 16;
   constexpr int kStats = LANES < (int)kMostPieces ? (int)kMostPieces / LANES : 1, kColumns = 256 / LANES;  // a lane's; of the workgroup at once
@@ -200,7 +211,7 @@ __device__ __forceinline__ void join(const Partials& p, uint32_t first, uint32_t
       if (out) {
         const float inv = 1.f / sum;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) out[(long)c * p.hd + d + e] = o[e] * inv;
+        for (int e = 0; e < VEC; ++e) out[(long)c * p.hd + d + e] = average(o[e], o[e] * inv, large);
       } else {
         if constexpr (VEC == 4)
           p.put(p.at(to) + row, o, false);
@@ -244,6 +255,7 @@ __device__ __forceinline__ float paged_value(const PagedView& w, bool is_v, size
 // sums of f32; 20 the tiles at 104).
 template <typename T>
 struct Plain {
+  static constexpr bool kF32 = std::is_same<T, float>::value;
   static constexpr int kPer = kMaxHalf * 2 / 64;
   static constexpr int kVec = 1, kLanes = 64;
   struct Shared {
@@ -254,7 +266,7 @@ struct Plain {
   // output where `whole`, else the partial that where() names.
   template <typename Where>
   static __device__ __forceinline__ void segment(const PagedView& w, const AttnArgs& a, Shared& sh, uint32_t s, int h,
-                                                 int qh, int, uint32_t p0, uint32_t p1, bool whole,
+                                                 int qh, int, uint32_t p0, uint32_t p1, float unit, bool whole,
                                                  const Partials& pt, Where where) {
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const float* q = a.q + s * a.q_stride + (long)qh * w.hd;
@@ -314,9 +326,9 @@ struct Plain {
       }
     }
     __syncthreads();
-    if (lane == 0) sh.m[wv] = m, sh.l[wv] = (float)l;
+    if (lane == 0) sh.m[wv] = m, sh.l[wv] = (float)(l * unit);
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) sh.o[wv][lane + 64 * j] = (float)o[j];
+    for (int j = 0; j < kPer; ++j) sh.o[wv][lane + 64 * j] = (float)(o[j] * unit);
     __syncthreads();
     bool here = false;
     const uint32_t part = whole ? 0 : where(here);
@@ -331,7 +343,7 @@ struct Plain {
       for (int i = 0; i < 4; ++i)
         if (f[i] != 0.f) y += f[i] * sh.o[i][d];
       if (whole)
-        a.out[s * a.out_stride + (long)qh * w.hd + d] = y / sum;
+        a.out[s * a.out_stride + (long)qh * w.hd + d] = average(y, y / sum, unit != 1.f);
       else
         pt.put(part + 4u * d, y, here);
     }
@@ -482,7 +494,7 @@ struct Tiled {
 
   template <typename Where>
   static __device__ __forceinline__ void segment(const PagedView& w, const AttnArgs& a, Shared& sh, uint32_t s, int h,
-                                                 int qh, int ncols, uint32_t p0, uint32_t p1, bool whole,
+                                                 int qh, int ncols, uint32_t p0, uint32_t p1, float unit, bool whole,
                                                  const Partials& pt, Where where) {
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int wv = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -642,7 +654,7 @@ struct Tiled {
         float p[4 * kSub], lt[kSub];
 #pragma unroll
         for (int i = 0; i < 4 * kSub; ++i) {
-          p[i] = __builtin_amdgcn_exp2f(y[i] - m + (kF32 ? 0.f : 15.f));
+          p[i] = kF32 ? __builtin_amdgcn_exp2f(y[i] - m) * unit : __builtin_amdgcn_exp2f(y[i] - m + 15.f);
           lt[i >> 2] = i & 3 ? lt[i >> 2] + p[i] : p[i];
         }
         l += kSub == 2 ? lt[0] + lt[kSub - 1] : lt[0];
@@ -757,7 +769,11 @@ struct Tiled {
         sum += f * lk;
       }
       if (whole) {
-        *reinterpret_cast<f32x4u*>(a.out + s * a.out_stride + (long)(qh + c) * w.hd + d) = o * (1.f / sum);
+        const float inv = 1.f / sum;
+        const bool large = unit != 1.f;
+        *reinterpret_cast<f32x4u*>(a.out + s * a.out_stride + (long)(qh + c) * w.hd + d) =
+            f32x4{average(o[0], o[0] * inv, large), average(o[1], o[1] * inv, large),
+                  average(o[2], o[2] * inv, large), average(o[3], o[3] * inv, large)};
       } else {
         pt.put(part + (uint32_t)(c * w.hd + d) * 4u, o, here);
         if (d == 0) pt.put_stat(part, c, top, sum, here);
@@ -772,6 +788,7 @@ __global__ __launch_bounds__(256, WAVES) void paged_attn_kernel(PagedView w, Att
   __shared__ unsigned drawn;
   const int lane = threadIdx.x & 63;
   const uint32_t items = (uint32_t)(w.n_kv * a.blocks);
+  const bool large = Inner::kF32 && w.status[kLarge] != 0;
   const Turn turn = a.turns[own_turn(blockIdx.x, gridDim.x)];
   unsigned* const tickets = a.tickets + (turn.set ? a.set_words : 0);
   // Sequence i's rows, for the 64 from s0 on a lane each.
@@ -837,7 +854,8 @@ __global__ __launch_bounds__(256, WAVES) void paged_attn_kernel(PagedView w, Att
           uint32_t of_group = 0;
           bool once = false;   // joined at once, at device scope
           bool alone = false;  // the group's only piece of many: its partial as it is
-          Inner::segment(w, a, sh, s, h, qh, ncols, u0 * kUnitRows, min(n, u1 * kUnitRows), whole, pt, [&](bool& here) {
+          Inner::segment(w, a, sh, s, h, qh, ncols, u0 * kUnitRows, min(n, u1 * kUnitRows), large ? weight_unit(n) : 1.f,
+                         whole, pt, [&](bool& here) {
             const Group g = group_of(r, slot, in_slot);
             ps = pieces_of(g, divide(first, per), divide(first + units - 1, per), first, per, in_slot, divide);
             of_group = group_partial(g, first, per);
@@ -859,14 +877,14 @@ __global__ __launch_bounds__(256, WAVES) void paged_attn_kernel(PagedView w, Att
             if (!alone) {
               if (!last_of(only ? ticket : tickets + of_group, ps.count, drawn)) return;
               join<Inner::kVec, Inner::kLanes, kXcdScope>(pt, piece0, rest, ps.count, ncols, only ? out : nullptr,
-                                                          2 * ranges + of_group);
+                                                          2 * ranges + of_group, large);
             }
             if (only) return;
             piece0 = 2 * ranges + ps.group0;
             rest = (piece0 & ~1u) + 2;
           }
           if (last_of(ticket, count, drawn))
-            join<Inner::kVec, Inner::kLanes, kDeviceScope>(pt, piece0, rest, count, ncols, out, 0);
+            join<Inner::kVec, Inner::kLanes, kDeviceScope>(pt, piece0, rest, count, ncols, out, 0, large);
         },
         divide);
   }

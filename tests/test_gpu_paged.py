@@ -1190,3 +1190,40 @@ def test_calls_behind_a_capture_wait_for_those_before_it(back):
     torch.cuda.synchronize()
     again = rv.paged_attention(q, c, 1, t, n, scale_of(hd), torch.empty_like(out))
     assert np.array_equal(host(out).view(np.uint32), host(again).view(np.uint32))
+
+
+@pytest.mark.parametrize("hd", [128, 64, 96, 256, 192, 20, 512])
+@pytest.mark.parametrize("lens", [[300, 1, 16], [9000], [70] * 300])
+def test_values_at_the_end_of_the_range(hd, lens):
+    """f32 pages whose values' sums pass the floats' range: averages of them do not."""
+    torch = torch_cuda()
+    say(f"case largest values {(hd, lens[:3])}")
+    rng = np.random.default_rng(hd + len(lens))
+    n_kv, group, page = 2, 4, 16
+    top = float(np.finfo(np.float32).max)
+    table, pool = tables(rng, len(lens), -(-max(lens) // page))
+    c = rv.PagedKvCache(1, n_kv, hd, pool, page, "f32")
+    own = []
+    for i, n in enumerate(lens):
+        k, v = rows(rng, n, n_kv * hd), rng.uniform(-1, 1, (n, n_kv * hd))
+        v[:, :hd // 2] = 1.0  # half of kv head 0: all as large as can be
+        v = (v * top).astype(np.float32)
+        c.append_rows(0, dev(k), dev(v), ints(table), ints(np.arange(n)), ints(np.full(n, i)))
+        own.append((k, v))
+    q = rng.standard_normal((len(lens), n_kv * group * hd)).astype(np.float32)
+    out = torch.empty(q.shape, device="cuda")
+    rv.paged_attention(dev(q), c, 0, ints(table), ints(lens), scale_of(hd), out)
+    got = host(out).astype(np.float64) / top
+    assert np.isfinite(got).all()
+    for i in range(0, len(lens), 1 if len(lens) < 4 else 29):
+        k, v = own[i]
+        want, a = attend(q[i], k, v / np.float64(top), n_kv, hd, scale_of(hd))
+        check(got[i], want, a, 1.0, f"sequence {i}")
+    # Once they are overwritten the rest is as it was, to its last bits.
+    few = rows(rng, max(lens), n_kv * hd)
+    two = rv.PagedKvCache(1, n_kv, hd, pool, page, "f32")
+    for i, n in enumerate(lens):
+        for x in (c, two):
+            x.append_rows(0, dev(own[i][0]), dev(few[:n]), ints(table), ints(np.arange(n)), ints(np.full(n, i)))
+    outs = [rv.paged_attention(dev(q), x, 0, ints(table), ints(lens), scale_of(hd), torch.empty_like(out)) for x in (c, two)]
+    assert np.array_equal(host(outs[0]).view(np.uint32), host(outs[1]).view(np.uint32))
