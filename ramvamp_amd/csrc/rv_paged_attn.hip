@@ -379,9 +379,14 @@ struct Tiled {
   static constexpr int kStep = 4 * kRows;  // from one of a wave's tiles to its next
   // A sum of f32 drops what is below 2^-24 of it, the many small weights behind a large
   // one whole: a wave's sums are put aside (in LDS) and begun again after so many tiles.
-  // So at most 2^-18 of the largest value is lost: a product's rows (32, 16, of f32 4)
-  // count down to 2^-25 together.
+  // So at most 2^-18 of the largest value is lost in the tiles between: a product's rows
+  // (32, 16, of f32 4) count down to 2^-25 together. They begin again with what the addition to
+  // those put aside has rounded off (the sum s of a and b is off by (a - (s - (s - a))) +
+  // (b - (s - a)) exactly), so that nothing is added to that however many tiles there are;
+  // but with zero where whole heads of 256 leave no registers for it (f16 and Q8_0, two
+  // waves a SIMD: 41 to 56 values spilled): there up to 2^-25 more a time.
   static constexpr uint32_t kAside = kF32 ? 32 : 64;
+  static constexpr bool kKeepRest = HDP < 256 || !FULL || kF32;
   static constexpr int VD = kF32 || HDP == 64 ? 4 : 8;  // values of a row of V a lane loads together
   static constexpr int NH = HDP / (16 * VD);
   static constexpr int NK = kF32 ? HDP / 16 : kQ8 ? HDP / 64 : HDP / 32;  // 16-byte loads of a row of K a lane
@@ -530,22 +535,27 @@ struct Tiled {
     bool aside = false;
     auto place = [&](int r, int i) { return reinterpret_cast<f32x4*>(&sh.o[wv][4 * g + r][16 * VD * (i / VD) + VD * n + i % VD]); };
     auto put_aside = [&] {
+#pragma clang fp contract(off)
+      auto add = [](auto a, auto b, auto& rest) {
+        const auto sum = a + b, part = sum - a;
+        rest = (a - (sum - part)) + (b - part);
+        return sum;
+      };
       const float c = m_aside == m ? 1.f : __builtin_amdgcn_exp2f(m_aside - m);
-      l_aside = l_aside * c + l;
+      l_aside = add(l_aside * c, l, l);
       m_aside = m;
-      l = 0.f;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float f = __shfl(c, 4 * g + r, 64);
 #pragma unroll
         for (int i = 0; i < NH * VD; i += 4) {
-          f32x4 x = {acc[i][r], acc[i + 1][r], acc[i + 2][r], acc[i + 3][r]};
-          if (aside) x += *place(r, i) * f;
+          f32x4 x = {acc[i][r], acc[i + 1][r], acc[i + 2][r], acc[i + 3][r]}, rest{};
+          if (aside) x = add(*place(r, i) * f, x, rest);
           *place(r, i) = x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i + e][r] = kKeepRest ? rest[e] : 0.f;
         }
       }
-#pragma unroll
-      for (int i = 0; i < NH * VD; ++i) acc[i] = f32x4{};
       aside = true;
     };
     if (p1 - p0 > kAside * kStep) __syncthreads();  // (the last segment's reads)

@@ -1227,3 +1227,34 @@ def test_values_at_the_end_of_the_range(hd, lens):
             x.append_rows(0, dev(own[i][0]), dev(few[:n]), ints(table), ints(np.arange(n)), ints(np.full(n, i)))
     outs = [rv.paged_attention(dev(q), x, 0, ints(table), ints(lens), scale_of(hd), torch.empty_like(out)) for x in (c, two)]
     assert np.array_equal(host(outs[0]).view(np.uint32), host(outs[1]).view(np.uint32))
+
+
+@pytest.mark.parametrize("hd", [64, 96, 128, 192, 256])
+def test_very_long_sums_keep_small_weights(hd):
+    """1.5 million f32 rows to a workgroup, whose weights next to the first one's add up
+    to nothing within one period of the sums, but not over all periods."""
+    torch = torch_cuda()
+    say(f"case very long sums {hd}")
+    n, seqs = 1500000, 300
+    c = rv.PagedKvCache(1, 2, hd, -(-n // 1024), 1024, "f32")
+    k, v = torch.zeros(n, 2 * hd, device="cuda"), torch.ones(n, 2 * hd, device="cuda")
+    k[0, 0] = k[0, hd] = 1.0
+    v[1:, :hd] = -1.0  # kv head 0: the first row's value against all others'
+    v[0, hd:] = 0.0    # kv head 1: the others' alone
+    table = ints(np.random.default_rng(0).permutation(-(-n // 1024))[None])
+    c.append_rows(0, k, v, table, ints(np.arange(n)), ints(np.zeros(n)))
+    del k, v
+    gaps = np.array([28.2, 32.2, 34.2, 36.2]) * np.log(2)  # the first row's score above the others'
+    q = np.zeros((2, 4, hd), np.float32)
+    q[:, :, 0] = gaps / scale_of(hd)
+    q = np.tile(q.reshape(1, -1), (seqs, 1))
+    out = torch.empty(seqs, 8 * hd, device="cuda")
+    rv.paged_attention(dev(q), c, 0, table.repeat(seqs, 1), ints([n] * seqs), scale_of(hd), out)
+    first = np.float32(gaps / scale_of(hd)).astype(np.float64) * scale_of(hd)
+    rest = (n - 1) * np.exp(-first)
+    want = np.stack([(1 - rest) / (1 + rest), rest / (1 + rest)])
+    # A weight is off by the score's 2^-21 times the score, as in the tests above, which
+    # moves an average of values 2 apart by twice as much; and check()'s 96 half steps.
+    bound = 2 * rest / (1 + rest) * (2 * gaps + 1) * 2.0 ** -21 + 96 * EPS32
+    err = np.abs(host(out).reshape(seqs, 2, 4, hd) - want[None, :, :, None]).max((0, 3))
+    assert np.all(err <= bound), (err, bound)
