@@ -120,7 +120,7 @@ void rv_paged_free(rv_paged* pg);
 /* As rv_kv_set_tuning. RV_TUNE_PAGED_JOIN: how workgroups that share a
  * sequence's kv head join what they have: 0 within each XCD's L2 first where the
  * device deals workgroups to its XCDs in turn (checked when the cache is made),
- * else across them at once, 2 always so. */
+ * else across them at once, 2 always so; other values are RV_ERR_UNSUPPORTED. */
 #define RV_TUNE_PAGED_JOIN 1
 int32_t rv_paged_set_tuning(rv_paged* pg, int32_t knob, int64_t value, rv_error* err);
 /* As rv_kv_set_stream. Calls on one cache share its workspace: one stream at a

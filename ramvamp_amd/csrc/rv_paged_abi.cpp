@@ -354,6 +354,7 @@ void rv_paged_free(rv_paged* pg) {
 int32_t rv_paged_set_tuning(rv_paged* pg, int32_t knob, int64_t value, rv_error* err) {
   if (!pg) return null_arg(err, "pg");
   if (knob != RV_TUNE_PAGED_JOIN) return unsupported(err, (uint64_t)knob, "tuning knob");
+  if (value != 0 && value != 2) return unsupported(err, (uint64_t)value, "RV_TUNE_PAGED_JOIN (0 or 2)");
   pg->tune_join = value;
   return ok(err);
 }

@@ -1258,3 +1258,14 @@ def test_very_long_sums_keep_small_weights(hd):
     bound = 2 * rest / (1 + rest) * (2 * gaps + 1) * 2.0 ** -21 + 96 * EPS32
     err = np.abs(host(out).reshape(seqs, 2, 4, hd) - want[None, :, :, None]).max((0, 3))
     assert np.all(err <= bound), (err, bound)
+
+
+@pytest.mark.parametrize("value", [1, 3, -7, 2 ** 40])
+def test_join_values_that_mean_nothing_are_refused(value):
+    torch_cuda()
+    say(f"case join value {value}")
+    c = rv.PagedKvCache(1, 2, 64, 4, 16, "f16")
+    with pytest.raises(rv.DeviceError) as e:
+        c.set_tuning(rv.RV_TUNE_PAGED_JOIN, value)
+    assert e.value.variant == "Unsupported"
+    c.set_tuning(rv.RV_TUNE_PAGED_JOIN, 0)
