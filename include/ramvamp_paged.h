@@ -80,8 +80,8 @@ void rv_rope_free(rv_rope* rope);
 int32_t rv_rope_frequencies(const rv_rope* rope, double* freq, size_t n, double* gain, rv_error* err);
 /* Row r of x, `width` f32 (whole heads: else RV_ATTN_Q_LEN_INDIVISIBLE), rotated at
  * positions[r] (i32; negative turns backwards) into row r of out. out may be x
- * itself (same stride), or rows beside x's in one buffer; any other overlap is
- * RV_ERR_UNSUPPORTED. Queued on `stream` of the current device. */
+ * itself (same stride), or rows beside x's in one buffer; any other overlap, also
+ * with positions, is RV_ERR_UNSUPPORTED. Queued on `stream` of the current device. */
 int32_t rv_rope_rows(const rv_rope* rope, const float* x, size_t x_stride, size_t rows, size_t width,
                      const int32_t* positions, float* out, size_t out_stride, void* stream, uint32_t flags,
                      rv_error* err);
@@ -149,7 +149,8 @@ int32_t rv_paged_append_rows(rv_paged* pg, size_t layer, const rv_rope* rope, co
 /* The rows at positions[r] of sequence seqs[r], as attention reads them, into
  * row r of k and v (contiguous; either may be null): f32 of an F32 cache, else
  * f16. A row of a negative position or one refused on the device (as above) is
- * zeros. */
+ * zeros. k and v overlap neither each other nor what the call reads
+ * (RV_ERR_UNSUPPORTED). */
 int32_t rv_paged_read_rows(rv_paged* pg, size_t layer, size_t rows, const int32_t* positions, const int32_t* seqs,
                            const rv_page_table* table, void* k, void* v, uint32_t flags, rv_error* err);
 
@@ -170,7 +171,7 @@ int32_t rv_paged_read_rows(rv_paged* pg, size_t layer, size_t rows, const int32_
  * rows are more than 2^31 - 1 units (n_seqs * the tables' rows / 128 for each 16
  * query heads of a kv head; of every query head where head_dim is no multiple of
  * 8 or above 256). Checks, in order: q_dim, layer, the strides, the table, n_seqs,
- * out overlapping q (RV_ERR_UNSUPPORTED), the units. */
+ * out overlapping q, lens or the table (RV_ERR_UNSUPPORTED), the units. */
 int32_t rv_paged_attention(rv_paged* pg, size_t layer, const float* q, size_t q_stride, size_t n_seqs, size_t q_dim,
                            const rv_page_table* table, const int32_t* lens, float scale, float* out,
                            size_t out_stride, uint32_t flags, rv_error* err);
@@ -179,7 +180,9 @@ int32_t rv_paged_attention(rv_paged* pg, size_t layer, const float* q, size_t q_
  * may be null), rotated (rope may be null) at positions[i], k and v appended to
  * sequence i there, then attention over positions[i] + 1 rows. As
  * rv_paged_append_rows and rv_paged_attention one after the other; a negative
- * position gives zeros and writes nothing. Positions and tables are read when
+ * position gives zeros and writes nothing. out may overlap q, k, v and the weights,
+ * all read before it is written, but not positions or the table
+ * (RV_ERR_UNSUPPORTED). Positions and tables are read when
  * the step runs, so a captured step is replayed for every token (advance the
  * positions in the graph, or between replays on its stream); the first call of
  * a batch size may have to allocate and is not captured (RV_ERR_UNSUPPORTED). */

@@ -76,6 +76,21 @@ bool overlap(const float* x, size_t x_stride, const float* y, size_t y_stride, s
   return apart < need || apart + need > step;
 }
 
+// Whether `bytes` at p share memory with rows of f32 (with them, not what is between).
+bool meets(const void* p, size_t bytes, const float* y, size_t y_stride, size_t rows, size_t width) {
+  if (bytes == 0 || rows == 0 || width == 0) return false;
+  const uintptr_t a = (uintptr_t)p, b = (uintptr_t)y;
+  if (a + bytes <= b || b + extent(rows, width, y_stride) <= a) return false;
+  if (a < b || rows == 1) return true;
+  const size_t step = y_stride * sizeof(float), i = (a - b) / step, in_row = (a - b) % step;
+  return in_row < width * sizeof(float) || (i + 1 < rows && in_row + bytes > step);
+}
+
+// Bytes of a table from its first id to the last of n sequences.
+size_t table_bytes(const rv_page_table& t, size_t n) {
+  return n && t.pages ? ((n - 1) * t.stride + t.pages) * sizeof(int32_t) : 0;
+}
+
 // As rv_kv_new's geometry, for pages.
 int32_t geometry(size_t n_layers, size_t n_kv_heads, size_t head_dim, size_t n_pages, size_t page_rows, int elem,
                  size_t* bytes, rv_error* err) {
@@ -283,6 +298,8 @@ int32_t rv_rope_rows(const rv_rope* rope, const float* x, size_t x_stride, size_
   if (rows == 1) x_stride = out_stride = width;
   if (!(x == out && x_stride == out_stride) && overlap(x, x_stride, out, out_stride, rows, width))
     return unsupported(err, 0, "out overlaps x");
+  if (meets(positions, rows * sizeof(int32_t), out, out_stride, rows, width))
+    return unsupported(err, 0, "out overlaps positions");
   const rv::HipStatus st = rv::launch_rope_rows(*rope, x, x_stride, rows, width, positions, out,
                                                 out_stride, (hipStream_t)stream);
   return finish((hipStream_t)stream, flags, st, err);
@@ -435,6 +452,15 @@ int32_t rv_paged_read_rows(rv_paged* pg, size_t layer, size_t rows, const int32_
   if (queued.e != hipSuccess) return hip_fail(err, queued.e, "stream hand-over");
   if (rows == 0 || (!k && !v)) return finish(pg->order.stream, flags, {}, err);
   if (!positions) return null_arg(err, "positions");
+  const size_t es = pg->elem == RV_ELEM_F32 ? 4 : 2, n = rows * pg->kv_dim * es;
+  const auto apart = [&](const void* x, const void* y, size_t bytes) {
+    return !x || !y || (uintptr_t)x + n <= (uintptr_t)y || (uintptr_t)y + bytes <= (uintptr_t)x;
+  };
+  if (!apart(k, v, n)) return unsupported(err, 0, "k overlaps v");
+  const size_t ids = table_bytes(*table, seqs ? table->n_seqs : rows);
+  for (const void* x : {k, v})
+    if (!apart(x, positions, rows * sizeof(int32_t)) || !apart(x, seqs, rows * sizeof(int32_t)) || (ids && !apart(x, table->ids, ids)))
+      return unsupported(err, 0, "k or v overlaps positions, seqs or the table");
   return finish(pg->order.stream, flags,
                 rv::launch_paged_read(pg, rv::paged_view(pg, layer, *table), rows, positions, seqs, k, v, pg->order.stream),
                 err);
@@ -460,6 +486,9 @@ int32_t rv_paged_attention(rv_paged* pg, size_t layer, const float* q, size_t q_
   if (!q || !lens || !out) return null_arg(err, !q ? "q" : !lens ? "lens" : "out");
   if (n_seqs == 1) q_stride = out_stride = q_dim;
   if (overlap(q, q_stride, out, out_stride, n_seqs, q_dim)) return unsupported(err, 0, "out overlaps q");
+  if (meets(lens, n_seqs * sizeof(int32_t), out, out_stride, n_seqs, q_dim) ||
+      meets(table->ids, table_bytes(*table, n_seqs), out, out_stride, n_seqs, q_dim))
+    return unsupported(err, 0, "out overlaps lens or the table");
   const size_t n_q = q_dim / pg->head_dim;
   rv::PagedAttnPlan plan;
   if ((rc = ready_attn(pg, *table, n_seqs, n_q, &plan, err))) return rc;
@@ -492,6 +521,10 @@ int32_t rv_paged_decode_step(rv_paged* pg, size_t layer, const rv_rope* rope, co
   if (n_seqs == 0) return finish(pg->order.stream, flags, {}, err);
   for (const auto& p : {std::pair<const void*, const char*>{q, "q"}, {k, "k"}, {v, "v"}, {positions, "positions"}, {out, "out"}})
     if (!p.first) return null_arg(err, p.second);
+  // (q, k and v are read, and q copied, before the first output is written.)
+  if (meets(positions, n_seqs * sizeof(int32_t), out, out_stride, n_seqs, q_dim) ||
+      meets(table->ids, table_bytes(*table, n_seqs), out, out_stride, n_seqs, q_dim))
+    return unsupported(err, 0, "out overlaps positions or the table");
   const size_t n_q = q_dim / pg->head_dim;
   rv::PagedAttnPlan plan;
   if ((rc = ready_attn(pg, *table, n_seqs, n_q, &plan, err))) return rc;

@@ -300,7 +300,8 @@ def paged_decode_step(cache: PagedKvCache, layer: int, q_rows, k_rows, v_rows, q
     """rv_paged_decode_step: one token of each sequence through a layer's attention:
     q and k RMS-normed per head (a weight may be None) and rotated at positions[i], k
     and v appended there, then attention over positions[i] + 1 rows. A negative
-    position gives zeros and writes nothing."""
+    position gives zeros and writes nothing. out may be q_rows, or overlap any of the
+    float inputs."""
     d = cache.device
     qp, n, width, qs = _rows(q_rows, "q_rows", d)
     kp, k_n, k_width, ks = _rows(k_rows, "k_rows", d)

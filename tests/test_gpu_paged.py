@@ -1269,3 +1269,73 @@ def test_join_values_that_mean_nothing_are_refused(value):
         c.set_tuning(rv.RV_TUNE_PAGED_JOIN, value)
     assert e.value.variant == "Unsupported"
     c.set_tuning(rv.RV_TUNE_PAGED_JOIN, 0)
+
+
+def test_outputs_over_what_is_still_read_are_refused():
+    """Lengths, positions, tables and sequences inside the rows written; between the rows
+    they are none of the call's business."""
+    torch = torch_cuda()
+    say("case outputs over what is read")
+    c = rv.PagedKvCache(1, 2, 64, 8, 16, "f16")
+    f = lambda *s: torch.zeros(*s, device="cuda")
+    t, at = ints([[0], [1], [2]]), ints([0, 0, 0])
+    as_ints = lambda x: x.view(torch.int32)
+    wide = f(3, 256 + 8)
+    out, flat = wide[:, :256], as_ints(wide).view(-1)
+    q, k = f(3, 256), f(3, 128)
+    step = lambda pos, tab, o, x=q, y=k, z=k: rv.paged_decode_step(c, 0, x, y, z, None, None, EPS, None, tab, pos, 0.125, o)
+    for start in (0, 100, 255, 262, 264 * 2 + 253):  # (of 262's three the last is in a row)
+        inside = flat[start:start + 3]
+        for call in (lambda: rv.paged_attention(q, c, 0, t, inside, 0.125, out),
+                     lambda: rv.paged_attention(q, c, 0, inside.view(3, 1), at, 0.125, out),
+                     lambda: step(inside, t, out), lambda: step(at, inside.view(3, 1), out)):
+            with pytest.raises(rv.DeviceError) as e:
+                call()
+            assert e.value.variant == "Unsupported"
+    between = flat[264 + 257:264 + 260]
+    rv.paged_attention(q, c, 0, t, between, 0.125, out)
+    rv.paged_attention(q, c, 0, between.view(3, 1), at, 0.125, out)
+    step(between, t, out)
+    x = f(3, 256)
+    rope = rv.Rope(64, THETA)
+    rv.rope_rows(x, between, rope, out)
+    with pytest.raises(rv.DeviceError):
+        rv.rope_rows(x, flat[250:253], rope, out)
+    half = lambda n: torch.zeros(n, dtype=torch.float16, device="cuda")
+    kv = half(2 * 3 * 128)
+    ok = kv[:384].view(3, 128), kv[384:].view(3, 128)
+    c.read_rows(0, t, at, k=ok[0], v=ok[1])
+    over = as_ints(ok[0]).view(-1)[10:13]
+    for kw in (dict(k=ok[0], v=ok[0]), dict(k=ok[0], v=kv[100:484].view(3, 128))):
+        with pytest.raises(rv.DeviceError):
+            c.read_rows(0, t, at, **kw)
+    for tab, pos, seq in ((t, over, None), (over.view(3, 1), at, None), (t, at, over)):
+        with pytest.raises(rv.DeviceError):
+            c.read_rows(0, tab, pos, seq, k=ok[0], v=ok[1])
+    c.device_status()
+
+
+@pytest.mark.parametrize("elem", ["f16", "f32", "q8_0"])
+@pytest.mark.parametrize("over", ["q", "k", "v", "all"])
+def test_step_over_its_inputs(elem, over):
+    """out over any of q, k and v: the bits of a step with rows of its own."""
+    torch = torch_cuda()
+    say(f"case step over its inputs {(elem, over)}")
+    rng = np.random.default_rng(56)
+    lens, n_kv, group, hd = [70, 0, 300], 4, 1, 64
+    (c, table, _), (d, _, _) = [filled(np.random.default_rng(1), elem, n_kv, hd, 16, lens, extra=1) for _ in range(2)]
+    q, k, v, (wq, wk) = step_inputs(rng, 3, n_kv, group, hd)
+    args = (dev(wq), dev(wk), EPS, rv.Rope(hd, THETA), ints(table), ints(lens), scale_of(hd))
+    want = rv.paged_decode_step(c, 1, dev(q), dev(k), dev(v), *args, torch.empty(q.shape, device="cuda"))
+    x = {"q": dev(q), "k": dev(k), "v": dev(v)}
+    if over == "all":  # rows that overlap q's, k's and v's in one matrix
+        fused = torch.cat([x["q"], x["k"], x["v"]], 1).contiguous()
+        w = q.shape[1]
+        x = {"q": fused[:, :w], "k": fused[:, w:2 * w], "v": fused[:, 2 * w:]}
+        out = fused[:, w // 2:w // 2 + w]
+    else:
+        out = x[over]
+    rv.paged_decode_step(d, 1, x["q"], x["k"], x["v"], *args, out)
+    assert np.array_equal(host(out).copy().view(np.uint32), host(want).view(np.uint32))
+    for a, b in zip(everything(c, 1), everything(d, 1)):
+        assert np.array_equal(a, b, equal_nan=True)

@@ -231,3 +231,17 @@ def test_a_cache_passes_from_stream_to_stream_on_the_host(tmp_path):
                    check=True, capture_output=True)
     out = subprocess.run([exe], capture_output=True, text=True, timeout=100)
     assert out.returncode == 0 and not out.stdout, out.stdout
+
+
+@pytest.mark.parametrize("at,code", [
+    (8192, 33), (8188, 33), (8192 + 4 * 127, 33), (8192 + 4 * 255, 33), (8192 + 4 * 128 * 7 + 4 * 127, 33),
+    (8192 + 4 * 256 * 7 + 4 * 127, 33), (8192 + 4 * 249, 33), (8192 - 4 * 7, 33), (4096, 33), (4096 + 4 * 120, 33),
+])
+def test_rotated_rows_over_their_positions_are_refused(at, code):
+    """8 rows of 128 of a wider buffer, and positions that they reach, or a place of x
+    that they are; the addresses are never read."""
+    rope, err = rv.Rope(128, 1e6), L.RvError()
+    out = 4096 if at < 8000 else 8192
+    call = lambda p, rows: L.load().rv_rope_rows(rope._h, out, 256, rows, 128, p, out, 256, None, 0, ctypes.byref(err))
+    assert call(at, 8) == code == err.code
+    assert b"positions" in err.what
