@@ -67,7 +67,8 @@ extern "C" {
 typedef struct rv_rope rv_rope;
 
 /* head_dim at most 512; rotary_dim even, 2 .. head_dim (RV_PRIM_INVALID_HEAD_DIM,
- * a = rotary_dim, b = head_dim). theta finite and positive (YARN: above 1).
+ * a = rotary_dim, b = head_dim). theta finite and positive (YARN: above 1), and so
+ * that NTK's base and 2^31 f_i are finite.
  * factor (finite, at least 1) counts with a scaling, trained_positions (at least
  * 1) and the betas (finite, beta_fast > beta_slow > 0) with YARN alone; NTK needs
  * rotary_dim above 2. Else RV_ERR_UNSUPPORTED with `what`. */

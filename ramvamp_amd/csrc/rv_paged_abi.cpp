@@ -265,6 +265,10 @@ int32_t rv_rope_new(size_t head_dim, size_t rotary_dim, uint32_t layout, double 
       const double ramp = std::min(std::max(((double)i - lo) / std::max(hi - lo, 0.001), 0.0), 1.0);
       f = f * (1.0 - ramp) + f / factor * ramp;
     }
+    if (!std::isfinite(base) || !std::isfinite(f * 0x1p31)) {
+      delete r;
+      return unsupported(err, 0, "rope theta (angles past the range of f64)");
+    }
     r->freq[i] = f;
   }
   *out = r;

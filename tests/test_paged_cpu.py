@@ -245,3 +245,17 @@ def test_rotated_rows_over_their_positions_are_refused(at, code):
     call = lambda p, rows: L.load().rv_rope_rows(rope._h, out, 256, rows, 128, p, out, 256, None, 0, ctypes.byref(err))
     assert call(at, 8) == code == err.code
     assert b"positions" in err.what
+
+
+@pytest.mark.parametrize("kw", [dict(theta=5e-324), dict(theta=1e-308), dict(theta=1e308, scaling="ntk", factor=1e10),
+                                dict(theta=1e6, rotary_dim=4, scaling="ntk", factor=1e200)])
+def test_rope_bases_whose_angles_are_not_finite_are_refused(kw):
+    with pytest.raises(rv.RamvampError) as e:
+        rv.Rope(**{"head_dim": 512, **kw})
+    assert e.value.variant == "Unsupported"
+
+
+def test_rope_bases_at_the_ends_of_the_range():
+    for theta in (1e-290, 1e308):
+        f, _ = rv.Rope(512, theta).frequencies()
+        assert np.all(np.isfinite(f * 2.0 ** 31)) and f[0] == 1.0
