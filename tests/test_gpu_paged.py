@@ -1339,3 +1339,60 @@ def test_step_over_its_inputs(elem, over):
     assert np.array_equal(host(out).copy().view(np.uint32), host(want).view(np.uint32))
     for a, b in zip(everything(c, 1), everything(d, 1)):
         assert np.array_equal(a, b, equal_nan=True)
+
+
+@pytest.mark.parametrize("elem", ["f16", "f32", "q8_0"])
+@pytest.mark.parametrize("n_kv,group,hd,r,layout,scaling,lens", [
+    (4, 8, 128, 128, "half", "yarn", [0, 1, 63, 300, 4000]), (2, 3, 64, 32, "interleaved", "ntk", [5, -1, 129, 0]),
+    (1, 16, 96, 96, "half", "none", [40, 700]), (2, 1, 256, 64, "interleaved", "linear", [7, 130]),
+    (1, 2, 512, 512, "half", "none", [9]), (2, 4, 192, 100, "half", "yarn", [33, 0]),
+])
+def test_step_in_64_bits(elem, n_kv, group, hd, r, layout, scaling, lens):
+    """A normed, rotated step against its definition, from the rows given to the output."""
+    torch = torch_cuda()
+    say(f"case step in 64 bits {(elem, n_kv, group, hd, r, layout, scaling, lens)}")
+    rng = np.random.default_rng(hd + r + len(lens))
+    n, at, page = len(lens), np.array(lens), 16
+    rope = rv.Rope(hd, THETA, r, layout, scaling, factor=4.0, trained_positions=32768)
+    gain = rope.frequencies()[1]
+    c, table, own = filled(rng, elem, n_kv, hd, page, [max(x, 0) for x in lens], extra=1)
+    q, k, v, (wq, wk) = step_inputs(rng, n, n_kv, group, hd)
+    out = torch.full(q.shape, 3.0, device="cuda")
+    rv.paged_decode_step(c, 1, dev(q), dev(k), dev(v), dev(wq), dev(wk), EPS, rope, ints(table), ints(lens),
+                         scale_of(hd), out)
+    gk, gv = (host(x).astype(np.float32) for x in c.read_rows(1, ints(table), ints(lens)))
+    c.device_status()
+    cos, sin = turns(rope, np.maximum(at, 0))
+
+    def exact(x, w):
+        """The normed and rotated rows, and how far 32 bits may be from them: the norm's
+        reciprocal root and two products (half a step each, one spare), then the rotation."""
+        x = x.reshape(n, -1, hd).astype(np.float64)
+        x = x / np.sqrt((x * x).mean(-1, keepdims=True) + float(np.float32(EPS))) * w
+        off = 4 * EPS32 * np.abs(x)
+        off[..., :r] = rotation_bound(x, r, layout, gain)[..., :r] * 2
+        return rotated(x, cos, sin, r, layout), off
+
+    (q64, q_off), (k64, k_off) = exact(q, wq), exact(k, wk)
+    for got, want, off in ((gk, k64, k_off), (gv, v.reshape(n, n_kv, hd).astype(np.float64), 0.0)):
+        got = got.reshape(n, n_kv, hd)
+        if elem == "f32":
+            bound = off + 0 * np.abs(want)
+        elif elem == "f16":
+            bound = off + 2.0 ** -11 * (np.abs(want) + off) + 2.0 ** -25
+        else:  # half a code, what 32 bits take off or add to it, and the scale's and the value's f16
+            top = np.abs(want + off).reshape(n, n_kv, -1, 32).max(-1).repeat(32, -1)
+            bound = off + top / 127 * (0.5 + 2.0 ** -16) + 2 * 2.0 ** -11 * top + 2.0 ** -18
+        for i in range(n):
+            assert np.all(np.abs(got[i] - want[i]) <= bound[i]) if lens[i] >= 0 else not got[i].any()
+    for i in range(n):
+        if lens[i] < 0:
+            assert not host(out)[i].any()
+            continue
+        ks, vs = np.concatenate([own[i][0], gk[i:i + 1]]), np.concatenate([own[i][1], gv[i:i + 1]])
+        want, a = attend(q64[i].reshape(-1), ks, vs, n_kv, hd, scale_of(hd))
+        # q's own error moves a score by at most its product with |k|: as much as a larger
+        # A would at check()'s 37 half steps.
+        kk = np.abs(ks.reshape(-1, n_kv, hd).astype(np.float64))
+        moved = max(float((q_off[i].reshape(n_kv, group, hd)[j] @ kk[:, j].T).max()) for j in range(n_kv))
+        check(host(out)[i], want, a + moved * scale_of(hd) / np.log(2) / (37 * EPS32), float(np.abs(vs).max()), f"sequence {i}")

@@ -259,3 +259,19 @@ def test_rope_bases_at_the_ends_of_the_range():
     for theta in (1e-290, 1e308):
         f, _ = rv.Rope(512, theta).frequencies()
         assert np.all(np.isfinite(f * 2.0 ** 31)) and f[0] == 1.0
+
+
+def test_masks_are_spelled_as_the_check_of_saves_reads_them(tmp_path):
+    """A divergent branch of this compiler ends in a label and the mask's restoring below
+    it, in the words that partial_saves looks for: another spelling fails here."""
+    src, out = tmp_path / "k.hip", str(tmp_path / "k.s")
+    src.write_text("#include <hip/hip_runtime.h>\n"
+                   "__global__ void k(float* x, int n) {\n"
+                   "  float y = x[threadIdx.x];\n"
+                   "  if ((int)threadIdx.x < n) { y += x[threadIdx.x + 64]; __syncthreads(); x[threadIdx.x + 128] = y; }\n"
+                   "  x[threadIdx.x] = y;\n}\n")
+    subprocess.run([B.HIPCC, *B.FLAGS, "--offload-device-only", "-S", "-o", out, str(src)], check=True, capture_output=True)
+    with open(out) as f:
+        body = re.search(r"^_Z\S+:\s.*?\.Lfunc_end", f.read(), re.M | re.S).group()
+    assert re.search(r"s_and_saveexec_b64 [^\n]*\n(?:[^\n]*\n)*?\s*s_cbranch_execz (\.LBB\d+_\d+)\n(?:[^\n]*\n)*?"
+                     r"\1:[^\n]*\n(?:\s*;[^\n]*\n)*\s*s_or_b64 exec, exec,", body), body
