@@ -84,10 +84,9 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 // A power of two that n weights of at most 1 each times it make less than one half of.
 __device__ __forceinline__ float weight_unit(uint32_t n) { return ldexpf(1.f, __builtin_clz(n) - 33); }
 
-// y, the average that a sum o gives of values that may be `large`: of finite ones finite,
-// whatever its last rounding.
-__device__ __forceinline__ float average(float o, float y, bool large) {
-  return large && __builtin_isinf(y) && !__builtin_isinf(o) ? __builtin_copysignf(0x1.fffffep127f, y) : y;
+// The average y that a sum o gives: of finite values finite, whatever its last rounding.
+__device__ __forceinline__ float finite(float o, float y) {
+  return __builtin_isinf(y) && !__builtin_isinf(o) ? __builtin_copysignf(0x1.fffffep127f, y) : y;
 }
 
 // ---- partials ---------------------------------------------------------------------
@@ -210,8 +209,13 @@ __device__ __forceinline__ void join(const Partials& p, uint32_t first, uint32_t
       if (cc >= ncols || d >= p.hd) continue;
       if (out) {
         const float inv = 1.f / sum;
+        Row y = o * inv;
+        if (large) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) out[(long)c * p.hd + d + e] = average(o[e], o[e] * inv, large);
+          for (int e = 0; e < VEC; ++e) y[e] = finite(o[e], y[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) out[(long)c * p.hd + d + e] = y[e];
       } else {
         if constexpr (VEC == 4)
           p.put(p.at(to) + row, o, false);
@@ -343,7 +347,7 @@ struct Plain {
       for (int i = 0; i < 4; ++i)
         if (f[i] != 0.f) y += f[i] * sh.o[i][d];
       if (whole)
-        a.out[s * a.out_stride + (long)qh * w.hd + d] = average(y, y / sum, unit != 1.f);
+        a.out[s * a.out_stride + (long)qh * w.hd + d] = unit != 1.f ? finite(y, y / sum) : y / sum;
       else
         pt.put(part + 4u * d, y, here);
     }
@@ -534,8 +538,9 @@ struct Tiled {
     float m_aside = -INFINITY, l_aside = 0.f;
     bool aside = false;
     auto place = [&](int r, int i) { return reinterpret_cast<f32x4*>(&sh.o[wv][4 * g + r][16 * VD * (i / VD) + VD * n + i % VD]); };
-    auto put_aside = [&] {
+    auto put_aside = [&](auto is_last) {
 #pragma clang fp contract(off)
+      constexpr bool kRest = kKeepRest && !decltype(is_last)::value;
       auto add = [](auto a, auto b, auto& rest) {
         const auto sum = a + b, part = sum - a;
         rest = (a - (sum - part)) + (b - part);
@@ -550,10 +555,15 @@ struct Tiled {
 #pragma unroll
         for (int i = 0; i < NH * VD; i += 4) {
           f32x4 x = {acc[i][r], acc[i + 1][r], acc[i + 2][r], acc[i + 3][r]}, rest{};
-          if (aside) x = add(*place(r, i) * f, x, rest);
+          if (aside) {
+            if constexpr (kRest)
+              x = add(*place(r, i) * f, x, rest);
+            else
+              x += *place(r, i) * f;
+          }
           *place(r, i) = x;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i + e][r] = kKeepRest ? rest[e] : 0.f;
+          for (int e = 0; e < 4; ++e) acc[i + e][r] = rest[e];
         }
       }
       aside = true;
@@ -732,17 +742,18 @@ struct Tiled {
         if constexpr (!kLast) load_v(w, v_hp, v_row, n, t);
       };
       const bool only = b + kStep >= p1;
-      uint32_t left = kAside;
-      for (; b + kStep < p1; b += kStep) {
-        step(std::false_type{}, false);
-        if (--left == 0) {
-          put_aside();
-          left = kAside;
-        }
+      // (A loop of its own for what lies between: its sums stay in their registers.)
+      while (b + kStep < p1) {
+        uint32_t left = kAside;
+        do {
+          step(std::false_type{}, false);
+          b += kStep;
+        } while (--left && b + kStep < p1);
+        if (left == 0) put_aside(std::false_type{});
       }
       step(std::true_type{}, only);
       if (aside) {
-        put_aside();
+        put_aside(std::true_type{});
         l = l_aside;
       }
       l = swap_sum<32>(swap_sum<16>(l));
@@ -780,10 +791,12 @@ struct Tiled {
       }
       if (whole) {
         const float inv = 1.f / sum;
-        const bool large = unit != 1.f;
-        *reinterpret_cast<f32x4u*>(a.out + s * a.out_stride + (long)(qh + c) * w.hd + d) =
-            f32x4{average(o[0], o[0] * inv, large), average(o[1], o[1] * inv, large),
-                  average(o[2], o[2] * inv, large), average(o[3], o[3] * inv, large)};
+        f32x4 y = o * inv;
+        if (unit != 1.f) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = finite(o[e], y[e]);
+        }
+        *reinterpret_cast<f32x4u*>(a.out + s * a.out_stride + (long)(qh + c) * w.hd + d) = y;
       } else {
         pt.put(part + (uint32_t)(c * w.hd + d) * 4u, o, here);
         if (d == 0) pt.put_stat(part, c, top, sum, here);
