@@ -241,7 +241,7 @@ __device__ __forceinline__ double head_sum(double x, int log) {
 // a Q8_0 block). Normed values pass through LDS, where a thread finds the other halves
 // of its pairs. k' = rot(k / sqrt(mean k^2 + eps) w): sum of squares and angles in f64.
 // Bound by a row's chain (position, page id, angles, store) rather than its bytes: one
-// row 3.4 us, 5734 rows of 4 + 4 heads of 128 into f16 pages 11.1, 3.2 TB/s
+// row 3.4 us, 5734 rows of 4 + 4 heads of 128 into f16 pages 11.5, 3.2 TB/s
 // (16.6 with the sums through LDS and single values turned).
 template <typename T, int N>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedView w, RopeArgs<N> rope, AppendArgs a) {

@@ -23,9 +23,9 @@
 //
 // Bound by the pages' bytes where there are many: f16, 32 query heads over 4 of 128, 64
 // sequences of up to 16000 rows 188 us, 6.6 TB/s (a streaming read's rate); one of 131000
-// 46.5, 5.8 TB/s. Q8_0 is bound by issue (32 of up to 8192 rows 38 us, 3.8 TB/s, vector
-// instructions 55 % of the cycles); few rows by one phase after the other: 100 rows 5.8,
-// 4096 11.5 us, a third of it the joins.
+// 46.5, 5.8 TB/s. Q8_0 by no one unit (32 of up to 8192 rows 38 us, 3.8 TB/s: vector
+// instructions 56 % of the cycles, matrix instructions 12 %, waves waiting 24 %); few rows
+// by one phase after the other: 100 rows 5.8, 4096 11.3 us, a third of it the joins.
 #include "rv_paged.hpp"
 
 #include <algorithm>
