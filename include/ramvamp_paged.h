@@ -163,11 +163,12 @@ int32_t rv_paged_read_rows(rv_paged* pg, size_t layer, size_t rows, const int32_
  * is NaN. Rows of out behind the last are not touched. f32 arithmetic: f16 and
  * Q8_0 rows are matrix operands as stored, q and probabilities f16 hi + lo
  * halves scaled by powers of two (to 2^-22 of themselves, or 2^-38 of the
- * largest of a head's), sums in f32. V may be any finite values; scale * (q . k) has
- * to stay within f32's range, with f32 rows q . k and its partial sums too. An infinity or NaN in a row that is
- * attended reaches the outputs of that kv head's query heads alone: NaN, but for
- * an infinity of K that may, where it makes a score minus infinity, leave its row
- * without weight. What lies in rows past lens[i] never counts.
+ * largest of a head's), sums in f32. V may be any finite values; scale * (q . k)
+ * has to stay within f32's range, over f32 rows q . k and its partial sums too. An
+ * infinity or NaN in a row that is attended reaches the outputs of that kv head's
+ * query heads alone: NaN, but for an infinity of K that may, where it makes a score
+ * minus infinity, leave its row without weight, and one of V that may stay an
+ * infinity. What lies in rows past lens[i] never counts.
  * RV_ERR_UNSUPPORTED: n_seqs past 2^23, query heads past 65535, and tables whose
  * rows are more than 2^31 - 1 units (n_seqs * the tables' rows / 128 for each 16
  * query heads of a kv head; of every query head where head_dim is no multiple of
