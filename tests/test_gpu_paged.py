@@ -1396,3 +1396,91 @@ def test_step_in_64_bits(elem, n_kv, group, hd, r, layout, scaling, lens):
         kk = np.abs(ks.reshape(-1, n_kv, hd).astype(np.float64))
         moved = max(float((q_off[i].reshape(n_kv, group, hd)[j] @ kk[:, j].T).max()) for j in range(n_kv))
         check(host(out)[i], want, a + moved * scale_of(hd) / np.log(2) / (37 * EPS32), float(np.abs(vs).max()), f"sequence {i}")
+
+
+def test_a_blocking_streams_capture_is_not_broken_by_the_hand_over():
+    """A stream that the null stream waits for is captured while that holds a call: no
+    event may be recorded on the null stream then, and the call behind the capture, on
+    a third stream, waits for it all the same."""
+    import ctypes
+
+    from ramvamp_amd import _lib as L
+
+    torch = torch_cuda()
+    say("case blocking capture")
+    hip = L.load()  # (its HIP runtime is the process's)
+    rng = np.random.default_rng(57)
+    lens, n_kv, hd = [300, 40], 2, 128
+    c, table, _ = filled(rng, "f16", n_kv, hd, 16, lens)
+    k, v = rows(rng, 2, n_kv * hd), rows(rng, 2, n_kv * hd)
+    t, n, last, seq = ints(table), ints(lens), ints([m - 1 for m in lens]), ints([0, 1])
+    kd, vd, q = dev(k), dev(v), dev(rng.standard_normal((2, 2 * 4 * hd)))
+    out = torch.empty(2, 2 * 4 * hd, device="cuda")
+    gk, gv = (torch.zeros(2, n_kv * hd, dtype=torch.float16, device="cuda") for _ in range(2))
+    big = torch.ones(8192, 8192, device="cuda")
+    hold = big @ big
+    rv.paged_attention(q, c, 1, t, n, scale_of(hd), out)  # (allocates)
+    third = torch.cuda.Stream()
+    blocking, graph = ctypes.c_void_p(), ctypes.c_void_p()
+    assert hip.hipStreamCreate(ctypes.byref(blocking)) == 0
+    second = torch.cuda.ExternalStream(blocking.value)
+    torch.cuda.synchronize()
+    for _ in range(8):
+        torch.mm(big, big, out=hold)
+    c.append_rows(1, kd, vd, t, last, seq)
+    assert hip.hipStreamBeginCapture(blocking, 0) == 0
+    with torch.cuda.stream(second):
+        rv.paged_attention(q, c, 1, t, n, scale_of(hd), out)
+    assert hip.hipStreamEndCapture(blocking, ctypes.byref(graph)) == 0 and graph.value
+    with torch.cuda.stream(third):
+        c.read_rows(1, t, last, seq, k=gk, v=gv)
+    torch.cuda.synchronize()
+    assert np.array_equal(host(gk), k.astype(np.float16)) and np.array_equal(host(gv), v.astype(np.float16))
+    assert hip.hipGraphDestroy(graph) == 0
+    c.synchronize()  # (on the null stream again)
+    assert hip.hipStreamDestroy(blocking) == 0
+
+
+@pytest.mark.parametrize("elem", ["f16", "f32", "q8_0"])
+def test_calls_of_many_shapes_in_turn(elem):
+    """Grids, batches and joins that differ from call to call, eager and replayed, share
+    one cache's partials and tickets: each gives its own bits every time."""
+    torch = torch_cuda()
+    say(f"case many shapes in turn {elem}")
+    rng = np.random.default_rng(58)
+    n_kv, hd, lens = 2, 64, [9000, 1, 700, 0, 130, 4000] + [int(x) for x in rng.integers(0, 300, 200)]
+    c, table, own = filled(rng, elem, n_kv, hd, 16, lens, junk=False)
+    t, all_lens = ints(table), ints(lens)
+    calls = []
+    for k, group, join in ((1, 4, 0), (len(lens), 4, 0), (2, 1, 0), (6, 20, 0), (6, 4, 2), (3, 16, 0)):
+        q = rng.standard_normal((k, n_kv * group * hd)).astype(np.float32)
+        calls.append((k, join, dev(q), torch.empty(q.shape, device="cuda"), expect(q, own[:k], n_kv, hd)))
+
+    def run(i):
+        k, join, q, out, _ = calls[i]
+        c.set_tuning(rv.RV_TUNE_PAGED_JOIN, join)
+        rv.paged_attention(q, c, 1, t[:k], all_lens[:k], scale_of(hd), out)
+
+    for i in sorted(range(len(calls)), key=lambda i: -calls[i][3].numel()):
+        run(i)  # (allocates)
+    torch.cuda.synchronize()
+    bits = [host(x[3]).view(np.uint32) for x in calls]
+    for b, (k, _, _, _, (want, a, vmax)) in zip(bits, calls):
+        for s in range(k):
+            check(b[s].view(np.float32), want[s], a, vmax, f"sequence {s} of {k}")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for i in (1, 0, 4, 2):
+            run(i)
+    for rep in range(6):
+        order = [int(x) for x in rng.permutation(len(calls))]
+        for x in calls:
+            x[3].fill_(float("nan"))
+        g.replay()
+        for i in order[:3]:
+            run(i)
+        g.replay()
+        for i in order[3:]:
+            run(i)
+        for b, x in zip(bits, calls):
+            assert np.array_equal(host(x[3]).view(np.uint32), b), f"turn {rep}"
